@@ -2,8 +2,8 @@
 
     python chill-attention_b200/build.py            # -> chill_attention/_lib/libchill_b200.so
 
-Each mask functor's tensor-core kernels and its CUDA-core kernels are translation units of their own
-(csrc/tc_inst.cu, csrc/simt_inst.cu with -DCHILL_INST_MASK=<functor>), compiled in parallel.
+Each mask functor's tensor-core kernels, its CUDA-core kernels and its kernels over a paged cache are translation units of their own
+(csrc/tc_inst.cu, csrc/simt_inst.cu, csrc/cache_inst.cu with -DCHILL_INST_MASK=<functor>), compiled in parallel.
 ``build_library`` is also what ``chill_attention.custom`` calls to produce a private
 library for a user-defined mask functor.  The objects of the built-in functors, nine tenths of a build, are kept beside the
 library and linked into such private libraries as they are.
@@ -41,7 +41,7 @@ def _nvcc():
 
 def _sources_digest(extra=()):
     h = hashlib.sha256()
-    names = sorted(n for n in os.listdir(CSRC) if n != "torch_ext.cpp") + [os.path.join(INCLUDE, "chill_b200.h")]
+    names = sorted(n for n in os.listdir(CSRC) if not n.startswith("torch_")) + [os.path.join(INCLUDE, "chill_b200.h")]
     for name in names:
         path = name if os.path.isabs(name) else os.path.join(CSRC, name)
         if os.path.isfile(path):
@@ -92,10 +92,10 @@ def build_library(out_path=None, custom_header=None, custom_functor=None, verbos
         os.replace(part, obj)
         return out
 
-    units = [(defines, src + ".cu", os.path.join(obj_dir, src + ".o")) for src in ("chill_abi", "host_pipeline")]
+    units = [(defines, src + ".cu", os.path.join(obj_dir, src + ".o")) for src in ("chill_abi", "host_pipeline", "cache_pages")]
     for fn in functors:
         builtin = fn in BUILTIN_FUNCTORS
-        for unit in ("tc", "simt"):
+        for unit in ("tc", "simt", "cache"):
             units.append((list(common if builtin else defines) + [f"-DCHILL_INST_MASK={fn}"], f"{unit}_inst.cu",
                           os.path.join(kept_dir if builtin else obj_dir, f"{unit}_{fn}.o")))
     with cf.ThreadPoolExecutor(max_workers=8) as ex:
@@ -114,16 +114,16 @@ def build_library(out_path=None, custom_header=None, custom_functor=None, verbos
 
 
 def build_extension(force=False):
-    """Compile the native eager-mode call path (csrc/torch_ext.cpp) against the installed torch; returns its path."""
+    """Compile the native eager-mode call path (csrc/torch_ext.cpp, csrc/torch_cache.cpp) against the installed torch; returns its path."""
     import sysconfig
 
     import torch
     from torch.utils.cpp_extension import include_paths, library_paths
 
     out = os.path.join(LIB_DIR, "_chill_torch.so")
-    src = os.path.join(CSRC, "torch_ext.cpp")
+    sources = [os.path.join(CSRC, name) for name in ("torch_ext.cpp", "torch_cache.cpp")]
     h = hashlib.sha256((torch.__version__ + sys.version).encode())
-    for path in (src, os.path.join(INCLUDE, "chill_b200.h")):
+    for path in sources + [os.path.join(CSRC, "torch_ext.h"), os.path.join(INCLUDE, "chill_b200.h")]:
         with open(path, "rb") as f:
             h.update(f.read())
     stamp = out + ".stamp"
@@ -133,7 +133,7 @@ def build_extension(force=False):
     cuda = os.path.dirname(os.path.dirname(_nvcc()))
     includes = include_paths() + [os.path.join(cuda, "include"), sysconfig.get_paths()["include"], INCLUDE]
     _run(["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
-          "-DTORCH_EXTENSION_NAME=_chill_torch"] + [x for i in includes for x in ("-isystem", i)] + [src, "-o", out]
+          "-DTORCH_EXTENSION_NAME=_chill_torch"] + [x for i in includes for x in ("-isystem", i)] + sources + ["-o", out]
          + [f"-L{p}" for p in library_paths()] + ["-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch", "-ltorch_python"])
     with open(stamp, "w") as f:
         f.write(h.hexdigest())

@@ -1,0 +1,195 @@
+// Attention of new tokens over a paged cache on the CUDA cores: fp32 (IEEE arithmetic) and every layout that the tensor-core
+// kernels can not take.  See cache_common.cuh for units and shares.
+//
+// A CTA of 128 threads works on 16 rows and 64 keys at a time, everything as fp32 in shared memory:
+//   S = Q K^T   a thread has one key and 8 rows: one vector of K and 8 (broadcast) of Q for 32 FMAs
+//   softmax     a warp has 4 rows; running maximum and sum in base 2
+//   O += P V    a thread has 4 channels of 2 D / 64 rows (registers)
+#pragma once
+#include "cache_common.cuh"
+#include "tc_common.cuh"
+
+namespace chill {
+namespace cache {
+
+constexpr int kSimtThreads = 128;
+constexpr int kSimtRows = 16;
+
+template <int DP>
+struct SimtSmem {
+  static constexpr int kKRow = DP + 4;  // floats of a K row: 16-byte vectors of 8 consecutive keys fall into different banks
+  static constexpr int kQ = 0;
+  static constexpr int kK = kQ + kSimtRows * DP;
+  static constexpr int kV = kK + kKeyTile * kKRow;
+  static constexpr int kS = kV + kKeyTile * DP;
+  static constexpr int kM = kS + kSimtRows * kKeyTile;  // alpha of every row
+  static constexpr int kBad = kM + kSimtRows;           // a key has no page
+  static constexpr int kCum = kBad + kKeyTile;
+  static constexpr int kBytes = (kCum + kScanEntries + 1) * 4;
+};
+
+template <typename T, int DP, class M>
+__global__ void __launch_bounds__(kSimtThreads) cached_simt_kernel(CachedP p) {
+  using L = SimtSmem<DP>;
+  extern __shared__ __align__(16) float smem[];
+  float *sq = smem + L::kQ, *sk = smem + L::kK, *sv = smem + L::kV, *ss = smem + L::kS, *sa = smem + L::kM;
+  int* bad = reinterpret_cast<int*>(smem + L::kBad);
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  constexpr int kChunks = DP / 4;                                                   // channel quads
+  constexpr int kGroups = kSimtThreads / kChunks < kSimtRows ? kSimtThreads / kChunks : kSimtRows;  // threads of a quad
+  constexpr int kOwn = kSimtRows / kGroups;                                         // rows of a thread in O += P V
+  const int quad = tid % kChunks, group = tid / kChunks;
+  const bool pv = group < kGroups;
+  const int* cum;
+  Share share = begin_share<M, kSimtThreads>(p, reinterpret_cast<int*>(smem + L::kCum), cum);
+  pdl_launch_dependents();
+  Piece piece;
+  while (share.next(p, cum, piece)) {
+    const RowTile t = row_tile<M>(p, piece.entry);
+    const int tiles = t.n_tiles == 0 ? 0 : piece.t1;
+    __syncthreads();
+    for (int idx = tid; idx < kSimtRows * DP; idx += kSimtThreads) {
+      const int r = idx / DP, d = idx % DP;
+      float x = 0.f;
+      if (r < t.rows && d < p.D) {
+        const int i = (t.r0 + r) / p.G, h = piece.head * p.G + (t.r0 + r) % p.G;
+        x = to_f(row_ptr<T>(p.q, t.b, h, i)[d * p.q.sd]);
+      }
+      sq[r * DP + d] = x;
+    }
+    float m[4], l[4];  // rows 4 * warp + n, the same in all lanes
+    float acc[kOwn][4];
+#pragma unroll
+    for (int n = 0; n < 4; ++n) m[n] = -CUDART_INF_F, l[n] = 0.f;
+#pragma unroll
+    for (int n = 0; n < kOwn; ++n) acc[n][0] = acc[n][1] = acc[n][2] = acc[n][3] = 0.f;
+
+    for (int kt = piece.t0; kt < tiles; ++kt) {
+      const int k0 = t.k_lo + kt * kKeyTile;
+      __syncthreads();  // the tile before has been used
+      for (int idx = tid; idx < kKeyTile * kChunks; idx += kSimtThreads) {
+        const int key = idx / kChunks, d = (idx % kChunks) * 4, at = k0 + key;
+        const int page = at < t.total ? p.table[t.b * p.table_sb + at / p.page] : -1;
+        const bool there = page >= 0 && page < p.num_pages;
+        float4 kx = make_float4(0.f, 0.f, 0.f, 0.f), vx = kx;
+        if (there) {
+          const int row = at % p.page;
+          const T* ks = reinterpret_cast<const T*>(p.k.p) + page * p.k.sb + piece.head * p.k.sh + row * p.k.sl;
+          const T* vs = reinterpret_cast<const T*>(p.v.p) + page * p.v.sb + piece.head * p.v.sh + row * p.v.sl;
+          float* kf = &kx.x;
+          float* vf = &vx.x;
+#pragma unroll
+          for (int u = 0; u < 4; ++u) {
+            if (d + u < p.D) {
+              kf[u] = to_f(ks[(d + u) * p.k.sd]);
+              vf[u] = to_f(vs[(d + u) * p.v.sd]);
+            }
+          }
+        }
+        *reinterpret_cast<float4*>(sk + key * L::kKRow + d) = kx;
+        *reinterpret_cast<float4*>(sv + key * DP + d) = vx;
+        if (d == 0) bad[key] = !there;
+      }
+      __syncthreads();
+      {  // S: key tid % 64, rows 8 * (tid / 64) on
+        const int key = tid & 63, r0 = (tid >> 6) * 8;
+        float s[8];
+#pragma unroll
+        for (int n = 0; n < 8; ++n) s[n] = 0.f;
+#pragma unroll 4
+        for (int d = 0; d < DP; d += 4) {
+          const float4 kx = *reinterpret_cast<const float4*>(sk + key * L::kKRow + d);
+#pragma unroll
+          for (int n = 0; n < 8; ++n) {
+            const float4 qx = *reinterpret_cast<const float4*>(sq + (r0 + n) * DP + d);
+            s[n] = fmaf(qx.x, kx.x, fmaf(qx.y, kx.y, fmaf(qx.z, kx.z, fmaf(qx.w, kx.w, s[n]))));
+          }
+        }
+        const int at = k0 + key;
+        const bool full = at >= t.full_lo && at < t.full_hi;
+#pragma unroll
+        for (int n = 0; n < 8; ++n) {
+          const int r = r0 + n;
+          bool ok = r < t.rows && at < t.total && !bad[key];
+          if (ok && !full) {
+            const int i = (t.r0 + r) / p.G;
+            ok = sees<M>(p, t, i, token_position(p, t, i), at);
+          }
+          ss[r * kKeyTile + key] = ok ? s[n] * p.scale_log2 : -CUDART_INF_F;
+        }
+      }
+      __syncthreads();
+#pragma unroll
+      for (int n = 0; n < 4; ++n) {  // softmax of row 4 * warp + n
+        float* row = ss + (warp * 4 + n) * kKeyTile;
+        const float x = row[lane], y = row[lane + 32];
+        float top = fmaxf(x, y);
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+        const float m_new = fmaxf(m[n], top), safe = m_new == -CUDART_INF_F ? 0.f : m_new;
+        const float a = exp2f(m[n] - safe);  // m = -inf: 0
+        const float ex = exp2f(x - safe), ey = exp2f(y - safe);
+        l[n] = l[n] * a + warp_sum(ex + ey);
+        m[n] = m_new;
+        row[lane] = ex;
+        row[lane + 32] = ey;
+        if (lane == 0) sa[warp * 4 + n] = a;
+      }
+      __syncthreads();
+      if (pv) {
+#pragma unroll
+        for (int n = 0; n < kOwn; ++n) {
+          const float a = sa[group * kOwn + n];
+#pragma unroll
+          for (int u = 0; u < 4; ++u) acc[n][u] *= a;
+        }
+#pragma unroll 4
+        for (int key = 0; key < kKeyTile; ++key) {
+          const float4 vx = *reinterpret_cast<const float4*>(sv + key * DP + quad * 4);
+#pragma unroll
+          for (int n = 0; n < kOwn; ++n) {
+            const float w = ss[(group * kOwn + n) * kKeyTile + key];
+            if (w != 0.f) {  // a hidden key may hold anything
+              acc[n][0] = fmaf(w, vx.x, acc[n][0]); acc[n][1] = fmaf(w, vx.y, acc[n][1]);
+              acc[n][2] = fmaf(w, vx.z, acc[n][2]); acc[n][3] = fmaf(w, vx.w, acc[n][3]);
+            }
+          }
+        }
+      }
+    }
+
+    // maximum and sum of every row, for the threads that hold its O
+    __syncthreads();
+    float* sm = ss;
+    if (lane < 4) {
+#pragma unroll
+      for (int n = 0; n < 4; ++n)
+        if (lane == n) sm[warp * 4 + n] = m[n], sm[kSimtRows + warp * 4 + n] = l[n];
+    }
+    __syncthreads();
+    if (pv) {
+#pragma unroll
+      for (int n = 0; n < kOwn; ++n) {
+        const int r = group * kOwn + n, all = p.N * p.G;
+        if (t.r0 + r >= all) continue;
+        const float mr = sm[r], lr = sm[kSimtRows + r];
+        if (piece.whole) {
+          const int i = (t.r0 + r) / p.G, h = piece.head * p.G + (t.r0 + r) % p.G;
+          const float inv = r < t.rows && lr > 0.f ? 1.f / lr : 0.f;
+          T* to = o_row<T>(p, t.b, h, i);
+#pragma unroll
+          for (int u = 0; u < 4; ++u)
+            if (quad * 4 + u < p.D) to[(quad * 4 + u) * p.o.sd] = from_f<T>(acc[n][u] * inv);
+          if (quad == 0) store_lse(p, t.b, h, i, r < t.rows, mr, lr);
+        } else {
+          const long long at = (long long)piece.slot * p.rows + r;
+          if (quad * 4 < p.D) *reinterpret_cast<float4*>(p.part_o + at * p.D + quad * 4) = make_float4(acc[n][0], acc[n][1], acc[n][2], acc[n][3]);
+          if (quad == 0) p.part_ml[at] = make_float2(mr, lr);
+        }
+      }
+    }
+  }
+}
+
+}  // namespace cache
+}  // namespace chill

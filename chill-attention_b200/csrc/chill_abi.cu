@@ -9,6 +9,8 @@
 #include <mutex>
 
 #include "bwd_tc.cuh"
+#include "cache_common.cuh"
+#include "cache_launch.h"
 #include "chill_b200.h"
 #include "fwd_tc.cuh"
 #include "generic.cuh"
@@ -27,6 +29,7 @@ static int cuda_fail(cudaError_t e, const char* what) {
 }
 
 int record_cuda_failure(cudaError_t e, const char* what) { return cuda_fail(e, what); }  // for host_pipeline.cu
+void count_launches(int n) { g_launches += n; }                                                       // for cache_pages.cu
 
 static int* device_status_ptr() {
   // one word per device (the symbol is instantiated in every device's module image)
@@ -46,6 +49,19 @@ static int* split_status_ptr() {
 // ------------------------------------------------------------------------- validation
 static size_t esize(int dtype) { return dtype == CHILL_F32 ? 4 : 2; }
 
+static int check_mask(const chill_mask_desc& m) {
+  if (m.n_args < 0 || m.n_args > CHILL_MAX_MASK_ARGS) return CHILL_E_INVALID;
+#ifdef CHILL_CUSTOM_MASK
+  if (m.id < 0 || m.id > CHILL_MASK_CUSTOM) return CHILL_E_UNSUPPORTED;
+#else
+  if (m.id < 0 || m.id >= CHILL_MASK_CUSTOM) return CHILL_E_UNSUPPORTED;
+#endif
+  if (m.id == CHILL_MASK_CHUNKWISE && (m.n_args < 2 || m.i[0] <= 0)) return CHILL_E_INVALID;
+  if (m.id == CHILL_MASK_SLIDING && m.n_args < 2) return CHILL_E_INVALID;
+  if (m.id == CHILL_MASK_PREFIXLM && m.n_args < 1) return CHILL_E_INVALID;
+  return CHILL_OK;
+}
+
 static int check_shape(const chill_shape& s) {
   if (s.B <= 0 || s.H <= 0 || s.H_kv <= 0 || s.Lq <= 0 || s.Lk <= 0 || s.D <= 0) return CHILL_E_INVALID;
   if (s.H % s.H_kv != 0) return CHILL_E_INVALID;
@@ -53,16 +69,7 @@ static int check_shape(const chill_shape& s) {
   if (s.D > kMaxD) return CHILL_E_UNSUPPORTED;
   if (s.seq_len <= 0 || s.q_offset < 0 || s.k_offset < 0) return CHILL_E_INVALID;
   if (s.B > 65535 || s.H > 65535) return CHILL_E_TOO_LARGE;
-  if (s.mask.n_args < 0 || s.mask.n_args > CHILL_MAX_MASK_ARGS) return CHILL_E_INVALID;
-#ifdef CHILL_CUSTOM_MASK
-  if (s.mask.id < 0 || s.mask.id > CHILL_MASK_CUSTOM) return CHILL_E_UNSUPPORTED;
-#else
-  if (s.mask.id < 0 || s.mask.id >= CHILL_MASK_CUSTOM) return CHILL_E_UNSUPPORTED;
-#endif
-  if (s.mask.id == CHILL_MASK_CHUNKWISE && (s.mask.n_args < 2 || s.mask.i[0] <= 0)) return CHILL_E_INVALID;
-  if (s.mask.id == CHILL_MASK_SLIDING && s.mask.n_args < 2) return CHILL_E_INVALID;
-  if (s.mask.id == CHILL_MASK_PREFIXLM && s.mask.n_args < 1) return CHILL_E_INVALID;
-  return CHILL_OK;
+  return check_mask(s.mask);
 }
 
 // The functors do their index arithmetic in 32 bits (position + constant), so the 64-bit constants of the ABI are
@@ -642,6 +649,9 @@ static int bwd_wide(const chill_bwd_args& a, cudaStream_t st) {
   return e == 0 ? CHILL_OK : cuda_fail((cudaError_t)e, "bwd_wide launch");
 }
 
+// --------------------------------------------------------------------- attention over a paged cache
+#include "cache_dispatch.cuh"
+
 // ------------------------------------------------------------- backward without a scratch argument
 // Library-owned scratch for chill_bwd_noalloc: lives in the device image of this file, one copy per
 // GPU that loads the library.  In host code the name below is only a handle for the runtime; the
@@ -808,6 +818,21 @@ int chill_bwd_noalloc(const chill_bwd_args* a, void* stream) {
   if (bwd_tf32_eligible(b)) return bwd_tf32(b, (cudaStream_t)stream);
   if (b.s.flags & CHILL_FLAG_REQUIRE_TC) return CHILL_E_UNSUPPORTED;
   return bwd_generic(b, (cudaStream_t)stream);
+}
+
+size_t chill_cached_workspace_bytes(const chill_cached_args* a) {
+  CachedPlan c;
+  return check_cached(a, false) == CHILL_OK && plan_cached(*a, c) == CHILL_OK ? c.bytes : 0;
+}
+
+int chill_cached_kernel(const chill_cached_args* a) {
+  const int st = check_cached(a, true);
+  return st != CHILL_OK ? st : cached_kernel(*a);
+}
+
+int chill_cached_fwd(const chill_cached_args* a, void* stream) {
+  const int st = check_cached(a, true);
+  return st != CHILL_OK ? st : cached_fwd(*a, (cudaStream_t)stream);
 }
 
 int chill_mask_tabulate(const chill_mask_desc* m, int32_t n, int32_t tile, uint8_t* dense, int32_t* k_lims,

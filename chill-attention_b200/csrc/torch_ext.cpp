@@ -22,6 +22,7 @@
 #include <vector>
 
 #include "chill_b200.h"
+#include "torch_ext.h"
 
 namespace py = pybind11;
 using at::Tensor;
@@ -186,6 +187,8 @@ bool arguments_ok(const Tensor& q, const Tensor& k, const Tensor& v, const std::
   return true;
 }
 
+}  // namespace
+
 // Mask constants as both members of the descriptor.  The whole number is what Python's int() makes of the constant, which
 // refuses NaN and infinity; what 64 bits do not hold is saturated (the library clamps further).
 void set_mask_constants(chill_mask_desc& desc, const py::tuple& mask_args) {
@@ -202,6 +205,10 @@ void set_mask_constants(chill_mask_desc& desc, const py::tuple& mask_args) {
     if (PyErr_Occurred()) throw py::error_already_set();
   }
 }
+
+void throw_chill_error(const std::string& message) { throw ChillError(message); }
+
+namespace {
 
 // O, (O, LSE) when return_lse, or None when the arguments do not pass the checks.
 py::object attention(std::shared_ptr<Library> lib, const Tensor& q, const Tensor& k, const Tensor& v, std::optional<Tensor> lens,
@@ -257,5 +264,6 @@ PYBIND11_MODULE(_chill_torch, m) {
   });
   m.def("set_deterministic", [](bool flag) { g_deterministic = flag; });
   m.def("backward_counts", [] { return std::make_pair(g_bwd_tc.load(), g_bwd_generic.load()); });
+  bind_cache(m);
   m.attr("abi_version") = CHILL_ABI_VERSION;
 }

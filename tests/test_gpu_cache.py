@@ -1,0 +1,515 @@
+"""Paged cache on the GPU: pages, storing, attention of new tokens, accepted paths; against the 64-bit oracle."""
+import pytest
+import torch
+
+from cache_helpers import Problem, check_attention, masks
+from helpers import ensure_built
+from oracle import cache_oracle as orc
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module", autouse=True)
+def _lib():
+    ensure_built()
+    from chill_attention import _cabi
+
+    lib = _cabi.load_library()
+    yield lib
+    assert lib.chill_read_device_status() == 0
+
+
+def ints(x):
+    return torch.tensor(x, dtype=torch.int32, device="cuda")
+
+
+def strided(t, layout):
+    """The same values with other strides."""
+    t = t.cuda()
+    if layout == "transposed":  # [.., head, row, channel] kept as [.., row, head, channel]
+        return t.transpose(1, 2).contiguous().transpose(1, 2)
+    if layout == "padded":      # rows 16-byte aligned, with gaps of NaN
+        wide = torch.full((*t.shape[:3], t.shape[3] + 16), float("nan"), dtype=t.dtype, device="cuda")
+        wide[..., :t.shape[3]] = t
+        return wide[..., :t.shape[3]]
+    if layout == "odd":         # channels two apart, base not aligned
+        wide = torch.full((*t.shape[:3], 2 * t.shape[3] + 1), float("nan"), dtype=t.dtype, device="cuda")
+        wide[..., 1::2] = t
+        return wide[..., 1::2]
+    return t
+
+
+def attend(p, mask, layout="plain", flags=0):
+    from chill_attention import cache
+
+    scale = p.q.shape[3] ** -0.5
+    q, k, v = (strided(t, layout) for t in (p.q, p.k_cache, p.v_cache))
+    return cache._attention(q, k, v, p.table.cuda(), p.step(), mask, scale, True, flags), scale
+
+
+def kernel_of(p, flags=0):
+    """Which kernel serves the contiguous call."""
+    import ctypes
+
+    from chill_attention import _cabi
+
+    B, H, N, D = p.q.shape
+    a = _cabi.CachedArgs()
+    a.mask = _cabi.mask_desc(_cabi.MASK_CAUSAL, ())
+    a.B, a.H, a.H_kv, a.N, a.D, a.dtype = B, H, p.k_cache.shape[1], N, D, _cabi._DTYPES[p.dtype]
+    a.page_size, a.num_pages, a.table_width, a.sm_scale, a.flags = p.page, p.k_cache.shape[0], p.table.shape[1], 1.0, flags
+    a.q = a.k_cache = a.v_cache = a.o = a.table = a.lens = a.new_lens = 4096
+    for name, t in (("q_strides", p.q), ("o_strides", p.q), ("k_cache_strides", p.k_cache), ("v_cache_strides", p.v_cache)):
+        setattr(a, name, (ctypes.c_int64 * 4)(*t.stride()))
+    return _cabi.load_library().chill_cached_kernel(ctypes.byref(a))
+
+
+def run_and_check(p, mask, layout="plain", flags=0):
+    (o, lse), scale = attend(p, mask, layout, flags)
+    assert o.shape == p.q.shape and o.is_contiguous()
+    from chill_attention import _cabi
+
+    tensor_cores = layout not in ("odd",) and kernel_of(p, flags) != _cabi.CACHED_CUDA_CORES
+    check_attention(o, lse, p, mask, scale, tensor_cores)
+    return o, lse
+
+
+DTYPES = [torch.float32, torch.float16, torch.bfloat16]
+RAGGED = [300, 0, 1, 64, 63, 129, 17, 200]
+
+
+@pytest.mark.parametrize("kind", ["one", "chain", "tree"])
+@pytest.mark.parametrize("mask", list(masks()))
+@pytest.mark.parametrize("dtype", DTYPES, ids=["fp32", "fp16", "bf16"])
+def test_masks_and_ragged_lengths(dtype, mask, kind):
+    N = 1 if kind == "one" else 9
+    new = [N, N, 0, max(N - 2, 1), N, 1, N, 0]
+    p = Problem(dtype, 6, 2, 64, RAGGED, new, N, 16, tree=kind == "tree", seed=len(mask) + N)
+    run_and_check(p, masks()[mask])
+
+
+@pytest.mark.parametrize("D", [16, 32, 64, 128, 256])
+@pytest.mark.parametrize("group", [1, 3, 8])
+@pytest.mark.parametrize("dtype", DTYPES, ids=["fp32", "fp16", "bf16"])
+def test_head_dims_and_groups(dtype, group, D):
+    p = Problem(dtype, 2 * group, 2, D, [70, 3, 128, 0], [5, 2, 5, 5], 5, 32, tree=group != 3, seed=D + group)
+    run_and_check(p, masks()["causal"])
+
+
+@pytest.mark.parametrize("layout", ["transposed", "padded", "odd"])
+@pytest.mark.parametrize("dtype", DTYPES, ids=["fp32", "fp16", "bf16"])
+def test_strides(dtype, layout):
+    for N, D in ((3, 64), (40, 128)):
+        p = Problem(dtype, 8, 2, D, [90, 31, 64], [N, N - 1, N], N, 16, tree=True, seed=D)
+        run_and_check(p, masks()["window"], layout)
+
+
+@pytest.mark.parametrize("page", [1, 5, 8, 16, 48, 64, 100, 128, 512])
+def test_page_sizes(page):
+    for N, dtype in ((2, torch.bfloat16), (33, torch.float16)):
+        p = Problem(dtype, 4, 2, 64, [257, 40, 0, 99], [N, 1, N, N], N, page, tree=True, seed=page)
+        run_and_check(p, masks()["causal"])
+
+
+@pytest.mark.parametrize("N", [15, 16, 17, 31, 32, 33, 64, 65, 130])
+@pytest.mark.parametrize("kind", ["chain", "tree"])
+def test_row_tiles(kind, N):
+    for D, dtype in ((64, torch.bfloat16), (128, torch.float16)):
+        p = Problem(dtype, 4, 1, D, [150, 10, 64], [N, N - 3, 1], N, 64, tree=kind == "tree", seed=N)
+        run_and_check(p, masks()["window_ahead" if N % 2 else "causal"])
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=["fp32", "fp16", "bf16"])
+def test_one_long_request_is_split(dtype):
+    for N in (1, 6, 70):
+        p = Problem(dtype, 4, 1, 64, [5000], [N], N, 64, tree=N == 6, seed=N)
+        run_and_check(p, masks()["causal"])
+
+
+def test_sharp_scores_over_many_parts():
+    """Scores of tens: parts whose maxima differ by hundreds of powers of two."""
+    p = Problem(torch.float16, 8, 2, 128, [3000, 2000], [4, 4], 4, 32, tree=True, seed=4, sharp=16.0)
+    run_and_check(p, masks()["causal"])
+
+
+def test_many_short_requests():
+    """More (request, tile of rows) pairs than every CTA sums up by itself."""
+    B = 1100
+    p = Problem(torch.bfloat16, 2, 1, 64, [(7 * b) % 40 for b in range(B)], [(b % 3) for b in range(B)], 2, 16, seed=1)
+    run_and_check(p, masks()["causal"])
+
+
+@pytest.mark.parametrize("N", [2, 40])
+@pytest.mark.parametrize("dtype", DTYPES, ids=["fp32", "fp16", "bf16"])
+def test_keys_without_a_page_are_not_there(dtype, N):
+    holes = [(0, 0, -1), (0, 3, 10 ** 6), (1, 0, -1), (1, 1, -7), (1, 2, -1), (1, 3, 2 ** 30), (1, 4, -1), (2, 2, -2 ** 31)]
+    p = Problem(dtype, 4, 2, 64, [130, 30, 80], [N, N, N], N, 16, tree=True, seed=9, holes=holes)
+    o, lse = run_and_check(p, masks()["causal"])
+    q = Problem(dtype, 4, 2, 64, [130, 30], [N, N], N, 16, seed=9, holes=[(b, j, -1) for b in (0, 1) for j in range((130 if b == 0 else 30) // 16 + 1 + N // 16)])
+    o, lse = run_and_check(q, masks()["causal"])
+    if N == 2:
+        assert torch.isneginf(lse).all() and (o == 0).all()
+
+
+def test_lengths_beyond_the_table_and_below_zero():
+    p = Problem(torch.bfloat16, 4, 2, 64, [60, 50, 20], [8, 8, 8], 8, 16, seed=2)
+    from chill_attention import ChillStep, chill_attention_cached
+
+    s = p.step()
+    step = ChillStep(ints([10 ** 9, -5, 20]), ints([10 ** 9, -3, 2 ** 31 - 1]), s.slots, s.positions, None)
+    o, lse = chill_attention_cached(p.q.cuda(), p.k_cache.nan_to_num(0.5).cuda(), p.v_cache.nan_to_num(0.5).cuda(), p.table.cuda(), step, masks()["causal"],
+                                    return_lse=True)
+    assert torch.isfinite(o).all() and (o[1] == 0).all() and (lse[1] == 0).all()
+    want, _ = chill_attention_cached(p.q.cuda(), p.k_cache.nan_to_num(0.5).cuda(), p.v_cache.nan_to_num(0.5).cuda(), p.table.cuda(), s, masks()["causal"],
+                                     return_lse=True)
+    assert torch.equal(o[2], want[2])
+
+
+def test_same_result_every_time():
+    p = Problem(torch.bfloat16, 8, 2, 128, [2500, 900, 100], [6, 6, 2], 6, 64, tree=True, seed=3)
+    (a, la), _ = attend(p, masks()["causal"])
+    for _ in range(3):
+        (b, lb), _ = attend(p, masks()["causal"])
+        assert torch.equal(a, b) and torch.equal(la, lb)
+
+
+def test_custom_mask():
+    import os
+
+    import chill_attention as ca
+
+    here = os.path.dirname(os.path.abspath(__file__))
+
+    class DilatedCausalMask(ca.ChillMask):
+        cuda_functor_header = os.path.join(here, "custom_masks", "dilated_causal_mask.h")
+        cuda_functor = "DilatedCausalMask"
+
+    dilation = 3
+    mask = DilatedCausalMask((dilation,))
+    p = Problem(torch.float16, 4, 2, 64, [100, 33], [4, 4], 4, 16, seed=5)
+    (o, lse), scale = attend(p, mask)
+    real = orc.builtin_mask_dense
+    orc.builtin_mask_dense = lambda name, args, q, k: (q[:, None] >= k[None]) & ((q[:, None] - k[None]) % dilation == 0)
+    try:
+        check_attention(o, lse, p, mask, scale, True)
+    finally:
+        orc.builtin_mask_dense = real
+
+
+# ------------------------------------------------------------------------------------------------------- pages
+def check_pages(pages, table, held, stack, missing=None):
+    assert pages.table.tolist() == table and pages.held.tolist() == held
+    assert pages.n_free.item() == len(stack) and pages.free[:len(stack)].tolist() == stack
+    if missing is not None:
+        assert pages.missing.item() == missing
+
+
+@pytest.mark.parametrize("B,N,page", [(1, 1, 16), (3, 5, 1), (8, 1, 16), (70, 33, 7), (600, 4, 16), (1500, 1, 64), (2, 3000, 16)])
+def test_reserve_and_trim_follow_the_oracle(B, N, page):
+    import chill_attention as ca
+
+    g = torch.Generator().manual_seed(B + N)
+    draw = lambda hi: torch.randint(0, hi + 1, (B,), generator=g).tolist()  # noqa: E731
+    num = B * (-(-(60 + N) // page)) * 2 // 3 + 3  # not always enough
+    pages = ca.ChillPages.empty(B, 60 + N, num, page)
+    table, held, stack = pages.table.tolist(), pages.held.tolist(), pages.free.tolist()
+    lens = [0] * B
+    for turn in range(4):
+        new = draw(N)
+        parents = [[int(x) for x in torch.randint(-2, i + 2, (1,), generator=g)] [0] for _ in range(B) for i in range(N)] if turn == 2 and N < 100 else None
+        parents = [parents[b * N:(b + 1) * N] for b in range(B)] if parents else None
+        step = ca.chill_pages_reserve(pages, ints(lens), ints(new), N, page, ints(parents) if parents else None)
+        table, held, n, missing, slots, positions, sets = orc.reserve(table, held, stack, len(stack), lens, new, N, page, parents)
+        stack = stack[:n]
+        check_pages(pages, table, held, stack, missing)
+        assert step.slots.tolist() == slots and step.positions.tolist() == positions
+        if parents is None:
+            assert step.ancestors is None
+        else:
+            bits = step.ancestors.cpu()
+            for b in range(B):
+                for i in range(N):
+                    assert {j for j in range(N) if (int(bits[b, i, j // 32]) >> (j % 32)) & 1} == sets[b][i]
+        lens = [min(c + n, len(table[0]) * page) if turn != 1 else 0 if b % 3 == 0 else c for b, (c, n) in enumerate(zip(lens, new))]
+        lens = [min(c, h * page) for c, h in zip(lens, held)]
+        ca.chill_pages_trim(pages, ints(lens), page)
+        table, held, stack = orc.trim(table, held, stack, len(stack), lens, page)
+        check_pages(pages, table, held, stack)
+    ca.chill_pages_trim(pages, ints([0] * B), page)
+    assert pages.n_free.item() == num and sorted(pages.free.tolist()) == list(range(num)) and (pages.table == -1).all()
+
+
+def test_reserve_survives_nonsense():
+    import chill_attention as ca
+
+    pages = ca.ChillPages.empty(4, 64, 6, 16)
+    step = ca.chill_pages_reserve(pages, ints([-9, 2 ** 31 - 1, 10, 0]), ints([-1, 2 ** 31 - 1, 3, 7]), 8, 16)
+    assert pages.held.tolist() == [0, 4, 1, 1] and pages.n_free.item() == 0 and pages.missing.item() == 0
+    assert step.slots[0].tolist() == [-1] * 8 and step.slots[1].tolist() == [-1] * 8 and (step.slots[2, :3] >= 0).all()
+    pages.held.fill_(100)
+    pages.n_free.fill_(1000)
+    ca.chill_pages_trim(pages, ints([0, 0, 0, 0]), 16)  # a stack that is full already takes nothing more
+    assert pages.n_free.item() == 6 and (pages.table == -1).all()
+
+
+# -------------------------------------------------------------------------------------------- storing and keeping
+@pytest.mark.parametrize("layout", ["plain", "transposed", "padded", "odd"])
+@pytest.mark.parametrize("dtype", DTYPES, ids=["fp32", "fp16", "bf16"])
+def test_append(dtype, layout):
+    import chill_attention as ca
+
+    for D, N, page in ((64, 7, 16), (16, 1, 5), (256, 70, 64)):
+        p = Problem(dtype, 3, 3, D, [10, 0, 77], [N, 0, N - 1], N, page, seed=D)
+        k, v = torch.randn(3, 3, N, D).to(dtype), torch.randn(3, 3, N, D).to(dtype)
+        want_k, want_v = p.k_cache.clone(), p.v_cache.clone()
+        for b in range(3):
+            for i, s in enumerate(p.slots[b]):
+                if s >= 0:
+                    want_k[s // page, :, s % page], want_v[s // page, :, s % page] = k[b, :, i], v[b, :, i]
+        slots = p.step().slots
+        slots[1, 0] = p.k_cache.shape[0] * page  # outside the cache
+        kc, vc = strided(p.k_cache, layout), strided(p.v_cache, layout)
+        ca.chill_cache_append(kc, vc, strided(k, layout), strided(v, layout), slots)
+        assert torch.equal(kc.cpu().nan_to_num(7), want_k.nan_to_num(7))
+        assert torch.equal(vc.cpu().nan_to_num(7), want_v.nan_to_num(7))
+
+
+@pytest.mark.parametrize("layout", ["plain", "transposed", "odd"])
+@pytest.mark.parametrize("dtype", DTYPES, ids=["fp32", "fp16", "bf16"])
+def test_commit(dtype, layout):
+    import chill_attention as ca
+
+    N, page, lens = 40, 16, [10, 0, 77, 15, 30]
+    paths = [[0, 3, 4, 9, 20, 21, 22, 30, 31, 35, 38, 39], [0, 1, 2, 3, 4, 5, 6, 7, 8, 9, 10, 11], [39] + [0] * 11,
+             [1, 2, 3, 4, 5, 6, 7, 8, 9, 10, 11, 50], [5, 3, -1, 90, 4, 39, 39, 7, 8, 9, 10, 11]]
+    accepted, new = [12, 11, 1, 99, 8], [40, 40, 40, 12, 40]
+    for D in (64, 256):
+        p = Problem(dtype, 2, 2, D, lens, new, N, page, tree=True, seed=D)
+        want_k, want_v = p.k_cache.clone(), p.v_cache.clone()
+        for b, c in enumerate(lens):
+            for j in range(min(accepted[b], 12, new[b])):
+                f = paths[b][j]
+                if j < f < new[b]:
+                    for w, have in ((want_k, p.k_cache), (want_v, p.v_cache)):
+                        w[p.table[b, (c + j) // page], :, (c + j) % page] = have[p.table[b, (c + f) // page], :, (c + f) % page]
+        kc, vc = strided(p.k_cache, layout), strided(p.v_cache, layout)
+        out = ca.chill_cache_commit(kc, vc, p.table.cuda(), p.step(), ints(paths), ints(accepted))
+        assert out.tolist() == [22, 11, 78, 27, 38]
+        assert torch.equal(kc.cpu().nan_to_num(7), want_k.nan_to_num(7)) and torch.equal(vc.cpu().nan_to_num(7), want_v.nan_to_num(7))
+
+
+# ------------------------------------------------------------------------------------------------ the operators together
+def run_session(mask, dtype, total, chunks, page, H, Hkv, D, seed=0):
+    """A batch of two, fed in chunks through the cache; returns the rows of q, k, v, o as whole sequences."""
+    import chill_attention as ca
+
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    q, k, v = (torch.randn(2, h, total, D, device="cuda", generator=g).to(dtype) for h in (H, Hkv, Hkv))
+    pages = ca.ChillPages.empty(2, total, 2 * (-(-total // page)), page)
+    kc, vc = (torch.full((2 * (-(-total // page)), Hkv, page, D), float("nan"), dtype=dtype, device="cuda") for _ in range(2))
+    lens, parts = ints([0, 0]), []
+    at = 0
+    for n in chunks:
+        new = ints([n, n])
+        step = ca.chill_pages_reserve(pages, lens, new, n, page)
+        ca.chill_cache_append(kc, vc, k[:, :, at:at + n], v[:, :, at:at + n], step.slots)
+        parts.append(ca.chill_attention_cached(q[:, :, at:at + n], kc, vc, pages.table, step, mask, return_lse=True))
+        lens = lens + new
+        at += n
+    assert at == total and pages.missing.item() == 0
+    return q, k, v, torch.cat([o for o, _ in parts], 2), torch.cat([s for _, s in parts], 2)
+
+
+@pytest.mark.parametrize("name", ["causal", "window", "prefix_lm", "chunkwise"])
+@pytest.mark.parametrize("dtype", DTYPES, ids=["fp32", "fp16", "bf16"])
+def test_a_sequence_through_the_cache_is_the_sequence_at_once(dtype, name):
+    """Chunks of any size and single tokens give what chill_attention gives for the whole sequence (a chunk of a chunkwise mask has to
+    come at once, a prefix too)."""
+    import chill_attention as ca
+    from helpers import O_ATOL
+
+    mask = masks()[name]
+    chunks = [24, 48, 24, 72, 24] if name == "chunkwise" else [60, 1, 1, 70, 3, 1, 55, 1]
+    q, k, v, o, lse = run_session(mask, dtype, 192, chunks, 16, 4, 2, 64)
+    want, want_lse = ca.chill_attention(q, k, v, mask=mask, return_lse=True)
+    # both are within the operator's bar of the exact result
+    assert (o.float() - want.float()).abs().max().item() <= 2 * O_ATOL[dtype]
+    assert (lse - want_lse).abs().max().item() <= 1e-3 * 8
+
+
+def test_speculative_steps():
+    """Trees of drafts, an accepted path kept, the next tree: the cache then holds what feeding the accepted tokens one by one gives, and
+    every node's attention is that of its own path as a sequence."""
+    import chill_attention as ca
+
+    D, page, N, B = 64, 16, 12, 2
+    g = torch.Generator().manual_seed(3)
+    pages = ca.ChillPages.empty(B, 200, 40, page)
+    kc, vc = (torch.full((40, 2, page, D), float("nan"), device="cuda") for _ in range(2))
+    lens = ints([0, 0])
+    kept_k, kept_v = [[] for _ in range(B)], [[] for _ in range(B)]
+    for turn in range(6):
+        parents = [[int(torch.randint(max(-1, i - 3), i, (1,), generator=g)) for i in range(N)] for _ in range(B)]
+        new = [N, N - turn]
+        q, k, v = torch.randn(B, 4, N, D, generator=g), torch.randn(B, 2, N, D, generator=g), torch.randn(B, 2, N, D, generator=g)
+        step = ca.chill_pages_reserve(pages, lens, ints(new), N, page, ints(parents))
+        ca.chill_cache_append(kc, vc, k.cuda(), v.cuda(), step.slots)
+        o = ca.chill_attention_cached(q.cuda(), kc, vc, pages.table, step, ca.CausalChillMask())
+        path, accepted = [], []
+        for b in range(B):
+            chain = []  # the longest way down to the last real node
+            node = new[b] - 1
+            while node >= 0:
+                chain.append(node)
+                node = parents[b][node]
+            chain = chain[::-1]
+            if chain:  # attention of the path's last node, from the kept tokens and its own path alone
+                ks = torch.stack(kept_k[b] + [k[b, :, i] for i in chain], 1).double()
+                vs = torch.stack(kept_v[b] + [v[b, :, i] for i in chain], 1).double()
+                for h in range(4):
+                    w = torch.softmax(ks[h // 2] @ q[b, h, chain[-1]].double() * D ** -0.5, 0)
+                    assert ((w @ vs[h // 2]) - o[b, h, chain[-1]].cpu().double()).abs().max() < 1e-5
+            take = min(len(chain), turn + 1)
+            path.append((chain + [0] * N)[:N])
+            accepted.append(take)
+            kept_k[b] += [k[b, :, i] for i in chain[:take]]
+            kept_v[b] += [v[b, :, i] for i in chain[:take]]
+        lens = ca.chill_cache_commit(kc, vc, pages.table, step, ints(path), ints(accepted))
+        assert lens.tolist() == [len(x) for x in kept_k]
+        ca.chill_pages_trim(pages, lens, page)
+        assert pages.held.tolist() == [-(-len(x) // page) for x in kept_k]
+    for b in range(B):
+        for t, (x, y) in enumerate(zip(kept_k[b], kept_v[b])):
+            where = int(pages.table[b, t // page])
+            assert torch.equal(kc[where, :, t % page].cpu(), x) and torch.equal(vc[where, :, t % page].cpu(), y)
+
+
+def test_a_captured_step_is_replayed_with_other_lengths():
+    """One graph of all operators; lengths, tokens and pages change between replays, two graphs are alive at once."""
+    import chill_attention as ca
+
+    D, page, N, B = 64, 16, 4, 3
+    mask = ca.CausalChillMask()
+
+    class Session:
+        def __init__(self):
+            self.pages = ca.ChillPages.empty(B, 400, 80, page)
+            self.kc, self.vc = (torch.full((80, 2, page, D), float("nan"), dtype=torch.bfloat16, device="cuda") for _ in range(2))
+            self.lens, self.new = ints([0] * B), ints([N] * B)
+            self.q, self.k, self.v = (torch.zeros(B, h, N, D, dtype=torch.bfloat16, device="cuda") for h in (8, 2, 2))
+
+        def pass_(self):
+            step = ca.chill_pages_reserve(self.pages, self.lens, self.new, N, page)
+            ca.chill_cache_append(self.kc, self.vc, self.k, self.v, step.slots)
+            o = ca.chill_attention_cached(self.q, self.kc, self.vc, self.pages.table, step, mask)
+            self.lens.add_(self.new)
+            return o
+
+        def reset(self):
+            ca.chill_pages_trim(self.pages, ints([0] * B), page)
+            self.lens.zero_()
+            self.kc.fill_(float("nan"))
+            self.vc.fill_(float("nan"))
+
+    eager, one, two = Session(), Session(), Session()
+    graphs = []
+    for s in (one, two):
+        s.pass_()  # warm-up
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            o = s.pass_()
+        s.reset()
+        graphs.append((s, graph, o))
+    for turn in range(20):
+        data = [torch.randn_like(t) for t in (eager.q, eager.k, eager.v)]
+        new = ints([turn % (N + 1), N, (3 * turn) % (N + 1)])
+        for s in (eager, one, two):
+            for t, d in zip((s.q, s.k, s.v), data):
+                t.copy_(d)
+            s.new.copy_(new)
+        want = eager.pass_()
+        for s, graph, o in graphs:
+            graph.replay()
+        for s, graph, o in graphs:
+            assert torch.equal(o, want) and torch.equal(s.lens, eager.lens) and torch.equal(s.pages.table, eager.pages.table)
+
+
+def test_another_stream():
+    import chill_attention as ca
+
+    p = Problem(torch.bfloat16, 8, 2, 128, [2500, 900], [6, 6], 6, 64, tree=True, seed=3)
+    args = [p.q.cuda(), p.k_cache.cuda(), p.v_cache.cuda(), p.table.cuda(), p.step(), ca.CausalChillMask()]
+    want = ca.chill_attention_cached(*args)
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(3)]
+    outs = []
+    for turn in range(4):
+        for s in streams:  # calls that can overlap: each has a workspace of its own
+            with torch.cuda.stream(s):
+                outs.append(ca.chill_attention_cached(*args))
+    torch.cuda.synchronize()
+    assert all(torch.equal(o, want) for o in outs)
+
+
+def test_dispatcher_ops_give_the_same():
+    from chill_attention import cache
+
+    p = Problem(torch.float16, 8, 2, 64, [250, 90], [6, 5], 6, 16, tree=True, seed=3)
+    mask = masks()["window"]
+    (o, lse), scale = attend(p, mask)
+    s = p.step()
+    o2, lse2 = torch.ops.chill_attention.cached_forward(p.q.cuda(), p.k_cache.cuda(), p.v_cache.cuda(), p.table.cuda(), s.lens, s.new_lens, s.positions,
+                                                        s.ancestors, mask.name, list(mask.constargs), scale, 0)
+    assert torch.equal(o, o2) and torch.equal(lse, lse2)
+    import chill_attention as ca
+
+    a, b = (ca.ChillPages.empty(2, 300, 50, 16) for _ in range(2))
+    want = ca.chill_pages_reserve(a, s.lens, s.new_lens, 6, 16, ints(p.parents))
+    got = torch.ops.chill_attention.pages_reserve(*b, s.lens, s.new_lens, 6, 16, ints(p.parents))
+    assert all(torch.equal(x, y) for x, y in zip(want[2:], got)) and all(torch.equal(x, y) for x, y in zip(a, b))
+    torch.library.opcheck(torch.ops.chill_attention.cache_append.default,
+                          (p.k_cache.cuda(), p.v_cache.cuda(), torch.randn(2, 2, 6, 64).half().cuda(), torch.randn(2, 2, 6, 64).half().cuda(), s.slots),
+                          test_utils=("test_schema", "test_faketensor"))
+    assert cache._MASKS[mask.name][1] >= 0
+
+
+def test_refusals():
+    import chill_attention as ca
+
+    p = Problem(torch.bfloat16, 4, 2, 64, [40, 20], [3, 3], 3, 16, tree=True, seed=1)
+    q, kc, vc, table, step, mask = p.q.cuda(), p.k_cache.cuda(), p.v_cache.cuda(), p.table.cuda(), p.step(), ca.CausalChillMask()
+    call = ca.chill_attention_cached
+    bad = [
+        (q.half(), kc, vc, table, step), (q[:, :3], kc, vc, table, step), (q, kc, vc[1:], table, step), (q, kc.float(), vc, table, step),
+        (q, kc, vc, table.long(), step), (q, kc, vc, table[:1], step), (q[..., :48], kc[..., :48], vc[..., :48], table, step), (q[:0], kc, vc, table[:0], step),
+        (q, kc, vc, table, step._replace(lens=step.lens.long())), (q, kc, vc, table, step._replace(new_lens=step.new_lens[:1])),
+        (q, kc, vc, table, step._replace(positions=step.positions[:, :2])), (q, kc, vc, table, step._replace(ancestors=step.ancestors[..., :0])),
+        (q, kc, vc, table, step._replace(lens=step.lens.cpu())), (q.cpu(), kc, vc, table, step),
+        (q.clone().requires_grad_(True), kc, vc, table, step),
+    ]
+    for args in bad:
+        with pytest.raises(AssertionError):
+            call(*args, mask)
+    with torch.no_grad():
+        call(q.clone().requires_grad_(True), kc, vc, table, step, mask)
+    for scale in (0.0, -1.0, float("nan"), float("inf")):
+        with pytest.raises(RuntimeError, match="invalid argument"):
+            call(q, kc, vc, table, step, mask, sm_scale=scale)
+    k = torch.randn(2, 2, 3, 64, device="cuda", dtype=torch.bfloat16)
+    for args in [(kc, vc, k.float(), k, step.slots), (kc, vc, k[:, :1], k[:, :1], step.slots), (kc, vc, k, k, step.slots.long()),
+                 (kc, vc, k, k, step.slots[:, :2]), (kc, vc, k.clone().requires_grad_(True), k, step.slots)]:
+        with pytest.raises(AssertionError):
+            ca.chill_cache_append(*args)
+    path, accepted = ints([[0, 1], [0, 2]]), ints([1, 2])
+    for args in [(kc, vc, table, step, path[:1], accepted), (kc, vc, table, step, path, accepted.long()), (kc, vc, table, step, path[:, :0], accepted)]:
+        with pytest.raises(AssertionError):
+            ca.chill_cache_commit(*args)
+    pages = ca.ChillPages.empty(2, 100, 8, 16)
+    for args in [(pages, step.lens.long(), step.new_lens, 3, 16), (pages, step.lens, step.new_lens[:1], 3, 16), (pages, step.lens, step.new_lens, 0, 16),
+                 (pages, step.lens, step.new_lens, 3, 0), (pages, step.lens, step.new_lens, 3, 16, ints([[0, 1], [0, 1]])),
+                 (pages._replace(held=pages.held[:1]), step.lens, step.new_lens, 3, 16)]:
+        with pytest.raises(AssertionError):
+            ca.chill_pages_reserve(*args)
+    with pytest.raises(AssertionError):
+        ca.chill_pages_trim(pages, step.lens[:1], 16)
