@@ -1,12 +1,12 @@
 """Build the CUDA library for sm_100a with nvcc (no other toolchain needed).
 
-    python chill-attention_b200/build.py            # -> chill_attention/_lib/libchill_b200.so
+    python chill-attention_b200/build.py            # -> chill_attention/_lib/libchill_b200.so, libchill_cache_b200.so, _chill_torch.so
 
-Each mask functor's tensor-core kernels, its CUDA-core kernels and its kernels over a paged cache are translation units of their own
-(csrc/tc_inst.cu, csrc/simt_inst.cu, csrc/cache_inst.cu with -DCHILL_INST_MASK=<functor>), compiled in parallel.
+Each mask functor's tensor-core kernels and its CUDA-core kernels are translation units of their own
+(csrc/tc_inst.cu, csrc/simt_inst.cu with -DCHILL_INST_MASK=<functor>), compiled in parallel.
 ``build_library`` is also what ``chill_attention.custom`` calls to produce a private
 library for a user-defined mask functor.  The objects of the built-in functors, nine tenths of a build, are kept beside the
-library and linked into such private libraries as they are.
+library and linked into such private libraries as they are.  The paged cache is a library of its own (csrc/cache_*.cu).
 """
 from __future__ import annotations
 
@@ -39,9 +39,12 @@ def _nvcc():
     return nvcc
 
 
-def _sources_digest(extra=()):
+def _sources_digest(extra=(), cache=False):
+    """Of the kernel library's sources, or of those of the paged cache's library (csrc/cache_* and what they include)."""
     h = hashlib.sha256()
-    names = sorted(n for n in os.listdir(CSRC) if not n.startswith("torch_")) + [os.path.join(INCLUDE, "chill_b200.h")]
+    headers = ("abi_common.cuh", "generic.cuh", "masks.cuh", "tc_common.cuh", "tc_launch.h")
+    names = sorted(n for n in os.listdir(CSRC) if not n.startswith("torch_") and (n.startswith("cache_") or n in headers if cache else not n.startswith("cache_")))
+    names += [os.path.join(INCLUDE, n) for n in (("chill_b200.h", "chill_cache.h") if cache else ("chill_b200.h",))]
     for name in names:
         path = name if os.path.isabs(name) else os.path.join(CSRC, name)
         if os.path.isfile(path):
@@ -92,10 +95,10 @@ def build_library(out_path=None, custom_header=None, custom_functor=None, verbos
         os.replace(part, obj)
         return out
 
-    units = [(defines, src + ".cu", os.path.join(obj_dir, src + ".o")) for src in ("chill_abi", "host_pipeline", "cache_pages")]
+    units = [(defines, src + ".cu", os.path.join(obj_dir, src + ".o")) for src in ("chill_abi", "host_pipeline")]
     for fn in functors:
         builtin = fn in BUILTIN_FUNCTORS
-        for unit in ("tc", "simt", "cache"):
+        for unit in ("tc", "simt"):
             units.append((list(common if builtin else defines) + [f"-DCHILL_INST_MASK={fn}"], f"{unit}_inst.cu",
                           os.path.join(kept_dir if builtin else obj_dir, f"{unit}_{fn}.o")))
     with cf.ThreadPoolExecutor(max_workers=8) as ex:
@@ -113,6 +116,39 @@ def build_library(out_path=None, custom_header=None, custom_functor=None, verbos
     return out_path
 
 
+def build_cache_library(out_path=None, custom_header=None, custom_functor=None, verbose=False, force=False):
+    """The paged cache's library (csrc/cache_*.cu): entry points and page kernels, and the attention kernels of each functor
+    (a custom library: of the custom one alone).  Returns its path; skips work when sources are unchanged."""
+    out_path = out_path or os.path.join(LIB_DIR, "libchill_cache_b200.so")
+    os.makedirs(os.path.dirname(out_path), exist_ok=True)
+    defines, functors, extra = os.environ.get("CHILL_B200_NVCC_FLAGS", "").split(), list(BUILTIN_FUNCTORS), ()
+    if custom_header is not None:
+        custom_header = os.path.abspath(custom_header)
+        with open(custom_header, "rb") as f:
+            extra = (custom_functor, hashlib.sha256(f.read()).hexdigest())
+        defines = defines + [f'-DCHILL_CUSTOM_MASK_HEADER="{custom_header}"', f"-DCHILL_CUSTOM_MASK={custom_functor}", "-DCHILL_CUSTOM_MASK_ONLY"]
+        functors = [custom_functor]
+    digest = _sources_digest(extra + tuple(os.environ.get("CHILL_B200_NVCC_FLAGS", "").split()), cache=True)
+    stamp = out_path + ".stamp"
+    if not force and os.path.exists(out_path) and os.path.exists(stamp) and open(stamp).read() == digest:
+        return out_path
+    obj_dir = os.path.join(os.path.dirname(out_path), "obj_" + os.path.basename(out_path))
+    os.makedirs(obj_dir, exist_ok=True)
+    nvcc = [_nvcc()] + (["-Xptxas", "-v"] if verbose else []) + NVCC_FLAGS
+    units = [(defines, src + ".cu", os.path.join(obj_dir, src + ".o")) for src in ("cache_abi", "cache_pages")]
+    units += [(defines + [f"-DCHILL_INST_MASK={fn}", f"-DCHILL_INST_PART={part}"], "cache_inst.cu", os.path.join(obj_dir, f"cache_{fn}_{part}.o"))
+              for fn in functors for part in range(3)]
+    with cf.ThreadPoolExecutor(max_workers=8) as ex:
+        outs = list(ex.map(lambda u: _run(nvcc + u[0] + ["-c", os.path.join(CSRC, u[1]), "-o", u[2]]), units))
+    if verbose:
+        print("\n".join(outs))
+    _run([_nvcc(), "-shared", "-gencode", "arch=compute_100a,code=sm_100a", "-o", out_path] + [obj for _, _, obj in units])
+    with open(stamp, "w") as f:
+        f.write(digest)
+    shutil.rmtree(obj_dir, ignore_errors=True)
+    return out_path
+
+
 def build_extension(force=False):
     """Compile the native eager-mode call path (csrc/torch_ext.cpp, csrc/torch_cache.cpp) against the installed torch; returns its path."""
     import sysconfig
@@ -123,7 +159,7 @@ def build_extension(force=False):
     out = os.path.join(LIB_DIR, "_chill_torch.so")
     sources = [os.path.join(CSRC, name) for name in ("torch_ext.cpp", "torch_cache.cpp")]
     h = hashlib.sha256((torch.__version__ + sys.version).encode())
-    for path in sources + [os.path.join(CSRC, "torch_ext.h"), os.path.join(INCLUDE, "chill_b200.h")]:
+    for path in sources + [os.path.join(CSRC, "torch_ext.h")] + [os.path.join(INCLUDE, n) for n in ("chill_b200.h", "chill_cache.h")]:
         with open(path, "rb") as f:
             h.update(f.read())
     stamp = out + ".stamp"
@@ -143,4 +179,5 @@ def build_extension(force=False):
 if __name__ == "__main__":
     path = build_library(verbose="-v" in sys.argv, force="-f" in sys.argv)
     print(path)
+    print(build_cache_library(verbose="-v" in sys.argv, force="-f" in sys.argv))
     print(build_extension(force="-f" in sys.argv))

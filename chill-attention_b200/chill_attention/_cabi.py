@@ -38,8 +38,6 @@ FLAG_NARROW_HEAD = 64
 SELFTEST_STATUS = 901
 #: answers of chill_fwd_kernel
 FWD_CUDA_CORES, FWD_ONE_STREAM, FWD_TWO_STREAMS, FWD_TF32 = range(4)
-#: answers of chill_cached_kernel
-CACHED_CUDA_CORES = 0
 #: answers of chill_bwd_kernels
 BWD_CUDA_CORES, BWD_TWO_KERNELS, BWD_SINGLE, BWD_SINGLE_PAIR, BWD_WIDE, BWD_TF32 = range(6)
 
@@ -51,8 +49,6 @@ EXPORTS = (
     "chill_read_device_status", "chill_selftest_bounded_wait",
     "chill_launch_count", "chill_abi_version", "chill_status_string", "chill_last_cuda_error",
     "chill_host_workspace_bytes", "chill_fwd_bwd_host", "chill_host_chunk_schedule",
-    "chill_pages_reserve", "chill_pages_trim", "chill_cache_append", "chill_cache_commit",
-    "chill_cached_workspace_bytes", "chill_cached_fwd", "chill_cached_kernel",
 )
 
 
@@ -93,33 +89,6 @@ class HostArgs(C.Structure):
                 ("o", C.c_void_p), ("dq", C.c_void_p), ("dk", C.c_void_p), ("dv", C.c_void_p),
                 ("workspace", C.c_void_p), ("workspace_bytes", C.c_size_t), ("chunk_groups", C.c_int32),
                 ("reserved", C.c_int32)]
-
-
-class PagesArgs(C.Structure):
-    _fields_ = [("B", C.c_int32), ("N", C.c_int32), ("page_size", C.c_int32), ("num_pages", C.c_int32), ("table_width", C.c_int32),
-                ("reserved", C.c_int32), ("table", C.c_void_p), ("table_stride", C.c_int64), ("held", C.c_void_p),
-                ("free_pages", C.c_void_p), ("n_free", C.c_void_p), ("missing", C.c_void_p), ("lens", C.c_void_p),
-                ("new_lens", C.c_void_p), ("parents", C.c_void_p), ("slots", C.c_void_p), ("positions", C.c_void_p),
-                ("ancestors", C.c_void_p)]
-
-
-class CacheRowsArgs(C.Structure):
-    _fields_ = [("B", C.c_int32), ("H_kv", C.c_int32), ("N", C.c_int32), ("D", C.c_int32), ("dtype", C.c_int32),
-                ("page_size", C.c_int32), ("num_pages", C.c_int32), ("table_width", C.c_int32), ("A", C.c_int32),
-                ("reserved", C.c_int32), ("k_cache", C.c_void_p), ("v_cache", C.c_void_p), ("k_cache_strides", _S4),
-                ("v_cache_strides", _S4), ("k", C.c_void_p), ("v", C.c_void_p), ("k_strides", _S4), ("v_strides", _S4),
-                ("slots", C.c_void_p), ("table", C.c_void_p), ("table_stride", C.c_int64), ("lens", C.c_void_p),
-                ("new_lens", C.c_void_p), ("path", C.c_void_p), ("accepted", C.c_void_p), ("out_lens", C.c_void_p)]
-
-
-class CachedArgs(C.Structure):
-    _fields_ = [("mask", MaskDesc), ("B", C.c_int32), ("H", C.c_int32), ("H_kv", C.c_int32), ("N", C.c_int32), ("D", C.c_int32),
-                ("dtype", C.c_int32), ("page_size", C.c_int32), ("num_pages", C.c_int32), ("table_width", C.c_int32),
-                ("sm_scale", C.c_float), ("flags", C.c_uint32), ("reserved", C.c_int32), ("q", C.c_void_p),
-                ("k_cache", C.c_void_p), ("v_cache", C.c_void_p), ("o", C.c_void_p), ("lse", C.c_void_p), ("q_strides", _S4),
-                ("k_cache_strides", _S4), ("v_cache_strides", _S4), ("o_strides", _S4), ("lse_strides", _S3),
-                ("table", C.c_void_p), ("table_stride", C.c_int64), ("lens", C.c_void_p), ("new_lens", C.c_void_p),
-                ("positions", C.c_void_p), ("ancestors", C.c_void_p), ("workspace", C.c_void_p), ("workspace_bytes", C.c_size_t)]
 
 
 class ChillLibraryError(RuntimeError):
@@ -169,14 +138,6 @@ def load_library(path: str | None = None) -> C.CDLL:
         lib.chill_fwd_bwd_host.restype = C.c_int
         lib.chill_host_chunk_schedule.argtypes = [C.POINTER(HostArgs), C.POINTER(C.c_int32), C.c_int32]
         lib.chill_host_chunk_schedule.restype = C.c_int
-        for name, args in (("chill_pages_reserve", PagesArgs), ("chill_pages_trim", PagesArgs), ("chill_cache_append", CacheRowsArgs),
-                           ("chill_cache_commit", CacheRowsArgs), ("chill_cached_fwd", CachedArgs)):
-            getattr(lib, name).argtypes = [C.POINTER(args), C.c_void_p]
-            getattr(lib, name).restype = C.c_int
-        lib.chill_cached_workspace_bytes.argtypes = [C.POINTER(CachedArgs)]
-        lib.chill_cached_workspace_bytes.restype = C.c_size_t
-        lib.chill_cached_kernel.argtypes = [C.POINTER(CachedArgs)]
-        lib.chill_cached_kernel.restype = C.c_int
         for name in ("chill_fwd", "chill_bwd_delta", "chill_bwd", "chill_bwd_noalloc", "chill_fwd_uses_tensor_cores",
                      "chill_bwd_uses_tensor_cores", "chill_fwd_kernel", "chill_bwd_kernels", "chill_mask_tabulate", "chill_mask_tabulate_blocks",
                      "chill_mask_traits", "chill_selftest_bounded_wait",

@@ -26,15 +26,15 @@ import typing
 
 import torch
 
-from . import _cabi, _eager, chill
+from . import _cabi, _cache_abi, _eager, chill
 from .mask import ChillMask
 
 _HEAD_DIMS = chill._HEAD_DIMS
 _DTYPES = (torch.float32, torch.float16, torch.bfloat16)
 #: entry points a native CacheLibrary object is made of, in its order
 _ENTRY_POINTS = ("chill_cached_fwd", "chill_cached_workspace_bytes", "chill_pages_reserve", "chill_pages_trim", "chill_cache_append",
-                 "chill_cache_commit", "chill_status_string", "chill_last_cuda_error")
-#: kernel library -> its native call object; mask class name -> (call object, functor id)
+                 "chill_cache_commit")
+#: library -> its native call object; mask class name -> (call object, functor id)
 _NATIVE: dict = {}
 _MASKS: dict[str, tuple] = {}
 
@@ -72,11 +72,11 @@ class ChillStep(typing.NamedTuple):
 
 
 def _native(lib=None):
-    lib = lib or _cabi.load_library()
+    lib = lib or _cache_abi.load_library()
     native = _NATIVE.get(lib)
     if native is None:
-        native = _eager.extension().CacheLibrary([C.cast(getattr(lib, name), C.c_void_p).value for name in _ENTRY_POINTS])
-        _NATIVE[lib] = native
+        functions = [getattr(lib, name) for name in _ENTRY_POINTS] + [_cabi.load_library().chill_status_string, lib.chill_cache_last_cuda_error]
+        native = _NATIVE[lib] = _eager.extension().CacheLibrary([C.cast(f, C.c_void_p).value for f in functions])
     return native
 
 
@@ -299,12 +299,20 @@ def chill_cache_commit(k_cache: torch.Tensor, v_cache: torch.Tensor, table: torc
 
 
 def _mask_functor(mask: ChillMask):
-    found = _MASKS.get(mask.name)
-    if found is None:
-        if mask.name not in chill._REGISTRY:
-            chill.register_chill_mask(mask)
-        lib, functor_id = chill._REGISTRY[mask.name]
-        found = _MASKS[mask.name] = (_native(lib), functor_id)
+    """Native call object and functor id serving this mask class (builds the custom library if needed)."""
+    functor, header = getattr(mask, "cuda_functor", None), getattr(mask, "cuda_functor_header", None)
+    if header is not None:
+        from .custom import build_custom_cache_library
+
+        if not functor:
+            raise ValueError(f"{mask.name}: cuda_functor_header is set but cuda_functor (struct name) is not")
+        found = _native(_cache_abi.load_library(build_custom_cache_library(header, functor))), _cabi.MASK_CUSTOM
+    elif functor in _cabi.BUILTIN_FUNCTOR_IDS:
+        found = _native(), _cabi.BUILTIN_FUNCTOR_IDS[functor]
+    else:
+        raise NotImplementedError(f"{mask.name} has no CUDA functor: set `cuda_functor` to a built-in functor name or provide "
+                                  "`cuda_functor_header` + `cuda_functor` (see chill_attention/custom.py)")
+    _MASKS[mask.name] = found
     return found
 
 

@@ -36,3 +36,12 @@ def build_custom_library(header: str, functor: str) -> str:
         tag = hashlib.sha256(f.read() + functor.encode()).hexdigest()[:16]
     out = os.path.join(_HERE, "_lib", f"libchill_b200_{functor}_{tag}.so")
     return _build_module().build_library(out_path=out, custom_header=header, custom_functor=functor)
+
+
+def build_custom_cache_library(header: str, functor: str) -> str:
+    """The same for attention over a paged cache: a library with the functor's kernels alone."""
+    header = os.path.abspath(header)
+    with open(header, "rb") as f:
+        tag = hashlib.sha256(f.read() + functor.encode()).hexdigest()[:16]
+    out = os.path.join(_HERE, "_lib", f"libchill_cache_b200_{functor}_{tag}.so")
+    return _build_module().build_cache_library(out_path=out, custom_header=header, custom_functor=functor)

@@ -25,6 +25,8 @@ CHILL_HD int clamp_len(int x) { return imin(imax(x, 0), kMaxLen); }
 struct CachedP {
   int B, H, Hkv, G, N, D;
   int page, num_pages, width;
+  int box;              // rows of a TMA box (tensor-core kernels)
+  bool wide_q, wide_o;  // rows of Q / O can be moved in 16-byte vectors
   int rows, row_tiles;  // rows of a tile, tiles of N * G rows
   int words;            // 32-bit words of an ancestor row
   int min_share;        // tiles of keys a CTA takes at least

@@ -1,19 +1,19 @@
 // Pages of a key / value cache, kept on the GPU: which pages a request holds (table), which are free (a stack), where new tokens
 // go (slots), their positions and, for a tree of drafted tokens, their ancestors; the kernels that store new rows at their slots
 // and that move the accepted path of a tree together.  Entry points: chill_pages_reserve / _trim, chill_cache_append / _commit
-// (include/chill_b200.h).  Nothing here depends on the mask.
+// (include/chill_cache.h).  Nothing here depends on the mask.
 #include <cuda_runtime.h>
 #include <stdint.h>
 
 #include <atomic>
 
 #include "cache_common.cuh"
-#include "chill_b200.h"
+#include "chill_cache.h"
 
 namespace chill {
 
-int record_cuda_failure(cudaError_t e, const char* what);  // chill_abi.cu
-void count_launches(int n);                                // chill_abi.cu
+int record_cuda_failure(cudaError_t e, const char* what);  // cache_abi.cu
+void count_launches(int n);                                // cache_abi.cu
 
 namespace cache {
 

@@ -1,0 +1,94 @@
+// The tensor-core kernels multiply whole tiles: a key that a row does not see has weight 0 there, and 0 * NaN or 0 * inf is NaN.  So
+// whenever a result that is not finite comes out of a piece, its rows are worked out again here, on the CUDA cores and from the
+// visible keys alone.  A NaN that the visible keys do hold comes out again; finite data never gets here.
+#pragma once
+#include "cache_common.cuh"
+#include "tc_common.cuh"
+
+namespace chill {
+namespace cache {
+
+// Four channels of a row of O.
+template <typename T>
+__device__ __forceinline__ void store4(const CachedP& p, T* row, int ch, float a, float b, float c, float d) {
+  if (p.wide_o) {  // channels side by side, rows on 16-byte boundaries
+    if constexpr (sizeof(T) == 2) {
+      *reinterpret_cast<uint2*>(row + ch) = make_uint2(tc::pack2<T>(a, b), tc::pack2<T>(c, d));
+    } else {
+      *reinterpret_cast<float4*>(row + ch) = make_float4(a, b, c, d);
+    }
+  } else {
+    row[ch * p.o.sd] = from_f<T>(a); row[(ch + 1) * p.o.sd] = from_f<T>(b);
+    row[(ch + 2) * p.o.sd] = from_f<T>(c); row[(ch + 3) * p.o.sd] = from_f<T>(d);
+  }
+}
+
+// Whether any of the 128 consumer threads says so; also a barrier between their stores before and after it.
+__device__ __forceinline__ bool consumers_any(bool x) {
+  uint32_t any;
+  asm volatile(
+      "{\n\t"
+      ".reg .pred p, q;\n\t"
+      "setp.ne.u32 p, %1, 0;\n\t"
+      "barrier.cta.red.or.pred q, 2, 128, p;\n\t"
+      "selp.u32 %0, 1, 0, q;\n\t"
+      "}\n"
+      : "=r"(any)
+      : "r"((uint32_t)x)
+      : "memory");
+  return any != 0;
+}
+
+// Rows of a piece again, one row a warp, lanes over the channels, key by key.
+template <typename T, int DP, class M>
+__device__ __noinline__ void repair_piece(const CachedP& p, const RowTile& t, const Piece& piece, int warp, int warps) {
+  const int lane = threadIdx.x & 31;
+  constexpr int kOwn = DP / 32;  // channels of a lane: lane, lane + 32, ...
+  const int last = imin(t.k_lo + piece.t1 * kKeyTile, t.total);
+  for (int r = warp; r < t.rows; r += warps) {
+    const int i = (t.r0 + r) / p.G, h = piece.head * p.G + (t.r0 + r) % p.G, pos = token_position(p, t, i);
+    const T* qr = row_ptr<T>(p.q, t.b, h, i);
+    float q[kOwn], o[kOwn], m = -CUDART_INF_F, l = 0.f;
+#pragma unroll
+    for (int c = 0; c < kOwn; ++c) {
+      q[c] = lane + 32 * c < p.D ? to_f(qr[(lane + 32 * c) * p.q.sd]) : 0.f;
+      o[c] = 0.f;
+    }
+    for (int key = t.k_lo + piece.t0 * kKeyTile; key < last; ++key) {
+      const int page = p.table[t.b * p.table_sb + key / p.page];
+      if (page < 0 || page >= p.num_pages || !sees<M>(p, t, i, pos, key)) continue;
+      const int row = key % p.page;
+      const T* kr = reinterpret_cast<const T*>(p.k.p) + page * p.k.sb + piece.head * p.k.sh + row * p.k.sl;
+      const T* vr = reinterpret_cast<const T*>(p.v.p) + page * p.v.sb + piece.head * p.v.sh + row * p.v.sl;
+      float s = 0.f;
+#pragma unroll
+      for (int c = 0; c < kOwn; ++c)
+        if (lane + 32 * c < p.D) s = fmaf(q[c], to_f(kr[(lane + 32 * c) * p.k.sd]), s);
+      s = warp_sum(s) * p.scale_log2;
+      const float m_new = fmaxf(m, s), safe = m_new == -CUDART_INF_F ? 0.f : m_new;
+      const float a = exp2f(m - safe), w = exp2f(s - safe);
+      m = m_new;
+      l = l * a + w;
+#pragma unroll
+      for (int c = 0; c < kOwn; ++c)
+        if (lane + 32 * c < p.D) o[c] = fmaf(w, to_f(vr[(lane + 32 * c) * p.v.sd]), o[c] * a);
+    }
+    const float inv = l == 0.f ? 0.f : 1.f / l;
+    const long long at = (long long)piece.slot * p.rows + r;
+    T* to = o_row<T>(p, t.b, h, i);
+#pragma unroll
+    for (int c = 0; c < kOwn; ++c) {
+      const int d = lane + 32 * c;
+      if (d >= p.D) continue;
+      if (piece.whole) to[d * p.o.sd] = from_f<T>(o[c] * inv);
+      else p.part_o[at * p.D + d] = o[c];
+    }
+    if (lane == 0) {
+      if (piece.whole) store_lse(p, t.b, h, i, true, m, l);
+      else p.part_ml[at] = make_float2(m, l);
+    }
+  }
+}
+
+}  // namespace cache
+}  // namespace chill

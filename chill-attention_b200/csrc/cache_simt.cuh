@@ -29,7 +29,7 @@ struct SimtSmem {
 };
 
 template <typename T, int DP, class M>
-__global__ void __launch_bounds__(kSimtThreads) cached_simt_kernel(CachedP p) {
+__global__ void __launch_bounds__(kSimtThreads) cached_simt_kernel(const __grid_constant__ CachedP p) {
   using L = SimtSmem<DP>;
   extern __shared__ __align__(16) float smem[];
   float *sq = smem + L::kQ, *sk = smem + L::kK, *sv = smem + L::kV, *ss = smem + L::kS, *sa = smem + L::kM;

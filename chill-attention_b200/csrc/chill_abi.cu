@@ -8,9 +8,8 @@
 #include <atomic>
 #include <mutex>
 
+#include "abi_common.cuh"
 #include "bwd_tc.cuh"
-#include "cache_common.cuh"
-#include "cache_launch.h"
 #include "chill_b200.h"
 #include "fwd_tc.cuh"
 #include "generic.cuh"
@@ -19,24 +18,7 @@
 
 namespace chill {
 
-static thread_local char g_cuda_err[256] = "";
-__device__ int g_device_status = 0;
-static std::atomic<unsigned long long> g_launches{0};  // kernels launched by this library (chill_launch_count)
-
-static int cuda_fail(cudaError_t e, const char* what) {
-  snprintf(g_cuda_err, sizeof(g_cuda_err), "%s: %s", what, cudaGetErrorString(e));
-  return CHILL_E_CUDA;
-}
-
 int record_cuda_failure(cudaError_t e, const char* what) { return cuda_fail(e, what); }  // for host_pipeline.cu
-void count_launches(int n) { g_launches += n; }                                                       // for cache_pages.cu
-
-static int* device_status_ptr() {
-  // one word per device (the symbol is instantiated in every device's module image)
-  int* p = nullptr;
-  if (cudaGetSymbolAddress((void**)&p, g_device_status) != cudaSuccess) return nullptr;
-  return p;
-}
 
 // The same for the split fp32 kernels, which the CUDA-core kernels can stand in for: without the word they are left out, and the
 // error that says so is not left behind for the launch that follows.
@@ -47,21 +29,6 @@ static int* split_status_ptr() {
 }
 
 // ------------------------------------------------------------------------- validation
-static size_t esize(int dtype) { return dtype == CHILL_F32 ? 4 : 2; }
-
-static int check_mask(const chill_mask_desc& m) {
-  if (m.n_args < 0 || m.n_args > CHILL_MAX_MASK_ARGS) return CHILL_E_INVALID;
-#ifdef CHILL_CUSTOM_MASK
-  if (m.id < 0 || m.id > CHILL_MASK_CUSTOM) return CHILL_E_UNSUPPORTED;
-#else
-  if (m.id < 0 || m.id >= CHILL_MASK_CUSTOM) return CHILL_E_UNSUPPORTED;
-#endif
-  if (m.id == CHILL_MASK_CHUNKWISE && (m.n_args < 2 || m.i[0] <= 0)) return CHILL_E_INVALID;
-  if (m.id == CHILL_MASK_SLIDING && m.n_args < 2) return CHILL_E_INVALID;
-  if (m.id == CHILL_MASK_PREFIXLM && m.n_args < 1) return CHILL_E_INVALID;
-  return CHILL_OK;
-}
-
 static int check_shape(const chill_shape& s) {
   if (s.B <= 0 || s.H <= 0 || s.H_kv <= 0 || s.Lq <= 0 || s.Lk <= 0 || s.D <= 0) return CHILL_E_INVALID;
   if (s.H % s.H_kv != 0) return CHILL_E_INVALID;
@@ -72,54 +39,12 @@ static int check_shape(const chill_shape& s) {
   return check_mask(s.mask);
 }
 
-// The functors do their index arithmetic in 32 bits (position + constant), so the 64-bit constants of the ABI are
-// saturated first.  For the built-in masks every constant is a distance or a size measured in positions, and any value
-// beyond +-seq_len selects the same pairs as +-seq_len itself, so they are clamped there ("unbounded" written as
-// 2**31 - 1 or 2**40 stays unbounded).  Constants of a custom functor are saturated to +-2^30, which still leaves
-// room for adding a position.
-static MaskArgs to_mask_args(const chill_mask_desc& m, long long seq_len) {
-  MaskArgs a;
-  const long long lim = (m.id >= 0 && m.id < CHILL_MASK_CUSTOM && seq_len > 0) ? seq_len : (1ll << 30);
-  for (int i = 0; i < 8; ++i) {
-    long long v = i < m.n_args ? (long long)m.i[i] : 0;
-    v = v > lim ? lim : (v < -lim ? -lim : v);
-    a.i[i] = (int)v;
-    a.f[i] = i < m.n_args ? (float)m.f[i] : 0.f;
-  }
-  if (m.id == CHILL_MASK_CHUNKWISE && a.i[0] > 0 && seq_len > 0) {
-    // back_contexts counts chunks: more chunks than the sequence has changes nothing, and (chunk + back + 1) * size
-    // then stays far below 2^31
-    const int n_chunks = (int)((seq_len + a.i[0] - 1) / a.i[0]);
-    a.i[1] = a.i[1] > n_chunks ? n_chunks : (a.i[1] < -n_chunks ? -n_chunks : a.i[1]);
-  }
-  return a;
-}
-
 static Geo to_geo(const chill_shape& s) {
   Geo g;
   g.B = s.B; g.H = s.H; g.Hkv = s.H_kv; g.Lq = s.Lq; g.Lk = s.Lk; g.D = s.D;
   g.q_off = s.q_offset; g.k_off = s.k_offset; g.seq_len = s.seq_len;
   g.scale = s.sm_scale; g.lens = s.lens; g.margs = to_mask_args(s.mask, s.seq_len);
   return g;
-}
-
-static TRef to_ref(const void* p, const int64_t* st) {
-  TRef r;
-  r.p = const_cast<void*>(p);
-  r.sb = st[0]; r.sh = st[1]; r.sl = st[2]; r.sd = st[3];
-  return r;
-}
-
-// A [B][H][L][D] tensor can be described to TMA when channels are contiguous and everything
-// else is 16-byte aligned.
-static bool tma_ok(const void* p, const int64_t* st, int B, int H, int L, size_t es) {
-  if (st[3] != 1) return false;
-  if (((uintptr_t)p) % 16 != 0) return false;
-  if ((st[2] * (int64_t)es) % 16 != 0 || st[2] <= 0) return false;
-  if (H > 1 && ((st[1] * (int64_t)es) % 16 != 0 || st[1] <= 0)) return false;
-  if (B > 1 && ((st[0] * (int64_t)es) % 16 != 0 || st[0] <= 0)) return false;
-  (void)L;
-  return true;
 }
 
 // Channels of the tensor-core tiles that serve 16-bit head dim D (0: none below 256).  Narrow heads take the 64-channel
@@ -137,78 +62,6 @@ static bool shape_tc_ok(const chill_shape& s) {
   if (!(s.sm_scale > 0.f)) return false;
   return true;
 }
-
-// ------------------------------------------------------------------------ TMA encoding
-typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
-                                  const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
-                                  CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
-
-static EncodeTiledFn encode_fn() {
-  static EncodeTiledFn fn = nullptr;
-  if (fn == nullptr) {
-    void* p = nullptr;
-    cudaDriverEntryPointQueryResult qres;
-    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &qres) == cudaSuccess &&
-        qres == cudaDriverEntryPointSuccess)
-      fn = (EncodeTiledFn)p;
-  }
-  return fn;
-}
-
-// Box = 64 channels x `box_rows` positions of one (batch, head), 128B swizzle.
-static int make_map(CUtensorMap* m, const void* p, const int64_t* st, int B, int H, int L, int D, int dtype,
-                    int box_rows, CUtensorMapSwizzle swizzle = CU_TENSOR_MAP_SWIZZLE_128B) {
-  EncodeTiledFn fn = encode_fn();
-  if (fn == nullptr) {
-    snprintf(g_cuda_err, sizeof(g_cuda_err), "cuTensorMapEncodeTiled entry point not available");
-    return CHILL_E_CUDA;
-  }
-  const cuuint64_t es = esize(dtype);
-  cuuint64_t dims[4] = {(cuuint64_t)D, (cuuint64_t)L, (cuuint64_t)H, (cuuint64_t)B};
-  const cuuint64_t row = (cuuint64_t)st[2] * es;
-  cuuint64_t strides[3] = {row, H > 1 ? (cuuint64_t)st[1] * es : row * (cuuint64_t)L,
-                           B > 1 ? (cuuint64_t)st[0] * es : row * (cuuint64_t)L * (cuuint64_t)H};
-  cuuint32_t box[4] = {(cuuint32_t)(128 / es), (cuuint32_t)box_rows, 1, 1};  // 128-byte rows
-  cuuint32_t estr[4] = {1, 1, 1, 1};
-  const CUtensorMapDataType dt = dtype == CHILL_BF16   ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16
-                                 : dtype == CHILL_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16
-                                                      : CU_TENSOR_MAP_DATA_TYPE_FLOAT32;
-  CUresult r = fn(m, dt, 4, const_cast<void*>(p), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle,
-                  CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-  if (r != CUDA_SUCCESS) {
-    snprintf(g_cuda_err, sizeof(g_cuda_err), "cuTensorMapEncodeTiled failed with CUresult %d", (int)r);
-    return CHILL_E_CUDA;
-  }
-  return CHILL_OK;
-}
-
-// --------------------------------------------------------------------------- dispatch
-#ifdef CHILL_CUSTOM_MASK
-#define CHILL_CUSTOM_CASE(CALL) \
-  case CHILL_MASK_CUSTOM: { using MaskT = CHILL_CUSTOM_MASK; CALL; break; }
-#else
-#define CHILL_CUSTOM_CASE(CALL)
-#endif
-
-#define CHILL_MASK_SWITCH(ID, CALL) CHILL_MASK_SWITCH_OR(ID, CALL, return CHILL_E_UNSUPPORTED)
-#define CHILL_MASK_SWITCH_OR(ID, CALL, OTHERWISE)                          \
-  switch (ID) {                                                            \
-    case CHILL_MASK_FULL: { using MaskT = FullMask; CALL; break; }         \
-    case CHILL_MASK_CAUSAL: { using MaskT = CausalMask; CALL; break; }     \
-    case CHILL_MASK_SLIDING: { using MaskT = SlidingWindowMask; CALL; break; } \
-    case CHILL_MASK_CHUNKWISE: { using MaskT = ChunkwiseMask; CALL; break; } \
-    case CHILL_MASK_PREFIXLM: { using MaskT = PrefixLMMask; CALL; break; } \
-    CHILL_CUSTOM_CASE(CALL)                                                \
-    default: OTHERWISE;                                                    \
-  }
-
-#define CHILL_DTYPE_SWITCH(DT, CALL)                                  \
-  switch (DT) {                                                       \
-    case CHILL_F32: { using ElemT = float; CALL; break; }             \
-    case CHILL_F16: { using ElemT = __half; CALL; break; }            \
-    case CHILL_BF16: { using ElemT = __nv_bfloat16; CALL; break; }    \
-    default: return CHILL_E_UNSUPPORTED;                              \
-  }
 
 // fp32 tensors whose caller allowed TF32: forward on the tensor cores (fwd_tf32.cuh)
 static bool shape_tf32_ok(const chill_shape& s) {
@@ -649,9 +502,6 @@ static int bwd_wide(const chill_bwd_args& a, cudaStream_t st) {
   return e == 0 ? CHILL_OK : cuda_fail((cudaError_t)e, "bwd_wide launch");
 }
 
-// --------------------------------------------------------------------- attention over a paged cache
-#include "cache_dispatch.cuh"
-
 // ------------------------------------------------------------- backward without a scratch argument
 // Library-owned scratch for chill_bwd_noalloc: lives in the device image of this file, one copy per
 // GPU that loads the library.  In host code the name below is only a handle for the runtime; the
@@ -818,21 +668,6 @@ int chill_bwd_noalloc(const chill_bwd_args* a, void* stream) {
   if (bwd_tf32_eligible(b)) return bwd_tf32(b, (cudaStream_t)stream);
   if (b.s.flags & CHILL_FLAG_REQUIRE_TC) return CHILL_E_UNSUPPORTED;
   return bwd_generic(b, (cudaStream_t)stream);
-}
-
-size_t chill_cached_workspace_bytes(const chill_cached_args* a) {
-  CachedPlan c;
-  return check_cached(a, false) == CHILL_OK && plan_cached(*a, c) == CHILL_OK ? c.bytes : 0;
-}
-
-int chill_cached_kernel(const chill_cached_args* a) {
-  const int st = check_cached(a, true);
-  return st != CHILL_OK ? st : cached_kernel(*a);
-}
-
-int chill_cached_fwd(const chill_cached_args* a, void* stream) {
-  const int st = check_cached(a, true);
-  return st != CHILL_OK ? st : cached_fwd(*a, (cudaStream_t)stream);
 }
 
 int chill_mask_tabulate(const chill_mask_desc* m, int32_t n, int32_t tile, uint8_t* dense, int32_t* k_lims,

@@ -13,7 +13,7 @@
 #include <string>
 #include <vector>
 
-#include "chill_b200.h"
+#include "chill_cache.h"
 #include "torch_ext.h"
 
 namespace py = pybind11;
@@ -29,7 +29,7 @@ struct CacheLibrary {
   decltype(&chill_cache_append) append;
   decltype(&chill_cache_commit) commit;
   decltype(&chill_status_string) status_string;
-  decltype(&chill_last_cuda_error) cuda_error;
+  decltype(&chill_cache_last_cuda_error) cuda_error;
 };
 
 void check(const CacheLibrary& lib, int status, const char* what) {
@@ -209,7 +209,7 @@ void bind_cache(py::module_& m) {
     return std::make_shared<CacheLibrary>(CacheLibrary{pointer<decltype(&chill_cached_fwd)>(fn[0]), pointer<decltype(&chill_cached_workspace_bytes)>(fn[1]),
                           pointer<decltype(&chill_pages_reserve)>(fn[2]), pointer<decltype(&chill_pages_trim)>(fn[3]),
                           pointer<decltype(&chill_cache_append)>(fn[4]), pointer<decltype(&chill_cache_commit)>(fn[5]),
-                          pointer<decltype(&chill_status_string)>(fn[6]), pointer<decltype(&chill_last_cuda_error)>(fn[7])});
+                          pointer<decltype(&chill_status_string)>(fn[6]), pointer<decltype(&chill_cache_last_cuda_error)>(fn[7])});
   }));
   m.def("pages_reserve", &reserve);
   m.def("pages_trim", &trim);

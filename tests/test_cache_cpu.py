@@ -11,15 +11,15 @@ from oracle import cache_oracle as orc
 @pytest.fixture(scope="module")
 def lib():
     ensure_built()
-    from chill_attention import _cabi
+    from chill_attention import _cache_abi
 
-    return _cabi.load_library()
+    return _cache_abi.load_library()
 
 
 def cached_args(**changes):
-    from chill_attention import _cabi
+    from chill_attention import _cabi, _cache_abi
 
-    a = _cabi.CachedArgs()
+    a = _cache_abi.CachedArgs()
     a.mask = _cabi.mask_desc(_cabi.MASK_CAUSAL, ())
     a.B, a.H, a.H_kv, a.N, a.D, a.dtype = 2, 8, 2, 4, 64, 2
     a.page_size, a.num_pages, a.table_width, a.sm_scale = 16, 100, 20, 0.125
@@ -35,11 +35,11 @@ def cached_args(**changes):
 
 
 def test_struct_sizes_match_header():
-    from chill_attention import _cabi
+    from chill_attention import _cache_abi
 
-    assert ctypes.sizeof(_cabi.PagesArgs) == 24 + 8 * 2 + 8 * 10
-    assert ctypes.sizeof(_cabi.CacheRowsArgs) == 40 + 16 + 64 + 16 + 64 + 8 + 16 + 8 * 5
-    assert ctypes.sizeof(_cabi.CachedArgs) == 136 + 48 + 40 + 128 + 24 + 16 + 48
+    assert ctypes.sizeof(_cache_abi.PagesArgs) == 24 + 8 * 2 + 8 * 10
+    assert ctypes.sizeof(_cache_abi.CacheRowsArgs) == 40 + 16 + 64 + 16 + 64 + 8 + 16 + 8 * 5
+    assert ctypes.sizeof(_cache_abi.CachedArgs) == 136 + 48 + 40 + 128 + 24 + 16 + 48
 
 
 def test_attention_refusals(lib):
@@ -67,10 +67,10 @@ def test_attention_refusals(lib):
 
 
 def test_page_and_row_refusals(lib):
-    from chill_attention import _cabi
+    from chill_attention import _cache_abi
 
     def pages(**changes):
-        a = _cabi.PagesArgs()
+        a = _cache_abi.PagesArgs()
         a.B, a.N, a.page_size, a.num_pages, a.table_width, a.table_stride = 4, 3, 16, 100, 20, 20
         for name in ("table", "held", "free_pages", "n_free", "missing", "lens", "new_lens", "slots", "positions"):
             setattr(a, name, 4096)
@@ -92,7 +92,7 @@ def test_page_and_row_refusals(lib):
     assert lib.chill_pages_trim(pages(table_width=2 ** 26), None) == -4
 
     def rows(**changes):
-        a = _cabi.CacheRowsArgs()
+        a = _cache_abi.CacheRowsArgs()
         a.B, a.H_kv, a.N, a.D, a.dtype, a.page_size, a.num_pages, a.table_width, a.A = 4, 2, 3, 64, 2, 16, 100, 20, 2
         for name in ("k_cache", "v_cache", "k", "v", "slots", "table", "lens", "new_lens", "path", "accepted", "out_lens"):
             setattr(a, name, 4096)
@@ -140,3 +140,29 @@ def test_oracle_trim_undoes_reserve():
     assert slots[0][:7] == [5 * 16 + 10 + i for i in range(6)] + [0] and positions[1][:3] == [0, 1, 2] and slots[2] == [-1] * 32
     t, h, stack = orc.trim(t, h, free, n, lens, 16)
     assert (t, h, stack) == (table, held, free)
+
+
+def test_header_and_exports(lib, tmp_path):
+    """Everything include/chill_cache.h declares is exported, and the header is plain C99."""
+    import os
+    import re
+    import shutil
+    import subprocess
+
+    from chill_attention import _cache_abi
+    from helpers import ROOT
+
+    text = open(os.path.join(ROOT, "include", "chill_cache.h")).read()
+    names = set(re.findall(r"\b(chill_[a-z_0-9]+)\s*\(", re.sub(r"/\*.*?\*/", "", text, flags=re.S)))
+    assert names == set(_cache_abi.EXPORTS) and all(hasattr(lib, n) for n in names)
+    gcc = shutil.which("gcc")
+    if gcc is None:
+        pytest.skip("no gcc")
+    src = tmp_path / "use.c"
+    src.write_text('#include "chill_cache.h"\nint main(void) { chill_cached_args a = {0}; chill_pages_args b = {0}; chill_cache_rows_args c = {0};\n'
+                   "  (void)b; (void)c; return chill_cached_fwd(&a, 0) == CHILL_E_INVALID && chill_cache_abi_version() == CHILL_CACHE_ABI_VERSION ? 0 : 1; }\n")
+    exe, lib_dir = tmp_path / "use", os.path.dirname(_cache_abi.DEFAULT_LIB)
+    r = subprocess.run([gcc, "-std=c99", "-Wall", "-Werror", "-I", os.path.join(ROOT, "include"), str(src), "-o", str(exe), "-L", lib_dir,
+                        "-l:libchill_cache_b200.so", f"-Wl,-rpath,{lib_dir}"], capture_output=True, text=True)
+    assert r.returncode == 0, r.stderr
+    assert subprocess.run([str(exe)]).returncode == 0

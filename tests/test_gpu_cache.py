@@ -12,11 +12,11 @@ pytestmark = pytest.mark.gpu
 @pytest.fixture(scope="module", autouse=True)
 def _lib():
     ensure_built()
-    from chill_attention import _cabi
+    from chill_attention import _cache_abi
 
-    lib = _cabi.load_library()
+    lib = _cache_abi.load_library()
     yield lib
-    assert lib.chill_read_device_status() == 0
+    assert lib.chill_cache_read_device_status() == 0
 
 
 def ints(x):
@@ -51,25 +51,25 @@ def kernel_of(p, flags=0):
     """Which kernel serves the contiguous call."""
     import ctypes
 
-    from chill_attention import _cabi
+    from chill_attention import _cabi, _cache_abi
 
     B, H, N, D = p.q.shape
-    a = _cabi.CachedArgs()
+    a = _cache_abi.CachedArgs()
     a.mask = _cabi.mask_desc(_cabi.MASK_CAUSAL, ())
     a.B, a.H, a.H_kv, a.N, a.D, a.dtype = B, H, p.k_cache.shape[1], N, D, _cabi._DTYPES[p.dtype]
     a.page_size, a.num_pages, a.table_width, a.sm_scale, a.flags = p.page, p.k_cache.shape[0], p.table.shape[1], 1.0, flags
     a.q = a.k_cache = a.v_cache = a.o = a.table = a.lens = a.new_lens = 4096
     for name, t in (("q_strides", p.q), ("o_strides", p.q), ("k_cache_strides", p.k_cache), ("v_cache_strides", p.v_cache)):
         setattr(a, name, (ctypes.c_int64 * 4)(*t.stride()))
-    return _cabi.load_library().chill_cached_kernel(ctypes.byref(a))
+    return _cache_abi.load_library().chill_cached_kernel(ctypes.byref(a))
 
 
 def run_and_check(p, mask, layout="plain", flags=0):
     (o, lse), scale = attend(p, mask, layout, flags)
     assert o.shape == p.q.shape and o.is_contiguous()
-    from chill_attention import _cabi
+    from chill_attention import _cache_abi
 
-    tensor_cores = layout not in ("odd",) and kernel_of(p, flags) != _cabi.CACHED_CUDA_CORES
+    tensor_cores = layout not in ("odd",) and kernel_of(p, flags) != _cache_abi.CACHED_CUDA_CORES
     check_attention(o, lse, p, mask, scale, tensor_cores)
     return o, lse
 
@@ -149,6 +149,36 @@ def test_keys_without_a_page_are_not_there(dtype, N):
     o, lse = run_and_check(q, masks()["causal"])
     if N == 2:
         assert torch.isneginf(lse).all() and (o == 0).all()
+
+
+@pytest.mark.parametrize("value", [float("nan"), float("inf"), float("-inf")], ids=str)
+@pytest.mark.parametrize("kind,N", [("tree", 9), ("tree", 70), ("chain", 9), ("chain", 70)])
+@pytest.mark.parametrize("dtype", DTYPES, ids=["fp32", "fp16", "bf16"])
+def test_what_hidden_keys_hold_does_not_matter(dtype, kind, N, value):
+    """Keys and values that are not finite reach the rows that see them and no others."""
+    mask = masks()["causal" if kind == "tree" else "window"]
+    p = Problem(dtype, 4, 2, 64, [150, 64, 3000], [N, N - 1, N], N, 16, tree=kind == "tree", seed=N)
+    clean = p.k_cache.clone(), p.v_cache.clone()
+    poisoned = [[1, 4], [0], [2]] if kind == "tree" else [[-30, 1], [-36], [-35, -1]]  # new tokens; below zero: cached ones before them
+    sees = torch.zeros(3, N, dtype=torch.bool)
+    for b, keys in enumerate(poisoned):
+        c = p.lens[b]
+        for n, j in enumerate(keys):
+            page, row = int(p.table[b, (c + j) // 16]), (c + j) % 16
+            p.v_cache[page, :, row, 3] = value
+            if n == 0:
+                p.k_cache[page, 1, row] = value
+            for i in range(p.new[b]):
+                sees[b, i] |= j in p.sets[b][i] if kind == "tree" else i - 37 <= j <= i
+    assert sees.any() and not sees.all()
+    (o, lse), scale = attend(p, mask)
+    o_cpu = o.cpu()
+    for b in range(3):
+        for i in range(p.new[b]):
+            if sees[b, i]:
+                assert not torch.isfinite(o_cpu[b, :, i, 3]).any()
+    p.k_cache, p.v_cache = clean
+    check_attention(o, lse, p, mask, scale, dtype != torch.float32, rows=~sees)
 
 
 def test_lengths_beyond_the_table_and_below_zero():
