@@ -48,7 +48,7 @@ static int cached_kernel(const chill_cached_args& a) {
   const size_t es = esize(a.dtype);
   if (!tma_ok(a.k_cache, a.k_cache_strides, a.num_pages, a.H_kv, a.page_size, es) || !tma_ok(a.v_cache, a.v_cache_strides, a.num_pages, a.H_kv, a.page_size, es))
     return CHILL_CACHED_CUDA_CORES;
-  return CHILL_CACHED_ROWS;
+  return (long long)a.N * (a.H / a.H_kv) <= (a.D <= 128 ? 32 : 16) ? CHILL_CACHED_ROWS : CHILL_CACHED_TILES;
 }
 
 // Kernel, tiles, CTAs and workspace of a call, from the sizes that the host knows.
@@ -66,7 +66,7 @@ static int make_plan(const chill_cached_args& a, Plan& c) {
     c.rows = 16;
     c.grid = sm_count() * (a.D <= 64 ? 4 : (a.D <= 128 ? 2 : 1));
   } else {
-    c.rows = group_rows <= 16 || a.D > 128 ? 16 : 32;
+    c.rows = c.kernel == CHILL_CACHED_TILES ? 128 : (group_rows <= 16 ? 16 : 32);
     c.grid = sm_count() * (a.D <= 128 ? 2 : 1);
   }
   c.row_tiles = (int)((group_rows + c.rows - 1) / c.rows);

@@ -221,6 +221,24 @@ __device__ __forceinline__ Share begin_share(const CachedP& p, int* smem_cum, co
   return s;
 }
 
+// One tile of 64 keys by TMA: lane i of a warp copies box i % boxes.  The page of box i of the tile at k0; without one, page
+// num_pages, which is outside the map: TMA fills the box with zeros.
+__device__ __forceinline__ int tile_page(const CachedP& p, const RowTile& t, int k0, int i, bool& there) {
+  const int at = k0 + i * p.box;
+  int page = -1;
+  if (at < t.total) page = p.table[t.b * p.table_sb + at / p.page];
+  there = page >= 0 && page < p.num_pages;
+  return there ? page : p.num_pages;
+}
+// Groups of 8 keys without a page, from the boxes without one.
+__device__ __forceinline__ int lost_groups(const CachedP& p, unsigned lost, int boxes) {
+  int groups = 0;
+  if (lost != 0)
+    for (int i = 0; i < boxes; ++i)
+      if ((lost >> i) & 1u) groups |= ((1 << (p.box / 8)) - 1) << (i * (p.box / 8));
+  return groups;
+}
+
 __device__ __forceinline__ void pdl_launch_dependents() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 __device__ __forceinline__ void pdl_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 

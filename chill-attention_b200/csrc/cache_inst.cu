@@ -3,6 +3,7 @@
 #include "cache_launch.h"
 #include "cache_rows.cuh"
 #include "cache_simt.cuh"
+#include "cache_tiles.cuh"
 #include "chill_cache.h"
 #include "tc_launch.h"
 
@@ -40,9 +41,25 @@ static int launch_rows(const CachedP& p, const CUtensorMap* maps, int grid, cuda
   return (int)cudaGetLastError();
 }
 
+template <typename T, int DP>
+static int launch_tiles(const CachedP& p, const CUtensorMap* maps, int grid, cudaStream_t st) {
+  auto kern = cached_tiles_kernel<T, DP, InstMask>;
+  constexpr int smem = TilesShape<DP>::kDynamic;
+  static_assert(smem <= 232448, "exceeds the 227 KB of shared memory a CTA can opt in to");
+  struct Tag {};
+  cudaError_t e = ensure_dynamic_smem<Tag>(kern, smem, /*prefer_max_carveout=*/true);
+  if (e != cudaSuccess) return (int)e;
+  kern<<<grid, kTilesThreads, smem, st>>>(maps[0], maps[1], p);
+  return (int)cudaGetLastError();
+}
+
 template <typename T>
 static int launch_typed(int kernel, const CachedP& p, const CUtensorMap* maps, int grid, cudaStream_t st) {
   if constexpr (sizeof(T) == 2) {
+    if (kernel == CHILL_CACHED_TILES) {
+      if (p.D > 128) return launch_tiles<T, 256>(p, maps, grid, st);
+      return p.D > 64 ? launch_tiles<T, 128>(p, maps, grid, st) : launch_tiles<T, 64>(p, maps, grid, st);
+    }
     if (kernel == CHILL_CACHED_ROWS) {
       if (p.D > 128) return launch_rows<T, 256, 1>(p, maps, grid, st);
       if (p.D > 64) return p.rows == 16 ? launch_rows<T, 128, 1>(p, maps, grid, st) : launch_rows<T, 128, 2>(p, maps, grid, st);

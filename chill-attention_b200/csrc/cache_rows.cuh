@@ -65,16 +65,6 @@ __device__ __forceinline__ void mma16816<__half>(float (&c)[4], const uint32_t (
 
 enum : int { kStRowsProducer = 701, kStRowsConsumer = 702 };
 
-// One tile of 64 keys by TMA: lane i of a warp copies box i % boxes of 64-channel block i / boxes.  Returns the groups of 8 keys
-// that have no page (their rows are filled with zeros: page num_pages is outside the map).
-__device__ __forceinline__ int tile_page(const CachedP& p, const RowTile& t, int k0, int box, int i, bool& there) {
-  const int at = k0 + i * box, block = at / p.page;
-  int page = -1;
-  if (at < t.total) page = p.table[t.b * p.table_sb + block];
-  there = page >= 0 && page < p.num_pages;
-  return there ? page : p.num_pages;
-}
-
 template <typename T, int DP, int MT, class M>
 __global__ void __launch_bounds__(kRowsThreads, RowsShape<DP, MT>::kCtasPerSm)
 cached_rows_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV, const __grid_constant__ CachedP p) {
@@ -117,22 +107,18 @@ cached_rows_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constan
       const int mine = lane % boxes;
       bool there = false, there_next = false;
       int page = 0, page_next = 0;
-      if (piece.t0 < tiles) page_next = tile_page(p, t, t.k_lo + piece.t0 * kKeyTile, p.box, mine, there_next);
+      if (piece.t0 < tiles) page_next = tile_page(p, t, t.k_lo + piece.t0 * kKeyTile, mine, there_next);
       for (int kt = piece.t0; kt < tiles; ++kt, ++n) {
         const int s = n % kStages, k0 = t.k_lo + kt * kKeyTile;
         page = page_next;
         there = there_next;
-        if (kt + 1 < tiles) page_next = tile_page(p, t, k0 + kKeyTile, p.box, mine, there_next);
+        if (kt + 1 < tiles) page_next = tile_page(p, t, k0 + kKeyTile, mine, there_next);
         const unsigned lost = __ballot_sync(0xffffffffu, !there && lane < boxes);
         ok = tc::mbar_wait(empty + 8 * s, ((uint32_t)(n / kStages) & 1u) ^ 1u, guard, kStRowsProducer);
         ok = __all_sync(0xffffffffu, ok);
         if (!ok) break;
         if (lane == 0) {
-          int groups = 0;  // of 8 keys
-          if (lost != 0)
-            for (int i = 0; i < boxes; ++i)
-              if ((lost >> i) & 1u) groups |= ((1 << (p.box / 8)) - 1) << (i * (p.box / 8));
-          holes[s] = groups;
+          holes[s] = lost_groups(p, lost, boxes);
           tc::mbar_arrive_expect_tx(full + 8 * s, 2 * S::kTileBytes);
         }
         __syncwarp();
