@@ -42,46 +42,79 @@ static int box_rows(int page) {
   return 0;
 }
 
+// Rows of a tile of the kernel for many rows: as many whole tokens as 128 rows hold (0: a token has more).
+static int tile_rows(int G) { return G <= kTileRows ? kTileRows / G * G : 0; }
+
 // CHILL_CACHED_*: few rows go through mma.sync, which reads the keys once for all of them, many through tiles of 128 rows.
 static int cached_kernel(const chill_cached_args& a) {
   if (a.dtype == CHILL_F32 || (a.flags & CHILL_FLAG_FORCE_GENERIC) || box_rows(a.page_size) == 0) return CHILL_CACHED_CUDA_CORES;
   const size_t es = esize(a.dtype);
   if (!tma_ok(a.k_cache, a.k_cache_strides, a.num_pages, a.H_kv, a.page_size, es) || !tma_ok(a.v_cache, a.v_cache_strides, a.num_pages, a.H_kv, a.page_size, es))
     return CHILL_CACHED_CUDA_CORES;
-  return (long long)a.N * (a.H / a.H_kv) <= (a.D <= 128 ? 32 : 16) ? CHILL_CACHED_ROWS : CHILL_CACHED_TILES;
+  const int G = a.H / a.H_kv;
+  if ((long long)a.N * G <= (a.D <= 128 ? 32 : 16) || tile_rows(G) == 0 || !tma_ok(a.q, a.q_strides, a.B, a.H, a.N, es)) return CHILL_CACHED_ROWS;
+  return CHILL_CACHED_TILES;
 }
 
 // Kernel, tiles, CTAs and workspace of a call, from the sizes that the host knows.
 struct Plan {
-  int kernel, rows, row_tiles, grid, min_share;
+  int kernel, rows, row_tiles, grid, min_share, tail_shares;
   bool scan;  // prefix sums by a launch of their own
-  size_t seam, all, cum, ml, o, bytes;
+  size_t queue, seams, cum, ml, o, bytes;
 };
 
 static int make_plan(const chill_cached_args& a, Plan& c) {
-  const long long group_rows = (long long)a.N * (a.H / a.H_kv);
+  const int G = a.H / a.H_kv, sms = sm_count();
+  const long long group_rows = (long long)a.N * G;
   c.kernel = cached_kernel(a);
   c.min_share = 2;
+  c.tail_shares = 0;
   if (c.kernel == CHILL_CACHED_CUDA_CORES) {
     c.rows = 16;
-    c.grid = sm_count() * (a.D <= 64 ? 4 : (a.D <= 128 ? 2 : 1));
+    c.grid = sms * (a.D <= 64 ? 4 : (a.D <= 128 ? 2 : 1));
+  } else if (c.kernel == CHILL_CACHED_ROWS) {
+    c.rows = group_rows <= 16 || a.D > 128 ? 16 : 32;
+    c.grid = sms * (a.D <= 128 ? 2 : 1);
+    c.tail_shares = 2 * c.grid;
   } else {
-    c.rows = c.kernel == CHILL_CACHED_TILES ? 128 : (group_rows <= 16 ? 16 : 32);
-    c.grid = sm_count() * (a.D <= 128 ? 2 : 1);
+    const int half = tile_rows(G);
+    const bool two = a.D <= 128 && group_rows > half;
+    c.rows = two ? 2 * half : half;
+    c.grid = sms * (a.D <= 128 ? 2 : 1) / (two ? 2 : 1);
   }
-  c.row_tiles = (int)((group_rows + c.rows - 1) / c.rows);
-  const long long entries = (long long)a.B * c.row_tiles;
+  const long long row_tiles = (group_rows + c.rows - 1) / c.rows, entries = (long long)a.B * row_tiles;
   const long long keys = (long long)a.table_width * a.page_size;
   if (entries * a.H_kv * (keys / kKeyTile + 2) > 0x7fffffffll) return CHILL_E_TOO_LARGE;
-  c.scan = entries > kScanEntries;
+  c.row_tiles = (int)row_tiles;
   auto up = [](size_t x) { return (x + 255) / 256 * 256; };
-  c.seam = 0;
-  c.all = up((size_t)c.grid * sizeof(int4));
-  c.cum = c.all + 256;
+  // small shares only where the tables have room for so many keys
+  if (entries * a.H_kv * (keys / kKeyTile + 1) < (long long)kTailFrom * c.grid) c.tail_shares = 0;
+  c.scan = entries > kScanEntries;
+  const int shares = c.grid + c.tail_shares;
+  c.queue = 0;
+  c.seams = c.queue + 256;
+  c.cum = c.seams + up((size_t)shares * sizeof(Seam));
   c.ml = c.cum + (c.scan ? up((size_t)(entries + 1) * 4) : 0);
-  c.o = c.ml + up((size_t)2 * c.grid * c.rows * sizeof(float2));
-  c.bytes = c.o + up((size_t)2 * c.grid * c.rows * a.D * sizeof(float));
+  c.o = c.ml + up((size_t)2 * shares * c.rows * sizeof(float2));
+  c.bytes = c.o + up((size_t)2 * shares * c.rows * a.D * sizeof(float));
   return CHILL_OK;
+}
+
+// Q by whole tokens: channels, heads of a group, tokens, kv heads, requests; a box is 64 channels of `tokens` tokens' rows of a group.
+static int make_q_map(CUtensorMap* m, const chill_cached_args& a, int tokens) {
+  EncodeTiledFn fn = encode_fn();
+  if (fn == nullptr) return cuda_fail(cudaErrorUnknown, "cuTensorMapEncodeTiled entry point not available");
+  const int G = a.H / a.H_kv;
+  const cuuint64_t es = esize(a.dtype), any = 16;  // strides of dimensions of size one are not looked at
+  cuuint64_t dims[5] = {(cuuint64_t)a.D, (cuuint64_t)G, (cuuint64_t)a.N, (cuuint64_t)a.H_kv, (cuuint64_t)a.B};
+  cuuint64_t strides[4] = {G > 1 ? (cuuint64_t)a.q_strides[1] * es : any, a.N > 1 ? (cuuint64_t)a.q_strides[2] * es : any,
+                           a.H_kv > 1 ? (cuuint64_t)a.q_strides[1] * es * (cuuint64_t)G : any, a.B > 1 ? (cuuint64_t)a.q_strides[0] * es : any};
+  cuuint32_t box[5] = {64, (cuuint32_t)G, (cuuint32_t)tokens, 1, 1}, estr[5] = {1, 1, 1, 1, 1};
+  const CUresult r = fn(m, a.dtype == CHILL_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 5, const_cast<void*>(a.q), dims, strides, box, estr,
+                        CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r == CUDA_SUCCESS) return CHILL_OK;
+  snprintf(g_cuda_err, sizeof(g_cuda_err), "cuTensorMapEncodeTiled failed with CUresult %d", (int)r);
+  return CHILL_E_CUDA;
 }
 
 // Rows can be moved in 16-byte vectors.
@@ -93,10 +126,10 @@ static bool wide(const void* p, const int64_t* st, size_t es) {
 }
 
 template <class M>
-static int launch_typed(int dtype, int kernel, const CachedP& p, const CUtensorMap* maps, int grid, int* cum, cudaStream_t st, int* launches) {
-  if (dtype == CHILL_F32) return launch_cached<M, CHILL_F32>(kernel, p, maps, grid, cum, st, launches);
-  if (dtype == CHILL_F16) return launch_cached<M, CHILL_F16>(kernel, p, maps, grid, cum, st, launches);
-  return launch_cached<M, CHILL_BF16>(kernel, p, maps, grid, cum, st, launches);
+static int launch_typed(int dtype, int kernel, const CachedP& p, const CUtensorMap* maps, int grid, int* cum, cudaStream_t st) {
+  if (dtype == CHILL_F32) return launch_cached<M, CHILL_F32>(kernel, p, maps, grid, cum, st);
+  if (dtype == CHILL_F16) return launch_cached<M, CHILL_F16>(kernel, p, maps, grid, cum, st);
+  return launch_cached<M, CHILL_BF16>(kernel, p, maps, grid, cum, st);
 }
 
 static int cached_fwd(const chill_cached_args& a, cudaStream_t st) {
@@ -109,7 +142,8 @@ static int cached_fwd(const chill_cached_args& a, cudaStream_t st) {
   p.B = a.B; p.H = a.H; p.Hkv = a.H_kv; p.G = a.H / a.H_kv; p.N = a.N; p.D = a.D;
   p.page = a.page_size; p.num_pages = a.num_pages; p.width = a.table_width; p.box = box_rows(a.page_size);
   p.wide_q = wide(a.q, a.q_strides, es); p.wide_o = wide(a.o, a.o_strides, es);
-  p.rows = c.rows; p.row_tiles = c.row_tiles; p.words = (a.N + 31) / 32; p.min_share = c.min_share;
+  p.rows = c.rows; p.row_tiles = c.row_tiles; p.words = (a.N + 31) / 32;
+  p.min_share = c.min_share; p.tail_shares = c.tail_shares;
   p.scale_log2 = a.sm_scale * kLog2e;
   p.margs = to_mask_args(a.mask, (long long)kMaxLen);
   p.q = to_ref(a.q, a.q_strides); p.k = to_ref(a.k_cache, a.k_cache_strides); p.v = to_ref(a.v_cache, a.v_cache_strides);
@@ -120,17 +154,18 @@ static int cached_fwd(const chill_cached_args& a, cudaStream_t st) {
   char* w = (char*)a.workspace;
   int* cum = c.scan ? (int*)(w + c.cum) : nullptr;
   p.cum = cum;
-  p.seam = (int4*)(w + c.seam); p.all = (int*)(w + c.all); p.part_ml = (float2*)(w + c.ml); p.part_o = (float*)(w + c.o);
+  p.queue = (int*)(w + c.queue); p.seams = (Seam*)(w + c.seams); p.part_ml = (float2*)(w + c.ml); p.part_o = (float*)(w + c.o);
   p.status = device_status_ptr();
   if (p.status == nullptr) return cuda_fail(cudaGetLastError(), "status symbol");
-  CUtensorMap maps[2];
+  CUtensorMap maps[3];
   if (c.kernel != CHILL_CACHED_CUDA_CORES) {
     if ((rc = make_map(&maps[0], a.k_cache, a.k_cache_strides, a.num_pages, a.H_kv, a.page_size, a.D, a.dtype, p.box)) != CHILL_OK) return rc;
     if ((rc = make_map(&maps[1], a.v_cache, a.v_cache_strides, a.num_pages, a.H_kv, a.page_size, a.D, a.dtype, p.box)) != CHILL_OK) return rc;
   }
-  int e = 0, launches = 0;
-  CHILL_MASK_SWITCH(a.mask.id, (e = launch_typed<MaskT>(a.dtype, c.kernel, p, maps, c.grid, cum, st, &launches)))
-  count_launches(launches);
+  if (c.kernel == CHILL_CACHED_TILES && (rc = make_q_map(&maps[2], a, tile_rows(p.G) / p.G)) != CHILL_OK) return rc;
+  int e = 0;
+  CHILL_MASK_SWITCH(a.mask.id, (e = launch_typed<MaskT>(a.dtype, c.kernel, p, maps, c.grid, cum, st)))
+  if (e == 0) count_launches(1 + (c.scan || c.tail_shares > 0) + (c.grid > 1));
   return e == 0 ? CHILL_OK : cuda_fail((cudaError_t)e, "cached attention launch");
 }
 

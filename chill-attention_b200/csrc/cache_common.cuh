@@ -1,12 +1,18 @@
-// What the kernels of the paged cache share: geometry of a call, how the work is cut into equal shares, what a new token may see.
+// What the kernels of the paged cache share: geometry of a call, how the work is cut into shares, what a new token may see, how parts
+// are joined.
 //
 // Attention of new tokens over a cache, one (request, kv head) at a time: its rows are the new tokens times the heads that share
 // the kv head, row r = token r / G, head r % G, in tiles of `rows` rows; its keys are the cached ones and the new ones, in tiles
 // of kKeyTile keys.  A "unit" is one tile of rows of one kv head with the tiles of keys that it can see; units are numbered
-// by request, tile of rows, kv head.  Lengths live on the GPU, so the host can not split long units: every CTA works out
-// the prefix sum over the units' tiles and takes an equal share of all of them, wherever it begins and ends (in the middle of
-// units, mostly).  What a CTA has of a unit that it does not cover alone goes to a workspace as (maximum, sum, un-normalised O), and
-// a second kernel, launched behind the first without a gap, joins the parts in order of the keys: results are the same each run.
+// by request, tile of rows, kv head.  Lengths live on the GPU, so the host can not split long units: every CTA sums up the units' tiles
+// (with very many units a kernel of its own does) and cuts all of them into the same shares, wherever these begin and end (in the middle
+// of units, mostly).  Every CTA has one large share; where the kernel is bound by memory the last sixth of the tiles is cut into small
+// shares that go to whoever is done first, because SMs get unequal parts of the bandwidth (equal shares of 160 us were done after
+// 143 to 184 us).
+// What a share has of a unit that it does not cover alone goes to a workspace as (maximum, sum, un-normalised O), and a kernel launched
+// behind joins the parts in order of the keys: results are the same each run, whichever CTA had which share.  (Joined by the CTA of the last
+// part instead, a unit of 16 rows in 148 parts kept one CTA busy for 80 us, and the fence that takes cost every piece 3 us.  A first kernel
+// that plans for all CTAs takes 6 us, this sum 2 us.)
 #pragma once
 #include <cuda_runtime.h>
 #include <stdint.h>
@@ -18,7 +24,10 @@ namespace cache {
 
 constexpr int kMaxLen = 1 << 29;    // positions; three of them added stay below 2^31
 constexpr int kKeyTile = 64;        // keys of a tile, in all kernels
-constexpr int kScanEntries = 1024;  // (request, tile of rows) pairs whose prefix sum every CTA works out by itself
+constexpr int kTileRows = 128;      // rows of a tile of the kernel for many rows, at most
+constexpr int kTailFrom = 24;       // tiles a CTA, from where on there are small shares
+constexpr int kScanEntries = 256;   // (request, tile of rows) pairs that every CTA sums up by itself
+constexpr int kScanThreads = 1024;
 
 CHILL_HD int clamp_len(int x) { return imin(imax(x, 0), kMaxLen); }
 
@@ -29,7 +38,8 @@ struct CachedP {
   bool wide_q, wide_o;  // rows of Q / O can be moved in 16-byte vectors
   int rows, row_tiles;  // rows of a tile, tiles of N * G rows
   int words;            // 32-bit words of an ancestor row
-  int min_share;        // tiles of keys a CTA takes at least
+  int min_share;        // tiles of keys of a share at least
+  int tail_shares;      // small shares behind the large ones, at most (0: none)
   float scale_log2;     // softmax scale * log2(e)
   MaskArgs margs;
   TRef q, o;            // [batch][head][token][channel]
@@ -41,11 +51,11 @@ struct CachedP {
   const int *lens, *new_lens;
   const int *positions, *ancestors;  // ancestors null: the new tokens are a chain
   // workspace
-  const int* cum;       // prefix sums of a launch of their own; null: every CTA works them out
-  int4* seam;           // [CTA]: the unit its share begins in: (entry, kv head, first tile, tiles)
-  int* all;             // number of all tiles
-  float2* part_ml;      // [2 * CTA + (0 first, 1 last unit of its share)][row]
-  float* part_o;        // the same, [D]
+  const int* cum;       // [entries + 1]: tiles of the entries before, of one kv head, by a kernel of its own; null: every CTA for itself
+  int* queue;           // [1]: small shares taken
+  struct Seam* seams;   // [share]: the unit that is cut at the share's end for the first time
+  float2* part_ml;      // [2 * share + (0 first, 1 last unit of the share)][row]
+  float* part_o;        // the same, [D]; of the kernel for many rows [D / 4][row][4]
   int* status;
 };
 
@@ -114,7 +124,11 @@ __device__ __forceinline__ bool sees(const CachedP& p, const RowTile& t, int i, 
   return ((word >> (j & 31)) & 1u) != 0 && M::mask(pos, p.positions[(long long)t.b * p.N + j], n, p.margs);
 }
 
-// cum[e] = tiles of the (request, tile of rows) pairs before e, of one kv head; e <= B * row_tiles.  THREADS threads.
+__device__ __forceinline__ void pdl_launch_dependents() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+__device__ __forceinline__ void pdl_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+
+// ------------------------------------------------------------------------------------------------------- shares
+// cum[e] = tiles of the entries before e, of one kv head; e <= entries.
 template <class M, int THREADS>
 __device__ __forceinline__ void scan_units(const CachedP& p, int entries, int* cum) {
   __shared__ int sums[THREADS / 32];
@@ -134,9 +148,9 @@ __device__ __forceinline__ void scan_units(const CachedP& p, int entries, int* c
     int before = carry;
 #pragma unroll
     for (int w = 0; w < THREADS / 32; ++w) {
-      const int s = sums[w];
-      if (w < warp) before += s;
-      carry += s;
+      const int y = sums[w];
+      if (w < warp) before += y;
+      carry += y;
     }
     if (e < entries) cum[e] = before + x - v;
     __syncthreads();
@@ -145,81 +159,148 @@ __device__ __forceinline__ void scan_units(const CachedP& p, int entries, int* c
   __syncthreads();
 }
 
+// How the tiles of all units are cut: `large` equal shares up to tile large_end, then small ones of `tail` tiles.
+struct Cut {
+  int total, large_end, large, tail, shares;
+  __device__ __forceinline__ int begin(int x) const {
+    return x < large ? (int)((long long)large_end * x / large) : imin(total, large_end + (x - large) * tail);
+  }
+  __device__ __forceinline__ int of(int t) const {  // the share that tile t is in
+    return t < large_end ? (int)((((long long)t + 1) * large - 1) / large_end) : large + (t - large_end) / tail;
+  }
+};
+__device__ __forceinline__ Cut make_cut(const CachedP& p, int total, int grid) {
+  Cut c;
+  c.total = c.large_end = total;
+  c.large = c.shares = imax(1, imin(grid, total / p.min_share));
+  c.tail = 1;
+  if (p.tail_shares > 0 && total >= kTailFrom * grid) {
+    const int rest = total / 6;
+    c.tail = (rest + p.tail_shares - 1) / p.tail_shares;
+    c.large_end = total - rest;
+    c.shares = c.large + (rest + c.tail - 1) / c.tail;
+  }
+  return c;
+}
+
+// Before the launch of the attention kernel, which it overlaps: the counter of small shares, and where there are many entries their sums.
 template <class M>
-__global__ void __launch_bounds__(1024) scan_kernel(CachedP p, int* cum) {
-  scan_units<M, 1024>(p, p.B * p.row_tiles, cum);
+__global__ void __launch_bounds__(kScanThreads) prepare_kernel(const __grid_constant__ CachedP p, int* cum) {
+  pdl_launch_dependents();
+  if (threadIdx.x == 0) *p.queue = 0;
+  if (cum != nullptr) scan_units<M, kScanThreads>(p, p.B * p.row_tiles, cum);
 }
 
-// The share of CTA c of `ctas`: tiles [first, last) of all Hkv * cum[entries].  With little work only as many CTAs take part as
-// have min_share tiles each.
-__device__ __forceinline__ int share_begin(int total, int ctas, int c) { return (int)((long long)total * c / ctas); }
-__device__ __forceinline__ int active_ctas(const CachedP& p, int total, int grid) {
-  return imin(grid, imax(1, total / p.min_share));
-}
-// The entry whose tiles (of all kv heads) hold tile t.
-__device__ __forceinline__ int find_entry(const int* cum, int entries, int hkv, int t) {
-  int lo = 0, hi = entries - 1;
-  while (lo < hi) {
-    const int mid = (lo + hi + 1) >> 1;
-    if (cum[mid] * hkv <= t) lo = mid;
-    else hi = mid - 1;
-  }
-  return lo;
-}
-
-// A piece of a CTA's share: tiles [t0, t1) of the keys of one unit.
-struct Piece {
-  int entry, head;
-  int t0, t1;
-  bool whole;  // the unit is this CTA's alone
-  int slot;    // of the workspace, when it is not
+// The parts of a unit that is cut: slot0 of the share it begins in, then slot 2 * share of the following ones.
+struct Seam {
+  int parts;  // 0: the share's last unit ends with it, or begins before it
+  int slot0;
+  int b, head, r0, rows;
 };
 
-// Walks a CTA's share piece by piece; all threads of the CTA call it alike.
-struct Share {
-  int first, last, at, entry;
-  __device__ __forceinline__ bool next(const CachedP& p, const int* cum, Piece& x) {
-    if (at >= last) return false;
-    while (cum[entry + 1] * p.Hkv <= at) ++entry;
-    const int tiles = cum[entry + 1] - cum[entry], base = cum[entry] * p.Hkv;
-    x.entry = entry;
-    x.head = (at - base) / tiles;
-    const int begin = base + x.head * tiles;
-    x.t0 = at - begin;
-    x.t1 = imin(last - begin, tiles);
-    x.whole = x.t0 == 0 && x.t1 == tiles;
-    x.slot = 2 * (int)blockIdx.x + (at == first ? 0 : 1);
-    at = begin + x.t1;
-    return true;
-  }
-};
-
-// Prefix sums, this CTA's share and, for the kernel that joins the parts, where the share begins.
+// The sums and the cut, by all threads of a CTA of the attention kernel.
 template <class M, int THREADS>
-__device__ __forceinline__ Share begin_share(const CachedP& p, int* smem_cum, const int*& cum) {
+__device__ __forceinline__ Cut begin_work(const CachedP& p, int* smem_cum, const int*& cum) {
   const int entries = p.B * p.row_tiles;
   cum = p.cum;
   if (cum == nullptr) {
     scan_units<M, THREADS>(p, entries, smem_cum);
     cum = smem_cum;
+  } else {
+    pdl_wait();
   }
-  const int total = cum[entries] * p.Hkv, ctas = active_ctas(p, total, (int)gridDim.x), c = (int)blockIdx.x;
-  Share s;
-  s.first = c < ctas ? share_begin(total, ctas, c) : total;
-  s.last = c < ctas ? share_begin(total, ctas, c + 1) : total;
-  s.at = s.first;
-  s.entry = s.first < s.last ? find_entry(cum, entries, p.Hkv, s.first) : 0;
-  if (threadIdx.x == 0) {
-    int4 seam = make_int4(0, 0, 0, 0);
-    if (s.first < s.last) {
-      const int tiles = cum[s.entry + 1] - cum[s.entry], head = (s.first - cum[s.entry] * p.Hkv) / tiles;
-      seam = make_int4(s.entry, head, cum[s.entry] * p.Hkv + head * tiles, tiles);
-    }
-    p.seam[c] = seam;
-    if (c == 0) *p.all = total;
-  }
-  return s;
+  const Cut cut = make_cut(p, cum[entries] * p.Hkv, (int)gridDim.x);
+  if (threadIdx.x == 0)  // shares that there are not have nothing to join
+    for (int c = (int)blockIdx.x; c < (int)gridDim.x + p.tail_shares; c += (int)gridDim.x)
+      if (c >= cut.shares) p.seams[c].parts = 0;
+  return cut;
 }
+
+// A piece of a share: tiles [t0, t1) of the keys of one unit.
+struct Piece {
+  int entry, head;  // entry < 0: there is no more
+  int t0, t1;
+  int slot;         // of the workspace; -1: the unit is this share's alone
+};
+struct Item {
+  RowTile t;
+  Piece x;
+  int tiles;  // t1, or 0 where nothing is visible
+};
+// Hands out the pieces of a CTA's large share, then of small ones; a warp walks it, all lanes alike.
+struct Work {
+  Cut cut;
+  const int* cum;
+  int share, ahead;  // ahead: the small share that comes next (lane 0)
+  int at, last, begin, tiles, entry, head;
+  template <class M>
+  __device__ __forceinline__ void open(const CachedP& p, int c) {
+    share = c;
+    if (c >= cut.shares) return;
+    at = cut.begin(c);
+    last = cut.begin(c + 1);
+    int lo = 0, hi = p.B * p.row_tiles - 1;  // the entry whose tiles, of all kv heads, hold the first tile
+    while (lo < hi) {
+      const int mid = (lo + hi + 1) >> 1;
+      if (cum[mid] * p.Hkv <= at) lo = mid;
+      else hi = mid - 1;
+    }
+    entry = lo;
+    tiles = cum[lo + 1] - cum[lo];
+    head = (at - cum[lo] * p.Hkv) / tiles;
+    begin = cum[lo] * p.Hkv + head * tiles;
+  }
+  template <class M>
+  __device__ __forceinline__ void start(const CachedP& p, const Cut& c, const int* sums) {
+    cut = c;
+    cum = sums;
+    ahead = 0;
+    open<M>(p, (int)blockIdx.x < cut.large ? (int)blockIdx.x : cut.shares);
+  }
+  template <class M>
+  __device__ __forceinline__ bool next(const CachedP& p, Item& it) {
+    const int lane = threadIdx.x & 31;
+    if (share < cut.shares && at >= last) open<M>(p, cut.shares > cut.large ? __shfl_sync(0xffffffffu, ahead, 0) : cut.shares);
+    if (share >= cut.shares) {
+      it.x.entry = -1;
+      return false;
+    }
+    if (at >= begin + tiles) {  // the next unit
+      begin += tiles;
+      if (++head == p.Hkv) {
+        head = 0;
+        ++entry;
+        tiles = cum[entry + 1] - cum[entry];
+      }
+    }
+    Piece& x = it.x;
+    x.entry = entry;
+    x.head = head;
+    x.t0 = at - begin;
+    x.t1 = imin(last - begin, tiles);
+    it.t = row_tile<M>(p, entry);
+    it.tiles = it.t.n_tiles == 0 ? 0 : x.t1;
+    const int share_begin = cut.begin(share);
+    const bool goes_on = x.t1 != tiles;
+    x.slot = x.t0 != 0 ? 2 * share : (goes_on ? 2 * share + (share_begin < begin ? 1 : 0) : -1);
+    at = begin + x.t1;
+    if (at >= last) {  // the share's last piece
+      if (lane == 0) {
+        Seam m;
+        m.parts = x.t0 == 0 && goes_on ? cut.of(begin + tiles - 1) - share + 1 : 0;
+        m.slot0 = x.slot;
+        m.b = it.t.b; m.head = head; m.r0 = it.t.r0; m.rows = it.t.rows;
+        p.seams[share] = m;
+        if (cut.shares > cut.large) {
+          pdl_wait();
+          ahead = cut.large + atomicAdd(p.queue, 1);
+        }
+      }
+      __syncwarp();
+    }
+    return true;
+  }
+};
 
 // One tile of 64 keys by TMA: lane i of a warp copies box i % boxes.  The page of box i of the tile at k0; without one, page
 // num_pages, which is outside the map: TMA fills the box with zeros.
@@ -239,9 +320,6 @@ __device__ __forceinline__ int lost_groups(const CachedP& p, unsigned lost, int 
   return groups;
 }
 
-__device__ __forceinline__ void pdl_launch_dependents() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
-__device__ __forceinline__ void pdl_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
-
 // Writes one element of O and, by whoever has channel 0, the LSE.
 template <typename T>
 __device__ __forceinline__ T* o_row(const CachedP& p, int b, int h, int i) {
@@ -254,53 +332,188 @@ __device__ __forceinline__ void store_lse(const CachedP& p, int b, int h, int i,
   p.lse[b * p.lse_sb + h * p.lse_sh + i * p.lse_sl] = x;
 }
 
-// ------------------------------------------------------------------------------------------------------- joining
-// Block (c, y): the unit that the boundary between the shares of CTAs c and c + 1 cuts, if that is the first boundary inside it;
-// rows y * rows / gridDim.y on.  O = sum_i 2^(m_i - m) O_i / sum_i 2^(m_i - m) l_i over the parts in order.
-template <typename T>
-__global__ void __launch_bounds__(256) join_kernel(CachedP p, int grid) {
-  pdl_wait();
-  const int c = (int)blockIdx.x + 1;
-  const int total = *p.all, ctas = active_ctas(p, total, grid);
-  if (c >= ctas) return;
-  const int4 u = p.seam[c];
-  const int cut = share_begin(total, ctas, c), before = share_begin(total, ctas, c - 1);
-  if (cut == u.z || before > u.z) return;  // a unit begins here; or an earlier block joins this one
-  const int end = u.z + u.w;
-  const int slot0 = 2 * (c - 1) + (before < u.z ? 1 : 0);
-  int parts = 2;  // CTAs c - 1, c, ... as long as their shares begin inside the unit
-  while (c - 1 + parts < ctas && share_begin(total, ctas, c - 1 + parts) < end) ++parts;
+// Keys k0 .. k0 + 63 that token i at position pos sees, as bits; `lost`: groups of 8 keys without a page.
+template <class M>
+__device__ __forceinline__ uint64_t visible_keys(const CachedP& p, const RowTile& t, int i, int pos, int k0, int lost) {
+  const int n = t.cached + t.fresh, there = imin(t.total - k0, kKeyTile);
+  if (i < 0 || there <= 0) return 0ull;
+  const bool tree = p.ancestors != nullptr;
+  auto below = [](int c) -> uint64_t { return c >= 64 ? ~0ull : (c <= 0 ? 0ull : (1ull << c) - 1ull); };
+  // by the mask functor: all keys of a chain, the cached ones of a tree
+  const int cols = tree ? imin(t.cached - k0, there) : there;
+  uint64_t vis = 0ull;
+  if (cols > 0) {
+    if (interval_rows<M>::value) {
+      int lo, hi;
+      row_window<M, true>(pos, k0, cols, n, p.margs, lo, hi);
+      vis = below(hi + 1) & ~below(lo);
+    } else {
+      for (int c = 0; c < cols; ++c)
+        if (M::mask(pos, k0 + c, n, p.margs)) vis |= 1ull << c;
+    }
+  }
+  if (tree && k0 + there > t.cached) {  // by ancestry, then by the mask at the ancestors' positions
+    const int* row = p.ancestors + ((long long)t.b * p.N + i) * p.words;
+    const int j0 = k0 - t.cached;  // number of the new token at the tile's first key
+    const int w = imax(j0, 0) >> 5, sh = imax(j0, 0) & 31;
+    auto word = [&](int x) -> uint64_t { return x < p.words ? (uint64_t)(unsigned)row[x] : 0ull; };
+    uint64_t bits = (word(w) | (word(w + 1) << 32)) >> sh;
+    if (sh != 0) bits |= word(w + 2) << (64 - sh);
+    if (j0 < 0) bits <<= -j0;
+    bits &= below(there);
+    const int* at = p.positions + (long long)t.b * p.N + j0;
+    for (uint64_t left = bits; left != 0ull;) {
+      const int c = __ffsll((long long)left) - 1;
+      left &= left - 1ull;
+      if (!M::mask(pos, at[c], n, p.margs)) bits &= ~(1ull << c);
+    }
+    vis |= bits;
+  }
+  for (int g = lost; g != 0; g &= g - 1) vis &= ~(0xffull << (8 * (__ffs(g) - 1)));
+  return vis;
+}
 
-  const int b = u.x / p.row_tiles, r0 = (u.x - b * p.row_tiles) * p.rows;
-  const int all = p.N * p.G, valid = imin(imax(p.new_lens[b], 0), p.N) * p.G;
-  const int per_row = p.D / 4, chunk = p.rows / (int)gridDim.y, from = (int)blockIdx.y * chunk;
-  for (int idx = threadIdx.x; idx < chunk * per_row; idx += 256) {
-    const int r = from + idx / per_row, d = (idx % per_row) * 4;
-    if (r0 + r >= all) break;
-    const int i = (r0 + r) / p.G, h = u.y * p.G + (r0 + r) % p.G;
-    const bool ok = r0 + r < valid;
-    float m = -CUDART_INF_F, l = 0.f;
-    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-    if (ok) {
-      for (int k = 0; k < parts; ++k) m = fmaxf(m, p.part_ml[(long long)(k == 0 ? slot0 : 2 * (c - 1 + k)) * p.rows + r].x);
-      if (m != -CUDART_INF_F) {
-        for (int k = 0; k < parts; ++k) {
-          const long long at = (long long)(k == 0 ? slot0 : 2 * (c - 1 + k)) * p.rows + r;
-          const float2 ml = p.part_ml[at];
-          const float4 x = *reinterpret_cast<const float4*>(p.part_o + at * p.D + d);
-          const float w = exp2f(ml.x - m);
-          l += w * ml.y;
-          o.x += w * x.x; o.y += w * x.y; o.z += w * x.z; o.w += w * x.w;
+// Four channels of a row of O.
+template <typename T>
+__device__ __forceinline__ void store4(const CachedP& p, T* row, int ch, float a, float b, float c, float d) {
+  if (p.wide_o) {  // channels side by side, rows on 16-byte boundaries
+    if constexpr (sizeof(T) == 2) {
+      T e[4] = {from_f<T>(a), from_f<T>(b), from_f<T>(c), from_f<T>(d)};
+      *reinterpret_cast<uint2*>(row + ch) = *reinterpret_cast<const uint2*>(e);
+    } else {
+      *reinterpret_cast<float4*>(row + ch) = make_float4(a, b, c, d);
+    }
+  } else {
+    row[ch * p.o.sd] = from_f<T>(a); row[(ch + 1) * p.o.sd] = from_f<T>(b);
+    row[(ch + 2) * p.o.sd] = from_f<T>(c); row[(ch + 3) * p.o.sd] = from_f<T>(d);
+  }
+}
+
+// ------------------------------------------------------------------------------------------------------- joining
+//   O = sum_i 2^(m_i - m) O_i / sum_i 2^(m_i - m) l_i, m = max_i m_i, over the parts of a unit in order.
+// Block (share, y): the unit that is cut at the share's end for the first time, if there is one.
+// Few rows: a lane has four channels (two times four beyond 128) of a row, eight parts' loads are in flight at a time.  With `many` parts a
+// block works on one row, every warp on every eighth part; otherwise a warp on one row.
+constexpr int kJoinThreads = 256;
+template <typename T, int QUADS>
+__global__ void __launch_bounds__(kJoinThreads, QUADS == 1 ? 4 : 2) join_few_kernel(const __grid_constant__ CachedP p, int many) {
+  __shared__ float4 sums[8][32 * QUADS];
+  __shared__ float2 stat[8];
+  pdl_wait();
+  const Seam j = p.seams[blockIdx.x];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, quads = p.D / 4;
+  const int r = many ? (int)blockIdx.y : (int)blockIdx.y * 8 + warp, row = j.r0 + r;
+  if (j.parts < 2 || (many != 0 && row >= p.N * p.G)) return;
+  const bool exists = r < p.rows && row < p.N * p.G, ok = exists && r < j.rows;
+  float m = -CUDART_INF_F, l = 0.f;
+  float4 o[QUADS];
+#pragma unroll
+  for (int v = 0; v < QUADS; ++v) o[v] = make_float4(0.f, 0.f, 0.f, 0.f);
+  const int step = many ? 8 : 1;
+  for (int k0 = many ? warp : 0; k0 < j.parts && ok; k0 += 8 * step) {
+    float2 ml[8];
+    float4 x[8][QUADS];
+#pragma unroll
+    for (int u = 0; u < 8; ++u) {
+      const int k = k0 + step * u;
+      ml[u] = make_float2(-CUDART_INF_F, 0.f);
+#pragma unroll
+      for (int v = 0; v < QUADS; ++v) x[u][v] = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (k < j.parts) {
+        const long long at = (long long)(k == 0 ? j.slot0 : 2 * ((int)blockIdx.x + k)) * p.rows + r;
+        ml[u] = p.part_ml[at];
+#pragma unroll
+        for (int v = 0; v < QUADS; ++v)
+          if (lane + 32 * v < quads) x[u][v] = *reinterpret_cast<const float4*>(p.part_o + at * p.D + (lane + 32 * v) * 4);
+      }
+    }
+    float top = m;
+#pragma unroll
+    for (int u = 0; u < 8; ++u) top = fmaxf(top, ml[u].x);
+    if (top == -CUDART_INF_F) continue;
+    const float a = exp2f(m - top);
+    m = top;
+    l *= a;
+#pragma unroll
+    for (int v = 0; v < QUADS; ++v) o[v].x *= a, o[v].y *= a, o[v].z *= a, o[v].w *= a;
+#pragma unroll
+    for (int u = 0; u < 8; ++u) {
+      const float w = exp2f(ml[u].x - top);
+      l = fmaf(w, ml[u].y, l);
+#pragma unroll
+      for (int v = 0; v < QUADS; ++v) {
+        o[v].x = fmaf(w, x[u][v].x, o[v].x); o[v].y = fmaf(w, x[u][v].y, o[v].y);
+        o[v].z = fmaf(w, x[u][v].z, o[v].z); o[v].w = fmaf(w, x[u][v].w, o[v].w);
+      }
+    }
+  }
+  if (many) {  // the warps' sums become the first warp's
+#pragma unroll
+    for (int v = 0; v < QUADS; ++v) sums[warp][lane + 32 * v] = o[v], o[v] = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (lane == 0) stat[warp] = make_float2(m, l);
+    __syncthreads();
+    if (warp != 0) return;
+    m = -CUDART_INF_F;
+    l = 0.f;
+#pragma unroll
+    for (int w = 0; w < 8; ++w) m = fmaxf(m, stat[w].x);
+    if (m != -CUDART_INF_F) {
+#pragma unroll
+      for (int w = 0; w < 8; ++w) {
+        const float a = exp2f(stat[w].x - m);
+        l = fmaf(a, stat[w].y, l);
+#pragma unroll
+        for (int v = 0; v < QUADS; ++v) {
+          const float4 y = sums[w][lane + 32 * v];
+          o[v].x = fmaf(a, y.x, o[v].x); o[v].y = fmaf(a, y.y, o[v].y); o[v].z = fmaf(a, y.z, o[v].z); o[v].w = fmaf(a, y.w, o[v].w);
         }
       }
-      const float inv = l > 0.f ? 1.f / l : 0.f;
-      o.x *= inv; o.y *= inv; o.z *= inv; o.w *= inv;
     }
-    T* to = o_row<T>(p, b, h, i);
-    to[d * p.o.sd] = from_f<T>(o.x); to[(d + 1) * p.o.sd] = from_f<T>(o.y);
-    to[(d + 2) * p.o.sd] = from_f<T>(o.z); to[(d + 3) * p.o.sd] = from_f<T>(o.w);
-    if (d == 0) store_lse(p, b, h, i, ok, m, l);
   }
+  if (!exists) return;
+  const float inv = l != 0.f ? 1.f / l : 0.f;
+  const int i = row / p.G, h = j.head * p.G + row % p.G;
+  T* to = o_row<T>(p, j.b, h, i);
+#pragma unroll
+  for (int v = 0; v < QUADS; ++v)
+    if (lane + 32 * v < quads) store4<T>(p, to, (lane + 32 * v) * 4, o[v].x * inv, o[v].y * inv, o[v].z * inv, o[v].w * inv);
+  if (lane == 0) store_lse(p, j.b, h, i, ok, m, l);
+}
+
+// Many rows: lanes over 32 rows (as the parts lie), a warp for eight channels at a time.
+template <typename T>
+__global__ void __launch_bounds__(kJoinThreads) join_many_kernel(const __grid_constant__ CachedP p) {
+  pdl_wait();
+  const Seam j = p.seams[blockIdx.x];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, r = (int)blockIdx.y * 32 + lane, row = j.r0 + r;
+  if (j.parts < 2 || r >= p.rows || row >= p.N * p.G) return;
+  const int i = row / p.G, h = j.head * p.G + row % p.G;
+  const bool ok = r < j.rows;
+  auto slot = [&](int k) -> long long { return k == 0 ? j.slot0 : 2 * ((int)blockIdx.x + k); };
+  float m = -CUDART_INF_F, l = 0.f;
+#pragma unroll 4
+  for (int k = 0; k < (ok ? j.parts : 0); ++k) {
+    const float2 x = p.part_ml[slot(k) * p.rows + r];
+    const float top = fmaxf(m, x.x), safe = top == -CUDART_INF_F ? 0.f : top;
+    l = l * exp2f(m - safe) + exp2f(x.x - safe) * x.y;
+    m = top;
+  }
+  const float inv = l != 0.f ? 1.f / l : 0.f;
+  T* to = o_row<T>(p, j.b, h, i);
+  for (int d = warp * 8; d < p.D; d += 64) {
+    float4 a = make_float4(0.f, 0.f, 0.f, 0.f), b = a;
+#pragma unroll 4
+    for (int k = 0; k < (m != -CUDART_INF_F ? j.parts : 0); ++k) {
+      const float w = exp2f(p.part_ml[slot(k) * p.rows + r].x - m);
+      const float4* x = reinterpret_cast<const float4*>(p.part_o) + (slot(k) * (p.D / 4) + d / 4) * p.rows + r;
+      const float4 y = x[0], z = x[p.rows];
+      a.x = fmaf(w, y.x, a.x); a.y = fmaf(w, y.y, a.y); a.z = fmaf(w, y.z, a.z); a.w = fmaf(w, y.w, a.w);
+      b.x = fmaf(w, z.x, b.x); b.y = fmaf(w, z.y, b.y); b.z = fmaf(w, z.z, b.z); b.w = fmaf(w, z.w, b.w);
+    }
+    store4<T>(p, to, d, a.x * inv, a.y * inv, a.z * inv, a.w * inv);
+    store4<T>(p, to, d + 4, b.x * inv, b.y * inv, b.z * inv, b.w * inv);
+  }
+  if (warp == 0) store_lse(p, j.b, h, i, ok, m, l);
 }
 
 }  // namespace cache

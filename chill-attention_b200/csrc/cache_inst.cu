@@ -17,92 +17,94 @@ namespace cache {
 using InstMask = CHILL_INST_MASK;
 using InstType = std::conditional_t<CHILL_INST_PART == CHILL_F32, float, std::conditional_t<CHILL_INST_PART == CHILL_F16, __half, __nv_bfloat16>>;
 
+// `behind`: launched while the kernel before it in the stream, one of this call, runs; it waits for that where it needs its results.
+// The first kernel of a call never is: what runs before it is not known.
+template <class... Args, class... Given>
+static int launch(bool behind, void (*kern)(Args...), dim3 grid, int threads, int smem, cudaStream_t st, const Given&... args) {
+  cudaLaunchConfig_t cfg{};
+  cudaLaunchAttribute attr[1];
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3((unsigned)threads);
+  cfg.dynamicSmemBytes = (size_t)smem;
+  cfg.stream = st;
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = behind ? 1 : 0;
+  return (int)cudaLaunchKernelEx(&cfg, kern, Args(args)...);
+}
+
 template <typename T, int DP>
-static int launch_simt(const CachedP& p, int grid, cudaStream_t st) {
+static int launch_simt(const CachedP& p, int grid, bool behind, cudaStream_t st) {
   auto kern = cached_simt_kernel<T, DP, InstMask>;
   constexpr int smem = SimtSmem<DP>::kBytes;
   static_assert(smem <= 232448, "exceeds the 227 KB of shared memory a CTA can opt in to");
   struct Tag {};
   cudaError_t e = ensure_dynamic_smem<Tag>(kern, smem, /*prefer_max_carveout=*/true);
-  if (e != cudaSuccess) return (int)e;
-  kern<<<grid, kSimtThreads, smem, st>>>(p);
-  return (int)cudaGetLastError();
+  return e != cudaSuccess ? (int)e : launch(behind, kern, dim3((unsigned)grid), kSimtThreads, smem, st, p);
 }
 
 template <typename T, int DP, int MT>
-static int launch_rows(const CachedP& p, const CUtensorMap* maps, int grid, cudaStream_t st) {
+static int launch_rows(const CachedP& p, const CUtensorMap* maps, int grid, bool behind, cudaStream_t st) {
   auto kern = cached_rows_kernel<T, DP, MT, InstMask>;
   constexpr int smem = RowsShape<DP, MT>::kDynamic;
   static_assert(smem <= 232448, "exceeds the 227 KB of shared memory a CTA can opt in to");
   struct Tag {};
   cudaError_t e = ensure_dynamic_smem<Tag>(kern, smem, /*prefer_max_carveout=*/true);
-  if (e != cudaSuccess) return (int)e;
-  kern<<<grid, kRowsThreads, smem, st>>>(maps[0], maps[1], p);
-  return (int)cudaGetLastError();
+  return e != cudaSuccess ? (int)e : launch(behind, kern, dim3((unsigned)grid), kRowsThreads, smem, st, maps[0], maps[1], p);
 }
 
-template <typename T, int DP>
-static int launch_tiles(const CachedP& p, const CUtensorMap* maps, int grid, cudaStream_t st) {
-  auto kern = cached_tiles_kernel<T, DP, InstMask>;
-  constexpr int smem = TilesShape<DP>::kDynamic;
-  static_assert(smem <= 232448, "exceeds the 227 KB of shared memory a CTA can opt in to");
+template <typename T, int DP, int NQ>
+static int launch_tiles(const CachedP& p, const CUtensorMap* maps, int grid, bool behind, cudaStream_t st) {
+  using S = TilesShape<DP, NQ>;
+  auto kern = cached_tiles_kernel<T, DP, NQ, InstMask>;
+  static_assert(S::kDynamic <= 232448, "exceeds the 227 KB of shared memory a CTA can opt in to");
   struct Tag {};
-  cudaError_t e = ensure_dynamic_smem<Tag>(kern, smem, /*prefer_max_carveout=*/true);
+  cudaError_t e = ensure_dynamic_smem<Tag>(kern, S::kDynamic, /*prefer_max_carveout=*/true);
   if (e != cudaSuccess) return (int)e;
-  kern<<<grid, kTilesThreads, smem, st>>>(maps[0], maps[1], p);
-  return (int)cudaGetLastError();
+  return launch(behind, kern, dim3((unsigned)grid), S::kThreads, S::kDynamic, st, maps[2], maps[0], maps[1], p);
 }
 
 template <typename T>
-static int launch_typed(int kernel, const CachedP& p, const CUtensorMap* maps, int grid, cudaStream_t st) {
+static int launch_typed(int kernel, const CachedP& p, const CUtensorMap* maps, int grid, bool behind, cudaStream_t st) {
   if constexpr (sizeof(T) == 2) {
     if (kernel == CHILL_CACHED_TILES) {
-      if (p.D > 128) return launch_tiles<T, 256>(p, maps, grid, st);
-      return p.D > 64 ? launch_tiles<T, 128>(p, maps, grid, st) : launch_tiles<T, 64>(p, maps, grid, st);
+      const bool two = p.rows > kTileRows;
+      if (p.D > 128) return launch_tiles<T, 256, 1>(p, maps, grid, behind, st);
+      if (p.D > 64) return two ? launch_tiles<T, 128, 2>(p, maps, grid, behind, st) : launch_tiles<T, 128, 1>(p, maps, grid, behind, st);
+      return two ? launch_tiles<T, 64, 2>(p, maps, grid, behind, st) : launch_tiles<T, 64, 1>(p, maps, grid, behind, st);
     }
     if (kernel == CHILL_CACHED_ROWS) {
-      if (p.D > 128) return launch_rows<T, 256, 1>(p, maps, grid, st);
-      if (p.D > 64) return p.rows == 16 ? launch_rows<T, 128, 1>(p, maps, grid, st) : launch_rows<T, 128, 2>(p, maps, grid, st);
-      return p.rows == 16 ? launch_rows<T, 64, 1>(p, maps, grid, st) : launch_rows<T, 64, 2>(p, maps, grid, st);
+      if (p.D > 128) return launch_rows<T, 256, 1>(p, maps, grid, behind, st);
+      if (p.D > 64) return p.rows == 16 ? launch_rows<T, 128, 1>(p, maps, grid, behind, st) : launch_rows<T, 128, 2>(p, maps, grid, behind, st);
+      return p.rows == 16 ? launch_rows<T, 64, 1>(p, maps, grid, behind, st) : launch_rows<T, 64, 2>(p, maps, grid, behind, st);
     }
   }
   if (kernel != CHILL_CACHED_CUDA_CORES) return (int)cudaErrorInvalidValue;
-  if (p.D <= 32) return launch_simt<T, 32>(p, grid, st);
-  if (p.D <= 64) return launch_simt<T, 64>(p, grid, st);
-  if (p.D <= 128) return launch_simt<T, 128>(p, grid, st);
-  return launch_simt<T, 256>(p, grid, st);
-}
-
-// The parts are joined by a kernel whose launch overlaps the end of the first one; it waits for that before it reads.
-template <typename T>
-static int launch_join(const CachedP& p, int grid, cudaStream_t st) {
-  cudaLaunchConfig_t cfg{};
-  cudaLaunchAttribute attr[1];
-  cfg.gridDim = dim3((unsigned)imax(grid - 1, 1), (unsigned)(p.rows / 16));
-  cfg.blockDim = dim3(256);
-  cfg.stream = st;
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = 1;
-  return (int)cudaLaunchKernelEx(&cfg, join_kernel<T>, p, grid);
+  if (p.D <= 32) return launch_simt<T, 32>(p, grid, behind, st);
+  if (p.D <= 64) return launch_simt<T, 64>(p, grid, behind, st);
+  if (p.D <= 128) return launch_simt<T, 128>(p, grid, behind, st);
+  return launch_simt<T, 256>(p, grid, behind, st);
 }
 
 template <>
-int launch_cached<InstMask, CHILL_INST_PART>(int kernel, const CachedP& p, const CUtensorMap* maps, int grid, int* cum, cudaStream_t st, int* launches) {
-  if (cum != nullptr) {
-    scan_kernel<InstMask><<<1, 1024, 0, st>>>(p, cum);
+int launch_cached<InstMask, CHILL_INST_PART>(int kernel, const CachedP& p, const CUtensorMap* maps, int grid, int* cum, cudaStream_t st) {
+  const bool prepare = cum != nullptr || p.tail_shares > 0;
+  if (prepare) {
+    prepare_kernel<InstMask><<<1, cum != nullptr ? kScanThreads : 32, 0, st>>>(p, cum);
     const cudaError_t e = cudaGetLastError();
     if (e != cudaSuccess) return (int)e;
-    *launches += 1;
   }
-  int e = launch_typed<InstType>(kernel, p, maps, grid, st);
-  if (e != 0) return e;
-  *launches += 1;
-  if (grid == 1) return 0;  // nothing is cut
-  e = launch_join<InstType>(p, grid, st);
-  if (e == 0) *launches += 1;
-  return e;
+  const int e = launch_typed<InstType>(kernel, p, maps, grid, prepare, st);
+  if (e != 0 || grid == 1) return e;  // one share: nothing is cut
+  const unsigned shares = (unsigned)(grid + p.tail_shares);
+  if (kernel == CHILL_CACHED_TILES) return launch(true, join_many_kernel<InstType>, dim3(shares, (unsigned)((p.rows + 31) / 32)), kJoinThreads, 0, st, p);
+  // units that are far fewer than shares have many parts each
+  const long long rows = imin(p.rows, p.N * p.G), units = (long long)p.B * p.row_tiles * p.Hkv;
+  const int many = 4 * units < shares;
+  const dim3 blocks(shares, (unsigned)(many ? rows : (rows + 7) / 8));
+  if (p.D > 128) return launch(true, join_few_kernel<InstType, 2>, blocks, kJoinThreads, 0, st, p, many);
+  return launch(true, join_few_kernel<InstType, 1>, blocks, kJoinThreads, 0, st, p, many);
 }
 
 }  // namespace cache

@@ -9,10 +9,10 @@ namespace chill {
 namespace cache {
 struct CachedP;
 
-// `kernel`: CHILL_CACHED_*; `grid` CTAs share the work; maps: K, V; `cum`: where the prefix sums go when they have a launch of their
-// own, or null.  Returns a cudaError_t cast to int and adds to `launches`.
+// `kernel`: CHILL_CACHED_*; `grid` CTAs share the work; maps: K, V, Q; `cum`: where the prefix sums go when they have a
+// launch of their own, or null.  Returns a cudaError_t cast to int.
 template <class M, int DTYPE>
-int launch_cached(int kernel, const CachedP& p, const CUtensorMap* maps, int grid, int* cum, cudaStream_t st, int* launches);
+int launch_cached(int kernel, const CachedP& p, const CUtensorMap* maps, int grid, int* cum, cudaStream_t st);
 
 }  // namespace cache
 }  // namespace chill

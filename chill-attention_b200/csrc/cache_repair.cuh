@@ -8,44 +8,29 @@
 namespace chill {
 namespace cache {
 
-// Four channels of a row of O.
-template <typename T>
-__device__ __forceinline__ void store4(const CachedP& p, T* row, int ch, float a, float b, float c, float d) {
-  if (p.wide_o) {  // channels side by side, rows on 16-byte boundaries
-    if constexpr (sizeof(T) == 2) {
-      *reinterpret_cast<uint2*>(row + ch) = make_uint2(tc::pack2<T>(a, b), tc::pack2<T>(c, d));
-    } else {
-      *reinterpret_cast<float4*>(row + ch) = make_float4(a, b, c, d);
-    }
-  } else {
-    row[ch * p.o.sd] = from_f<T>(a); row[(ch + 1) * p.o.sd] = from_f<T>(b);
-    row[(ch + 2) * p.o.sd] = from_f<T>(c); row[(ch + 3) * p.o.sd] = from_f<T>(d);
-  }
-}
-
-// Whether any of the 128 consumer threads says so; also a barrier between their stores before and after it.
-__device__ __forceinline__ bool consumers_any(bool x) {
+// Whether any of 128 threads (four warps) says so; also a barrier between their stores before and after it.
+__device__ __forceinline__ bool consumers_any(bool x, int bar = 2) {
   uint32_t any;
   asm volatile(
       "{\n\t"
       ".reg .pred p, q;\n\t"
       "setp.ne.u32 p, %1, 0;\n\t"
-      "barrier.cta.red.or.pred q, 2, 128, p;\n\t"
+      "barrier.cta.red.or.pred q, %2, 128, p;\n\t"
       "selp.u32 %0, 1, 0, q;\n\t"
       "}\n"
       : "=r"(any)
-      : "r"((uint32_t)x)
+      : "r"((uint32_t)x), "r"(bar)
       : "memory");
   return any != 0;
 }
 
-// Rows of a piece again, one row a warp, lanes over the channels, key by key.
-template <typename T, int DP, class M>
-__device__ __noinline__ void repair_piece(const CachedP& p, const RowTile& t, const Piece& piece, int warp, int warps) {
+// Rows row0, row0 + warps, ... below `end` of a piece again, one row a warp, lanes over the channels, key by key.
+template <typename T, int DP, class M, bool kMany = false>
+__device__ __noinline__ void repair_piece(const CachedP& p, const RowTile& t, const Piece& piece, int row0, int warps, int end = 1 << 30) {
   const int lane = threadIdx.x & 31;
   constexpr int kOwn = DP / 32;  // channels of a lane: lane, lane + 32, ...
   const int last = imin(t.k_lo + piece.t1 * kKeyTile, t.total);
-  for (int r = warp; r < t.rows; r += warps) {
+  for (int r = row0; r < imin(t.rows, end); r += warps) {
     const int i = (t.r0 + r) / p.G, h = piece.head * p.G + (t.r0 + r) % p.G, pos = token_position(p, t, i);
     const T* qr = row_ptr<T>(p.q, t.b, h, i);
     float q[kOwn], o[kOwn], m = -CUDART_INF_F, l = 0.f;
@@ -80,11 +65,12 @@ __device__ __noinline__ void repair_piece(const CachedP& p, const RowTile& t, co
     for (int c = 0; c < kOwn; ++c) {
       const int d = lane + 32 * c;
       if (d >= p.D) continue;
-      if (piece.whole) to[d * p.o.sd] = from_f<T>(o[c] * inv);
+      if (piece.slot < 0) to[d * p.o.sd] = from_f<T>(o[c] * inv);
+      else if (kMany) p.part_o[(((long long)piece.slot * (p.D / 4) + d / 4) * p.rows + r) * 4 + d % 4] = o[c];
       else p.part_o[at * p.D + d] = o[c];
     }
     if (lane == 0) {
-      if (piece.whole) store_lse(p, t.b, h, i, true, m, l);
+      if (piece.slot < 0) store_lse(p, t.b, h, i, true, m, l);
       else p.part_ml[at] = make_float2(m, l);
     }
   }

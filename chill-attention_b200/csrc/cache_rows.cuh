@@ -4,8 +4,9 @@
 // be one row a thread), and the kernel is about keeping copies in flight.
 //
 // A CTA (two on an SM up to head dim 128) is one producer warp and four consumer warps:
-//   producer   walks the CTA's share; a tile is 64 keys of K and of V, boxes of `box` rows of one page and 64 channels (128-byte
-//              rows, 128B swizzle), a lane for each box, into a ring of kStages tiles (96 KB a CTA).  It runs ahead into the next unit.
+//   producer   takes shares and hands their pieces to the consumers, two of them with their Q (a bulk copy for each row) ahead; a
+//              tile is 64 keys of K and of V, boxes of `box` rows of one page and 64 channels (128-byte rows, 128B swizzle), a lane
+//              for each box, into a ring of kStages tiles (64 to 192 KB a CTA).  It runs ahead into the next piece and the next share.
 //   consumers  warp w takes keys 16 w .. 16 w + 15 of every tile for all rows, with a running maximum, sum and O of its own
 //              in registers: no warp waits for another before the end of a piece.  S = Q K^T (B fragments of K by ldmatrix), softmax
 //              on the accumulator's layout, P is the A fragment of O += P V as it stands (V by ldmatrix.trans).
@@ -21,25 +22,29 @@ namespace chill {
 namespace cache {
 
 constexpr int kRowsThreads = 256;  // warps 0-3 consumers, 4 producer, 5-7 idle
-constexpr int kRowsConsumerRegs = 216, kRowsOtherRegs = 40;  // two CTAs on an SM: 2 * 128 * (216 + 40) = 65536
+constexpr int kRowsConsumerRegs = 184, kRowsOtherRegs = 72;  // two CTAs on an SM: 2 * 128 * (184 + 72) = 65536
 
 template <int DP, int MT>
 struct RowsShape {
   static constexpr int kCtasPerSm = DP <= 128 ? 2 : 1;
   static constexpr int kHalves = DP / 64;                      // 64-channel blocks
   static constexpr int kTileBytes = kKeyTile * DP * 2;         // K or V
-  static constexpr int kStages = (DP <= 128 ? 98304 : 196608) / (2 * kTileBytes);
+  static constexpr int kStages = DP == 64 ? 5 : (MT == 1 ? 3 : 2);  // what two CTAs (head dim 256: one) have room for
   static constexpr int kRows = 16 * MT;
-  static constexpr int kQBytes = kRows * DP * 2;
+  static constexpr int kQPitch = DP * 2 + 16;                  // bytes of a row of Q: eight rows in different banks
+  static constexpr int kQBytes = kRows * kQPitch;
   static constexpr int kMergeBytes = 4 * 16 * 32 * 4;          // four warps, 16 rows, 32 channels
   static constexpr int kRing = 0;                              // stage: K, then V
-  static constexpr int kQ = kStages * 2 * kTileBytes;          // Q; at the end of a piece the merge buffer
-  static constexpr int kStat = kQ + (kQBytes > kMergeBytes ? kQBytes : kMergeBytes);  // maximum and sum of each warp's rows
-  static constexpr int kBars = kStat + 4 * kRows * 8;          // full[stage], empty[stage]
-  static constexpr int kHoles = kBars + 2 * kStages * 8;       // groups of 8 keys without a page, a word per stage
+  // Two Q, what the merge buffer is longer than a Q between them: it lies over the Q that has been used, and over that
+  static constexpr int kQ = kStages * 2 * kTileBytes;
+  static constexpr int kBetween = kMergeBytes > kQBytes ? kMergeBytes - kQBytes : 0;
+  static constexpr int kStat = kQ + 2 * kQBytes + kBetween;    // maximum and sum of each warp's rows
+  static constexpr int kBars = kStat + 4 * kRows * 8;          // full[stage], empty[stage], item_full[2], item_empty[2]
+  static constexpr int kHoles = kBars + (2 * kStages + 4) * 8; // groups of 8 keys without a page, a word per stage
   static constexpr int kMisc = kHoles + kStages * 4;
-  static constexpr int kCum = (kMisc + 16 + 15) / 16 * 16;
-  static constexpr int kTotal = kCum + (kScanEntries + 4) * 4;
+  static constexpr int kItems = (kMisc + 16 + 15) / 16 * 16;
+  static constexpr int kCum = kItems + 2 * (int)sizeof(Item);
+  static constexpr int kTotal = kCum + (kScanEntries + 1) * 4;
   static constexpr int kDynamic = kTotal + 1024;               // slack for manual 1024-byte alignment
   static_assert(kCtasPerSm * (kDynamic + 1024) <= 233472, "shared memory of an SM");
 };
@@ -63,6 +68,11 @@ __device__ __forceinline__ void mma16816<__half>(float (&c)[4], const uint32_t (
                : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
+// size bytes (a multiple of 16) from global to shared memory, both on 16-byte boundaries.
+__device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_t size, uint32_t bar) {
+  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst), "l"(src), "r"(size), "r"(bar) : "memory");
+}
+
 enum : int { kStRowsProducer = 701, kStRowsConsumer = 702 };
 
 template <typename T, int DP, int MT, class M>
@@ -74,9 +84,10 @@ cached_rows_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constan
   const uint32_t base = (tc::smem_u32(smem_raw) + 1023u) & ~1023u;
   uint8_t* gen = smem_raw + (base - tc::smem_u32(smem_raw));
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const uint32_t full = base + S::kBars, empty = full + 8 * kStages;
+  const uint32_t full = base + S::kBars, empty = full + 8 * kStages, item_full = empty + 8 * kStages, item_empty = item_full + 16;
   volatile int* holes = reinterpret_cast<volatile int*>(gen + S::kHoles);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(gen + S::kMisc);
+  Item* items = reinterpret_cast<Item*>(gen + S::kItems);
   const tc::Guard guard{p.status, abort_flag};
   if (threadIdx.x == 0) {
     *abort_flag = 0;
@@ -84,11 +95,18 @@ cached_rows_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constan
       tc::mbar_init(full + 8 * s, 1);
       tc::mbar_init(empty + 8 * s, 4);
     }
+    for (int s = 0; s < 2; ++s) {
+      tc::mbar_init(item_full + 8 * s, 1);
+      tc::mbar_init(item_empty + 8 * s, 4);
+    }
     tc::fence_barrier_init();
-    tc::fence_proxy_async_smem();
   }
+  // channels of Q beyond the head stay 0: those of K are filled with zeros, and 0 * NaN is NaN
+  if (p.D < DP)
+    for (int idx = threadIdx.x; idx < (2 * S::kQBytes + S::kBetween) / 16; idx += kRowsThreads) *reinterpret_cast<uint4*>(gen + S::kQ + idx * 16) = make_uint4(0u, 0u, 0u, 0u);
+  tc::fence_proxy_async_smem();
   const int* cum;
-  Share share = begin_share<M, kRowsThreads>(p, reinterpret_cast<int*>(gen + S::kCum), cum);
+  const Cut cut = begin_work<M, kRowsThreads>(p, reinterpret_cast<int*>(gen + S::kCum), cum);
   __syncthreads();
   pdl_launch_dependents();
 
@@ -96,40 +114,64 @@ cached_rows_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constan
     if constexpr (S::kCtasPerSm > 1) tc::reg_dealloc<kRowsOtherRegs>();
     if (warp > 4) return;
     // ---------------------------------------------------------------------------------------------- producer
-    const int boxes = kKeyTile / p.box, jobs = boxes * S::kHalves;
+    const int boxes = kKeyTile / p.box, jobs = boxes * S::kHalves, mine = lane % boxes;
     const uint32_t box_bytes = (uint32_t)p.box * 128u;
     int n = 0;  // tiles so far
     bool ok = true;
-    Piece piece;
-    while (ok && share.next(p, cum, piece)) {
-      const RowTile t = row_tile<M>(p, piece.entry);
-      const int tiles = t.n_tiles == 0 ? 0 : piece.t1;
-      const int mine = lane % boxes;
+    Work work;
+    work.start<M>(p, cut, cum);
+    Item it;
+    for (int item = 0;; ++item) {
+      const bool more = work.next<M>(p, it);
+      const int slot = item & 1;
+      ok = __all_sync(0xffffffffu, tc::mbar_wait(item_empty + 8 * slot, ((uint32_t)(item >> 1) & 1u) ^ 1u, guard, kStRowsProducer));
+      if (!ok) break;
+      const RowTile& t = it.t;
+      const uint32_t sq = base + S::kQ + slot * (S::kQBytes + S::kBetween), bar = item_full + 8 * slot;
+      if (more && it.tiles > 0 && !p.wide_q) {  // rows of Q that can not be copied in bulk
+        for (int idx = lane; idx < t.rows * p.D; idx += 32) {
+          const int r = idx / p.D, d = idx - r * p.D, i = (t.r0 + r) / p.G, h = it.x.head * p.G + (t.r0 + r) % p.G;
+          *reinterpret_cast<T*>(gen + (sq - base) + r * S::kQPitch + d * 2) = row_ptr<T>(p.q, t.b, h, i)[d * p.q.sd];
+        }
+        __syncwarp();
+      }
+      const bool bulk = more && it.tiles > 0 && p.wide_q;
+      if (lane == 0) {
+        items[slot] = it;
+        if (bulk) tc::mbar_arrive_expect_tx(bar, (uint32_t)(t.rows * p.D * 2));
+        else tc::mbar_arrive(bar);
+      }
+      __syncwarp();
+      if (!more) break;
+      if (bulk && lane < t.rows) {
+        const int i = (t.r0 + lane) / p.G, h = it.x.head * p.G + (t.r0 + lane) % p.G;
+        bulk_load(sq + lane * S::kQPitch, row_ptr<T>(p.q, t.b, h, i), (uint32_t)(p.D * 2), bar);
+      }
       bool there = false, there_next = false;
       int page = 0, page_next = 0;
-      if (piece.t0 < tiles) page_next = tile_page(p, t, t.k_lo + piece.t0 * kKeyTile, mine, there_next);
-      for (int kt = piece.t0; kt < tiles; ++kt, ++n) {
+      if (it.x.t0 < it.tiles) page_next = tile_page(p, t, t.k_lo + it.x.t0 * kKeyTile, mine, there_next);
+      for (int kt = it.x.t0; kt < it.tiles; ++kt, ++n) {
         const int s = n % kStages, k0 = t.k_lo + kt * kKeyTile;
         page = page_next;
         there = there_next;
-        if (kt + 1 < tiles) page_next = tile_page(p, t, k0 + kKeyTile, mine, there_next);
+        if (kt + 1 < it.tiles) page_next = tile_page(p, t, k0 + kKeyTile, mine, there_next);
         const unsigned lost = __ballot_sync(0xffffffffu, !there && lane < boxes);
-        ok = tc::mbar_wait(empty + 8 * s, ((uint32_t)(n / kStages) & 1u) ^ 1u, guard, kStRowsProducer);
-        ok = __all_sync(0xffffffffu, ok);
+        ok = __all_sync(0xffffffffu, tc::mbar_wait(empty + 8 * s, ((uint32_t)(n / kStages) & 1u) ^ 1u, guard, kStRowsProducer));
         if (!ok) break;
         if (lane == 0) {
           holes[s] = lost_groups(p, lost, boxes);
           tc::mbar_arrive_expect_tx(full + 8 * s, 2 * S::kTileBytes);
         }
         __syncwarp();
+        const int row = (k0 + mine * p.box) % p.page;
         for (int j = lane; j < jobs; j += 32) {
           const int half = j / boxes;
           const uint32_t dst = base + S::kRing + s * 2 * S::kTileBytes + half * (kKeyTile * 128) + mine * box_bytes;
-          const int row = (k0 + mine * p.box) % p.page;
-          tc::tma_load_4d(dst, &tmK, full + 8 * s, half * 64, row, piece.head, page);
-          tc::tma_load_4d(dst + S::kTileBytes, &tmV, full + 8 * s, half * 64, row, piece.head, page);
+          tc::tma_load_4d(dst, &tmK, full + 8 * s, half * 64, row, it.x.head, page);
+          tc::tma_load_4d(dst + S::kTileBytes, &tmV, full + 8 * s, half * 64, row, it.x.head, page);
         }
       }
+      if (!ok) break;
     }
     if (!ok) {  // copies already in flight land before the CTA's shared memory goes away
       const uint64_t t0 = tc::globaltimer_ns();
@@ -141,42 +183,22 @@ cached_rows_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constan
   // ------------------------------------------------------------------------------------------------- consumers
   if constexpr (S::kCtasPerSm > 1) tc::reg_alloc<kRowsConsumerRegs>();
   const int g = lane >> 2, quad = lane & 3;  // the accumulator's rows g and g + 8, channels / keys 2 quad, 2 quad + 1 of 8
-  const uint32_t sq = base + S::kQ;
-  float* merge = reinterpret_cast<float*>(gen + S::kQ);
   float2* stat = reinterpret_cast<float2*>(gen + S::kStat);
   int n = 0;
-  Piece piece;
-  while (share.next(p, cum, piece)) {  // after a wait that ran out, too: all four warps meet at every barrier of the CTA's pieces
-    const RowTile t = row_tile<M>(p, piece.entry);
-    const int tiles = t.n_tiles == 0 ? 0 : piece.t1;
-    tc::named_bar_sync(1, 128);  // Q and the merge buffer are free
-    for (int idx = threadIdx.x; idx < S::kRows * (DP / 8); idx += 128) {  // Q in 16-byte units, swizzled like K
-      const int r = idx / (DP / 8), unit = idx % (DP / 8);
-      uint4 x = make_uint4(0u, 0u, 0u, 0u);
-      if (r < t.rows && unit * 8 < p.D) {
-        const int i = (t.r0 + r) / p.G, h = piece.head * p.G + (t.r0 + r) % p.G;
-        const T* src = row_ptr<T>(p.q, t.b, h, i);
-        if (p.wide_q) {
-          x = *reinterpret_cast<const uint4*>(src + unit * 8);
-        } else {
-          T e[8];
-#pragma unroll
-          for (int u = 0; u < 8; ++u) e[u] = src[(unit * 8 + u) * p.q.sd];
-          x = *reinterpret_cast<const uint4*>(e);
-        }
-      }
-      *reinterpret_cast<uint4*>(gen + S::kQ + (unit / 8) * (S::kRows * 128) + r * 128 + (((unit % 8) ^ (r & 7)) * 16)) = x;
-    }
-    int token[MT][2], pos[MT][2];
-#pragma unroll
-    for (int mt = 0; mt < MT; ++mt)
-#pragma unroll
-      for (int u = 0; u < 2; ++u) {
-        const int r = mt * 16 + g + 8 * u;
-        token[mt][u] = r < t.rows ? (t.r0 + r) / p.G : -1;
-        pos[mt][u] = r < t.rows ? token_position(p, t, token[mt][u]) : 0;
-      }
-    tc::named_bar_sync(1, 128);
+  bool ok = true;
+  for (int item = 0;; ++item) {
+    const int slot = item & 1;
+    // The four warps leave together: whether there is one more piece, and whether all of them saw it, is settled at a barrier
+    bool leave = !__all_sync(0xffffffffu, tc::mbar_wait(item_full + 8 * slot, (uint32_t)(item >> 1) & 1u, guard, kStRowsConsumer));
+    if (!leave) leave = items[slot].x.entry < 0;
+    if (consumers_any(leave)) break;
+    const RowTile& t = items[slot].t;
+    const Piece& piece = items[slot].x;
+    const int tiles = items[slot].tiles, k_lo = t.k_lo, total = t.total, full_lo = t.full_lo, full_hi = t.full_hi;
+    const uint32_t sq = base + S::kQ + slot * (S::kQBytes + S::kBetween);
+    float* merge = reinterpret_cast<float*>(gen + S::kQ + slot * S::kQBytes);
+    const int row_token = lane < t.rows ? (t.r0 + lane) / p.G : -1;  // of row `lane`
+    const int row_pos = lane < t.rows ? token_position(p, t, row_token) : 0;
 
     float o[MT][DP / 8][4], m[MT][2], l[MT][2];
 #pragma unroll
@@ -193,9 +215,10 @@ cached_rows_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constan
     const int x7 = lane & 7;  // row % 8 in all three
 
     for (int kt = piece.t0; kt < tiles; ++kt, ++n) {
-      const int s = n % kStages, k0 = t.k_lo + kt * kKeyTile;
+      const int s = n % kStages, k0 = k_lo + kt * kKeyTile;
       const uint32_t sk = base + S::kRing + s * 2 * S::kTileBytes, sv = sk + S::kTileBytes;
-      if (!__all_sync(0xffffffffu, tc::mbar_wait(full + 8 * s, (uint32_t)(n / kStages) & 1u, guard, kStRowsConsumer))) break;
+      ok = __all_sync(0xffffffffu, tc::mbar_wait(full + 8 * s, (uint32_t)(n / kStages) & 1u, guard, kStRowsConsumer));
+      if (!ok) break;  // the rest of the piece is skipped; the next one's wait fails at once
       float c[MT][2][4];
 #pragma unroll
       for (int mt = 0; mt < MT; ++mt)
@@ -208,31 +231,30 @@ cached_rows_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constan
 #pragma unroll
         for (int mt = 0; mt < MT; ++mt) {
           uint32_t a[4];
-          ldsm4(a, sq + (kk / 4) * (S::kRows * 128) + (mt * 16 + q_row) * 128 + ((((kk % 4) * 2 + q_unit) ^ x7) << 4));
+          ldsm4(a, sq + (mt * 16 + q_row) * S::kQPitch + (kk * 2 + q_unit) * 16);
           mma16816<T>(c[mt][0], a, b[0], b[1]);
           mma16816<T>(c[mt][1], a, b[2], b[3]);
         }
       }
       const int lost = holes[s];
-      if (lost != 0 || k0 < t.full_lo || k0 + kKeyTile > t.full_hi) {
+      if (lost != 0 || k0 < full_lo || k0 + kKeyTile > full_hi) {
+        // lane r works out row r's keys; a thread then takes those of its own rows
+        uint64_t vis = visible_keys<M>(p, t, row_token, row_pos, k0, lost);
+        __syncwarp();
+        const uint32_t half = warp < 2 ? (uint32_t)vis : (uint32_t)(vis >> 32);  // the 32 keys that hold this warp's 16
 #pragma unroll
-        for (int j = 0; j < 2; ++j)
+        for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            const int in_tile = warp * 16 + j * 8 + quad * 2 + e, key = k0 + in_tile;
-            const bool there = key < t.total && ((lost >> (in_tile >> 3)) & 1) == 0;
-            const bool all = key >= t.full_lo && key < t.full_hi;
+          for (int u = 0; u < 2; ++u) {
+            const uint32_t mine = __shfl_sync(0xffffffffu, half, mt * 16 + g + 8 * u) >> ((warp & 1) * 16 + quad * 2);
 #pragma unroll
-            for (int mt = 0; mt < MT; ++mt)
+            for (int j = 0; j < 2; ++j)
 #pragma unroll
-              for (int u = 0; u < 2; ++u) {
-                bool see = there && token[mt][u] >= 0;
-                if (see && !all) see = sees<M>(p, t, token[mt][u], pos[mt][u], key);
-                if (!see) c[mt][j][u * 2 + e] = -CUDART_INF_F;
-              }
+              for (int e = 0; e < 2; ++e)
+                if (((mine >> (j * 8 + e)) & 1u) == 0u) c[mt][j][u * 2 + e] = -CUDART_INF_F;
           }
-        if (k0 + kKeyTile > t.total) {  // rows behind the last key may hold anything, and 0 * NaN is NaN: this warp's become 0
-          const int gone = imax(t.total - k0, 0);
+        if (k0 + kKeyTile > total) {  // rows behind the last key may hold anything, and 0 * NaN is NaN: this warp's become 0
+          const int gone = imax(total - k0, 0);
           for (int idx = lane; idx < 16 * (DP / 8); idx += 32) {
             const int r = warp * 16 + idx / (DP / 8), unit = idx % (DP / 8);
             if (r >= gone) *reinterpret_cast<uint4*>(gen + (sv - base) + (unit / 8) * (kKeyTile * 128) + r * 128 + (unit % 8) * 16) = make_uint4(0u, 0u, 0u, 0u);
@@ -339,7 +361,7 @@ cached_rows_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constan
         const int ch = cb * 32 + out_c;
         if (ch >= p.D || t.r0 + r >= all_rows) continue;
         odd |= r < t.rows && !(fabsf(x.x) + fabsf(x.y) + fabsf(x.z) + fabsf(x.w) <= 3e38f);
-        if (piece.whole) {
+        if (piece.slot < 0) {
           T* to = o_row<T>(p, t.b, h, i);
           if (r >= t.rows) x = make_float4(0.f, 0.f, 0.f, 0.f);
           store4<T>(p, to, ch, x.x * inv, x.y * inv, x.z * inv, x.w * inv);
@@ -348,11 +370,18 @@ cached_rows_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constan
         }
       }
       if (out_c == 0 && t.r0 + r < all_rows) {
-        if (piece.whole) store_lse(p, t.b, h, i, r < t.rows, top, sum);
+        if (piece.slot < 0) store_lse(p, t.b, h, i, r < t.rows, top, sum);
         else p.part_ml[(long long)piece.slot * p.rows + r] = make_float2(top, sum);
       }
     }
     if (consumers_any(odd)) repair_piece<T, DP, M>(p, t, piece, warp, 4);
+    if (p.D < DP) {  // the channels beyond the head become 0 again
+      tc::named_bar_sync(1, 128);
+      for (int idx = threadIdx.x; idx < S::kQBytes / 16; idx += 128) *reinterpret_cast<uint4*>(gen + (sq - base) + idx * 16) = make_uint4(0u, 0u, 0u, 0u);
+      tc::fence_proxy_async_smem();
+    }
+    __syncwarp();
+    if (lane == 0) tc::mbar_arrive(item_empty + 8 * slot);
   }
 }
 

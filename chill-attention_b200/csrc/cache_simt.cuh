@@ -24,7 +24,8 @@ struct SimtSmem {
   static constexpr int kS = kV + kKeyTile * DP;
   static constexpr int kM = kS + kSimtRows * kKeyTile;  // alpha of every row
   static constexpr int kBad = kM + kSimtRows;           // a key has no page
-  static constexpr int kCum = kBad + kKeyTile;
+  static constexpr int kItem = kBad + kKeyTile;
+  static constexpr int kCum = kItem + (int)sizeof(Item) / 4;
   static constexpr int kBytes = (kCum + kScanEntries + 1) * 4;
 };
 
@@ -40,14 +41,24 @@ __global__ void __launch_bounds__(kSimtThreads) cached_simt_kernel(const __grid_
   constexpr int kOwn = kSimtRows / kGroups;                                         // rows of a thread in O += P V
   const int quad = tid % kChunks, group = tid / kChunks;
   const bool pv = group < kGroups;
+  Item& item = *reinterpret_cast<Item*>(smem + L::kItem);
   const int* cum;
-  Share share = begin_share<M, kSimtThreads>(p, reinterpret_cast<int*>(smem + L::kCum), cum);
+  const Cut cut = begin_work<M, kSimtThreads>(p, reinterpret_cast<int*>(smem + L::kCum), cum);
   pdl_launch_dependents();
-  Piece piece;
-  while (share.next(p, cum, piece)) {
-    const RowTile t = row_tile<M>(p, piece.entry);
-    const int tiles = t.n_tiles == 0 ? 0 : piece.t1;
+  Work work;
+  if (warp == 0) work.start<M>(p, cut, cum);
+  while (true) {
     __syncthreads();
+    if (warp == 0) {
+      Item it;
+      work.next<M>(p, it);
+      if (lane == 0) item = it;
+    }
+    __syncthreads();
+    if (item.x.entry < 0) break;
+    const RowTile& t = item.t;
+    const Piece& piece = item.x;
+    const int tiles = item.tiles;
     for (int idx = tid; idx < kSimtRows * DP; idx += kSimtThreads) {
       const int r = idx / DP, d = idx % DP;
       float x = 0.f;
@@ -173,7 +184,7 @@ __global__ void __launch_bounds__(kSimtThreads) cached_simt_kernel(const __grid_
         const int r = group * kOwn + n, all = p.N * p.G;
         if (t.r0 + r >= all) continue;
         const float mr = sm[r], lr = sm[kSimtRows + r];
-        if (piece.whole) {
+        if (piece.slot < 0) {
           const int i = (t.r0 + r) / p.G, h = piece.head * p.G + (t.r0 + r) % p.G;
           const float inv = r < t.rows && lr > 0.f ? 1.f / lr : 0.f;
           T* to = o_row<T>(p, t.b, h, i);
