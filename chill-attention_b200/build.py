@@ -170,7 +170,7 @@ def build_extension(force=False):
     includes = include_paths() + [os.path.join(cuda, "include"), sysconfig.get_paths()["include"], INCLUDE]
     _run(["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
           "-DTORCH_EXTENSION_NAME=_chill_torch"] + [x for i in includes for x in ("-isystem", i)] + sources + ["-o", out]
-         + [f"-L{p}" for p in library_paths()] + ["-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch", "-ltorch_python"])
+         + [f"-L{p}" for p in library_paths()] + ["-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch_cuda", "-ltorch", "-ltorch_python"])
     with open(stamp, "w") as f:
         f.write(h.hexdigest())
     return out

@@ -72,22 +72,23 @@ class ChillStep(typing.NamedTuple):
 
 
 def _native(lib=None):
-    lib = lib or _cache_abi.load_library()
+    """The native call object of a library (None: the one of the built-in masks)."""
     native = _NATIVE.get(lib)
     if native is None:
-        functions = [getattr(lib, name) for name in _ENTRY_POINTS] + [_cabi.load_library().chill_status_string, lib.chill_cache_last_cuda_error]
+        found = lib or _cache_abi.load_library()
+        functions = [getattr(found, name) for name in _ENTRY_POINTS] + [_cabi.load_library().chill_status_string, found.chill_cache_last_cuda_error]
         native = _NATIVE[lib] = _eager.extension().CacheLibrary([C.cast(f, C.c_void_p).value for f in functions])
     return native
 
 
-def _plain(*tensors) -> bool:
-    """Whether a call can go to the native module directly: plain CUDA tensors and nothing that watches the dispatcher."""
-    if torch.compiler.is_compiling() or not _eager._PROBES_OK:
-        return False
-    for t in tensors:
-        if type(t) is not torch.Tensor or not t.is_cuda:
-            return False
-    return _eager._dispatch_depth() == 0 and _eager._function_depth() == 0 and _eager._functorch_top() is None
+_is_compiling = torch.compiler.is_compiling
+_dispatch_depth, _function_depth, _functorch_top = _eager._dispatch_depth, _eager._function_depth, _eager._functorch_top
+
+
+def _direct() -> bool:
+    """Whether a call can go to the native module: nothing watches the dispatcher.  (The module itself turns away tensors that are
+    watched, or not on a GPU.)"""
+    return not _is_compiling() and _eager._PROBES_OK and _dispatch_depth() == 0 and _function_depth() == 0 and _functorch_top() is None
 
 
 # --------------------------------------------------------------------------------------------- argument checks, with messages
@@ -249,8 +250,9 @@ def chill_pages_reserve(pages: ChillPages, lens: torch.Tensor, new_lens: torch.T
 
     Returns: the step's ChillStep; positions are lens[b] + depth (chain: lens[b] + number).
     """
-    if _plain(pages.table, lens, new_lens):
-        out = _eager.extension().pages_reserve(_native(), *pages, lens, new_lens, max_new, page_size, parents)
+    if _direct():
+        native = _NATIVE.get(None) or _native()
+        out = _eager._extension.pages_reserve(native, *pages, lens, new_lens, max_new, page_size, parents)
         if out is not None:
             return ChillStep(lens, new_lens, *out)
     _check_pages(pages, lens, page_size)
@@ -263,7 +265,7 @@ def chill_pages_trim(pages: ChillPages, lens: torch.Tensor, page_size: int) -> N
     """Gives the pages behind ``lens[b]`` tokens of every request back (``lens[b] = 0``: all of them), in place.
 
     The exact inverse of a reservation: what it gives back is what the same reservation takes again, in the same order."""
-    if _plain(pages.table, lens) and _eager.extension().pages_trim(_native(), pages.table, pages.held, pages.free, pages.n_free, lens, page_size):
+    if _direct() and _eager.extension().pages_trim(_NATIVE.get(None) or _native(), pages.table, pages.held, pages.free, pages.n_free, lens, page_size):
         return
     _check_pages(pages, lens, page_size)
     _trim_op(pages.table, pages.held, pages.free, pages.n_free, lens, page_size)
@@ -273,7 +275,7 @@ def chill_cache_append(k_cache: torch.Tensor, v_cache: torch.Tensor, k: torch.Te
     """Stores the rows of ``k`` and ``v`` ([batch, kv_heads, max_new, head_dim], any strides) at ``slots`` of the caches
     ([num_pages, kv_heads, page_size, head_dim], any strides), in place.  Tokens whose slot is outside the cache (-1) are left out; rows that
     no slot names stay as they are."""
-    if _plain(k_cache, v_cache, k, v, slots) and _eager.extension().cache_append(_native(), k_cache, v_cache, k, v, slots):
+    if _direct() and _eager.extension().cache_append(_NATIVE.get(None) or _native(), k_cache, v_cache, k, v, slots):
         return
     _check_rows(k_cache, v_cache, k, v, slots)
     _append_op(k_cache, v_cache, k, v, slots)
@@ -290,8 +292,8 @@ def chill_cache_commit(k_cache: torch.Tensor, v_cache: torch.Tensor, table: torc
     Returns: int32 [batch], the new lengths ``lens + accepted``.  Pages stay reserved; ``chill_pages_trim`` gives spare ones back.
     """
     N = step.slots.shape[1]
-    if _plain(k_cache, v_cache, table, path, accepted):
-        out = _eager.extension().cache_commit(_native(), k_cache, v_cache, table, step.lens, step.new_lens, N, path, accepted)
+    if _direct():
+        out = _eager.extension().cache_commit(_NATIVE.get(None) or _native(), k_cache, v_cache, table, step.lens, step.new_lens, N, path, accepted)
         if out is not None:
             return out
     _check_commit(k_cache, v_cache, table, step.lens, step.new_lens, path, accepted)
@@ -340,11 +342,9 @@ def chill_attention_cached(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torc
 def _attention(q, k_cache, v_cache, table, step, mask, sm_scale, return_lse, flags):
     if sm_scale is None:
         sm_scale = q.shape[-1] ** -0.5
-    if mask.name not in _MASKS:
-        _mask_functor(mask)
+    native, functor_id = _MASKS.get(mask.name) or _mask_functor(mask)
     lens, new_lens, _, positions, ancestors = step
-    if _plain(q, k_cache, v_cache, table, lens):
-        native, functor_id = _MASKS[mask.name]
+    if _direct():
         out = _eager._extension.cached_attention(native, functor_id, q, k_cache, v_cache, table, lens, new_lens, positions, ancestors,
                                                  mask.constargs, sm_scale, return_lse, flags)
         if out is not None:

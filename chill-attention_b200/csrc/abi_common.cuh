@@ -24,9 +24,14 @@ static int cuda_fail(cudaError_t e, const char* what) {
 }
 
 static int* device_status_ptr() {
-  // one word per device (the symbol is instantiated in every device's module image)
+  // one word per device (the symbol is instantiated in every device's module image); its address is looked up once
+  constexpr int kMaxDevices = 64;
+  static std::atomic<int*> known[kMaxDevices];
+  int dev = 0;
   int* p = nullptr;
+  if (cudaGetDevice(&dev) == cudaSuccess && dev >= 0 && dev < kMaxDevices && (p = known[dev].load(std::memory_order_acquire)) != nullptr) return p;
   if (cudaGetSymbolAddress((void**)&p, g_device_status) != cudaSuccess) return nullptr;
+  if (dev >= 0 && dev < kMaxDevices) known[dev].store(p, std::memory_order_release);
   return p;
 }
 

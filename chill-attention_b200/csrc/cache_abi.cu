@@ -70,8 +70,9 @@ static int make_plan(const chill_cached_args& a, Plan& c) {
   c.min_share = 2;
   c.tail_shares = 0;
   if (c.kernel == CHILL_CACHED_CUDA_CORES) {
-    c.rows = 16;
-    c.grid = sms * (a.D <= 64 ? 4 : (a.D <= 128 ? 2 : 1));
+    c.rows = group_rows <= 4 ? 4 : (group_rows <= 8 ? 8 : 16);
+    c.grid = sms * (c.rows < 16 ? 4 : (a.D <= 64 ? 4 : (a.D <= 128 ? 2 : 1)));
+    if (c.rows < 16) c.tail_shares = c.grid;
   } else if (c.kernel == CHILL_CACHED_ROWS) {
     c.rows = group_rows <= 16 || a.D > 128 ? 16 : 32;
     c.grid = sms * (a.D <= 128 ? 2 : 1);
@@ -141,6 +142,7 @@ static int cached_fwd(const chill_cached_args& a, cudaStream_t st) {
   CachedP p{};
   p.B = a.B; p.H = a.H; p.Hkv = a.H_kv; p.G = a.H / a.H_kv; p.N = a.N; p.D = a.D;
   p.page = a.page_size; p.num_pages = a.num_pages; p.width = a.table_width; p.box = box_rows(a.page_size);
+  p.wide_kv = wide(a.k_cache, a.k_cache_strides, es) && wide(a.v_cache, a.v_cache_strides, es);
   p.wide_q = wide(a.q, a.q_strides, es); p.wide_o = wide(a.o, a.o_strides, es);
   p.rows = c.rows; p.row_tiles = c.row_tiles; p.words = (a.N + 31) / 32;
   p.min_share = c.min_share; p.tail_shares = c.tail_shares;

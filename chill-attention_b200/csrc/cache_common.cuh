@@ -26,6 +26,7 @@ constexpr int kMaxLen = 1 << 29;    // positions; three of them added stay below
 constexpr int kKeyTile = 64;        // keys of a tile, in all kernels
 constexpr int kTileRows = 128;      // rows of a tile of the kernel for many rows, at most
 constexpr int kTailFrom = 24;       // tiles a CTA, from where on there are small shares
+constexpr int kTailTiles = 8;       // tiles of a small share, at least
 constexpr int kScanEntries = 256;   // (request, tile of rows) pairs that every CTA sums up by itself
 constexpr int kScanThreads = 1024;
 
@@ -36,6 +37,7 @@ struct CachedP {
   int page, num_pages, width;
   int box;              // rows of a TMA box (tensor-core kernels)
   bool wide_q, wide_o;  // rows of Q / O can be moved in 16-byte vectors
+  bool wide_kv;         // those of the caches too
   int rows, row_tiles;  // rows of a tile, tiles of N * G rows
   int words;            // 32-bit words of an ancestor row
   int min_share;        // tiles of keys of a share at least
@@ -162,11 +164,14 @@ __device__ __forceinline__ void scan_units(const CachedP& p, int entries, int* c
 // How the tiles of all units are cut: `large` equal shares up to tile large_end, then small ones of `tail` tiles.
 struct Cut {
   int total, large_end, large, tail, shares;
+  int each, more;  // tiles of a large share; so many of them have one more
   __device__ __forceinline__ int begin(int x) const {
-    return x < large ? (int)((long long)large_end * x / large) : imin(total, large_end + (x - large) * tail);
+    return x < large ? x * each + imin(x, more) : imin(total, large_end + (x - large) * tail);
   }
   __device__ __forceinline__ int of(int t) const {  // the share that tile t is in
-    return t < large_end ? (int)((((long long)t + 1) * large - 1) / large_end) : large + (t - large_end) / tail;
+    if (t >= large_end) return large + (t - large_end) / tail;
+    const int longer = more * (each + 1);
+    return t < longer ? t / (each + 1) : more + (t - longer) / each;
   }
 };
 __device__ __forceinline__ Cut make_cut(const CachedP& p, int total, int grid) {
@@ -176,10 +181,12 @@ __device__ __forceinline__ Cut make_cut(const CachedP& p, int total, int grid) {
   c.tail = 1;
   if (p.tail_shares > 0 && total >= kTailFrom * grid) {
     const int rest = total / 6;
-    c.tail = (rest + p.tail_shares - 1) / p.tail_shares;
+    c.tail = imax(kTailTiles, (rest + p.tail_shares - 1) / p.tail_shares);
     c.large_end = total - rest;
     c.shares = c.large + (rest + c.tail - 1) / c.tail;
   }
+  c.each = c.large_end / c.large;
+  c.more = c.large_end - c.each * c.large;
   return c;
 }
 
@@ -332,9 +339,16 @@ __device__ __forceinline__ void store_lse(const CachedP& p, int b, int h, int i,
   p.lse[b * p.lse_sb + h * p.lse_sh + i * p.lse_sl] = x;
 }
 
-// Keys k0 .. k0 + 63 that token i at position pos sees, as bits; `lost`: groups of 8 keys without a page.
+// The first 64 of token i's ancestor bits, loaded ahead of the tiles that need them.
+__device__ __forceinline__ uint64_t first_ancestors(const CachedP& p, int b, int i) {
+  if (p.ancestors == nullptr || i < 0) return 0ull;
+  const int* row = p.ancestors + ((long long)b * p.N + i) * p.words;
+  return (uint64_t)(unsigned)row[0] | (p.words > 1 ? (uint64_t)(unsigned)row[1] << 32 : 0ull);
+}
+
+// Keys k0 .. k0 + 63 that token i at position pos sees, as bits; `near`: first_ancestors; `lost`: groups of 8 keys without a page.
 template <class M>
-__device__ __forceinline__ uint64_t visible_keys(const CachedP& p, const RowTile& t, int i, int pos, int k0, int lost) {
+__device__ __forceinline__ uint64_t visible_keys(const CachedP& p, const RowTile& t, int i, int pos, uint64_t near, int k0, int lost) {
   const int n = t.cached + t.fresh, there = imin(t.total - k0, kKeyTile);
   if (i < 0 || there <= 0) return 0ull;
   const bool tree = p.ancestors != nullptr;
@@ -353,19 +367,29 @@ __device__ __forceinline__ uint64_t visible_keys(const CachedP& p, const RowTile
     }
   }
   if (tree && k0 + there > t.cached) {  // by ancestry, then by the mask at the ancestors' positions
-    const int* row = p.ancestors + ((long long)t.b * p.N + i) * p.words;
     const int j0 = k0 - t.cached;  // number of the new token at the tile's first key
-    const int w = imax(j0, 0) >> 5, sh = imax(j0, 0) & 31;
-    auto word = [&](int x) -> uint64_t { return x < p.words ? (uint64_t)(unsigned)row[x] : 0ull; };
-    uint64_t bits = (word(w) | (word(w + 1) << 32)) >> sh;
-    if (sh != 0) bits |= word(w + 2) << (64 - sh);
-    if (j0 < 0) bits <<= -j0;
+    uint64_t bits;
+    if (p.words <= 2) {
+      bits = j0 >= 64 ? 0ull : (j0 >= 0 ? near >> j0 : near << -j0);
+    } else {
+      const int* row = p.ancestors + ((long long)t.b * p.N + i) * p.words;
+      const int w = imax(j0, 0) >> 5, sh = imax(j0, 0) & 31;
+      auto word = [&](int x) -> uint64_t { return x < p.words ? (uint64_t)(unsigned)row[x] : 0ull; };
+      bits = (word(w) | (word(w + 1) << 32)) >> sh;
+      if (sh != 0) bits |= word(w + 2) << (64 - sh);
+      if (j0 < 0) bits <<= -j0;
+    }
     bits &= below(there);
-    const int* at = p.positions + (long long)t.b * p.N + j0;
-    for (uint64_t left = bits; left != 0ull;) {
-      const int c = __ffsll((long long)left) - 1;
-      left &= left - 1ull;
-      if (!M::mask(pos, at[c], n, p.margs)) bits &= ~(1ull << c);
+    // ancestors stand at positions [cached, pos]: one look where the mask shows the token all of these
+    int lo = 0, hi = 0;
+    if (M::kHasKFullRange) M::k_full_range_for_q(pos, 1, n, p.margs, lo, hi);
+    if (lo > t.cached || hi <= pos) {
+      const int* at = p.positions + (long long)t.b * p.N + j0;
+      for (uint64_t left = bits; left != 0ull;) {
+        const int c = __ffsll((long long)left) - 1;
+        left &= left - 1ull;
+        if (!M::mask(pos, at[c], n, p.margs)) bits &= ~(1ull << c);
+      }
     }
     vis |= bits;
   }

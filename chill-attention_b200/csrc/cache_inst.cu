@@ -36,6 +36,8 @@ static int launch(bool behind, void (*kern)(Args...), dim3 grid, int threads, in
 
 template <typename T, int DP>
 static int launch_simt(const CachedP& p, int grid, bool behind, cudaStream_t st) {
+  if (p.rows == 4) return launch(behind, cached_simt_few_kernel<T, DP, 4, InstMask>, dim3((unsigned)grid), kSimtThreads, 0, st, p);
+  if (p.rows == 8) return launch(behind, cached_simt_few_kernel<T, DP, 8, InstMask>, dim3((unsigned)grid), kSimtThreads, 0, st, p);
   auto kern = cached_simt_kernel<T, DP, InstMask>;
   constexpr int smem = SimtSmem<DP>::kBytes;
   static_assert(smem <= 232448, "exceeds the 227 KB of shared memory a CTA can opt in to");

@@ -184,7 +184,8 @@ cached_rows_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constan
   if constexpr (S::kCtasPerSm > 1) tc::reg_alloc<kRowsConsumerRegs>();
   const int g = lane >> 2, quad = lane & 3;  // the accumulator's rows g and g + 8, channels / keys 2 quad, 2 quad + 1 of 8
   float2* stat = reinterpret_cast<float2*>(gen + S::kStat);
-  int n = 0;
+  int stage = 0;
+  uint32_t phase = 0;
   bool ok = true;
   for (int item = 0;; ++item) {
     const int slot = item & 1;
@@ -199,6 +200,7 @@ cached_rows_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constan
     float* merge = reinterpret_cast<float*>(gen + S::kQ + slot * S::kQBytes);
     const int row_token = lane < t.rows ? (t.r0 + lane) / p.G : -1;  // of row `lane`
     const int row_pos = lane < t.rows ? token_position(p, t, row_token) : 0;
+    const uint64_t row_near = first_ancestors(p, t.b, row_token);
 
     float o[MT][DP / 8][4], m[MT][2], l[MT][2];
 #pragma unroll
@@ -214,10 +216,10 @@ cached_rows_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constan
     const int v_row = warp * 16 + ((lane >> 3) & 1) * 8 + (lane & 7), v_unit = lane >> 4;
     const int x7 = lane & 7;  // row % 8 in all three
 
-    for (int kt = piece.t0; kt < tiles; ++kt, ++n) {
-      const int s = n % kStages, k0 = k_lo + kt * kKeyTile;
+    for (int kt = piece.t0; kt < tiles; ++kt) {
+      const int s = stage, k0 = k_lo + kt * kKeyTile;
       const uint32_t sk = base + S::kRing + s * 2 * S::kTileBytes, sv = sk + S::kTileBytes;
-      ok = __all_sync(0xffffffffu, tc::mbar_wait(full + 8 * s, (uint32_t)(n / kStages) & 1u, guard, kStRowsConsumer));
+      ok = __all_sync(0xffffffffu, tc::mbar_wait(full + 8 * s, phase, guard, kStRowsConsumer));
       if (!ok) break;  // the rest of the piece is skipped; the next one's wait fails at once
       float c[MT][2][4];
 #pragma unroll
@@ -239,7 +241,7 @@ cached_rows_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constan
       const int lost = holes[s];
       if (lost != 0 || k0 < full_lo || k0 + kKeyTile > full_hi) {
         // lane r works out row r's keys; a thread then takes those of its own rows
-        uint64_t vis = visible_keys<M>(p, t, row_token, row_pos, k0, lost);
+        uint64_t vis = visible_keys<M>(p, t, row_token, row_pos, row_near, k0, lost);
         __syncwarp();
         const uint32_t half = warp < 2 ? (uint32_t)vis : (uint32_t)(vis >> 32);  // the 32 keys that hold this warp's 16
 #pragma unroll
@@ -263,23 +265,47 @@ cached_rows_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constan
           __syncwarp();
         }
       }
-      uint32_t pa[MT][4];
+      // All rows' maxima first, then one look whether any of them moved far: the rows' chains run side by side
+      float top[MT][2];
 #pragma unroll
-      for (int mt = 0; mt < MT; ++mt) {
+      for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+        for (int u = 0; u < 2; ++u) top[mt][u] = fmaxf(fmaxf(c[mt][0][2 * u], c[mt][0][2 * u + 1]), fmaxf(c[mt][1][2 * u], c[mt][1][2 * u + 1]));
+#pragma unroll
+      for (int x = 1; x <= 2; x <<= 1)
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+          for (int u = 0; u < 2; ++u) top[mt][u] = fmaxf(top[mt][u], __shfl_xor_sync(0xffffffffu, top[mt][u], x));
+      bool far = false;
+#pragma unroll
+      for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
-          float top = fmaxf(fmaxf(c[mt][0][2 * u], c[mt][0][2 * u + 1]), fmaxf(c[mt][1][2 * u], c[mt][1][2 * u + 1]));
-          top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-          top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2)) * p.scale_log2;
-          // The maximum is followed lazily: O is rescaled when it grew by more than 2^8 (weights stay below that, exact in fp32
-          // sums and far from the 16-bit types' limits), so most tiles do not touch O
-          if (__any_sync(0xffffffffu, top - m[mt][u] > 8.f)) {
-            const float m_new = fmaxf(m[mt][u], top), a = m_new == -CUDART_INF_F ? 1.f : tc::ex2(m[mt][u] - m_new);
-            m[mt][u] = m_new;
+          top[mt][u] *= p.scale_log2;
+          far |= top[mt][u] - m[mt][u] > 8.f;
+        }
+      // The maximum is followed lazily: O is rescaled when it grew by more than 2^8 (weights stay below that, exact in fp32 sums and far
+      // from the 16-bit types' limits), so most tiles do not touch O
+      if (__any_sync(0xffffffffu, far)) {
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+          for (int u = 0; u < 2; ++u) {
+            // a row goes by itself: rows that do not exist hold anything
+            const bool moves = top[mt][u] - m[mt][u] > 8.f;
+            const float a = moves ? tc::ex2(m[mt][u] - top[mt][u]) : 1.f;
+            m[mt][u] = moves ? top[mt][u] : m[mt][u];
             l[mt][u] *= a;
 #pragma unroll
             for (int d = 0; d < DP / 8; ++d) o[mt][d][2 * u] *= a, o[mt][d][2 * u + 1] *= a;
           }
+      }
+      uint32_t pa[MT][4];
+#pragma unroll
+      for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
           const float safe = m[mt][u] == -CUDART_INF_F ? 0.f : m[mt][u];
 #pragma unroll
           for (int j = 0; j < 2; ++j) {
@@ -288,7 +314,6 @@ cached_rows_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constan
             pa[mt][j * 2 + u] = tc::pack2<T>(w0, w1);
           }
         }
-      }
 #pragma unroll
       for (int nn = 0; nn < DP / 16; ++nn) {
         uint32_t b[4];
@@ -301,6 +326,7 @@ cached_rows_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constan
       }
       __syncwarp();
       if (lane == 0) tc::mbar_arrive(empty + 8 * s);
+      if (++stage == kStages) stage = 0, phase ^= 1u;
     }
 
     // ---- the four warps' states become one
@@ -350,12 +376,13 @@ cached_rows_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constan
         for (int d = 0; d < 4; ++d)
 #pragma unroll
           for (int u = 0; u < 2; ++u)
-            *reinterpret_cast<float2*>(merge + (warp * 16 + g + 8 * u) * 32 + d * 8 + quad * 2) = make_float2(o[mt][cb * 4 + d][2 * u], o[mt][cb * 4 + d][2 * u + 1]);
+            *reinterpret_cast<float2*>(merge + (warp * 16 + g + 8 * u) * 32 + ((d ^ (g & 3)) * 8) + quad * 2) = make_float2(o[mt][cb * 4 + d][2 * u], o[mt][cb * 4 + d][2 * u + 1]);
         tc::named_bar_sync(1, 128);
-        float4 x = *reinterpret_cast<const float4*>(merge + out_r * 32 + out_c);
+        const int swizzled = out_c ^ ((out_r & 3) * 8);  // rows that lie 128 bytes apart are stored from different banks
+        float4 x = *reinterpret_cast<const float4*>(merge + out_r * 32 + swizzled);
 #pragma unroll
         for (int w = 1; w < 4; ++w) {
-          const float4 y = *reinterpret_cast<const float4*>(merge + (w * 16 + out_r) * 32 + out_c);
+          const float4 y = *reinterpret_cast<const float4*>(merge + (w * 16 + out_r) * 32 + swizzled);
           x.x += y.x; x.y += y.y; x.z += y.z; x.w += y.w;
         }
         const int ch = cb * 32 + out_c;

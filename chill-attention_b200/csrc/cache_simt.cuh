@@ -1,7 +1,12 @@
 // Attention of new tokens over a paged cache on the CUDA cores: fp32 (IEEE arithmetic) and every layout that the tensor-core
 // kernels can not take.  See cache_common.cuh for units and shares.
 //
-// A CTA of 128 threads works on 16 rows and 64 keys at a time, everything as fp32 in shared memory:
+// Up to 8 rows (simt_few): bound by memory, so nothing goes through shared memory.  D / 4 lanes (32 at most) share a key, a warp has
+// 16 keys of every tile of 64; a lane keeps four channels (eight at head dim 256) of Q and O of every row, reads those of K and V of
+// 8 keys at once, and gets the scores by butterflies over its lanes.  Every group of lanes has a maximum and a sum of its own: no warp,
+// and no group, waits for another before the end of a piece.
+//
+// More rows: a CTA of 128 threads works on 16 rows and 64 keys at a time, everything as fp32 in shared memory:
 //   S = Q K^T   a thread has one key and 8 rows: one vector of K and 8 (broadcast) of Q for 32 FMAs
 //   softmax     a warp has 4 rows; running maximum and sum in base 2
 //   O += P V    a thread has 4 channels of 2 D / 64 rows (registers)
@@ -197,6 +202,188 @@ __global__ void __launch_bounds__(kSimtThreads) cached_simt_kernel(const __grid_
           if (quad * 4 < p.D) *reinterpret_cast<float4*>(p.part_o + at * p.D + quad * 4) = make_float4(acc[n][0], acc[n][1], acc[n][2], acc[n][3]);
           if (quad == 0) p.part_ml[at] = make_float2(mr, lr);
         }
+      }
+    }
+  }
+}
+
+// Four channels from global memory, as fp32.
+template <typename T>
+__device__ __forceinline__ float4 load4(const T* p, long long sd, bool wide) {
+  if (wide) {
+    if constexpr (sizeof(T) == 4) {
+      return *reinterpret_cast<const float4*>(p);
+    } else {
+      const uint2 x = *reinterpret_cast<const uint2*>(p);
+      float4 f;
+      tc::unpack2<T>(x.x, f.x, f.y);
+      tc::unpack2<T>(x.y, f.z, f.w);
+      return f;
+    }
+  }
+  return make_float4(to_f(p[0]), to_f(p[sd]), to_f(p[2 * sd]), to_f(p[3 * sd]));
+}
+
+template <typename T, int DP, int R, class M>
+__global__ void __launch_bounds__(kSimtThreads) cached_simt_few_kernel(const __grid_constant__ CachedP p) {
+  constexpr int kLanes = DP / 4 < 32 ? DP / 4 : 32;     // of a key
+  constexpr int kVecs = DP / 4 / kLanes;                // vectors of four channels of a lane
+  constexpr int kKeys = 32 / kLanes;                    // keys of a warp at a time: its groups of lanes
+  constexpr int kSteps = 16 / kKeys;                    // of the warp's 16 keys of a tile
+  constexpr int kAhead = kSteps < 8 / kVecs ? kSteps : 8 / kVecs;  // steps whose loads are in flight
+  __shared__ float4 sums[4][R][DP / 4];
+  __shared__ float2 stat[4][R];
+  __shared__ Item item;
+  __shared__ int smem_cum[kScanEntries + 1];
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, group = lane / kLanes, ch = (lane % kLanes) * 4;
+  const int* cum;
+  const Cut cut = begin_work<M, kSimtThreads>(p, smem_cum, cum);
+  pdl_launch_dependents();
+  Work work;
+  if (warp == 0) work.start<M>(p, cut, cum);
+  while (true) {
+    __syncthreads();
+    if (warp == 0) {
+      Item it;
+      work.next<M>(p, it);
+      if (lane == 0) item = it;
+    }
+    __syncthreads();
+    if (item.x.entry < 0) break;
+    const RowTile& t = item.t;
+    const Piece piece = item.x;
+    const int tiles = item.tiles, total = t.total, rows = t.rows, k_lo = t.k_lo, full_lo = t.full_lo, full_hi = t.full_hi;
+    float4 q[R][kVecs], o[R][kVecs];
+    float m[R], l[R];
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      m[r] = -CUDART_INF_F;
+      l[r] = 0.f;
+#pragma unroll
+      for (int v = 0; v < kVecs; ++v) {
+        const int d = ch + v * 128;
+        q[r][v] = o[r][v] = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (r < rows && d < p.D) {
+          const int i = (t.r0 + r) / p.G, h = piece.head * p.G + (t.r0 + r) % p.G;
+          q[r][v] = load4<T>(row_ptr<T>(p.q, t.b, h, i) + d * p.q.sd, p.q.sd, p.wide_q);
+        }
+      }
+    }
+    const int* table = p.table + t.b * p.table_sb;
+    const char* kb = reinterpret_cast<const char*>(p.k.p) + (piece.head * p.k.sh + ch * p.k.sd) * (long long)sizeof(T);
+    const char* vb = reinterpret_cast<const char*>(p.v.p) + (piece.head * p.v.sh + ch * p.v.sd) * (long long)sizeof(T);
+    for (int kt = piece.t0; kt < tiles; ++kt) {
+      const int k0 = k_lo + kt * kKeyTile + warp * 16;
+      if (k0 >= total) break;
+      const bool full = k0 >= full_lo && k0 + 16 <= full_hi;
+#pragma unroll 1
+      for (int s0 = 0; s0 < kSteps; s0 += kAhead) {
+        float4 kx[kAhead][kVecs], vx[kAhead][kVecs];
+        bool there[kAhead];
+        int key = k0 + s0 * kKeys + group, block = key / p.page, row = key - block * p.page;
+#pragma unroll
+        for (int s = 0; s < kAhead; ++s) {
+          const int page = key < total ? table[block] : -1;
+          there[s] = page >= 0 && page < p.num_pages;
+#pragma unroll
+          for (int v = 0; v < kVecs; ++v) {
+            kx[s][v] = vx[s][v] = make_float4(0.f, 0.f, 0.f, 0.f);
+            if (there[s] && ch + v * 128 < p.D) {
+              kx[s][v] = load4<T>(reinterpret_cast<const T*>(kb) + page * p.k.sb + row * p.k.sl + v * 128 * p.k.sd, p.k.sd, p.wide_kv);
+              vx[s][v] = load4<T>(reinterpret_cast<const T*>(vb) + page * p.v.sb + row * p.v.sl + v * 128 * p.v.sd, p.v.sd, p.wide_kv);
+            }
+          }
+          key += kKeys;
+          for (row += kKeys; row >= p.page; row -= p.page) ++block;
+        }
+        key = k0 + s0 * kKeys + group;
+#pragma unroll
+        for (int s = 0; s < kAhead; ++s, key += kKeys) {
+#pragma unroll
+          for (int r = 0; r < R; ++r) {
+            float x = 0.f;
+#pragma unroll
+            for (int v = 0; v < kVecs; ++v)
+              x = fmaf(q[r][v].x, kx[s][v].x, fmaf(q[r][v].y, kx[s][v].y, fmaf(q[r][v].z, kx[s][v].z, fmaf(q[r][v].w, kx[s][v].w, x))));
+#pragma unroll
+            for (int d = kLanes / 2; d > 0; d >>= 1) x += __shfl_xor_sync(0xffffffffu, x, d);
+            bool see = there[s] && r < rows;
+            if (see && !full) {
+              const int i = (t.r0 + r) / p.G;
+              see = sees<M>(p, t, i, token_position(p, t, i), key);
+            }
+            if (see) {  // the same in all lanes of the group; a hidden key may hold anything
+              x *= p.scale_log2;
+              const float top = fmaxf(m[r], x);
+              const float safe = top == -CUDART_INF_F ? 0.f : top;
+              if (top != m[r]) {
+                const float a = exp2f(m[r] - safe);
+                m[r] = top;
+                l[r] *= a;
+#pragma unroll
+                for (int v = 0; v < kVecs; ++v) o[r][v].x *= a, o[r][v].y *= a, o[r][v].z *= a, o[r][v].w *= a;
+              }
+              const float w = exp2f(x - safe);
+              l[r] += w;
+#pragma unroll
+              for (int v = 0; v < kVecs; ++v) {
+                o[r][v].x = fmaf(w, vx[s][v].x, o[r][v].x); o[r][v].y = fmaf(w, vx[s][v].y, o[r][v].y);
+                o[r][v].z = fmaf(w, vx[s][v].z, o[r][v].z); o[r][v].w = fmaf(w, vx[s][v].w, o[r][v].w);
+              }
+            }
+          }
+        }
+      }
+    }
+
+    // the groups' states, then the warps', become one
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+#pragma unroll
+      for (int d = kLanes; d < 32; d <<= 1) {
+        const float m2 = __shfl_xor_sync(0xffffffffu, m[r], d), l2 = __shfl_xor_sync(0xffffffffu, l[r], d), top = fmaxf(m[r], m2);
+        const float safe = top == -CUDART_INF_F ? 0.f : top, a = exp2f(m[r] - safe), b = exp2f(m2 - safe);
+        m[r] = top;
+        l[r] = l[r] * a + l2 * b;
+#pragma unroll
+        for (int v = 0; v < kVecs; ++v) {
+          o[r][v].x = o[r][v].x * a + __shfl_xor_sync(0xffffffffu, o[r][v].x, d) * b;
+          o[r][v].y = o[r][v].y * a + __shfl_xor_sync(0xffffffffu, o[r][v].y, d) * b;
+          o[r][v].z = o[r][v].z * a + __shfl_xor_sync(0xffffffffu, o[r][v].z, d) * b;
+          o[r][v].w = o[r][v].w * a + __shfl_xor_sync(0xffffffffu, o[r][v].w, d) * b;
+        }
+      }
+      if (group == 0) {
+#pragma unroll
+        for (int v = 0; v < kVecs; ++v) sums[warp][r][ch / 4 + v * 32] = o[r][v];
+      }
+      if (lane == 0) stat[warp][r] = make_float2(m[r], l[r]);
+    }
+    __syncthreads();
+    for (int idx = tid; idx < R * (DP / 4); idx += kSimtThreads) {
+      const int r = idx / (DP / 4), d = (idx % (DP / 4)) * 4;
+      if (d >= p.D || t.r0 + r >= p.N * p.G) continue;
+      float top = -CUDART_INF_F, sum = 0.f;
+#pragma unroll
+      for (int w = 0; w < 4; ++w) top = fmaxf(top, stat[w][r].x);
+      float4 z = make_float4(0.f, 0.f, 0.f, 0.f);
+      const float safe = top == -CUDART_INF_F ? 0.f : top;
+#pragma unroll
+      for (int w = 0; w < 4; ++w) {
+        const float a = exp2f(stat[w][r].x - safe);
+        const float4 y = sums[w][r][d / 4];
+        sum = fmaf(a, stat[w][r].y, sum);
+        z.x = fmaf(a, y.x, z.x); z.y = fmaf(a, y.y, z.y); z.z = fmaf(a, y.z, z.z); z.w = fmaf(a, y.w, z.w);
+      }
+      if (piece.slot < 0) {
+        const int i = (t.r0 + r) / p.G, h = piece.head * p.G + (t.r0 + r) % p.G;
+        const float inv = r < rows && sum != 0.f ? 1.f / sum : 0.f;
+        store4<T>(p, o_row<T>(p, t.b, h, i), d, z.x * inv, z.y * inv, z.z * inv, z.w * inv);
+        if (d == 0) store_lse(p, t.b, h, i, r < rows, top, sum);
+      } else {
+        const long long at = (long long)piece.slot * p.rows + r;
+        *reinterpret_cast<float4*>(p.part_o + at * p.D + d) = z;
+        if (d == 0) p.part_ml[at] = make_float2(top, sum);
       }
     }
   }

@@ -265,6 +265,7 @@ cached_tiles_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_consta
       const int row = grp * half + r;  // of the unit
       const int i = r < half && row < t.rows ? (t.r0 + row) / p.G : -1;
       const int pos = i >= 0 ? token_position(p, t, i) : 0;
+      const uint64_t near = first_ancestors(p, t.b, i);
       float m_used = -CUDART_INF_F, l = 0.f;
       bool ok = true;
       for (int j = 0; j < count; ++j, ++n) {
@@ -276,7 +277,7 @@ cached_tiles_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_consta
         const int lost = holes[s];
         const bool full = lost == 0 && k0 >= full_lo && k0 + kKeyTile <= full_hi;
         uint64_t vis = ~0ull;
-        if (!full) vis = visible_keys<M>(p, t, i, pos, k0, lost);
+        if (!full) vis = visible_keys<M>(p, t, i, pos, near, k0, lost);
         __syncwarp();
         uint32_t x[kKeyTile];
         tc::tmem_ld32(tS, x);
@@ -308,9 +309,10 @@ cached_tiles_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_consta
           ok = __all_sync(0xffffffffu, tc::mbar_wait(done, parity, guard, kStTilesSoftmax));
           if (!ok) break;
           tc::tc_fence_after();
-          const float a = m_cand == -CUDART_INF_F ? 1.f : tc::ex2(m_used - m_cand);
+          const bool moves = m_cand - m_used > 8.f;  // a row goes by itself: rows that do not exist hold anything
+          const float a = moves ? tc::ex2(m_used - m_cand) : 1.f;
           l *= a;
-          m_used = m_cand;
+          m_used = moves ? m_cand : m_used;
 #pragma unroll 1
           for (int d = 0; d < DP; d += 16) {
             uint32_t o[16];
