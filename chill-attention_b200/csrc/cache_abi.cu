@@ -58,16 +58,24 @@ static int cached_kernel(const chill_cached_args& a) {
 
 // Kernel, tiles, CTAs and workspace of a call, from the sizes that the host knows.
 struct Plan {
-  int kernel, rows, row_tiles, grid, min_share, tail_shares;
-  bool scan;  // prefix sums by a launch of their own
+  int kernel, rows, row_tiles, grid, pad, min_share, tail_shares;
+  bool scan;   // prefix sums by a launch of their own
+  bool whole;  // CTAs take whole units
   size_t queue, seams, cum, ml, o, bytes;
 };
+
+// What a CTA spends on a unit beside its tiles (Q, the parts of O, the next piece's start), in tiles.  Kernel for few rows: 0 / 2 / 4 tiles
+// 184.5 / 182.3 / 183.4 us (64 requests of up to 8192 tokens, one new each), 48.5 / 46.9 / 54.5 us (24 drafts each for 32 requests, window
+// of 1024).  Kernel for many rows: 0 / 3 / 5 / 7 / 10 tiles 110 / 96.3 / 92.4 / 90.1 / 92.9 us (64 drafts for 16 requests), 453 / 463 / 449 / 450 / 454
+// us (1024 new tokens for 4 requests).
+constexpr int kRowsPad = 2, kTilesPad = 6;
 
 static int make_plan(const chill_cached_args& a, Plan& c) {
   const int G = a.H / a.H_kv, sms = sm_count();
   const long long group_rows = (long long)a.N * G;
   c.kernel = cached_kernel(a);
   c.min_share = 2;
+  c.pad = 0;
   c.tail_shares = 0;
   if (c.kernel == CHILL_CACHED_CUDA_CORES) {
     c.rows = group_rows <= 4 ? 4 : (group_rows <= 8 ? 8 : 16);
@@ -77,20 +85,29 @@ static int make_plan(const chill_cached_args& a, Plan& c) {
     c.rows = group_rows <= 16 || a.D > 128 ? 16 : 32;
     c.grid = sms * (a.D <= 128 ? 2 : 1);
     c.tail_shares = 2 * c.grid;
+    c.pad = kRowsPad;
   } else {
     const int half = tile_rows(G);
     const bool two = a.D <= 128 && group_rows > half;
     c.rows = two ? 2 * half : half;
+    c.pad = kTilesPad;
     c.grid = sms * (a.D <= 128 ? 2 : 1) / (two ? 2 : 1);
   }
   const long long row_tiles = (group_rows + c.rows - 1) / c.rows, entries = (long long)a.B * row_tiles;
   const long long keys = (long long)a.table_width * a.page_size;
-  if (entries * a.H_kv * (keys / kKeyTile + 2) > 0x7fffffffll) return CHILL_E_TOO_LARGE;
+  if (entries * a.H_kv * (keys / kKeyTile + 8) > 0x7fffffffll) return CHILL_E_TOO_LARGE;
   c.row_tiles = (int)row_tiles;
   auto up = [](size_t x) { return (x + 255) / 256 * 256; };
+  // Tables of a few tiles: one launch and no sum, whatever the lengths (2 requests of 300 cached tokens, fp32: 6 tiles in one CTA each take
+  // 8 us, 3 CTAs and the kernel that joins them 16 us)
+  c.whole = keys <= 8 * kKeyTile;
+  if (c.whole) {
+    c.grid = entries * a.H_kv < c.grid ? (int)(entries * a.H_kv) : c.grid;
+    c.tail_shares = 0;
+  }
   // small shares only where the tables have room for so many keys
   if (entries * a.H_kv * (keys / kKeyTile + 1) < (long long)kTailFrom * c.grid) c.tail_shares = 0;
-  c.scan = entries > kScanEntries;
+  c.scan = !c.whole && entries > kScanEntries;
   const int shares = c.grid + c.tail_shares;
   c.queue = 0;
   c.seams = c.queue + 256;
@@ -145,7 +162,7 @@ static int cached_fwd(const chill_cached_args& a, cudaStream_t st) {
   p.wide_kv = wide(a.k_cache, a.k_cache_strides, es) && wide(a.v_cache, a.v_cache_strides, es);
   p.wide_q = wide(a.q, a.q_strides, es); p.wide_o = wide(a.o, a.o_strides, es);
   p.rows = c.rows; p.row_tiles = c.row_tiles; p.words = (a.N + 31) / 32;
-  p.min_share = c.min_share; p.tail_shares = c.tail_shares;
+  p.whole = c.whole; p.pad = c.pad; p.min_share = c.min_share; p.tail_shares = c.tail_shares;
   p.scale_log2 = a.sm_scale * kLog2e;
   p.margs = to_mask_args(a.mask, (long long)kMaxLen);
   p.q = to_ref(a.q, a.q_strides); p.k = to_ref(a.k_cache, a.k_cache_strides); p.v = to_ref(a.v_cache, a.v_cache_strides);
@@ -167,7 +184,7 @@ static int cached_fwd(const chill_cached_args& a, cudaStream_t st) {
   if (c.kernel == CHILL_CACHED_TILES && (rc = make_q_map(&maps[2], a, tile_rows(p.G) / p.G)) != CHILL_OK) return rc;
   int e = 0;
   CHILL_MASK_SWITCH(a.mask.id, (e = launch_typed<MaskT>(a.dtype, c.kernel, p, maps, c.grid, cum, st)))
-  if (e == 0) count_launches(1 + (c.scan || c.tail_shares > 0) + (c.grid > 1));
+  if (e == 0) count_launches(1 + (c.scan || c.tail_shares > 0) + (c.grid > 1 && !c.whole));
   return e == 0 ? CHILL_OK : cuda_fail((cudaError_t)e, "cached attention launch");
 }
 

@@ -40,6 +40,8 @@ struct CachedP {
   bool wide_kv;         // those of the caches too
   int rows, row_tiles;  // rows of a tile, tiles of N * G rows
   int words;            // 32-bit words of an ancestor row
+  bool whole;           // short tables: CTAs take whole units in turn, nothing is summed up, cut or joined
+  int pad;              // tiles that a unit counts for beside its own
   int min_share;        // tiles of keys of a share at least
   int tail_shares;      // small shares behind the large ones, at most (0: none)
   float scale_log2;     // softmax scale * log2(e)
@@ -107,10 +109,11 @@ __device__ __forceinline__ RowTile row_tile(const CachedP& p, int entry) {
   return t;
 }
 
-// Tiles a unit counts for in the shares: one at least, so that every unit has a CTA that writes its rows.
+// What a unit counts for in the shares: its tiles, one at least, so that every unit has a CTA that writes its rows; and ahead of
+// them `pad` for what a CTA spends on a unit beside its tiles.
 template <class M>
 __device__ __forceinline__ int unit_tiles(const CachedP& p, int entry) {
-  return imax(row_tile<M>(p, entry).n_tiles, 1);
+  return imax(row_tile<M>(p, entry).n_tiles, 1) + p.pad;
 }
 
 // Position of row r (token i) of a tile, and whether it sees key t (a place in the cache), t < total.
@@ -210,6 +213,11 @@ template <class M, int THREADS>
 __device__ __forceinline__ Cut begin_work(const CachedP& p, int* smem_cum, const int*& cum) {
   const int entries = p.B * p.row_tiles;
   cum = p.cum;
+  if (p.whole) {
+    Cut units{};
+    units.shares = entries * p.Hkv;
+    return units;
+  }
   if (cum == nullptr) {
     scan_units<M, THREADS>(p, entries, smem_cum);
     cum = smem_cum;
@@ -240,10 +248,14 @@ struct Work {
   const int* cum;
   int share, ahead;  // ahead: the small share that comes next (lane 0)
   int at, last, begin, tiles, entry, head;
+  int pieces;        // of the share so far
+  Seam seam;
   template <class M>
   __device__ __forceinline__ void open(const CachedP& p, int c) {
     share = c;
     if (c >= cut.shares) return;
+    pieces = 0;
+    seam.parts = 0;
     at = cut.begin(c);
     last = cut.begin(c + 1);
     int lo = 0, hi = p.B * p.row_tiles - 1;  // the entry whose tiles, of all kv heads, hold the first tile
@@ -262,49 +274,67 @@ struct Work {
     cut = c;
     cum = sums;
     ahead = 0;
-    open<M>(p, (int)blockIdx.x < cut.large ? (int)blockIdx.x : cut.shares);
+    share = (int)blockIdx.x;
+    if (!p.whole) open<M>(p, (int)blockIdx.x < cut.large ? (int)blockIdx.x : cut.shares);
+  }
+  // The share has been handed out: what of it is to be joined, and which one comes next.
+  __device__ __forceinline__ void close(const CachedP& p) {
+    if ((threadIdx.x & 31) == 0) {
+      p.seams[share] = seam;
+      if (cut.shares > cut.large) {
+        pdl_wait();
+        ahead = cut.large + atomicAdd(p.queue, 1);
+      }
+    }
+    __syncwarp();
   }
   template <class M>
   __device__ __forceinline__ bool next(const CachedP& p, Item& it) {
-    const int lane = threadIdx.x & 31;
-    if (share < cut.shares && at >= last) open<M>(p, cut.shares > cut.large ? __shfl_sync(0xffffffffu, ahead, 0) : cut.shares);
-    if (share >= cut.shares) {
-      it.x.entry = -1;
-      return false;
-    }
-    if (at >= begin + tiles) {  // the next unit
-      begin += tiles;
-      if (++head == p.Hkv) {
-        head = 0;
-        ++entry;
-        tiles = cum[entry + 1] - cum[entry];
-      }
-    }
     Piece& x = it.x;
-    x.entry = entry;
-    x.head = head;
-    x.t0 = at - begin;
-    x.t1 = imin(last - begin, tiles);
-    it.t = row_tile<M>(p, entry);
-    it.tiles = it.t.n_tiles == 0 ? 0 : x.t1;
-    const int share_begin = cut.begin(share);
-    const bool goes_on = x.t1 != tiles;
-    x.slot = x.t0 != 0 ? 2 * share : (goes_on ? 2 * share + (share_begin < begin ? 1 : 0) : -1);
-    at = begin + x.t1;
-    if (at >= last) {  // the share's last piece
-      if (lane == 0) {
-        Seam m;
-        m.parts = x.t0 == 0 && goes_on ? cut.of(begin + tiles - 1) - share + 1 : 0;
-        m.slot0 = x.slot;
-        m.b = it.t.b; m.head = head; m.r0 = it.t.r0; m.rows = it.t.rows;
-        p.seams[share] = m;
-        if (cut.shares > cut.large) {
-          pdl_wait();
-          ahead = cut.large + atomicAdd(p.queue, 1);
+    x.entry = -1;
+    if (p.whole) {  // share: a unit
+      if (share >= cut.shares) return false;
+      x.entry = share / p.Hkv;
+      x.head = share - x.entry * p.Hkv;
+      x.t0 = 0;
+      x.slot = -1;
+      it.t = row_tile<M>(p, x.entry);
+      x.t1 = it.tiles = it.t.n_tiles;
+      share += (int)gridDim.x;
+      return true;
+    }
+    while (true) {
+      if (share < cut.shares && at >= last) open<M>(p, cut.shares > cut.large ? __shfl_sync(0xffffffffu, ahead, 0) : cut.shares);
+      if (share >= cut.shares) return false;
+      if (at >= begin + tiles) {  // the next unit
+        begin += tiles;
+        if (++head == p.Hkv) {
+          head = 0;
+          ++entry;
+          tiles = cum[entry + 1] - cum[entry];
         }
       }
-      __syncwarp();
+      at = imax(at, imin(begin + p.pad, last));
+      if (at < last) break;
+      close(p);
     }
+    const int first = begin + p.pad, real = tiles - p.pad;  // the unit's tiles
+    x.entry = entry;
+    x.head = head;
+    x.t0 = at - first;
+    x.t1 = imin(last - first, real);
+    it.t = row_tile<M>(p, entry);
+    it.tiles = it.t.n_tiles == 0 ? 0 : x.t1;
+    const bool goes_on = x.t1 != real;
+    x.slot = x.t0 != 0 || goes_on ? 2 * share + (pieces > 0 ? 1 : 0) : -1;
+    if (x.t0 == 0 && goes_on) {
+      seam.parts = cut.of(first + real - 1) - share + 1;
+      seam.slot0 = x.slot;
+      seam.b = it.t.b; seam.head = head; seam.r0 = it.t.r0; seam.rows = it.t.rows;
+    }
+    ++pieces;
+    at = first + x.t1;
+    if (at >= last) close(p);
     return true;
   }
 };
@@ -415,93 +445,99 @@ __device__ __forceinline__ void store4(const CachedP& p, T* row, int ch, float a
 
 // ------------------------------------------------------------------------------------------------------- joining
 //   O = sum_i 2^(m_i - m) O_i / sum_i 2^(m_i - m) l_i, m = max_i m_i, over the parts of a unit in order.
-// Block (share, y): the unit that is cut at the share's end for the first time, if there is one.
-// Few rows: a lane has four channels (two times four beyond 128) of a row, eight parts' loads are in flight at a time.  With `many` parts a
-// block works on one row, every warp on every eighth part; otherwise a warp on one row.
+// Few rows: block (x, y) has the units that are cut at the ends of shares x, x + gridDim.x, ...; a lane has four channels (two times four
+// beyond 128) of a row, eight parts' loads are in flight at a time.  With `many` parts a block works on one row, every warp on every
+// eighth part; otherwise a warp on one row.
 constexpr int kJoinThreads = 256;
 template <typename T, int QUADS>
-__global__ void __launch_bounds__(kJoinThreads, QUADS == 1 ? 4 : 2) join_few_kernel(const __grid_constant__ CachedP p, int many) {
+__global__ void __launch_bounds__(kJoinThreads, QUADS == 1 ? 4 : 2) join_few_kernel(const __grid_constant__ CachedP p, int many, int shares) {
   __shared__ float4 sums[8][32 * QUADS];
   __shared__ float2 stat[8];
   pdl_wait();
-  const Seam j = p.seams[blockIdx.x];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, quads = p.D / 4;
-  const int r = many ? (int)blockIdx.y : (int)blockIdx.y * 8 + warp, row = j.r0 + r;
-  if (j.parts < 2 || (many != 0 && row >= p.N * p.G)) return;
-  const bool exists = r < p.rows && row < p.N * p.G, ok = exists && r < j.rows;
-  float m = -CUDART_INF_F, l = 0.f;
-  float4 o[QUADS];
+  const int mine = (int)blockIdx.x + lane * (int)gridDim.x;  // gridDim.x >= shares / 32
+  unsigned cut_here = __ballot_sync(0xffffffffu, mine < shares && p.seams[mine].parts > 1);
+  for (; cut_here != 0; cut_here &= cut_here - 1) {
+    const int share = (int)blockIdx.x + (__ffs(cut_here) - 1) * (int)gridDim.x;
+    const Seam j = p.seams[share];
+    const int r = many ? (int)blockIdx.y : (int)blockIdx.y * 8 + warp, row = j.r0 + r;
+    if (many != 0 && row >= p.N * p.G) continue;
+    const bool exists = r < p.rows && row < p.N * p.G, ok = exists && r < j.rows;
+    float m = -CUDART_INF_F, l = 0.f;
+    float4 o[QUADS];
 #pragma unroll
-  for (int v = 0; v < QUADS; ++v) o[v] = make_float4(0.f, 0.f, 0.f, 0.f);
-  const int step = many ? 8 : 1;
-  for (int k0 = many ? warp : 0; k0 < j.parts && ok; k0 += 8 * step) {
-    float2 ml[8];
-    float4 x[8][QUADS];
+    for (int v = 0; v < QUADS; ++v) o[v] = make_float4(0.f, 0.f, 0.f, 0.f);
+    const int step = many ? 8 : 1;
+    for (int k0 = many ? warp : 0; k0 < j.parts && ok; k0 += 8 * step) {
+      float2 ml[8];
+      float4 x[8][QUADS];
 #pragma unroll
-    for (int u = 0; u < 8; ++u) {
-      const int k = k0 + step * u;
-      ml[u] = make_float2(-CUDART_INF_F, 0.f);
+      for (int u = 0; u < 8; ++u) {
+        const int k = k0 + step * u;
+        ml[u] = make_float2(-CUDART_INF_F, 0.f);
 #pragma unroll
-      for (int v = 0; v < QUADS; ++v) x[u][v] = make_float4(0.f, 0.f, 0.f, 0.f);
-      if (k < j.parts) {
-        const long long at = (long long)(k == 0 ? j.slot0 : 2 * ((int)blockIdx.x + k)) * p.rows + r;
-        ml[u] = p.part_ml[at];
+        for (int v = 0; v < QUADS; ++v) x[u][v] = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (k < j.parts) {
+          const long long at = (long long)(k == 0 ? j.slot0 : 2 * (share + k)) * p.rows + r;
+          ml[u] = p.part_ml[at];
 #pragma unroll
-        for (int v = 0; v < QUADS; ++v)
-          if (lane + 32 * v < quads) x[u][v] = *reinterpret_cast<const float4*>(p.part_o + at * p.D + (lane + 32 * v) * 4);
+          for (int v = 0; v < QUADS; ++v)
+            if (lane + 32 * v < quads) x[u][v] = *reinterpret_cast<const float4*>(p.part_o + at * p.D + (lane + 32 * v) * 4);
+        }
       }
-    }
-    float top = m;
+      float top = m;
 #pragma unroll
-    for (int u = 0; u < 8; ++u) top = fmaxf(top, ml[u].x);
-    if (top == -CUDART_INF_F) continue;
-    const float a = exp2f(m - top);
-    m = top;
-    l *= a;
+      for (int u = 0; u < 8; ++u) top = fmaxf(top, ml[u].x);
+      if (top == -CUDART_INF_F) continue;
+      const float a = exp2f(m - top);
+      m = top;
+      l *= a;
 #pragma unroll
-    for (int v = 0; v < QUADS; ++v) o[v].x *= a, o[v].y *= a, o[v].z *= a, o[v].w *= a;
+      for (int v = 0; v < QUADS; ++v) o[v].x *= a, o[v].y *= a, o[v].z *= a, o[v].w *= a;
 #pragma unroll
-    for (int u = 0; u < 8; ++u) {
-      const float w = exp2f(ml[u].x - top);
-      l = fmaf(w, ml[u].y, l);
-#pragma unroll
-      for (int v = 0; v < QUADS; ++v) {
-        o[v].x = fmaf(w, x[u][v].x, o[v].x); o[v].y = fmaf(w, x[u][v].y, o[v].y);
-        o[v].z = fmaf(w, x[u][v].z, o[v].z); o[v].w = fmaf(w, x[u][v].w, o[v].w);
-      }
-    }
-  }
-  if (many) {  // the warps' sums become the first warp's
-#pragma unroll
-    for (int v = 0; v < QUADS; ++v) sums[warp][lane + 32 * v] = o[v], o[v] = make_float4(0.f, 0.f, 0.f, 0.f);
-    if (lane == 0) stat[warp] = make_float2(m, l);
-    __syncthreads();
-    if (warp != 0) return;
-    m = -CUDART_INF_F;
-    l = 0.f;
-#pragma unroll
-    for (int w = 0; w < 8; ++w) m = fmaxf(m, stat[w].x);
-    if (m != -CUDART_INF_F) {
-#pragma unroll
-      for (int w = 0; w < 8; ++w) {
-        const float a = exp2f(stat[w].x - m);
-        l = fmaf(a, stat[w].y, l);
+      for (int u = 0; u < 8; ++u) {
+        const float w = exp2f(ml[u].x - top);
+        l = fmaf(w, ml[u].y, l);
 #pragma unroll
         for (int v = 0; v < QUADS; ++v) {
-          const float4 y = sums[w][lane + 32 * v];
-          o[v].x = fmaf(a, y.x, o[v].x); o[v].y = fmaf(a, y.y, o[v].y); o[v].z = fmaf(a, y.z, o[v].z); o[v].w = fmaf(a, y.w, o[v].w);
+          o[v].x = fmaf(w, x[u][v].x, o[v].x); o[v].y = fmaf(w, x[u][v].y, o[v].y);
+          o[v].z = fmaf(w, x[u][v].z, o[v].z); o[v].w = fmaf(w, x[u][v].w, o[v].w);
         }
       }
     }
-  }
-  if (!exists) return;
-  const float inv = l != 0.f ? 1.f / l : 0.f;
-  const int i = row / p.G, h = j.head * p.G + row % p.G;
-  T* to = o_row<T>(p, j.b, h, i);
+    if (many) {  // the warps' sums become the first warp's
+      __syncthreads();  // those of the unit before have been read
 #pragma unroll
-  for (int v = 0; v < QUADS; ++v)
-    if (lane + 32 * v < quads) store4<T>(p, to, (lane + 32 * v) * 4, o[v].x * inv, o[v].y * inv, o[v].z * inv, o[v].w * inv);
-  if (lane == 0) store_lse(p, j.b, h, i, ok, m, l);
+      for (int v = 0; v < QUADS; ++v) sums[warp][lane + 32 * v] = o[v], o[v] = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (lane == 0) stat[warp] = make_float2(m, l);
+      __syncthreads();
+      if (warp != 0) continue;
+      m = -CUDART_INF_F;
+      l = 0.f;
+#pragma unroll
+      for (int w = 0; w < 8; ++w) m = fmaxf(m, stat[w].x);
+      if (m != -CUDART_INF_F) {
+#pragma unroll
+        for (int w = 0; w < 8; ++w) {
+          const float a = exp2f(stat[w].x - m);
+          l = fmaf(a, stat[w].y, l);
+#pragma unroll
+          for (int v = 0; v < QUADS; ++v) {
+            const float4 y = sums[w][lane + 32 * v];
+            o[v].x = fmaf(a, y.x, o[v].x); o[v].y = fmaf(a, y.y, o[v].y); o[v].z = fmaf(a, y.z, o[v].z); o[v].w = fmaf(a, y.w, o[v].w);
+          }
+        }
+      }
+    }
+    if (!exists) continue;
+    const float inv = l != 0.f ? 1.f / l : 0.f;
+    const int i = row / p.G, h = j.head * p.G + row % p.G;
+    T* to = o_row<T>(p, j.b, h, i);
+#pragma unroll
+    for (int v = 0; v < QUADS; ++v)
+      if (lane + 32 * v < quads) store4<T>(p, to, (lane + 32 * v) * 4, o[v].x * inv, o[v].y * inv, o[v].z * inv, o[v].w * inv);
+    if (lane == 0) store_lse(p, j.b, h, i, ok, m, l);
+  }
 }
 
 // Many rows: lanes over 32 rows (as the parts lie), a warp for eight channels at a time.

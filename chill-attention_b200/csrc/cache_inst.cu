@@ -36,8 +36,10 @@ static int launch(bool behind, void (*kern)(Args...), dim3 grid, int threads, in
 
 template <typename T, int DP>
 static int launch_simt(const CachedP& p, int grid, bool behind, cudaStream_t st) {
-  if (p.rows == 4) return launch(behind, cached_simt_few_kernel<T, DP, 4, InstMask>, dim3((unsigned)grid), kSimtThreads, 0, st, p);
-  if (p.rows == 8) return launch(behind, cached_simt_few_kernel<T, DP, 8, InstMask>, dim3((unsigned)grid), kSimtThreads, 0, st, p);
+  const dim3 blocks((unsigned)grid);
+  if (p.rows == 4 && p.whole) return launch(behind, cached_simt_few_kernel<T, DP, 4, 8, InstMask>, blocks, 256, 0, st, p);
+  if (p.rows == 4) return launch(behind, cached_simt_few_kernel<T, DP, 4, 4, InstMask>, blocks, 128, 0, st, p);
+  if (p.rows == 8) return launch(behind, cached_simt_few_kernel<T, DP, 8, 4, InstMask>, blocks, 128, 0, st, p);
   auto kern = cached_simt_kernel<T, DP, InstMask>;
   constexpr int smem = SimtSmem<DP>::kBytes;
   static_assert(smem <= 232448, "exceeds the 227 KB of shared memory a CTA can opt in to");
@@ -98,15 +100,15 @@ int launch_cached<InstMask, CHILL_INST_PART>(int kernel, const CachedP& p, const
     if (e != cudaSuccess) return (int)e;
   }
   const int e = launch_typed<InstType>(kernel, p, maps, grid, prepare, st);
-  if (e != 0 || grid == 1) return e;  // one share: nothing is cut
-  const unsigned shares = (unsigned)(grid + p.tail_shares);
-  if (kernel == CHILL_CACHED_TILES) return launch(true, join_many_kernel<InstType>, dim3(shares, (unsigned)((p.rows + 31) / 32)), kJoinThreads, 0, st, p);
+  if (e != 0 || grid == 1 || p.whole) return e;  // nothing is cut
+  const int shares = grid + p.tail_shares;
+  if (kernel == CHILL_CACHED_TILES) return launch(true, join_many_kernel<InstType>, dim3((unsigned)shares, (unsigned)((p.rows + 31) / 32)), kJoinThreads, 0, st, p);
   // units that are far fewer than shares have many parts each
   const long long rows = imin(p.rows, p.N * p.G), units = (long long)p.B * p.row_tiles * p.Hkv;
   const int many = 4 * units < shares;
-  const dim3 blocks(shares, (unsigned)(many ? rows : (rows + 7) / 8));
-  if (p.D > 128) return launch(true, join_few_kernel<InstType, 2>, blocks, kJoinThreads, 0, st, p, many);
-  return launch(true, join_few_kernel<InstType, 1>, blocks, kJoinThreads, 0, st, p, many);
+  const dim3 blocks((unsigned)imin(shares, (many ? 1 : 3) * sm_count()), (unsigned)(many ? rows : (rows + 7) / 8));
+  if (p.D > 128) return launch(true, join_few_kernel<InstType, 2>, blocks, kJoinThreads, 0, st, p, many, shares);
+  return launch(true, join_few_kernel<InstType, 1>, blocks, kJoinThreads, 0, st, p, many, shares);
 }
 
 }  // namespace cache

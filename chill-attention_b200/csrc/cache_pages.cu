@@ -22,10 +22,11 @@ namespace cache {
 //           before b; the j-th page taken for b is free[n_free - 1 - (off_b + j)], while there is one.
 // trim:     give_b = max(0, held_b - pages of lens[b]), r_b = sum of give before b, K = all; the j-th page given back by b goes to
 //           free[n_free + K - 1 - (r_b + j)]: the exact inverse, so pages that were reserved last come first again.
-// Both are one prefix sum over the requests and a few words for each: latency is all there is.  One launch of one cluster:
-// every CTA sums up the requests before its own ones (they are a few KB in L2), the cluster barrier separates these reads of
-// `held` and `n_free` from the writes to them, and after it each CTA works on its own share of the requests.
-constexpr int kPageThreads = 512;
+// Both are one prefix sum over the requests and a few words for each: latency is all there is.  One launch; its first cluster has
+// the pages: every CTA sums up the requests before its own ones (they are a few KB in L2), the cluster barrier separates these reads
+// of `held` and `n_free` from the writes to them, and after it each CTA works on its own share of the requests.  Further clusters
+// work out positions and ancestors, which do not depend on pages, beside it.
+constexpr int kPageThreads = 1024;
 constexpr int kPageCtas = 8;             // CTAs of the cluster (one where there is little to write)
 constexpr int kMaxRequests = 65535;      // check_pages
 constexpr int kOwnRequests = (kMaxRequests + kPageCtas - 1) / kPageCtas;
@@ -75,10 +76,42 @@ __device__ __forceinline__ void pages_of(const PagesP& p, int b, int& held, int&
   need = imin((cached + fresh + p.page - 1) / p.page, p.width);
 }
 
+// Positions and ancestors of the new tokens, token by token.  Parents come before their children, so the walk from a token up to its root
+// meets the words of its bit row from the last to the first and ends after at most i steps.
+__device__ __forceinline__ void place_tokens(const PagesP& p, long long first, long long step) {
+  const long long items = (long long)p.B * p.N;
+  for (long long at = first; at < items; at += step) {
+    const int b = (int)(at / p.N), i = (int)(at - (long long)b * p.N);
+    const int cached = clamp_len(p.lens[b]), fresh = imin(imax(p.new_lens[b], 0), p.N);
+    const bool real = i < fresh;
+    int depth = i;
+    if (p.parents != nullptr) {
+      const int* parent = p.parents + (long long)b * p.N;
+      unsigned* bits = reinterpret_cast<unsigned*>(p.ancestors) + at * p.words;
+      int w = p.words - 1;
+      unsigned word = 0;
+      depth = -1;
+      for (int node = real ? i : -1; node >= 0;) {
+        const int up = parent[node];
+        for (; w > (node >> 5); --w, word = 0) bits[w] = word;
+        word |= 1u << (node & 31);
+        ++depth;
+        node = up < node ? up : -1;
+      }
+      for (; w >= 0; --w, word = 0) bits[w] = word;
+    }
+    p.positions[at] = real ? cached + depth : 0;
+  }
+}
+
 template <bool kTrim>
-__global__ void __launch_bounds__(kPageThreads) pages_kernel(PagesP p) {
+__global__ void __launch_bounds__(kPageThreads) pages_kernel(PagesP p, int ctas) {
   __shared__ int before[kOwnRequests];  // off_b or r_b of this CTA's requests
-  const int ctas = (int)gridDim.x, rank = (int)blockIdx.x;
+  const int rank = (int)blockIdx.x;
+  if (!kTrim && rank >= ctas) {  // another cluster than the one with the pages
+    place_tokens(p, (long long)(rank - ctas) * kPageThreads + threadIdx.x, (long long)((int)gridDim.x - ctas) * kPageThreads);
+    return;
+  }
   const int per = (p.B + ctas - 1) / ctas, b0 = imin(rank * per, p.B), b1 = imin(b0 + per, p.B);
   const int n_free = imin(imax(*p.n_free, 0), p.num_pages);
   int sum = 0;
@@ -129,55 +162,38 @@ __global__ void __launch_bounds__(kPageThreads) pages_kernel(PagesP p) {
   if (kTrim) return;
 
   __syncthreads();  // the tables' new entries are written
-  // Slot, position and ancestors of every new token of this CTA's requests.  Parents come before their children, so the walk from
-  // a token up to its root meets the words of its bit row from the last to the first and ends after at most i steps.
   const int items = (b1 - b0) * p.N;
   for (int it = threadIdx.x; it < items; it += kPageThreads) {
     const int own = it / p.N, i = it - own * p.N, b = b0 + own;
     const int cached = clamp_len(p.lens[b]), fresh = imin(imax(p.new_lens[b], 0), p.N);
-    const bool real = i < fresh;
     const int t = cached + i, block = t / p.page;
     int slot = -1;
-    if (real && block < p.width) {
+    if (i < fresh && block < p.width) {
       const int page = p.table[b * p.table_sb + block];
       if (page >= 0 && page < p.num_pages) slot = page * p.page + (t - block * p.page);
     }
-    const long long at = (long long)b * p.N + i;
-    p.slots[at] = slot;
-    int depth = i;
-    if (p.parents != nullptr) {
-      const int* parent = p.parents + (long long)b * p.N;
-      unsigned* bits = reinterpret_cast<unsigned*>(p.ancestors) + at * p.words;
-      int w = p.words - 1;
-      unsigned word = 0;
-      depth = -1;
-      for (int node = real ? i : -1; node >= 0;) {
-        for (; w > (node >> 5); --w, word = 0) bits[w] = word;
-        word |= 1u << (node & 31);
-        ++depth;
-        const int up = parent[node];
-        node = up < node ? up : -1;
-      }
-      for (; w >= 0; --w, word = 0) bits[w] = word;
-    }
-    p.positions[at] = real ? cached + depth : 0;
+    p.slots[(long long)b * p.N + i] = slot;
   }
+  if ((int)gridDim.x == ctas) place_tokens(p, (long long)rank * kPageThreads + threadIdx.x, (long long)ctas * kPageThreads);
 }
 
 template <bool kTrim>
 static int launch_pages(const PagesP& p, cudaStream_t st) {
+  const long long tokens = (long long)p.B * p.N;
+  const int ctas = p.B <= 64 && tokens <= 2 * kPageThreads ? 1 : kPageCtas;
+  // tokens of large trees: a thread each, up to 16 clusters of them
+  const int more = kTrim || ctas == 1 ? 0 : (int)((tokens + kPageCtas * kPageThreads - 1) / (kPageCtas * kPageThreads) < 16 ? (tokens + kPageCtas * kPageThreads - 1) / (kPageCtas * kPageThreads) : 16);
   cudaLaunchConfig_t cfg{};
   cudaLaunchAttribute attr[1];
-  const bool small = p.B <= 64 && (long long)p.B * p.N <= 2 * kPageThreads;
-  cfg.gridDim = dim3(small ? 1 : kPageCtas);
+  cfg.gridDim = dim3((unsigned)(ctas + more * kPageCtas));
   cfg.blockDim = dim3(kPageThreads);
   cfg.stream = st;
   attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = cfg.gridDim.x;
+  attr[0].val.clusterDim.x = (unsigned)ctas;
   attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
   cfg.attrs = attr;
-  cfg.numAttrs = 1;
-  const cudaError_t e = cudaLaunchKernelEx(&cfg, pages_kernel<kTrim>, p);
+  cfg.numAttrs = ctas > 1 ? 1 : 0;
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, pages_kernel<kTrim>, p, ctas);
   if (e != cudaSuccess) return record_cuda_failure(e, "pages launch");
   count_launches(1);
   return CHILL_OK;
@@ -269,26 +285,29 @@ __global__ void __launch_bounds__(128) commit_kernel(RowsP p) {
       if (page < 0 || page >= p.num_pages) return nullptr;
       return base + page * st[0] + (t - block * p.page) * st[2];
     };
+    int from[kBatch];  // asked for before it is known how many count: one trip to memory less
+#pragma unroll
+    for (int u = 0; u < kBatch; ++u) from[u] = u < p.A ? path[u] : 0;
     for (int j0 = 0; j0 < take; j0 += kBatch) {
+      if (j0 != 0) {
+#pragma unroll
+        for (int u = 0; u < kBatch; ++u) from[u] = j0 + u < take ? path[j0 + u] : 0;
+      }
+      const char* src[kBatch];
+      char* dst[kBatch];
+#pragma unroll
+      for (int u = 0; u < kBatch; ++u) {  // in place already, or not a drafted token: no move
+        const bool moves = j0 + u < take && from[u] > j0 + u && from[u] < fresh;
+        src[u] = moves ? row_of(cached + from[u]) : nullptr;
+        dst[u] = moves ? row_of(cached + j0 + u) : nullptr;
+      }
       V x[kBatch];
-      bool moves[kBatch];
 #pragma unroll
-      for (int u = 0; u < kBatch; ++u) {
-        moves[u] = false;
-        if (j0 + u >= take) continue;
-        const int from = path[j0 + u];
-        if (from <= j0 + u || from >= fresh) continue;  // in place already, or not a drafted token
-        const char* src = row_of(cached + from);
-        if (src == nullptr) continue;
-        x[u] = *reinterpret_cast<const V*>(src);
-        moves[u] = true;
-      }
+      for (int u = 0; u < kBatch; ++u)
+        if (src[u] != nullptr) x[u] = *reinterpret_cast<const V*>(src[u]);
 #pragma unroll
-      for (int u = 0; u < kBatch; ++u) {
-        if (!moves[u]) continue;
-        char* dst = row_of(cached + j0 + u);
-        if (dst != nullptr) *reinterpret_cast<V*>(dst) = x[u];
-      }
+      for (int u = 0; u < kBatch; ++u)
+        if (src[u] != nullptr && dst[u] != nullptr) *reinterpret_cast<V*>(dst[u]) = x[u];
     }
   }
 }

@@ -3,7 +3,7 @@
 //
 // Up to 8 rows (simt_few): bound by memory, so nothing goes through shared memory.  D / 4 lanes (32 at most) share a key, a warp has
 // 16 keys of every tile of 64; a lane keeps four channels (eight at head dim 256) of Q and O of every row, reads those of K and V of
-// 8 keys at once, and gets the scores by butterflies over its lanes.  Every group of lanes has a maximum and a sum of its own: no warp,
+// four or eight steps at once, and gets the scores by butterflies over its lanes.  Every group of lanes has a maximum and a sum of its own: no warp,
 // and no group, waits for another before the end of a piece.
 //
 // More rows: a CTA of 128 threads works on 16 rows and 64 keys at a time, everything as fp32 in shared memory:
@@ -224,20 +224,21 @@ __device__ __forceinline__ float4 load4(const T* p, long long sd, bool wide) {
   return make_float4(to_f(p[0]), to_f(p[sd]), to_f(p[2 * sd]), to_f(p[3 * sd]));
 }
 
-template <typename T, int DP, int R, class M>
-__global__ void __launch_bounds__(kSimtThreads) cached_simt_few_kernel(const __grid_constant__ CachedP p) {
+// WARPS: four of them have a tile; with eight (units taken whole, where one CTA has all of a unit's tiles) two tiles are under way.
+template <typename T, int DP, int R, int WARPS, class M>
+__global__ void __launch_bounds__(WARPS * 32) cached_simt_few_kernel(const __grid_constant__ CachedP p) {
   constexpr int kLanes = DP / 4 < 32 ? DP / 4 : 32;     // of a key
   constexpr int kVecs = DP / 4 / kLanes;                // vectors of four channels of a lane
   constexpr int kKeys = 32 / kLanes;                    // keys of a warp at a time: its groups of lanes
   constexpr int kSteps = 16 / kKeys;                    // of the warp's 16 keys of a tile
-  constexpr int kAhead = kSteps < 8 / kVecs ? kSteps : 8 / kVecs;  // steps whose loads are in flight
-  __shared__ float4 sums[4][R][DP / 4];
-  __shared__ float2 stat[4][R];
+  constexpr int kAhead = kSteps < (R == 4 ? 8 / kVecs : 4) ? kSteps : (R == 4 ? 8 / kVecs : 4);  // steps whose loads are in flight
+  __shared__ float4 sums[WARPS][R][DP / 4];
+  __shared__ float2 stat[WARPS][R];
   __shared__ Item item;
   __shared__ int smem_cum[kScanEntries + 1];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, group = lane / kLanes, ch = (lane % kLanes) * 4;
   const int* cum;
-  const Cut cut = begin_work<M, kSimtThreads>(p, smem_cum, cum);
+  const Cut cut = begin_work<M, WARPS * 32>(p, smem_cum, cum);
   pdl_launch_dependents();
   Work work;
   if (warp == 0) work.start<M>(p, cut, cum);
@@ -270,25 +271,39 @@ __global__ void __launch_bounds__(kSimtThreads) cached_simt_few_kernel(const __g
       }
     }
     const int* table = p.table + t.b * p.table_sb;
+    const int my_token = lane < rows ? (t.r0 + lane) / p.G : -1, my_pos = lane < rows ? token_position(p, t, my_token) : 0;  // of row `lane`
+    const uint64_t my_near = first_ancestors(p, t.b, my_token);
     const char* kb = reinterpret_cast<const char*>(p.k.p) + (piece.head * p.k.sh + ch * p.k.sd) * (long long)sizeof(T);
     const char* vb = reinterpret_cast<const char*>(p.v.p) + (piece.head * p.v.sh + ch * p.v.sd) * (long long)sizeof(T);
-    for (int kt = piece.t0; kt < tiles; ++kt) {
-      const int k0 = k_lo + kt * kKeyTile + warp * 16;
+    const int quarter = (warp & 3) * 16;  // this warp's keys of a tile
+    for (int kt = piece.t0 + warp / 4; kt < tiles; kt += WARPS / 4) {
+      const int k0 = k_lo + kt * kKeyTile + quarter;
       if (k0 >= total) break;
-      const bool full = k0 >= full_lo && k0 + 16 <= full_hi;
+      unsigned seen = rows >= 32 ? 0xffffffffu : (1u << rows) - 1u, words[R];  // bit s * kKeys + g: the key of group g in step s
+      if (k0 < full_lo || k0 + 16 > full_hi) {
+        const uint64_t vis = visible_keys<M>(p, t, my_token, my_pos, my_near, k0 - quarter, 0);
+        __syncwarp();
+        seen = (unsigned)(vis >> quarter) & 0xffffu;  // row `lane`'s 16 keys of this warp
+#pragma unroll
+        for (int r = 0; r < R; ++r) words[r] = __shfl_sync(0xffffffffu, seen, r);
+      } else {
+#pragma unroll
+        for (int r = 0; r < R; ++r) words[r] = (seen >> r) & 1u ? 0xffffu : 0u;
+      }
 #pragma unroll 1
       for (int s0 = 0; s0 < kSteps; s0 += kAhead) {
         float4 kx[kAhead][kVecs], vx[kAhead][kVecs];
-        bool there[kAhead];
+        unsigned there = 0;
         int key = k0 + s0 * kKeys + group, block = key / p.page, row = key - block * p.page;
 #pragma unroll
         for (int s = 0; s < kAhead; ++s) {
           const int page = key < total ? table[block] : -1;
-          there[s] = page >= 0 && page < p.num_pages;
+          const bool is = page >= 0 && page < p.num_pages;
+          there |= (unsigned)is << s;
 #pragma unroll
           for (int v = 0; v < kVecs; ++v) {
             kx[s][v] = vx[s][v] = make_float4(0.f, 0.f, 0.f, 0.f);
-            if (there[s] && ch + v * 128 < p.D) {
+            if (is && ch + v * 128 < p.D) {
               kx[s][v] = load4<T>(reinterpret_cast<const T*>(kb) + page * p.k.sb + row * p.k.sl + v * 128 * p.k.sd, p.k.sd, p.wide_kv);
               vx[s][v] = load4<T>(reinterpret_cast<const T*>(vb) + page * p.v.sb + row * p.v.sl + v * 128 * p.v.sd, p.v.sd, p.wide_kv);
             }
@@ -296,34 +311,37 @@ __global__ void __launch_bounds__(kSimtThreads) cached_simt_few_kernel(const __g
           key += kKeys;
           for (row += kKeys; row >= p.page; row -= p.page) ++block;
         }
-        key = k0 + s0 * kKeys + group;
 #pragma unroll
-        for (int s = 0; s < kAhead; ++s, key += kKeys) {
+        for (int r = 0; r < R; ++r) {
+          float x[kAhead], top = m[r];
 #pragma unroll
-          for (int r = 0; r < R; ++r) {
-            float x = 0.f;
+          for (int s = 0; s < kAhead; ++s) {
+            x[s] = 0.f;
 #pragma unroll
             for (int v = 0; v < kVecs; ++v)
-              x = fmaf(q[r][v].x, kx[s][v].x, fmaf(q[r][v].y, kx[s][v].y, fmaf(q[r][v].z, kx[s][v].z, fmaf(q[r][v].w, kx[s][v].w, x))));
+              x[s] = fmaf(q[r][v].x, kx[s][v].x, fmaf(q[r][v].y, kx[s][v].y, fmaf(q[r][v].z, kx[s][v].z, fmaf(q[r][v].w, kx[s][v].w, x[s]))));
+          }
 #pragma unroll
-            for (int d = kLanes / 2; d > 0; d >>= 1) x += __shfl_xor_sync(0xffffffffu, x, d);
-            bool see = there[s] && r < rows;
-            if (see && !full) {
-              const int i = (t.r0 + r) / p.G;
-              see = sees<M>(p, t, i, token_position(p, t, i), key);
-            }
-            if (see) {  // the same in all lanes of the group; a hidden key may hold anything
-              x *= p.scale_log2;
-              const float top = fmaxf(m[r], x);
-              const float safe = top == -CUDART_INF_F ? 0.f : top;
-              if (top != m[r]) {
-                const float a = exp2f(m[r] - safe);
-                m[r] = top;
-                l[r] *= a;
+          for (int d = kLanes / 2; d > 0; d >>= 1)
 #pragma unroll
-                for (int v = 0; v < kVecs; ++v) o[r][v].x *= a, o[r][v].y *= a, o[r][v].z *= a, o[r][v].w *= a;
-              }
-              const float w = exp2f(x - safe);
+            for (int s = 0; s < kAhead; ++s) x[s] += __shfl_xor_sync(0xffffffffu, x[s], d);
+          unsigned see = 0;  // the same in all lanes of a group
+#pragma unroll
+          for (int s = 0; s < kAhead; ++s) {
+            const bool is = ((there >> s) & (words[r] >> ((s0 + s) * kKeys + group)) & 1u) != 0;
+            see |= (unsigned)is << s;
+            x[s] = is ? x[s] * p.scale_log2 : -CUDART_INF_F;
+            top = fmaxf(top, x[s]);
+          }
+          const float safe = top == -CUDART_INF_F ? 0.f : top, a = tc::ex2(m[r] - safe);
+          m[r] = top;
+          l[r] *= a;
+#pragma unroll
+          for (int v = 0; v < kVecs; ++v) o[r][v].x *= a, o[r][v].y *= a, o[r][v].z *= a, o[r][v].w *= a;
+#pragma unroll
+          for (int s = 0; s < kAhead; ++s) {
+            if ((see >> s) & 1u) {  // a hidden key may hold anything
+              const float w = tc::ex2(x[s] - safe);
               l[r] += w;
 #pragma unroll
               for (int v = 0; v < kVecs; ++v) {
@@ -360,16 +378,16 @@ __global__ void __launch_bounds__(kSimtThreads) cached_simt_few_kernel(const __g
       if (lane == 0) stat[warp][r] = make_float2(m[r], l[r]);
     }
     __syncthreads();
-    for (int idx = tid; idx < R * (DP / 4); idx += kSimtThreads) {
+    for (int idx = tid; idx < R * (DP / 4); idx += WARPS * 32) {
       const int r = idx / (DP / 4), d = (idx % (DP / 4)) * 4;
       if (d >= p.D || t.r0 + r >= p.N * p.G) continue;
       float top = -CUDART_INF_F, sum = 0.f;
 #pragma unroll
-      for (int w = 0; w < 4; ++w) top = fmaxf(top, stat[w][r].x);
+      for (int w = 0; w < WARPS; ++w) top = fmaxf(top, stat[w][r].x);
       float4 z = make_float4(0.f, 0.f, 0.f, 0.f);
       const float safe = top == -CUDART_INF_F ? 0.f : top;
 #pragma unroll
-      for (int w = 0; w < 4; ++w) {
+      for (int w = 0; w < WARPS; ++w) {
         const float a = exp2f(stat[w][r].x - safe);
         const float4 y = sums[w][r][d / 4];
         sum = fmaf(a, stat[w][r].y, sum);

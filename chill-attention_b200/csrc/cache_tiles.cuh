@@ -18,6 +18,8 @@
 #include "cache_repair.cuh"
 #include "tc_common.cuh"
 
+#include <type_traits>
+
 namespace chill {
 namespace cache {
 
@@ -58,6 +60,30 @@ __device__ __forceinline__ void tma_load_5d(uint32_t dst, const CUtensorMap* map
                : "memory");
 }
 
+// 2^x of a pair on the FMA pipe: x = n + f, n = round(x) by adding 1.5 * 2^23, f in [-1/2, 1/2]; 2^f by a polynomial of degree 5 (minimax
+// of the relative error by Remez' algorithm: 7.5e-8, evaluated in fp32 2.3e-7, as much as ex2.approx is off), n goes into the exponent.
+__device__ __forceinline__ uint64_t ex2_fma(uint64_t x2) {
+  float x0, x1;
+  tc::upk2(x2, x0, x1);
+  x2 = tc::pk2(fmaxf(x0, -126.f), fmaxf(x1, -126.f));  // below: 2^-126 beside a row's largest weight of 2^-8 or more; not for hidden keys, which need a 0
+  const uint64_t n2 = tc::fadd2(x2, tc::pk2(12582912.f, 12582912.f));
+  const uint64_t f2 = tc::ffma2(tc::fadd2(n2, tc::pk2(-12582912.f, -12582912.f)), tc::pk2(-1.f, -1.f), x2);
+  uint64_t p2 = tc::pk2(1.3276472e-3f, 1.3276472e-3f);
+  p2 = tc::ffma2(p2, f2, tc::pk2(9.6755413e-3f, 9.6755413e-3f));
+  p2 = tc::ffma2(p2, f2, tc::pk2(5.5507133e-2f, 5.5507133e-2f));
+  p2 = tc::ffma2(p2, f2, tc::pk2(0.24022120f, 0.24022120f));
+  p2 = tc::ffma2(p2, f2, tc::pk2(0.69314697f, 0.69314697f));
+  p2 = tc::ffma2(p2, f2, tc::pk2(1.0000001f, 1.0000001f));
+  float a, b, na, nb;
+  tc::upk2(p2, a, b);
+  tc::upk2(n2, na, nb);
+  return tc::pk2u(__float_as_uint(a) + (__float_as_uint(na) << 23), __float_as_uint(b) + (__float_as_uint(nb) << 23));
+}
+// Of every sixteen pairs of weights, half as many are worked out so.  The two groups' softmax warps on a scheduler ask its MUFU for 1024
+// of the 2100 clocks of a step, mostly at the same time: 1024 new tokens for each of 4 requests, 507 us with none, 480 with an eighth of
+// the pairs, 467 with a quarter, 512 with half of them.
+constexpr int kFmaShare = 8;
+
 enum : int { kStTilesProducer = 711, kStTilesMma = 712, kStTilesSoftmax = 713, kStTilesEpilogue = 714 };
 
 template <typename T, int DP, int NQ, class M>
@@ -65,7 +91,7 @@ __global__ void __launch_bounds__(TilesShape<DP, NQ>::kThreads, TilesShape<DP, N
 cached_tiles_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
                     const __grid_constant__ CachedP p) {
   using S = TilesShape<DP, NQ>;
-  constexpr int kStages = S::kStages, NSB = 2, kProducer = 4 * NQ;
+  constexpr int kStages = S::kStages, kProducer = 4 * NQ;
   extern __shared__ uint8_t smem_raw[];
   const uint32_t base = (tc::smem_u32(smem_raw) + 1023u) & ~1023u;
   uint8_t* gen = smem_raw + (base - tc::smem_u32(smem_raw));
@@ -249,7 +275,7 @@ cached_tiles_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_consta
     const int grp = NQ == 1 ? 0 : warp >> 2, r = (warp & 3) * 32 + lane;  // row of the group's tile == TMEM lane
     const uint32_t lane_sel = ((uint32_t)((warp & 3) * 32) << 16) + grp * S::kGroupCols;
     const uint32_t s_full = group_bars + 64 * grp, p_full = s_full + 16, o_full = s_full + 48, o_empty = s_full + 56;
-    const uint32_t tO = tmem + NSB * kKeyTile + lane_sel;
+    const uint32_t tO = tmem + 2 * kKeyTile + lane_sel;
     const float c = p.scale_log2;
     const int half = p.rows / NQ;
     int n = 0, pieces = 0;
@@ -269,9 +295,9 @@ cached_tiles_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_consta
       float m_used = -CUDART_INF_F, l = 0.f;
       bool ok = true;
       for (int j = 0; j < count; ++j, ++n) {
-        const int s = n % kStages, sb = n % NSB, k0 = k_lo + (t0 + j) * kKeyTile;
+        const int s = n % kStages, sb = n & 1, k0 = k_lo + (t0 + j) * kKeyTile;
         const uint32_t tS = tmem + sb * kKeyTile + lane_sel;
-        ok = __all_sync(0xffffffffu, tc::mbar_wait(s_full + 8 * sb, (uint32_t)(n / NSB) & 1u, guard, kStTilesSoftmax));
+        ok = __all_sync(0xffffffffu, tc::mbar_wait(s_full + 8 * sb, (uint32_t)(n >> 1) & 1u, guard, kStTilesSoftmax));
         if (!ok) break;
         tc::tc_fence_after();
         const int lost = holes[s];
@@ -326,18 +352,23 @@ cached_tiles_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_consta
         const float safe = m_used == -CUDART_INF_F ? 0.f : m_used;
         const uint64_t c2 = tc::pk2(c, c), nm2 = tc::pk2(-safe, -safe);
         uint64_t l0 = 0ull, l1 = 0ull;
+        auto weights = [&](auto fma) {
 #pragma unroll
-        for (int e = 0; e < kKeyTile / 2; e += 2) {
-          const uint64_t e0 = tc::ex2_pair(tc::ffma2(tc::pk2u(x[2 * e], x[2 * e + 1]), c2, nm2), false);
-          const uint64_t e1 = tc::ex2_pair(tc::ffma2(tc::pk2u(x[2 * e + 2], x[2 * e + 3]), c2, nm2), false);
-          l0 = tc::fadd2(l0, e0);
-          l1 = tc::fadd2(l1, e1);
-          float p0, p1, p2, p3;
-          tc::upk2(e0, p0, p1);
-          tc::upk2(e1, p2, p3);
-          x[e] = tc::pack2<T>(p0, p1);  // a slot that has been used already (e <= 2 e)
-          x[e + 1] = tc::pack2<T>(p2, p3);
-        }
+          for (int e = 0; e < kKeyTile / 2; e += 2) {
+            const uint64_t a0 = tc::ffma2(tc::pk2u(x[2 * e], x[2 * e + 1]), c2, nm2), a1 = tc::ffma2(tc::pk2u(x[2 * e + 2], x[2 * e + 3]), c2, nm2);
+            const uint64_t e0 = decltype(fma)::value && e % 16 < kFmaShare ? ex2_fma(a0) : tc::ex2_pair(a0, false);
+            const uint64_t e1 = tc::ex2_pair(a1, false);
+            l0 = tc::fadd2(l0, e0);
+            l1 = tc::fadd2(l1, e1);
+            float p0, p1, p2, p3;
+            tc::upk2(e0, p0, p1);
+            tc::upk2(e1, p2, p3);
+            x[e] = tc::pack2<T>(p0, p1);  // a slot that has been used already (e <= 2 e)
+            x[e + 1] = tc::pack2<T>(p2, p3);
+          }
+        };
+        if (full) weights(std::true_type{});
+        else weights(std::false_type{});
         float a0, a1, a2, a3;
         tc::upk2(l0, a0, a1);
         tc::upk2(l1, a2, a3);
