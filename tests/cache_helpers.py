@@ -16,13 +16,14 @@ def masks():
 class Problem:
     """CPU tensors of one call; .cuda() gives the arguments of the public functions."""
 
-    def __init__(self, dtype, H, Hkv, D, lens, new, N, page, tree=False, seed=0, holes=(), spare=2, sharp=1.0):
+    def __init__(self, dtype, H, Hkv, D, lens, new, N, page, tree=False, seed=0, holes=(), spare=2, sharp=1.0, room=0):
         g = torch.Generator().manual_seed(seed)
         self.dtype, self.page, self.N, self.chain = dtype, page, N, not tree
         B = len(lens)
         self.lens, self.new = list(lens), list(new)
         blocks = [-(-(c + min(max(n, 0), N)) // page) for c, n in zip(lens, new)]
         pages, width = sum(blocks) + spare, max(max(blocks), 1) + 1
+        width = max(width, -(-room // page))  # room: keys the table has room for
         order = torch.randperm(pages, generator=g).tolist()
         self.table = torch.full((B, width), -1, dtype=torch.int32)
         at = 0

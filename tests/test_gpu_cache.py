@@ -78,21 +78,27 @@ DTYPES = [torch.float32, torch.float16, torch.bfloat16]
 RAGGED = [300, 0, 1, 64, 63, 129, 17, 200]
 
 
+# Keys the tables have room for: up to 512 every CTA takes whole (request, kv head) units; beyond that the work is cut into shares.
+ROOMS = {"whole": 0, "shares": 600}
+
+
+@pytest.mark.parametrize("room", list(ROOMS))
 @pytest.mark.parametrize("kind", ["one", "chain", "tree"])
 @pytest.mark.parametrize("mask", list(masks()))
 @pytest.mark.parametrize("dtype", DTYPES, ids=["fp32", "fp16", "bf16"])
-def test_masks_and_ragged_lengths(dtype, mask, kind):
+def test_masks_and_ragged_lengths(dtype, mask, kind, room):
     N = 1 if kind == "one" else 9
     new = [N, N, 0, max(N - 2, 1), N, 1, N, 0]
-    p = Problem(dtype, 6, 2, 64, RAGGED, new, N, 16, tree=kind == "tree", seed=len(mask) + N)
+    p = Problem(dtype, 6, 2, 64, RAGGED, new, N, 16, tree=kind == "tree", seed=len(mask) + N, room=ROOMS[room])
     run_and_check(p, masks()[mask])
 
 
 @pytest.mark.parametrize("D", [16, 32, 64, 128, 256])
 @pytest.mark.parametrize("group", [1, 3, 8])
+@pytest.mark.parametrize("room", list(ROOMS))
 @pytest.mark.parametrize("dtype", DTYPES, ids=["fp32", "fp16", "bf16"])
-def test_head_dims_and_groups(dtype, group, D):
-    p = Problem(dtype, 2 * group, 2, D, [70, 3, 128, 0], [5, 2, 5, 5], 5, 32, tree=group != 3, seed=D + group)
+def test_head_dims_and_groups(dtype, room, group, D):
+    p = Problem(dtype, 2 * group, 2, D, [70, 3, 128, 0], [5, 2, 5, 5], 5, 32, tree=group != 3, seed=D + group, room=ROOMS[room])
     run_and_check(p, masks()["causal"])
 
 
@@ -100,23 +106,49 @@ def test_head_dims_and_groups(dtype, group, D):
 @pytest.mark.parametrize("dtype", DTYPES, ids=["fp32", "fp16", "bf16"])
 def test_strides(dtype, layout):
     for N, D in ((3, 64), (40, 128)):
-        p = Problem(dtype, 8, 2, D, [90, 31, 64], [N, N - 1, N], N, 16, tree=True, seed=D)
+        p = Problem(dtype, 8, 2, D, [90, 31, 64], [N, N - 1, N], N, 16, tree=True, seed=D, room=600 if N == 3 else 0)
         run_and_check(p, masks()["window"], layout)
+        if D == 128:
+            run_and_check(Problem(dtype, 8, 2, D, [90, 31, 64], [N, N - 1, N], N, 16, tree=True, seed=D, room=600), masks()["window"], layout)
 
 
 @pytest.mark.parametrize("page", [1, 5, 8, 16, 48, 64, 100, 128, 512])
 def test_page_sizes(page):
     for N, dtype in ((2, torch.bfloat16), (33, torch.float16)):
-        p = Problem(dtype, 4, 2, 64, [257, 40, 0, 99], [N, 1, N, N], N, page, tree=True, seed=page)
-        run_and_check(p, masks()["causal"])
+        for room in ROOMS.values():
+            p = Problem(dtype, 4, 2, 64, [257, 40, 0, 99], [N, 1, N, N], N, page, tree=True, seed=page, room=room)
+            run_and_check(p, masks()["causal"])
 
 
 @pytest.mark.parametrize("N", [15, 16, 17, 31, 32, 33, 64, 65, 130])
 @pytest.mark.parametrize("kind", ["chain", "tree"])
 def test_row_tiles(kind, N):
-    for D, dtype in ((64, torch.bfloat16), (128, torch.float16)):
-        p = Problem(dtype, 4, 1, D, [150, 10, 64], [N, N - 3, 1], N, 64, tree=kind == "tree", seed=N)
+    for D, dtype, room in ((64, torch.bfloat16, 600), (128, torch.float16, 600), (256, torch.bfloat16, 600), (128, torch.bfloat16, 0)):
+        p = Problem(dtype, 4, 1, D, [150, 10, 64], [N, N - 3, 1], N, 64, tree=kind == "tree", seed=N, room=room)
         run_and_check(p, masks()["window_ahead" if N % 2 else "causal"])
+
+
+@pytest.mark.parametrize("G", [5, 7, 48, 100, 128, 130])
+def test_groups_that_do_not_divide_a_tile(G):
+    """Tiles of rows hold whole tokens: 125, 126, 96, 100 and 128 of 128 rows; a token with more goes elsewhere."""
+    from chill_attention import _cache_abi
+
+    p = Problem(torch.bfloat16, 2 * G, 2, 64, [150, 70], [9, 6], 9, 16, tree=True, seed=G, room=600)
+    assert kernel_of(p) == (_cache_abi.CACHED_ROWS if G == 130 else _cache_abi.CACHED_TILES)
+    run_and_check(p, masks()["causal"])
+
+
+def test_which_kernel_serves_a_call():
+    from chill_attention import _cabi, _cache_abi
+
+    def ask(dtype=torch.bfloat16, H=4, Hkv=2, D=64, N=1, page=16, flags=0):
+        return kernel_of(Problem(dtype, H, Hkv, D, [10], [N], N, page), flags)
+
+    for D in (16, 32, 64, 128):
+        assert ask(D=D) == ask(D=D, N=16) == _cache_abi.CACHED_ROWS and ask(D=D, N=17) == _cache_abi.CACHED_TILES  # 32 rows at most
+    assert ask(D=256, N=8) == _cache_abi.CACHED_ROWS and ask(D=256, N=9) == _cache_abi.CACHED_TILES              # 16
+    assert ask(dtype=torch.float32) == ask(page=12) == ask(page=1) == ask(flags=_cabi.FLAG_FORCE_GENERIC) == _cache_abi.CACHED_CUDA_CORES
+    assert ask(page=8) == ask(page=24) == _cache_abi.CACHED_ROWS
 
 
 @pytest.mark.parametrize("dtype", DTYPES, ids=["fp32", "fp16", "bf16"])
@@ -132,19 +164,41 @@ def test_sharp_scores_over_many_parts():
     run_and_check(p, masks()["causal"])
 
 
-def test_many_short_requests():
+@pytest.mark.parametrize("room", list(ROOMS))
+def test_many_short_requests(room):
     """More (request, tile of rows) pairs than every CTA sums up by itself."""
     B = 1100
-    p = Problem(torch.bfloat16, 2, 1, 64, [(7 * b) % 40 for b in range(B)], [(b % 3) for b in range(B)], 2, 16, seed=1)
+    p = Problem(torch.bfloat16, 2, 1, 64, [(7 * b) % 40 for b in range(B)], [(b % 3) for b in range(B)], 2, 16, seed=1, room=ROOMS[room])
     run_and_check(p, masks()["causal"])
+
+
+@pytest.mark.parametrize("dtype,N,D", [(torch.bfloat16, 1, 64), (torch.float16, 5, 64), (torch.float32, 1, 16)], ids=str)
+def test_small_shares_for_whoever_is_done_first(dtype, N, D):
+    """Enough keys (24 tiles of 64 for each CTA) that the last sixth of them is handed out as the CTAs get done."""
+    lens = [57000, 120, 61000, 40000, 58000, 90]
+    heads = 6 if dtype == torch.float32 else 4
+    p = Problem(dtype, heads, heads, D, lens, [N] * 6, N, 64, tree=N > 1, seed=D, room=62000)
+    o, lse = run_and_check(p, masks()["causal"])
+    (again, _), _ = attend(p, masks()["causal"])
+    assert torch.equal(o, again)  # whoever had them
+    short = Problem(dtype, 4, 4, D, [300, 20], [N] * 2, N, 64, seed=D, room=400000)  # room for as many, few there
+    run_and_check(short, masks()["causal"])
+
+
+@pytest.mark.parametrize("name", ["full", "causal"])
+def test_a_batch_with_mixed_steps(name):
+    """Prompts, single tokens and idle requests in one call: tiles of rows that hold no token."""
+    p = Problem(torch.float16, 8, 2, 128, [0, 700, 30, 0, 256], [150, 1, 0, 3, 64], 150, 16, seed=8)
+    run_and_check(p, masks()[name])
 
 
 @pytest.mark.parametrize("N", [2, 40])
 @pytest.mark.parametrize("dtype", DTYPES, ids=["fp32", "fp16", "bf16"])
 def test_keys_without_a_page_are_not_there(dtype, N):
     holes = [(0, 0, -1), (0, 3, 10 ** 6), (1, 0, -1), (1, 1, -7), (1, 2, -1), (1, 3, 2 ** 30), (1, 4, -1), (2, 2, -2 ** 31)]
-    p = Problem(dtype, 4, 2, 64, [130, 30, 80], [N, N, N], N, 16, tree=True, seed=9, holes=holes)
-    o, lse = run_and_check(p, masks()["causal"])
+    for room in ROOMS.values():
+        p = Problem(dtype, 4, 2, 64, [130, 30, 80], [N, N, N], N, 16, tree=True, seed=9, holes=holes, room=room)
+        o, lse = run_and_check(p, masks()["causal"])
     q = Problem(dtype, 4, 2, 64, [130, 30], [N, N], N, 16, seed=9, holes=[(b, j, -1) for b in (0, 1) for j in range((130 if b == 0 else 30) // 16 + 1 + N // 16)])
     o, lse = run_and_check(q, masks()["causal"])
     if N == 2:
