@@ -83,7 +83,7 @@ static int make_plan(const chill_cached_args& a, Plan& c) {
     if (c.rows < 16) c.tail_shares = c.grid;
   } else if (c.kernel == CHILL_CACHED_ROWS) {
     c.rows = group_rows <= 16 || a.D > 128 ? 16 : 32;
-    c.grid = sms * (a.D <= 128 ? 2 : 1);
+    c.grid = sms * rows_ctas(a.D, c.rows);
     c.tail_shares = 2 * c.grid;
     c.pad = kRowsPad;
   } else {

@@ -3,16 +3,17 @@
 // go through mma.sync, whose tile is 16 rows (the smallest tcgen05 tile is 64, most of it would be padding, and its softmax would
 // be one row a thread), and the kernel is about keeping copies in flight.
 //
-// A CTA (two on an SM up to head dim 128) is one producer warp and four consumer warps:
+// A CTA (several on an SM, see rows_ctas) is one producer warp and four consumer warps:
 //   producer   takes shares and hands their pieces to the consumers, two of them with their Q (a bulk copy for each row) ahead; a
 //              tile is 64 keys of K and of V, boxes of `box` rows of one page and 64 channels (128-byte rows, 128B swizzle), a lane
-//              for each box, into a ring of kStages tiles (64 to 192 KB a CTA).  It runs ahead into the next piece and the next share.
+//              for each box, into a ring of kStages tiles (48 to 192 KB a CTA).  It runs ahead into the next piece and the next share.
 //   consumers  warp w takes keys 16 w .. 16 w + 15 of every tile for all rows, with a running maximum, sum and O of its own
 //              in registers: no warp waits for another before the end of a piece.  S = Q K^T (B fragments of K by ldmatrix), softmax
 //              on the accumulator's layout, P is the A fragment of O += P V as it stands (V by ldmatrix.trans).
 //   At the end of a piece the four states are joined through shared memory, 32 channels at a time.
-// P is rounded to the inputs' 16 bits for the second product (one rounding, half a step of the type relative to each weight, as
-// the other 16-bit kernels do; sums are of the unrounded weights, in fp32).
+// For the second product the weights are 16 bits wide like V.  With 16 rows each is given as two such numbers, the rounded one and the
+// rounded rest: twice the products, which the copies hide (64 requests, one token each: 180.7 us either way), and O is exact up to its own rounding.  With 32 rows once rounded, half a step of the type relative to each weight, as
+// the other 16-bit kernels do (24 drafts each for 32 requests: 46.9 us, in two parts 48.5).  Sums are of the unrounded weights, in fp32.
 #pragma once
 #include "cache_common.cuh"
 #include "cache_repair.cuh"
@@ -22,14 +23,16 @@ namespace chill {
 namespace cache {
 
 constexpr int kRowsThreads = 256;  // warps 0-3 consumers, 4 producer, 5-7 idle
-constexpr int kRowsConsumerRegs = 184, kRowsOtherRegs = 72;  // two CTAs on an SM: 2 * 128 * (184 + 72) = 65536
 
 template <int DP, int MT>
 struct RowsShape {
-  static constexpr int kCtasPerSm = DP <= 128 ? 2 : 1;
+  static constexpr int kCtasPerSm = rows_ctas(DP, 16 * MT);
+  // a CTA's pool is 256 threads x launch registers: consumers + others <= 2 * launch
+  static constexpr int kConsumerRegs = kCtasPerSm == 3 ? 104 : 184, kOtherRegs = kCtasPerSm == 3 ? 56 : 72;
+  static_assert(kCtasPerSm == 1 || kConsumerRegs + kOtherRegs <= 2 * (65536 / (256 * kCtasPerSm) / 8 * 8), "setmaxnreg.inc would never be granted");
   static constexpr int kHalves = DP / 64;                      // 64-channel blocks
   static constexpr int kTileBytes = kKeyTile * DP * 2;         // K or V
-  static constexpr int kStages = DP == 64 ? 5 : (MT == 1 ? 3 : 2);  // what two CTAs (head dim 256: one) have room for
+  static constexpr int kStages = DP == 64 ? (kCtasPerSm == 3 ? 3 : 5) : (MT == 1 ? 3 : 2);  // what the CTAs of an SM have room for
   static constexpr int kRows = 16 * MT;
   static constexpr int kQPitch = DP * 2 + 16;                  // bytes of a row of Q: eight rows in different banks
   static constexpr int kQBytes = kRows * kQPitch;
@@ -80,6 +83,7 @@ __global__ void __launch_bounds__(kRowsThreads, RowsShape<DP, MT>::kCtasPerSm)
 cached_rows_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV, const __grid_constant__ CachedP p) {
   using S = RowsShape<DP, MT>;
   constexpr int kStages = S::kStages;
+  constexpr bool kTwoParts = MT == 1;
   extern __shared__ uint8_t smem_raw[];
   const uint32_t base = (tc::smem_u32(smem_raw) + 1023u) & ~1023u;
   uint8_t* gen = smem_raw + (base - tc::smem_u32(smem_raw));
@@ -111,7 +115,7 @@ cached_rows_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constan
   pdl_launch_dependents();
 
   if (warp >= 4) {
-    if constexpr (S::kCtasPerSm > 1) tc::reg_dealloc<kRowsOtherRegs>();
+    if constexpr (S::kCtasPerSm > 1) tc::reg_dealloc<S::kOtherRegs>();
     if (warp > 4) return;
     // ---------------------------------------------------------------------------------------------- producer
     const int boxes = kKeyTile / p.box, jobs = boxes * S::kHalves, mine = lane % boxes;
@@ -181,7 +185,7 @@ cached_rows_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constan
   }
 
   // ------------------------------------------------------------------------------------------------- consumers
-  if constexpr (S::kCtasPerSm > 1) tc::reg_alloc<kRowsConsumerRegs>();
+  if constexpr (S::kCtasPerSm > 1) tc::reg_alloc<S::kConsumerRegs>();
   const int g = lane >> 2, quad = lane & 3;  // the accumulator's rows g and g + 8, channels / keys 2 quad, 2 quad + 1 of 8
   float2* stat = reinterpret_cast<float2*>(gen + S::kStat);
   int stage = 0;
@@ -301,7 +305,7 @@ cached_rows_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constan
             for (int d = 0; d < DP / 8; ++d) o[mt][d][2 * u] *= a, o[mt][d][2 * u + 1] *= a;
           }
       }
-      uint32_t pa[MT][4];
+      uint32_t pa[MT][4], rest[MT][4];
 #pragma unroll
       for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
@@ -312,6 +316,11 @@ cached_rows_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constan
             const float w0 = tc::ex2(fmaf(c[mt][j][2 * u], p.scale_log2, -safe)), w1 = tc::ex2(fmaf(c[mt][j][2 * u + 1], p.scale_log2, -safe));
             l[mt][u] += w0 + w1;
             pa[mt][j * 2 + u] = tc::pack2<T>(w0, w1);
+            if (kTwoParts) {
+              float h0, h1;
+              tc::unpack2<T>(pa[mt][j * 2 + u], h0, h1);
+              rest[mt][j * 2 + u] = tc::pack2<T>(w0 - h0, w1 - h1);
+            }
           }
         }
 #pragma unroll
@@ -322,6 +331,10 @@ cached_rows_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constan
         for (int mt = 0; mt < MT; ++mt) {
           mma16816<T>(o[mt][2 * nn], pa[mt], b[0], b[1]);
           mma16816<T>(o[mt][2 * nn + 1], pa[mt], b[2], b[3]);
+          if (kTwoParts) {
+            mma16816<T>(o[mt][2 * nn], rest[mt], b[0], b[1]);
+            mma16816<T>(o[mt][2 * nn + 1], rest[mt], b[2], b[3]);
+          }
         }
       }
       __syncwarp();
