@@ -70,6 +70,20 @@ struct Plan {
 // us (1024 new tokens for 4 requests).
 constexpr int kRowsPad = 2, kTilesPad = 6;
 
+// Keys a token can see at most in a table of `keys` (looked at for 32 positions: what is chosen by it is a matter of time alone).
+template <class M>
+static long long widest(const MaskArgs& margs, int keys) {
+  long long most = 0;
+  for (int i = 0; i < 32; ++i) {
+    int lo, hi;
+    M::k_range_for_q((int)((long long)(keys - 1) * i / 31), keys, margs, lo, hi);
+    lo = imax(lo, 0);
+    hi = imin(hi, keys - 1);
+    most = hi - lo + 1 > most ? hi - lo + 1 : most;
+  }
+  return most;
+}
+
 static int make_plan(const chill_cached_args& a, Plan& c) {
   const int G = a.H / a.H_kv, sms = sm_count();
   const long long group_rows = (long long)a.N * G;
@@ -98,15 +112,19 @@ static int make_plan(const chill_cached_args& a, Plan& c) {
   if (entries * a.H_kv * (keys / kKeyTile + 8) > 0x7fffffffll) return CHILL_E_TOO_LARGE;
   c.row_tiles = (int)row_tiles;
   auto up = [](size_t x) { return (x + 255) / 256 * 256; };
-  // Tables of a few tiles: one launch and no sum, whatever the lengths (2 requests of 300 cached tokens, fp32: 6 tiles in one CTA each take
-  // 8 us, 3 CTAs and the kernel that joins them 16 us)
-  c.whole = keys <= 8 * kKeyTile;
+  // what a unit can have to do, by the size of the table and the mask
+  long long seen = keys;
+  CHILL_MASK_SWITCH_OR(a.mask.id, (seen = widest<MaskT>(to_mask_args(a.mask, (long long)kMaxLen), (int)keys)), )
+  seen = seen + a.N < keys ? seen + a.N : keys;
+  // A few tiles: one launch and no sum, whatever the lengths (2 requests of 300 cached tokens, fp32: 12 us; cut in shares, with the kernel
+  // that joins them, 23 us)
+  c.whole = seen <= 8 * kKeyTile;
   if (c.whole) {
     c.grid = entries * a.H_kv < c.grid ? (int)(entries * a.H_kv) : c.grid;
     c.tail_shares = 0;
   }
-  // small shares only where the tables have room for so many keys
-  if (entries * a.H_kv * (keys / kKeyTile + 1) < (long long)kTailFrom * c.grid) c.tail_shares = 0;
+  // small shares only where there can be so many keys
+  if (entries * a.H_kv * (seen / kKeyTile + 1) < (long long)kTailFrom * c.grid) c.tail_shares = 0;
   c.scan = !c.whole && entries > kScanEntries;
   const int shares = c.grid + c.tail_shares;
   c.queue = 0;

