@@ -15,7 +15,8 @@ for each request, a chunk of a prompt, or a tree of drafted tokens) over the cac
     chill_pages_trim(pages, lens, page_size)                              # lens[b] = 0: request b is done
 
 Nothing here synchronises or copies to the host, lengths are read on the GPU, and every call can be captured into a CUDA graph and
-replayed with other lengths in the same tensors.  Work is enqueued on the current stream of the tensors' device; calls that use the
+replayed with other lengths in the same tensors; torch.compile traces the calls as dispatcher ops (a mask class after its first eager
+call).  Work is enqueued on the current stream of the tensors' device; calls that use the
 same pages on different streams are ordered by the caller.  There are no gradients: tensors that require them are refused.  The
 reference has no counterpart; a mask means here what it means to ``chill_attention``, for tokens at the positions of the step.
 """
@@ -54,6 +55,7 @@ class ChillPages(typing.NamedTuple):
     @classmethod
     def empty(cls, batch: int, max_len: int, num_pages: int, page_size: int, device="cuda") -> "ChillPages":
         """No request holds a page; a request can grow to max_len tokens (rounded up to whole pages)."""
+        assert batch >= 1 and max_len >= 1 and num_pages >= 1 and page_size >= 1
         ints = {"dtype": torch.int32, "device": device}
         return cls(torch.full((batch, -(-max_len // page_size)), -1, **ints), torch.zeros(batch, **ints),
                    torch.arange(num_pages - 1, -1, -1, **ints), torch.full((1,), num_pages, **ints), torch.zeros(1, **ints))
@@ -274,7 +276,7 @@ def chill_pages_trim(pages: ChillPages, lens: torch.Tensor, page_size: int) -> N
 def chill_cache_append(k_cache: torch.Tensor, v_cache: torch.Tensor, k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor) -> None:
     """Stores the rows of ``k`` and ``v`` ([batch, kv_heads, max_new, head_dim], any strides) at ``slots`` of the caches
     ([num_pages, kv_heads, page_size, head_dim], any strides), in place.  Tokens whose slot is outside the cache (-1) are left out; rows that
-    no slot names stay as they are."""
+    no slot names stay as they are, one that two tokens name holds either's."""
     if _direct() and _eager.extension().cache_append(_NATIVE.get(None) or _native(), k_cache, v_cache, k, v, slots):
         return
     _check_rows(k_cache, v_cache, k, v, slots)
@@ -342,9 +344,11 @@ def chill_attention_cached(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torc
 def _attention(q, k_cache, v_cache, table, step, mask, sm_scale, return_lse, flags):
     if sm_scale is None:
         sm_scale = q.shape[-1] ** -0.5
-    native, functor_id = _MASKS.get(mask.name) or _mask_functor(mask)
+    if mask.name not in _MASKS:
+        _mask_functor(mask)
     lens, new_lens, _, positions, ancestors = step
     if _direct():
+        native, functor_id = _MASKS[mask.name]
         out = _eager._extension.cached_attention(native, functor_id, q, k_cache, v_cache, table, lens, new_lens, positions, ancestors,
                                                  mask.constargs, sm_scale, return_lse, flags)
         if out is not None:

@@ -25,7 +25,7 @@ static int check_cached(const chill_cached_args* a, bool pointers) {
   if (a->B > 65535 || a->H > 65535 || a->N > kMaxLen / 2 || (long long)a->N * (a->H / a->H_kv) > kMaxLen ||
       (long long)a->num_pages * a->page_size > 0x7fffffffll || (long long)a->table_width * a->page_size > kMaxLen)
     return CHILL_E_TOO_LARGE;
-  if (!(a->sm_scale > 0.f) || a->sm_scale > 3e38f) return CHILL_E_INVALID;
+  if (!(a->sm_scale > 0.f) || a->sm_scale > 2e38f) return CHILL_E_INVALID;  // times log2(e) it stays finite
   const int st = check_mask(a->mask);
   if (st != CHILL_OK) return st;
   if (!pointers) return CHILL_OK;

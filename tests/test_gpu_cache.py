@@ -138,6 +138,13 @@ def test_groups_that_do_not_divide_a_tile(G):
     run_and_check(p, masks()["causal"])
 
 
+@pytest.mark.parametrize("G", [1, 2])
+@pytest.mark.parametrize("D", [32, 128, 256])
+def test_many_rows_of_few_heads(D, G):
+    p = Problem(torch.bfloat16, 2 * G, 2, D, [100, 0, 400], [130, 70, 129], 130, 32, tree=G == 2, seed=G, room=600)
+    run_and_check(p, masks()["chunkwise"])
+
+
 def test_which_kernel_serves_a_call():
     from chill_attention import _cabi, _cache_abi
 
@@ -517,6 +524,94 @@ def test_a_captured_step_is_replayed_with_other_lengths():
             graph.replay()
         for s, graph, o in graphs:
             assert torch.equal(o, want) and torch.equal(s.lens, eager.lens) and torch.equal(s.pages.table, eager.pages.table)
+
+
+def test_a_call_can_be_captured_before_any_ran():
+    import os
+    import subprocess
+    import sys
+
+    from helpers import ROOT
+
+    code = """
+import sys; sys.path[:0] = [%r, %r, %r]
+import torch, chill_attention as ca
+from cache_helpers import Problem
+for N, dtype in ((1, torch.bfloat16), (40, torch.float16), (1, torch.float32)):
+    p = Problem(dtype, 4, 2, 64, [900, 20], [N, N], N, 16, seed=N)
+    args = [p.q.cuda(), p.k_cache.cuda(), p.v_cache.cuda(), p.table.cuda(), p.step(), ca.CausalChillMask()]
+    pages, lens = ca.ChillPages.empty(2, 100, 20, 16), torch.zeros(2, dtype=torch.int32, device="cuda")
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        o = ca.chill_attention_cached(*args)
+        step = ca.chill_pages_reserve(pages, lens, args[4].new_lens, N, 16)
+    g.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(o, ca.chill_attention_cached(*args)) and (step.slots >= 0).all()
+print("captured")
+""" % (os.path.join(ROOT, "chill-attention_b200"), ROOT, os.path.join(ROOT, "tests"))
+    r = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=240)
+    assert r.returncode == 0 and "captured" in r.stdout, r.stderr[-2000:]
+
+
+def test_a_compiled_step():
+    import chill_attention as ca
+
+    p = Problem(torch.bfloat16, 8, 2, 64, [250, 90], [6, 5], 6, 16, tree=True, seed=3, room=600)
+    mask = masks()["window"]
+    q, table, parents = p.q.cuda(), p.table.cuda(), ints(p.parents)
+    k, v = torch.randn(2, 2, 6, 64, device="cuda", dtype=torch.bfloat16), torch.randn(2, 2, 6, 64, device="cuda", dtype=torch.bfloat16)
+    path, accepted = ints([[0, 2, 5], [1, 3, 4]]), ints([2, 3])
+
+    def step(pages, kc, vc, lens, new):
+        s = ca.chill_pages_reserve(pages, lens, new, 6, 16, parents)
+        ca.chill_cache_append(kc, vc, k, v, s.slots)
+        o, lse = ca.chill_attention_cached(q, kc, vc, pages.table, s, mask, return_lse=True)
+        lens = ca.chill_cache_commit(kc, vc, pages.table, s, path, accepted)
+        ca.chill_pages_trim(pages, lens, 16)
+        return o, lse, lens
+
+    def state():
+        pages = ca.ChillPages(table.clone(), ints(p.held), ints(p.spare_pages + [-1] * (p.k_cache.shape[0] - len(p.spare_pages))), ints([len(p.spare_pages)]), ints([0]))
+        return pages, p.k_cache.nan_to_num(0.25).cuda(), p.v_cache.nan_to_num(0.25).cuda(), ints(p.lens), ints(p.new)
+
+    a, b = state(), state()
+    want = step(*a)
+    got = torch.compile(step, fullgraph=True)(*b)
+    assert all(torch.equal(x, y) for x, y in zip(want, got))
+    assert all(torch.equal(x, y) for x, y in zip([*a[0], a[1], a[2]], [*b[0], b[1], b[2]]))
+
+
+def test_caches_with_more_than_two_to_the_31_elements():
+    """Pages whose offsets do not fit 32 bits, in elements and in bytes."""
+    import chill_attention as ca
+
+    page, Hkv, D, B, N = 64, 8, 64, 2, 3
+    pages = 2 ** 31 // (page * Hkv * D) + 40
+    kc, vc = (torch.empty(pages, Hkv, page, D, dtype=torch.float16, device="cuda") for _ in range(2))
+    assert kc.numel() > 2 ** 31
+    high = list(range(pages - 8, pages))
+    for tree in (False, True):
+        p = Problem(torch.float16, 16, Hkv, D, [100, 130], [N, N], N, page, tree=tree, seed=1, room=600)
+        where = {int(x): high[i] for i, x in enumerate(sorted(set(p.table[p.table >= 0].tolist())))}
+        for a, b in where.items():
+            kc[b], vc[b] = p.k_cache[a].cuda(), p.v_cache[a].cuda()
+        table = torch.tensor([[where.get(x, -1) for x in row] for row in p.table.tolist()], dtype=torch.int32, device="cuda")
+        for flags in (0, 1):
+            from chill_attention import cache
+
+            o, lse = cache._attention(p.q.cuda(), kc, vc, table, p.step(), masks()["causal"], D ** -0.5, True, flags)
+            check_attention(o, lse, p, masks()["causal"], D ** -0.5, flags == 0)
+        step = p.step()
+        slots = ints([[where[s // page] * page + s % page for s in row] for row in p.slots])
+        k, v = (torch.randn(B, Hkv, N, D, device="cuda").half() for _ in range(2))
+        ca.chill_cache_append(kc, vc, k, v, slots)
+        out = ca.chill_cache_commit(kc, vc, table, step, ints([[1, 2], [2, 2]]), ints([2, 1]))
+        assert out.tolist() == [102, 131]
+        for b, path in ((0, [1, 2, 2]), (1, [2, 1, 2])):
+            for i, f in enumerate(path):
+                s = int(slots[b, i])
+                assert torch.equal(kc[s // page, :, s % page], k[b, :, f]) and torch.equal(vc[s // page, :, s % page], v[b, :, f])
 
 
 def test_another_stream():
