@@ -92,7 +92,7 @@ static int make_plan(const chill_cached_args& a, Plan& c) {
   c.pad = 0;
   c.tail_shares = 0;
   if (c.kernel == CHILL_CACHED_CUDA_CORES) {
-    c.rows = group_rows <= 4 ? 4 : (group_rows <= 8 ? 8 : 16);
+    c.rows = group_rows <= 4 ? 4 : (group_rows <= 8 ? 8 : (group_rows <= 16 ? 16 : 32));
     c.grid = sms * (c.rows < 16 ? 4 : (a.D <= 64 ? 4 : (a.D <= 128 ? 2 : 1)));
     if (c.rows < 16) c.tail_shares = c.grid;
   } else if (c.kernel == CHILL_CACHED_ROWS) {

@@ -34,18 +34,23 @@ static int launch(bool behind, void (*kern)(Args...), dim3 grid, int threads, in
   return (int)cudaLaunchKernelEx(&cfg, kern, Args(args)...);
 }
 
+template <typename T, int DP, int RT>
+static int launch_simt_many(const CachedP& p, int grid, bool behind, cudaStream_t st) {
+  auto kern = cached_simt_many_kernel<T, DP, RT, InstMask>;
+  constexpr int smem = SimtSmem<DP, RT>::kBytes;
+  static_assert(smem <= 232448 && SimtSmem<DP, RT>::kCtasPerSm * (smem + 1024) <= 233472, "shared memory of an SM");
+  struct Tag {};
+  cudaError_t e = ensure_dynamic_smem<Tag>(kern, smem, /*prefer_max_carveout=*/true);
+  return e != cudaSuccess ? (int)e : launch(behind, kern, dim3((unsigned)grid), kSimtThreads, smem, st, p);
+}
+
 template <typename T, int DP>
 static int launch_simt(const CachedP& p, int grid, bool behind, cudaStream_t st) {
   const dim3 blocks((unsigned)grid);
   if (p.rows == 4 && p.whole) return launch(behind, cached_simt_few_kernel<T, DP, 4, 8, InstMask>, blocks, 256, 0, st, p);
   if (p.rows == 4) return launch(behind, cached_simt_few_kernel<T, DP, 4, 4, InstMask>, blocks, 128, 0, st, p);
   if (p.rows == 8) return launch(behind, cached_simt_few_kernel<T, DP, 8, 4, InstMask>, blocks, 128, 0, st, p);
-  auto kern = cached_simt_kernel<T, DP, InstMask>;
-  constexpr int smem = SimtSmem<DP>::kBytes;
-  static_assert(smem <= 232448, "exceeds the 227 KB of shared memory a CTA can opt in to");
-  struct Tag {};
-  cudaError_t e = ensure_dynamic_smem<Tag>(kern, smem, /*prefer_max_carveout=*/true);
-  return e != cudaSuccess ? (int)e : launch(behind, kern, dim3((unsigned)grid), kSimtThreads, smem, st, p);
+  return p.rows == 16 ? launch_simt_many<T, DP, 2>(p, grid, behind, st) : launch_simt_many<T, DP, 4>(p, grid, behind, st);
 }
 
 template <typename T, int DP, int MT>

@@ -6,206 +6,42 @@
 // four or eight steps at once, and gets the scores by butterflies over its lanes.  Every group of lanes has a maximum and a sum of its own: no warp,
 // and no group, waits for another before the end of a piece.
 //
-// More rows: a CTA of 128 threads works on 16 rows and 64 keys at a time, everything as fp32 in shared memory:
-//   S = Q K^T   a thread has one key and 8 rows: one vector of K and 8 (broadcast) of Q for 32 FMAs
-//   softmax     a warp has 4 rows; running maximum and sum in base 2
-//   O += P V    a thread has 4 channels of 2 D / 64 rows (registers)
+// More rows (simt_many): bound by the FMAs and what they read from shared memory, so a thread has a block of both products.  A CTA of 128
+// threads, 16 across and 8 down, works on 8 RT rows (16 or 32) and 64 keys at a time, everything as fp32 in shared memory:
+//   S = Q K^T   a thread has RT rows and 4 keys: RT + 4 vectors read for 16 RT FMAs, two at a time (even and odd channels)
+//   softmax     the 16 threads of a row agree on its maximum by butterflies; each keeps a sum of its own to the end
+//   O += P V    a thread has RT rows and D / 16 channels; P goes through shared memory, between threads of one warp only
+// K of the next tile is copied during the second product, V of this one during the first (asynchronous copies where the rows are fp32 on
+// 16-byte boundaries).  Vectors are put at chunk ^ (key mod 8) of a row, so that the reads of a warp fall into different banks.
 #pragma once
 #include "cache_common.cuh"
+#include "cache_repair.cuh"
 #include "tc_common.cuh"
 
 namespace chill {
 namespace cache {
 
 constexpr int kSimtThreads = 128;
-constexpr int kSimtRows = 16;
 
-template <int DP>
-struct SimtSmem {
-  static constexpr int kKRow = DP + 4;  // floats of a K row: 16-byte vectors of 8 consecutive keys fall into different banks
+template <int DP, int RT>
+struct SimtSmem {  // in floats
+  static constexpr int kRows = 8 * RT;
+  static constexpr int kCtasPerSm = DP <= 64 ? 4 : (DP <= 128 ? 2 : 1);
   static constexpr int kQ = 0;
-  static constexpr int kK = kQ + kSimtRows * DP;
-  static constexpr int kV = kK + kKeyTile * kKRow;
-  static constexpr int kS = kV + kKeyTile * DP;
-  static constexpr int kM = kS + kSimtRows * kKeyTile;  // alpha of every row
-  static constexpr int kBad = kM + kSimtRows;           // a key has no page
-  static constexpr int kItem = kBad + kKeyTile;
+  static constexpr int kK = kQ + kRows * DP;
+  static constexpr int kV = kK + kKeyTile * DP;
+  static constexpr int kP = kV + kKeyTile * DP;
+  static constexpr int kPlaces = kP + kRows * kKeyTile;  // page and row of every key of a tile, of two tiles
+  static constexpr int kThere = kPlaces + 4 * kKeyTile;  // a bit for every key: it has a page
+  static constexpr int kItem = kThere + 4;
   static constexpr int kCum = kItem + (int)sizeof(Item) / 4;
   static constexpr int kBytes = (kCum + kScanEntries + 1) * 4;
 };
 
-template <typename T, int DP, class M>
-__global__ void __launch_bounds__(kSimtThreads) cached_simt_kernel(const __grid_constant__ CachedP p) {
-  using L = SimtSmem<DP>;
-  extern __shared__ __align__(16) float smem[];
-  float *sq = smem + L::kQ, *sk = smem + L::kK, *sv = smem + L::kV, *ss = smem + L::kS, *sa = smem + L::kM;
-  int* bad = reinterpret_cast<int*>(smem + L::kBad);
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  constexpr int kChunks = DP / 4;                                                   // channel quads
-  constexpr int kGroups = kSimtThreads / kChunks < kSimtRows ? kSimtThreads / kChunks : kSimtRows;  // threads of a quad
-  constexpr int kOwn = kSimtRows / kGroups;                                         // rows of a thread in O += P V
-  const int quad = tid % kChunks, group = tid / kChunks;
-  const bool pv = group < kGroups;
-  Item& item = *reinterpret_cast<Item*>(smem + L::kItem);
-  const int* cum;
-  const Cut cut = begin_work<M, kSimtThreads>(p, reinterpret_cast<int*>(smem + L::kCum), cum);
-  pdl_launch_dependents();
-  Work work;
-  if (warp == 0) work.start<M>(p, cut, cum);
-  while (true) {
-    __syncthreads();
-    if (warp == 0) {
-      Item it;
-      work.next<M>(p, it);
-      if (lane == 0) item = it;
-    }
-    __syncthreads();
-    if (item.x.entry < 0) break;
-    const RowTile& t = item.t;
-    const Piece& piece = item.x;
-    const int tiles = item.tiles;
-    for (int idx = tid; idx < kSimtRows * DP; idx += kSimtThreads) {
-      const int r = idx / DP, d = idx % DP;
-      float x = 0.f;
-      if (r < t.rows && d < p.D) {
-        const int i = (t.r0 + r) / p.G, h = piece.head * p.G + (t.r0 + r) % p.G;
-        x = to_f(row_ptr<T>(p.q, t.b, h, i)[d * p.q.sd]);
-      }
-      sq[r * DP + d] = x;
-    }
-    float m[4], l[4];  // rows 4 * warp + n, the same in all lanes
-    float acc[kOwn][4];
-#pragma unroll
-    for (int n = 0; n < 4; ++n) m[n] = -CUDART_INF_F, l[n] = 0.f;
-#pragma unroll
-    for (int n = 0; n < kOwn; ++n) acc[n][0] = acc[n][1] = acc[n][2] = acc[n][3] = 0.f;
-
-    for (int kt = piece.t0; kt < tiles; ++kt) {
-      const int k0 = t.k_lo + kt * kKeyTile;
-      __syncthreads();  // the tile before has been used
-      for (int idx = tid; idx < kKeyTile * kChunks; idx += kSimtThreads) {
-        const int key = idx / kChunks, d = (idx % kChunks) * 4, at = k0 + key;
-        const int page = at < t.total ? p.table[t.b * p.table_sb + at / p.page] : -1;
-        const bool there = page >= 0 && page < p.num_pages;
-        float4 kx = make_float4(0.f, 0.f, 0.f, 0.f), vx = kx;
-        if (there) {
-          const int row = at % p.page;
-          const T* ks = reinterpret_cast<const T*>(p.k.p) + page * p.k.sb + piece.head * p.k.sh + row * p.k.sl;
-          const T* vs = reinterpret_cast<const T*>(p.v.p) + page * p.v.sb + piece.head * p.v.sh + row * p.v.sl;
-          float* kf = &kx.x;
-          float* vf = &vx.x;
-#pragma unroll
-          for (int u = 0; u < 4; ++u) {
-            if (d + u < p.D) {
-              kf[u] = to_f(ks[(d + u) * p.k.sd]);
-              vf[u] = to_f(vs[(d + u) * p.v.sd]);
-            }
-          }
-        }
-        *reinterpret_cast<float4*>(sk + key * L::kKRow + d) = kx;
-        *reinterpret_cast<float4*>(sv + key * DP + d) = vx;
-        if (d == 0) bad[key] = !there;
-      }
-      __syncthreads();
-      {  // S: key tid % 64, rows 8 * (tid / 64) on
-        const int key = tid & 63, r0 = (tid >> 6) * 8;
-        float s[8];
-#pragma unroll
-        for (int n = 0; n < 8; ++n) s[n] = 0.f;
-#pragma unroll 4
-        for (int d = 0; d < DP; d += 4) {
-          const float4 kx = *reinterpret_cast<const float4*>(sk + key * L::kKRow + d);
-#pragma unroll
-          for (int n = 0; n < 8; ++n) {
-            const float4 qx = *reinterpret_cast<const float4*>(sq + (r0 + n) * DP + d);
-            s[n] = fmaf(qx.x, kx.x, fmaf(qx.y, kx.y, fmaf(qx.z, kx.z, fmaf(qx.w, kx.w, s[n]))));
-          }
-        }
-        const int at = k0 + key;
-        const bool full = at >= t.full_lo && at < t.full_hi;
-#pragma unroll
-        for (int n = 0; n < 8; ++n) {
-          const int r = r0 + n;
-          bool ok = r < t.rows && at < t.total && !bad[key];
-          if (ok && !full) {
-            const int i = (t.r0 + r) / p.G;
-            ok = sees<M>(p, t, i, token_position(p, t, i), at);
-          }
-          ss[r * kKeyTile + key] = ok ? s[n] * p.scale_log2 : -CUDART_INF_F;
-        }
-      }
-      __syncthreads();
-#pragma unroll
-      for (int n = 0; n < 4; ++n) {  // softmax of row 4 * warp + n
-        float* row = ss + (warp * 4 + n) * kKeyTile;
-        const float x = row[lane], y = row[lane + 32];
-        float top = fmaxf(x, y);
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-        const float m_new = fmaxf(m[n], top), safe = m_new == -CUDART_INF_F ? 0.f : m_new;
-        const float a = exp2f(m[n] - safe);  // m = -inf: 0
-        const float ex = exp2f(x - safe), ey = exp2f(y - safe);
-        l[n] = l[n] * a + warp_sum(ex + ey);
-        m[n] = m_new;
-        row[lane] = ex;
-        row[lane + 32] = ey;
-        if (lane == 0) sa[warp * 4 + n] = a;
-      }
-      __syncthreads();
-      if (pv) {
-#pragma unroll
-        for (int n = 0; n < kOwn; ++n) {
-          const float a = sa[group * kOwn + n];
-#pragma unroll
-          for (int u = 0; u < 4; ++u) acc[n][u] *= a;
-        }
-#pragma unroll 4
-        for (int key = 0; key < kKeyTile; ++key) {
-          const float4 vx = *reinterpret_cast<const float4*>(sv + key * DP + quad * 4);
-#pragma unroll
-          for (int n = 0; n < kOwn; ++n) {
-            const float w = ss[(group * kOwn + n) * kKeyTile + key];
-            if (w != 0.f) {  // a hidden key may hold anything
-              acc[n][0] = fmaf(w, vx.x, acc[n][0]); acc[n][1] = fmaf(w, vx.y, acc[n][1]);
-              acc[n][2] = fmaf(w, vx.z, acc[n][2]); acc[n][3] = fmaf(w, vx.w, acc[n][3]);
-            }
-          }
-        }
-      }
-    }
-
-    // maximum and sum of every row, for the threads that hold its O
-    __syncthreads();
-    float* sm = ss;
-    if (lane < 4) {
-#pragma unroll
-      for (int n = 0; n < 4; ++n)
-        if (lane == n) sm[warp * 4 + n] = m[n], sm[kSimtRows + warp * 4 + n] = l[n];
-    }
-    __syncthreads();
-    if (pv) {
-#pragma unroll
-      for (int n = 0; n < kOwn; ++n) {
-        const int r = group * kOwn + n, all = p.N * p.G;
-        if (t.r0 + r >= all) continue;
-        const float mr = sm[r], lr = sm[kSimtRows + r];
-        if (piece.slot < 0) {
-          const int i = (t.r0 + r) / p.G, h = piece.head * p.G + (t.r0 + r) % p.G;
-          const float inv = r < t.rows && lr > 0.f ? 1.f / lr : 0.f;
-          T* to = o_row<T>(p, t.b, h, i);
-#pragma unroll
-          for (int u = 0; u < 4; ++u)
-            if (quad * 4 + u < p.D) to[(quad * 4 + u) * p.o.sd] = from_f<T>(acc[n][u] * inv);
-          if (quad == 0) store_lse(p, t.b, h, i, r < t.rows, mr, lr);
-        } else {
-          const long long at = (long long)piece.slot * p.rows + r;
-          if (quad * 4 < p.D) *reinterpret_cast<float4*>(p.part_o + at * p.D + quad * 4) = make_float4(acc[n][0], acc[n][1], acc[n][2], acc[n][3]);
-          if (quad == 0) p.part_ml[at] = make_float2(mr, lr);
-        }
-      }
-    }
-  }
+__device__ __forceinline__ void copy16(float* dst, const void* src, bool there) {  // zeros where there is nothing
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(tc::smem_u32(dst)), "l"(src), "r"(there ? 16 : 0) : "memory");
 }
+__device__ __forceinline__ void copies_done() { asm volatile("cp.async.wait_all;" ::: "memory"); }
 
 // Four channels from global memory, as fp32.
 template <typename T>
@@ -222,6 +58,202 @@ __device__ __forceinline__ float4 load4(const T* p, long long sd, bool wide) {
     }
   }
   return make_float4(to_f(p[0]), to_f(p[sd]), to_f(p[2 * sd]), to_f(p[3 * sd]));
+}
+
+template <typename T, int DP, int RT, class M>
+__global__ void __launch_bounds__(kSimtThreads, (SimtSmem<DP, RT>::kCtasPerSm)) cached_simt_many_kernel(const __grid_constant__ CachedP p) {
+  using L = SimtSmem<DP, RT>;
+  constexpr int kChunks = DP / 4, kVecs = DP > 64 ? DP / 64 : 1;
+  extern __shared__ __align__(16) float smem[];
+  float *sq = smem + L::kQ, *sk = smem + L::kK, *sv = smem + L::kV, *sp = smem + L::kP;
+  int2* places = reinterpret_cast<int2*>(smem + L::kPlaces);
+  volatile unsigned* there = reinterpret_cast<volatile unsigned*>(smem + L::kThere);
+  Item& item = *reinterpret_cast<Item*>(smem + L::kItem);
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, tx = tid & 15, ty = tid >> 4, odd_row = ty & 1;
+  const int* cum;
+  const Cut cut = begin_work<M, kSimtThreads>(p, reinterpret_cast<int*>(smem + L::kCum), cum);
+  pdl_launch_dependents();
+  Work work;
+  if (warp == 0) work.start<M>(p, cut, cum);
+  while (true) {
+    __syncthreads();
+    if (warp == 0) {
+      Item it;
+      work.next<M>(p, it);
+      if (lane == 0) item = it;
+    }
+    __syncthreads();
+    if (item.x.entry < 0) break;
+    const RowTile& t = item.t;
+    const Piece& piece = item.x;
+    const int tiles = item.tiles, t0 = piece.t0, total = t.total, k_lo = t.k_lo, full_lo = t.full_lo, full_hi = t.full_hi;
+    // page and row of this thread's key of a tile
+    auto place = [&](int kt) -> int2 {
+      const int at = k_lo + kt * kKeyTile + tid, block = at / p.page;
+      const int page = at < total ? p.table[t.b * p.table_sb + block] : -1;
+      return make_int2(page >= 0 && page < p.num_pages ? page : -1, at - block * p.page);
+    };
+    auto put_place = [&](int kt, int2 x) {
+      places[((kt - t0) & 1) * kKeyTile + tid] = x;
+      const unsigned is = __ballot_sync(0xffffffffu, x.x >= 0);
+      if (lane == 0) there[((kt - t0) & 1) * 2 + warp] = is;
+    };
+    auto copy = [&](int kt, const TRef& c, float* to, bool swizzle) {  // K or V of a tile
+#pragma unroll 4
+      for (int idx = tid; idx < kKeyTile * kChunks; idx += kSimtThreads) {
+        const int key = idx / kChunks, ch = idx % kChunks;
+        const int2 x = places[((kt - t0) & 1) * kKeyTile + key];
+        const bool is = x.x >= 0 && ch * 4 < p.D;
+        const T* from = reinterpret_cast<const T*>(c.p) + (is ? x.x * c.sb + piece.head * c.sh + x.y * c.sl + ch * 4 * c.sd : 0);
+        float* dst = to + key * DP + (swizzle ? ch ^ (key & 7) : ch) * 4;
+        if (sizeof(T) == 4 && p.wide_kv) copy16(dst, from, is);
+        else *reinterpret_cast<float4*>(dst) = is ? load4<T>(from, c.sd, p.wide_kv) : make_float4(0.f, 0.f, 0.f, 0.f);
+      }
+    };
+    if (t0 < tiles && tid < kKeyTile) put_place(t0, place(t0));
+    for (int idx = tid; idx < L::kRows * kChunks; idx += kSimtThreads) {
+      const int r = idx / kChunks, ch = idx % kChunks;
+      float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (r < t.rows && ch * 4 < p.D) {
+        const int i = (t.r0 + r) / p.G, h = piece.head * p.G + (t.r0 + r) % p.G;
+        x = load4<T>(row_ptr<T>(p.q, t.b, h, i) + ch * 4 * p.q.sd, p.q.sd, p.wide_q);
+      }
+      *reinterpret_cast<float4*>(sq + r * DP + (ch ^ (r / RT & 1)) * 4) = x;
+    }
+    // of row ty * RT + tx, where there is one
+    const int my_row = tx < RT ? ty * RT + tx : -1, my_token = my_row >= 0 && my_row < t.rows ? (t.r0 + my_row) / p.G : -1;
+    const int my_pos = my_token >= 0 ? token_position(p, t, my_token) : 0;
+    const uint64_t my_near = first_ancestors(p, t.b, my_token);
+    float m[RT], l[RT];  // the maximum is the same in the 16 threads of a row, the sum each one's own
+    uint64_t o[RT][kVecs][2];
+#pragma unroll
+    for (int n = 0; n < RT; ++n) {
+      m[n] = -CUDART_INF_F;
+      l[n] = 0.f;
+#pragma unroll
+      for (int v = 0; v < kVecs; ++v) o[n][v][0] = o[n][v][1] = 0ull;
+    }
+    __syncthreads();
+    if (t0 < tiles) copy(t0, p.k, sk, true);
+    for (int kt = t0; kt < tiles; ++kt) {
+      const int k0 = k_lo + kt * kKeyTile;
+      const bool more = kt + 1 < tiles;
+      int2 next = make_int2(-1, 0);
+      if (more && tid < kKeyTile) next = place(kt + 1);
+      copies_done();
+      __syncthreads();  // K is there; V of the tile before has been used
+      copy(kt, p.v, sv, false);
+      uint64_t s2[RT][4];
+#pragma unroll
+      for (int n = 0; n < RT; ++n) s2[n][0] = s2[n][1] = s2[n][2] = s2[n][3] = 0ull;
+#pragma unroll 4
+      for (int ch = 0; ch < kChunks; ++ch) {
+        ulonglong2 q[RT], k[4];
+#pragma unroll
+        for (int n = 0; n < RT; ++n) q[n] = *reinterpret_cast<const ulonglong2*>(sq + (ty * RT + n) * DP + (ch ^ odd_row) * 4);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) k[j] = *reinterpret_cast<const ulonglong2*>(sk + (tx + 16 * j) * DP + (ch ^ (tx & 7)) * 4);
+#pragma unroll
+        for (int n = 0; n < RT; ++n)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) s2[n][j] = tc::ffma2(q[n].y, k[j].y, tc::ffma2(q[n].x, k[j].x, s2[n][j]));
+      }
+      const unsigned th0 = there[((kt - t0) & 1) * 2], th1 = there[((kt - t0) & 1) * 2 + 1];
+      const bool full = (th0 & th1) == 0xffffffffu && k0 >= full_lo && k0 + kKeyTile <= full_hi;
+      uint64_t vis = ~0ull;
+      if (!full) {
+        vis = visible_keys<M>(p, t, my_token, my_pos, my_near, k0, 0) & ((uint64_t)th0 | (uint64_t)th1 << 32);
+        __syncwarp();
+      }
+#pragma unroll
+      for (int n = 0; n < RT; ++n) {
+        const uint64_t see = full ? ~0ull : __shfl_sync(0xffffffffu, (unsigned long long)vis, (lane & 16) + n);
+        float x[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          float lo, hi;
+          tc::upk2(s2[n][j], lo, hi);
+          x[j] = (see >> (tx + 16 * j)) & 1ull ? (lo + hi) * p.scale_log2 : -CUDART_INF_F;
+        }
+        float top = fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3]));
+#pragma unroll
+        for (int d = 8; d > 0; d >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
+        const float m_new = fmaxf(m[n], top), safe = m_new == -CUDART_INF_F ? 0.f : m_new;
+        const float a = exp2f(m[n] - safe);  // m = -inf: 0
+        m[n] = m_new;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          x[j] = exp2f(x[j] - safe);
+          sp[(ty * RT + n) * kKeyTile + ((tx + 16 * j) ^ (odd_row * 16))] = x[j];
+        }
+        l[n] = fmaf(l[n], a, (x[0] + x[1]) + (x[2] + x[3]));
+        if (a != 1.f) {
+#pragma unroll
+          for (int v = 0; v < kVecs; ++v) {
+            o[n][v][0] = tc::fmul2(o[n][v][0], tc::pk2(a, a));
+            o[n][v][1] = tc::fmul2(o[n][v][1], tc::pk2(a, a));
+          }
+        }
+      }
+      if (more && tid < kKeyTile) put_place(kt + 1, next);
+      copies_done();
+      __syncthreads();  // V is there; K has been used
+      if (more) copy(kt + 1, p.k, sk, true);
+      if (DP >= 64 || tx * 4 < DP) {
+#pragma unroll 1
+        for (int k4 = 0; k4 < kKeyTile; k4 += 4) {
+          float4 w[RT];
+#pragma unroll
+          for (int n = 0; n < RT; ++n) w[n] = *reinterpret_cast<const float4*>(sp + (ty * RT + n) * kKeyTile + (k4 ^ (odd_row * 16)));
+#pragma unroll
+          for (int u = 0; u < 4; ++u) {
+#pragma unroll
+            for (int v = 0; v < kVecs; ++v) {
+              const ulonglong2 x = *reinterpret_cast<const ulonglong2*>(sv + (k4 + u) * DP + v * 64 + tx * 4);
+#pragma unroll
+              for (int n = 0; n < RT; ++n) {
+                const float wn = u == 0 ? w[n].x : (u == 1 ? w[n].y : (u == 2 ? w[n].z : w[n].w));
+                o[n][v][0] = tc::ffma2(tc::pk2(wn, wn), x.x, o[n][v][0]);
+                o[n][v][1] = tc::ffma2(tc::pk2(wn, wn), x.y, o[n][v][1]);
+              }
+            }
+          }
+        }
+      }
+    }
+
+    bool odd = false;  // not finite: a hidden key's 0 times what it holds, maybe
+#pragma unroll
+    for (int n = 0; n < RT; ++n) {
+      const int r = ty * RT + n;
+#pragma unroll
+      for (int d = 8; d > 0; d >>= 1) l[n] += __shfl_xor_sync(0xffffffffu, l[n], d);
+      if (t.r0 + r >= p.N * p.G) continue;
+      const int i = (t.r0 + r) / p.G, h = piece.head * p.G + (t.r0 + r) % p.G;
+      const long long at = (long long)imax(piece.slot, 0) * p.rows + r;
+      const bool valid = r < t.rows;
+      const float inv = l[n] != 0.f ? 1.f / l[n] : 0.f;
+      T* to = o_row<T>(p, t.b, h, i);
+      odd |= valid && !(l[n] <= 3e38f);
+#pragma unroll
+      for (int v = 0; v < kVecs; ++v) {
+        const int d = v * 64 + tx * 4;
+        if (d >= p.D || (DP < 64 && d >= DP)) continue;
+        float f[4];
+        tc::upk2(o[n][v][0], f[0], f[1]);
+        tc::upk2(o[n][v][1], f[2], f[3]);
+        odd |= valid && !(fabsf(f[0]) + fabsf(f[1]) + fabsf(f[2]) + fabsf(f[3]) <= 3e38f);
+        if (piece.slot >= 0) *reinterpret_cast<float4*>(p.part_o + at * p.D + d) = make_float4(f[0], f[1], f[2], f[3]);
+        else if (valid) store4<T>(p, to, d, f[0] * inv, f[1] * inv, f[2] * inv, f[3] * inv);
+        else store4<T>(p, to, d, 0.f, 0.f, 0.f, 0.f);
+      }
+      if (tx == 0) {
+        if (piece.slot >= 0) p.part_ml[at] = make_float2(m[n], l[n]);
+        else store_lse(p, t.b, h, i, valid, m[n], l[n]);
+      }
+    }
+    if (consumers_any(odd)) repair_piece<T, DP, M>(p, t, piece, warp, 4);
+  }
 }
 
 // WARPS: four of them have a tile; with eight (units taken whole, where one CTA has all of a unit's tiles) two tiles are under way.
