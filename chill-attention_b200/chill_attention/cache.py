@@ -35,7 +35,7 @@ _DTYPES = (torch.float32, torch.float16, torch.bfloat16)
 #: entry points a native CacheLibrary object is made of, in its order
 _ENTRY_POINTS = ("chill_cached_fwd", "chill_cached_workspace_bytes", "chill_pages_reserve", "chill_pages_trim", "chill_cache_append",
                  "chill_cache_commit")
-#: library -> its native call object; mask class name -> (call object, functor id)
+#: library -> its native call object; mask class name -> (call object, functor id, class)
 _NATIVE: dict = {}
 _MASKS: dict[str, tuple] = {}
 
@@ -217,7 +217,7 @@ def _attention_op(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
                   positions: torch.Tensor, ancestors: typing.Optional[torch.Tensor], mask_name: str,
                   mask_args: typing.List[typing.Union[int, float, bool]], sm_scale: float, flags: int) -> tuple[torch.Tensor, torch.Tensor]:
     _check_attention(q, k_cache, v_cache, table, lens, new_lens, positions, ancestors)
-    native, functor_id = _MASKS[mask_name]
+    native, functor_id, _ = _MASKS[mask_name]
     return _eager.extension().cached_attention(native, functor_id, q, k_cache, v_cache, table, lens, new_lens, positions, ancestors,
                                                tuple(mask_args), sm_scale, True, flags)
 
@@ -303,7 +303,7 @@ def chill_cache_commit(k_cache: torch.Tensor, v_cache: torch.Tensor, table: torc
 
 
 def _mask_functor(mask: ChillMask):
-    """Native call object and functor id serving this mask class (builds the custom library if needed)."""
+    """Finds the native call object and the functor id that serve this mask class (builds the custom library if needed)."""
     functor, header = getattr(mask, "cuda_functor", None), getattr(mask, "cuda_functor_header", None)
     if header is not None:
         from .custom import build_custom_cache_library
@@ -316,8 +316,15 @@ def _mask_functor(mask: ChillMask):
     else:
         raise NotImplementedError(f"{mask.name} has no CUDA functor: set `cuda_functor` to a built-in functor name or provide "
                                   "`cuda_functor_header` + `cuda_functor` (see chill_attention/custom.py)")
-    _MASKS[mask.name] = found
-    return found
+    _MASKS[mask.name] = *found, type(mask)
+
+
+def _check_same_name(mask: ChillMask):
+    """The dispatcher op knows a mask by its class name: another class of that name has to mean the same functor."""
+    known = _MASKS[mask.name][2]
+    same = all(getattr(mask, a, None) == getattr(known, a, None) for a in ("cuda_functor", "cuda_functor_header"))
+    if not same:
+        raise ValueError(f"two mask classes are named {mask.name} and have different CUDA functors: give one of them another name")
 
 
 def chill_attention_cached(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, table: torch.Tensor, step: ChillStep, mask: ChillMask,
@@ -346,9 +353,11 @@ def _attention(q, k_cache, v_cache, table, step, mask, sm_scale, return_lse, fla
         sm_scale = q.shape[-1] ** -0.5
     if mask.name not in _MASKS:
         _mask_functor(mask)
+    elif not _is_compiling() and _MASKS[mask.name][2] is not type(mask):
+        _check_same_name(mask)
     lens, new_lens, _, positions, ancestors = step
     if _direct():
-        native, functor_id = _MASKS[mask.name]
+        native, functor_id, _ = _MASKS[mask.name]
         out = _eager._extension.cached_attention(native, functor_id, q, k_cache, v_cache, table, lens, new_lens, positions, ancestors,
                                                  mask.constargs, sm_scale, return_lse, flags)
         if out is not None:

@@ -132,6 +132,23 @@ def test_cpu_tensors_are_refused(lib):
         ca.chill_attention_cached(torch.zeros(2, 4, 3, 64), cache, cache, pages.table, step, ca.CausalChillMask())
 
 
+def test_two_mask_classes_of_one_name():
+    from chill_attention import CausalChillMask, cache
+
+    def make(functor, **more):
+        return type("OneName", (CausalChillMask,), {"cuda_functor": functor, **more})()
+
+    first = make("CausalMask")
+    cache._MASKS["OneName"] = (None, 0, type(first))
+    try:
+        cache._check_same_name(make("CausalMask"))  # the same functor: whichever class
+        for other in (make("FullMask"), make("CausalMask", cuda_functor_header="/tmp/x.h")):
+            with pytest.raises(ValueError, match="two mask classes"):
+                cache._attention(torch.zeros(1, 1, 1, 64), None, None, None, (None,) * 5, other, None, False, 0)
+    finally:
+        del cache._MASKS["OneName"]
+
+
 def test_oracle_trim_undoes_reserve():
     table, held, free = [[5, -1, -1, -1], [-1] * 4, [7, 2, -1, -1]], [1, 0, 2], [9, 8, 6, 4, 3, 1, 0]
     lens, new = [10, 0, 20], [30, 16, 0]
