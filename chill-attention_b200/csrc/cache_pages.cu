@@ -386,6 +386,7 @@ int chill_cache_commit(const chill_cache_rows_args* a, void* stream) {
   int st = check_rows(a);
   if (st != CHILL_OK) return st;
   if (!a->table || !a->lens || !a->new_lens || !a->path || !a->accepted || !a->out_lens || a->table_width <= 0 || a->A <= 0) return CHILL_E_INVALID;
+  if (a->out_lens == a->lens) return CHILL_E_INVALID;  // a request has several CTAs, all of them read its length
   if ((long long)a->table_width * a->page_size > kMaxLen) return CHILL_E_TOO_LARGE;
   const int es = a->dtype == CHILL_F32 ? 4 : 2;
   const bool wide = a->D * es % 16 == 0 && vec16(a->k_cache, a->k_cache_strides, es) && vec16(a->v_cache, a->v_cache_strides, es);

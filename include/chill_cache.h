@@ -66,7 +66,7 @@ typedef struct chill_cache_rows_args {
   const int32_t *lens, *new_lens; /* [B] */
   const int32_t* path;            /* [B][A]: numbers of the accepted tokens, increasing */
   const int32_t* accepted;        /* [B]: how many of them, clamped to [0, min(A, new_lens[b])] */
-  int32_t* out_lens;              /* [B]: lens[b] + accepted[b]; may be lens itself */
+  int32_t* out_lens;              /* [B]: lens[b] + accepted[b]; not lens itself */
 } chill_cache_rows_args;
 
 /* Row (b, head, i) of k and v goes to slot slots[b][i] of the caches; slots outside the cache are skipped. */

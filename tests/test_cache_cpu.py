@@ -109,6 +109,7 @@ def test_page_and_row_refusals(lib):
         assert lib.chill_cache_append(rows(**{name: None}), None) == -1
     for name in ("table", "lens", "new_lens", "path", "accepted", "out_lens"):
         assert lib.chill_cache_commit(rows(**{name: None}), None) == -1
+    assert lib.chill_cache_commit(rows(), None) == -1  # out_lens is lens: the CTAs of a request all read its length
     assert lib.chill_cache_commit(rows(A=0), None) == -1 and lib.chill_cache_commit(rows(table_width=0), None) == -1
 
 

@@ -128,6 +128,16 @@ def test_row_tiles(kind, N):
         run_and_check(p, masks()["window_ahead" if N % 2 else "causal"])
 
 
+@pytest.mark.parametrize("N", [9, 16, 17, 31, 33, 70])
+@pytest.mark.parametrize("kind", ["chain", "tree"])
+def test_row_tiles_on_the_cuda_cores(kind, N):
+    """Tiles of 16 and of 32 rows, every head dim, pages that are no multiple of anything."""
+    for D, dtype, page, room in ((16, torch.float32, 16, 600), (32, torch.float32, 48, 0), (64, torch.bfloat16, 5, 600),
+                                 (64, torch.float32, 7, 600), (128, torch.float32, 64, 600), (256, torch.float32, 5, 600), (256, torch.float16, 3, 0)):
+        p = Problem(dtype, 4, 4, D, [150, 10, 64], [N, N - 3, 1], N, page, tree=kind == "tree", seed=N, room=room)
+        run_and_check(p, masks()["window_ahead" if N % 2 else "causal"])
+
+
 @pytest.mark.parametrize("G", [5, 7, 48, 100, 128, 130])
 def test_groups_that_do_not_divide_a_tile(G):
     """Tiles of rows hold whole tokens: 125, 126, 96, 100 and 128 of 128 rows; a token with more goes elsewhere."""
