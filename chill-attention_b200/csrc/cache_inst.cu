@@ -49,7 +49,7 @@ static int launch_simt(const CachedP& p, int grid, bool behind, cudaStream_t st)
   const dim3 blocks((unsigned)grid);
   if (p.rows == 4 && p.whole) return launch(behind, cached_simt_few_kernel<T, DP, 4, 8, InstMask>, blocks, 256, 0, st, p);
   if (p.rows == 4) return launch(behind, cached_simt_few_kernel<T, DP, 4, 4, InstMask>, blocks, 128, 0, st, p);
-  if (p.rows == 8) return launch(behind, cached_simt_few_kernel<T, DP, 8, 4, InstMask>, blocks, 128, 0, st, p);
+  if (p.rows == 8) return launch_simt_many<T, DP, 1>(p, grid, behind, st);
   return p.rows == 16 ? launch_simt_many<T, DP, 2>(p, grid, behind, st) : launch_simt_many<T, DP, 4>(p, grid, behind, st);
 }
 

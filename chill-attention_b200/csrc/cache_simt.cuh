@@ -1,13 +1,13 @@
 // Attention of new tokens over a paged cache on the CUDA cores: fp32 (IEEE arithmetic) and every layout that the tensor-core
 // kernels can not take.  See cache_common.cuh for units and shares.
 //
-// Up to 8 rows (simt_few): bound by memory, so nothing goes through shared memory.  D / 4 lanes (32 at most) share a key, a warp has
+// Up to 4 rows (simt_few): bound by memory, so nothing goes through shared memory.  D / 4 lanes (32 at most) share a key, a warp has
 // 16 keys of every tile of 64; a lane keeps four channels (eight at head dim 256) of Q and O of every row, reads those of K and V of
-// four or eight steps at once, and gets the scores by butterflies over its lanes.  Every group of lanes has a maximum and a sum of its own: no warp,
+// eight steps at once, and gets the scores by butterflies over its lanes.  Every group of lanes has a maximum and a sum of its own: no warp,
 // and no group, waits for another before the end of a piece.
 //
 // More rows (simt_many): bound by the FMAs and what they read from shared memory, so a thread has a block of both products.  A CTA of 128
-// threads, 16 across and 8 down, works on 8 RT rows (16 or 32) and 64 keys at a time, everything as fp32 in shared memory:
+// threads, 16 across and 8 down, works on 8 RT rows (8, 16 or 32) and 64 keys at a time, everything as fp32 in shared memory:
 //   S = Q K^T   a thread has RT rows and 4 keys: RT + 4 vectors read for 16 RT FMAs, two at a time (even and odd channels)
 //   softmax     the 16 threads of a row agree on its maximum by butterflies; each keeps a sum of its own to the end
 //   O += P V    a thread has RT rows and D / 16 channels; P goes through shared memory, between threads of one warp only
@@ -15,6 +15,8 @@
 // 16-byte boundaries).  Vectors are put at chunk ^ (key mod 8) of a row, so that the reads of a warp fall into different banks.
 // fp32, 500 new tokens for 2 requests of up to 4000, 16 heads on 4 of 128: 1113 us, 25 TFLOP/s (an SM reads as long as it multiplies); 12 drafts
 // for 8 requests of up to 5000 tokens, 16 heads on 8 of 128: 137 us.  (One key and 8 rows a thread, nothing copied ahead: 3016 and 427 us.)
+// One new token for 16 requests of up to 8000, 8 heads of 128 a kv head: 148 us, in tiles of 16 rows 156, as in simt_few 182; with 4 heads a kv
+// head (64 requests of up to 4000) simt_few has 212, this 307.
 #pragma once
 #include "cache_common.cuh"
 #include "cache_repair.cuh"
@@ -265,7 +267,7 @@ __global__ void __launch_bounds__(WARPS * 32) cached_simt_few_kernel(const __gri
   constexpr int kVecs = DP / 4 / kLanes;                // vectors of four channels of a lane
   constexpr int kKeys = 32 / kLanes;                    // keys of a warp at a time: its groups of lanes
   constexpr int kSteps = 16 / kKeys;                    // of the warp's 16 keys of a tile
-  constexpr int kAhead = kSteps < (R == 4 ? 8 / kVecs : 4) ? kSteps : (R == 4 ? 8 / kVecs : 4);  // steps whose loads are in flight
+  constexpr int kAhead = kSteps < 8 / kVecs ? kSteps : 8 / kVecs;  // steps whose loads are in flight
   __shared__ float4 sums[WARPS][R][DP / 4];
   __shared__ float2 stat[WARPS][R];
   __shared__ Item item;
