@@ -92,7 +92,7 @@ static int make_plan(const chill_cached_args& a, Plan& c) {
   c.pad = 0;
   c.tail_shares = 0;
   if (c.kernel == CHILL_CACHED_CUDA_CORES) {
-    c.rows = group_rows <= 4 ? 4 : (group_rows <= 8 ? 8 : (group_rows <= 16 ? 16 : 32));
+    c.rows = group_rows <= 2 ? 2 : (group_rows <= 4 ? 4 : (group_rows <= 8 ? 8 : (group_rows <= 16 ? 16 : 32)));
     c.grid = sms * (c.rows < 8 ? 4 : (a.D <= 64 ? 4 : (a.D <= 128 ? 2 : 1)));
     if (c.rows < 8) c.tail_shares = c.grid;  // 16 rows and more: 1194 us with small shares, 1136 without (500 new tokens for 2 requests)
   } else if (c.kernel == CHILL_CACHED_ROWS) {
@@ -116,7 +116,7 @@ static int make_plan(const chill_cached_args& a, Plan& c) {
   long long seen = keys;
   CHILL_MASK_SWITCH_OR(a.mask.id, (seen = widest<MaskT>(to_mask_args(a.mask, (long long)kMaxLen), (int)keys)), )
   seen = seen + a.N < keys ? seen + a.N : keys;
-  // A few tiles: one launch and no sum, whatever the lengths (2 requests of 300 cached tokens, fp32: 12 us; cut in shares, with the kernel
+  // A few tiles: one launch and no sum, whatever the lengths (2 requests of 300 cached tokens, fp32: 10 us; cut in shares, with the kernel
   // that joins them, 23 us)
   c.whole = seen <= 8 * kKeyTile;
   if (c.whole) {

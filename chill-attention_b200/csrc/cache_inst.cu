@@ -47,6 +47,8 @@ static int launch_simt_many(const CachedP& p, int grid, bool behind, cudaStream_
 template <typename T, int DP>
 static int launch_simt(const CachedP& p, int grid, bool behind, cudaStream_t st) {
   const dim3 blocks((unsigned)grid);
+  if (p.rows == 2 && p.whole) return launch(behind, cached_simt_few_kernel<T, DP, 2, 8, InstMask>, blocks, 256, 0, st, p);
+  if (p.rows == 2) return launch(behind, cached_simt_few_kernel<T, DP, 2, 4, InstMask>, blocks, 128, 0, st, p);
   if (p.rows == 4 && p.whole) return launch(behind, cached_simt_few_kernel<T, DP, 4, 8, InstMask>, blocks, 256, 0, st, p);
   if (p.rows == 4) return launch(behind, cached_simt_few_kernel<T, DP, 4, 4, InstMask>, blocks, 128, 0, st, p);
   if (p.rows == 8) return launch_simt_many<T, DP, 1>(p, grid, behind, st);

@@ -1,11 +1,14 @@
 // Attention of new tokens over a paged cache on the CUDA cores: fp32 (IEEE arithmetic) and every layout that the tensor-core
 // kernels can not take.  See cache_common.cuh for units and shares.
 //
-// Up to 4 rows (simt_few): bound by memory, so nothing goes through shared memory.  D / 4 lanes (32 at most) share a key, a warp has
-// 16 keys of every tile of 64; a lane keeps four channels (eight at head dim 256) of Q and O of every row, reads those of K and V of
-// eight steps at once, and gets the scores by butterflies over its lanes.  Every group of lanes has a maximum and a sum of its own: no warp,
-// and no group, waits for another before the end of a piece.
-//
+// Up to 4 rows (simt_few, tiles of 2 or 4): bound by memory, so nothing goes through shared memory but the weights.  D / 4 lanes (32 at most)
+// share a key, a warp has 16 keys of every tile of 64; a lane keeps four channels (eight at head dim 256) of Q and O of every row and
+// reads those of K and V of eight steps at once.  The 16 or 32 scores of such a batch are summed over the lanes all together: lanes halve what they
+// hold at each step, each ends up with one or two scores, keeps the maximum and the sum of that row, and takes the exponential once.  Every group
+// of lanes has a state of its own: no warp, and no group, waits for another before the end of a piece.
+// fp32, one new token for 64 requests of up to 4000, 16 heads on 4 of 128: 127 us; with every score summed in all lanes and two CTAs on an SM
+// 206; with that sum and two CTAs 192, three 177, four (128 registers) 127, six with batches of half the size 133.
+// 8 heads on 8 of 128: 222 us (4.9 TB/s); in tiles of 4 rows and with sums in all lanes 416.
 // More rows (simt_many): bound by the FMAs and what they read from shared memory, so a thread has a block of both products.  A CTA of 128
 // threads, 16 across and 8 down, works on 8 RT rows (8, 16 or 32) and 64 keys at a time, everything as fp32 in shared memory:
 //   S = Q K^T   a thread has RT rows and 4 keys: RT + 4 vectors read for 16 RT FMAs, two at a time (even and odd channels)
@@ -15,8 +18,8 @@
 // 16-byte boundaries).  Vectors are put at chunk ^ (key mod 8) of a row, so that the reads of a warp fall into different banks.
 // fp32, 500 new tokens for 2 requests of up to 4000, 16 heads on 4 of 128: 1113 us, 25 TFLOP/s (an SM reads as long as it multiplies); 12 drafts
 // for 8 requests of up to 5000 tokens, 16 heads on 8 of 128: 137 us.  (One key and 8 rows a thread, nothing copied ahead: 3016 and 427 us.)
-// One new token for 16 requests of up to 8000, 8 heads of 128 a kv head: 148 us, in tiles of 16 rows 156, as in simt_few 182; with 4 heads a kv
-// head (64 requests of up to 4000) simt_few has 212, this 307.
+// One new token for 16 requests of up to 8000, 8 heads of 128 a kv head: 148 us, in tiles of 16 rows 156, as in simt_few 182 (before its
+// sums over the lanes).
 #pragma once
 #include "cache_common.cuh"
 #include "cache_repair.cuh"
@@ -260,15 +263,36 @@ __global__ void __launch_bounds__(kSimtThreads, (SimtSmem<DP, RT>::kCtasPerSm)) 
   }
 }
 
+// Sums N values over 2 STEP lanes, which halve the values that they hold at each step: lane `sub` of them ends up with those from
+// sub * N / (2 STEP) on, or, where there are fewer values than lanes, with the one it shares with its neighbours.
+template <int N, int STEP>
+__device__ __forceinline__ void lane_sums(float* x, int sub) {
+  if constexpr (N > 1) {
+    const bool upper = (sub & STEP) != 0;
+#pragma unroll
+    for (int i = 0; i < N / 2; ++i) {
+      const float keep = upper ? x[i + N / 2] : x[i], give = upper ? x[i] : x[i + N / 2];
+      x[i] = keep + __shfl_xor_sync(0xffffffffu, give, STEP);
+    }
+  } else {
+    x[0] += __shfl_xor_sync(0xffffffffu, x[0], STEP);
+  }
+  if constexpr (STEP > 1) lane_sums<(N > 1 ? N / 2 : 1), STEP / 2>(x, sub);
+}
+
 // WARPS: four of them have a tile; with eight (units taken whole, where one CTA has all of a unit's tiles) two tiles are under way.
 template <typename T, int DP, int R, int WARPS, class M>
-__global__ void __launch_bounds__(WARPS * 32) cached_simt_few_kernel(const __grid_constant__ CachedP p) {
+__global__ void __launch_bounds__(WARPS * 32, 16 / WARPS) cached_simt_few_kernel(const __grid_constant__ CachedP p) {
   constexpr int kLanes = DP / 4 < 32 ? DP / 4 : 32;     // of a key
   constexpr int kVecs = DP / 4 / kLanes;                // vectors of four channels of a lane
   constexpr int kKeys = 32 / kLanes;                    // keys of a warp at a time: its groups of lanes
   constexpr int kSteps = 16 / kKeys;                    // of the warp's 16 keys of a tile
   constexpr int kAhead = kSteps < 8 / kVecs ? kSteps : 8 / kVecs;  // steps whose loads are in flight
+  constexpr int kVals = R * kAhead, kOwn = kVals > kLanes ? kVals / kLanes : 1;  // scores of such a batch, and how many a lane ends up with
+  constexpr int kSame = kVals < kLanes ? kLanes / kVals : 1, kRowLanes = kLanes / R;  // lanes with the same score; lanes of a row
   __shared__ float4 sums[WARPS][R][DP / 4];
+  __shared__ float4 weights[WARPS][kKeys][kVals / 4];
+  __shared__ float alpha[WARPS][kKeys][R];
   __shared__ float2 stat[WARPS][R];
   __shared__ Item item;
   __shared__ int smem_cum[kScanEntries + 1];
@@ -291,11 +315,10 @@ __global__ void __launch_bounds__(WARPS * 32) cached_simt_few_kernel(const __gri
     const Piece piece = item.x;
     const int tiles = item.tiles, total = t.total, rows = t.rows, k_lo = t.k_lo, full_lo = t.full_lo, full_hi = t.full_hi;
     float4 q[R][kVecs], o[R][kVecs];
-    float m[R], l[R];
+    const int sub = lane % kLanes, my_r = sub / kRowLanes;  // this lane's row, and its maximum and part of the sum
+    float my_m = -CUDART_INF_F, my_l = 0.f;
 #pragma unroll
     for (int r = 0; r < R; ++r) {
-      m[r] = -CUDART_INF_F;
-      l[r] = 0.f;
 #pragma unroll
       for (int v = 0; v < kVecs; ++v) {
         const int d = ch + v * 128;
@@ -312,29 +335,30 @@ __global__ void __launch_bounds__(WARPS * 32) cached_simt_few_kernel(const __gri
     const char* kb = reinterpret_cast<const char*>(p.k.p) + (piece.head * p.k.sh + ch * p.k.sd) * (long long)sizeof(T);
     const char* vb = reinterpret_cast<const char*>(p.v.p) + (piece.head * p.v.sh + ch * p.v.sd) * (long long)sizeof(T);
     const int quarter = (warp & 3) * 16;  // this warp's keys of a tile
+    auto page_of = [&](int k) -> int {  // of key k + lane, for the first 16 lanes
+      const int page = lane < 16 && k + lane < total ? table[(k + lane) / p.page] : -1;
+      return page < p.num_pages ? page : -1;
+    };
+    int pages_next = page_of(k_lo + (piece.t0 + warp / 4) * kKeyTile + quarter);
     for (int kt = piece.t0 + warp / 4; kt < tiles; kt += WARPS / 4) {
-      const int k0 = k_lo + kt * kKeyTile + quarter;
+      const int k0 = k_lo + kt * kKeyTile + quarter, pages = pages_next;
+      pages_next = page_of(k0 + WARPS / 4 * kKeyTile);
       if (k0 >= total) break;
-      unsigned seen = rows >= 32 ? 0xffffffffu : (1u << rows) - 1u, words[R];  // bit s * kKeys + g: the key of group g in step s
+      unsigned seen = my_r < rows ? 0xffffu : 0u;  // bit s * kKeys + g: row my_r sees the key of group g in step s
       if (k0 < full_lo || k0 + 16 > full_hi) {
         const uint64_t vis = visible_keys<M>(p, t, my_token, my_pos, my_near, k0 - quarter, 0);
         __syncwarp();
-        seen = (unsigned)(vis >> quarter) & 0xffffu;  // row `lane`'s 16 keys of this warp
-#pragma unroll
-        for (int r = 0; r < R; ++r) words[r] = __shfl_sync(0xffffffffu, seen, r);
-      } else {
-#pragma unroll
-        for (int r = 0; r < R; ++r) words[r] = (seen >> r) & 1u ? 0xffffu : 0u;
+        seen = __shfl_sync(0xffffffffu, (unsigned)(vis >> quarter), my_r);  // what lane r holds is row r's
       }
 #pragma unroll 1
       for (int s0 = 0; s0 < kSteps; s0 += kAhead) {
         float4 kx[kAhead][kVecs], vx[kAhead][kVecs];
         unsigned there = 0;
-        int key = k0 + s0 * kKeys + group, block = key / p.page, row = key - block * p.page;
+        int row = (k0 + s0 * kKeys + group) % p.page;
 #pragma unroll
         for (int s = 0; s < kAhead; ++s) {
-          const int page = key < total ? table[block] : -1;
-          const bool is = page >= 0 && page < p.num_pages;
+          const int page = __shfl_sync(0xffffffffu, pages, (s0 + s) * kKeys + group);
+          const bool is = page >= 0;
           there |= (unsigned)is << s;
 #pragma unroll
           for (int v = 0; v < kVecs; ++v) {
@@ -344,52 +368,78 @@ __global__ void __launch_bounds__(WARPS * 32) cached_simt_few_kernel(const __gri
               vx[s][v] = load4<T>(reinterpret_cast<const T*>(vb) + page * p.v.sb + row * p.v.sl + v * 128 * p.v.sd, p.v.sd, p.wide_kv);
             }
           }
-          key += kKeys;
-          for (row += kKeys; row >= p.page; row -= p.page) ++block;
+          for (row += kKeys; row >= p.page;) row -= p.page;
         }
+        float x[kVals];
 #pragma unroll
-        for (int r = 0; r < R; ++r) {
-          float x[kAhead], top = m[r];
+        for (int r = 0; r < R; ++r)
 #pragma unroll
           for (int s = 0; s < kAhead; ++s) {
-            x[s] = 0.f;
+            float z = 0.f;
 #pragma unroll
             for (int v = 0; v < kVecs; ++v)
-              x[s] = fmaf(q[r][v].x, kx[s][v].x, fmaf(q[r][v].y, kx[s][v].y, fmaf(q[r][v].z, kx[s][v].z, fmaf(q[r][v].w, kx[s][v].w, x[s]))));
+              z = fmaf(q[r][v].x, kx[s][v].x, fmaf(q[r][v].y, kx[s][v].y, fmaf(q[r][v].z, kx[s][v].z, fmaf(q[r][v].w, kx[s][v].w, z))));
+            x[r * kAhead + s] = z;
+          }
+        lane_sums<kVals, kLanes / 2>(x, sub);  // score sub * kVals / kLanes and following ones
+        const int first = sub * kVals / kLanes % kAhead;  // step of its first score
+        float top = my_m;
+#pragma unroll
+        for (int i = 0; i < kOwn; ++i) {
+          const int s = first + i;
+          const bool is = ((there >> s) & (seen >> ((s0 + s) * kKeys + group)) & 1u) != 0;
+          x[i] = is ? x[i] * p.scale_log2 : -CUDART_INF_F;
+          top = fmaxf(top, x[i]);
+        }
+#pragma unroll
+        for (int d = kRowLanes / 2; d >= kSame; d >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
+        const float safe = top == -CUDART_INF_F ? 0.f : top, a = tc::ex2(my_m - safe);
+        my_m = top;
+        my_l *= a;
+#pragma unroll
+        for (int i = 0; i < kOwn; ++i) {
+          const float w = tc::ex2(x[i] - safe);
+          my_l += w;
+          if (sub % kSame == 0) reinterpret_cast<float*>(weights[warp][group])[sub * kVals / kLanes + i] = w;
+        }
+        if (sub % kRowLanes == 0) alpha[warp][group][my_r] = a;
+        const bool moved = __any_sync(0xffffffffu, a != 1.f);
+        __syncwarp();
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+          if (moved) {
+            const float ar = alpha[warp][group][r];
+#pragma unroll
+            for (int v = 0; v < kVecs; ++v) o[r][v].x *= ar, o[r][v].y *= ar, o[r][v].z *= ar, o[r][v].w *= ar;
           }
 #pragma unroll
-          for (int d = kLanes / 2; d > 0; d >>= 1)
+          for (int s4 = 0; s4 < kAhead; s4 += 4) {
+            const float4 w4 = weights[warp][group][(r * kAhead + s4) / 4];
 #pragma unroll
-            for (int s = 0; s < kAhead; ++s) x[s] += __shfl_xor_sync(0xffffffffu, x[s], d);
-          unsigned see = 0;  // the same in all lanes of a group
+            for (int u = 0; u < 4; ++u) {
+              const float w = u == 0 ? w4.x : (u == 1 ? w4.y : (u == 2 ? w4.z : w4.w));
+              if (w != 0.f) {  // a hidden key may hold anything
 #pragma unroll
-          for (int s = 0; s < kAhead; ++s) {
-            const bool is = ((there >> s) & (words[r] >> ((s0 + s) * kKeys + group)) & 1u) != 0;
-            see |= (unsigned)is << s;
-            x[s] = is ? x[s] * p.scale_log2 : -CUDART_INF_F;
-            top = fmaxf(top, x[s]);
-          }
-          const float safe = top == -CUDART_INF_F ? 0.f : top, a = tc::ex2(m[r] - safe);
-          m[r] = top;
-          l[r] *= a;
-#pragma unroll
-          for (int v = 0; v < kVecs; ++v) o[r][v].x *= a, o[r][v].y *= a, o[r][v].z *= a, o[r][v].w *= a;
-#pragma unroll
-          for (int s = 0; s < kAhead; ++s) {
-            if ((see >> s) & 1u) {  // a hidden key may hold anything
-              const float w = tc::ex2(x[s] - safe);
-              l[r] += w;
-#pragma unroll
-              for (int v = 0; v < kVecs; ++v) {
-                o[r][v].x = fmaf(w, vx[s][v].x, o[r][v].x); o[r][v].y = fmaf(w, vx[s][v].y, o[r][v].y);
-                o[r][v].z = fmaf(w, vx[s][v].z, o[r][v].z); o[r][v].w = fmaf(w, vx[s][v].w, o[r][v].w);
+                for (int v = 0; v < kVecs; ++v) {
+                  o[r][v].x = fmaf(w, vx[s4 + u][v].x, o[r][v].x); o[r][v].y = fmaf(w, vx[s4 + u][v].y, o[r][v].y);
+                  o[r][v].z = fmaf(w, vx[s4 + u][v].z, o[r][v].z); o[r][v].w = fmaf(w, vx[s4 + u][v].w, o[r][v].w);
+                }
               }
             }
           }
         }
+        __syncwarp();  // the weights have been read
       }
     }
 
+    float m[R], l[R];
+#pragma unroll
+    for (int d = kRowLanes / 2; d >= kSame; d >>= 1) my_l += __shfl_xor_sync(0xffffffffu, my_l, d);
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      m[r] = __shfl_sync(0xffffffffu, my_m, group * kLanes + r * kRowLanes);
+      l[r] = __shfl_sync(0xffffffffu, my_l, group * kLanes + r * kRowLanes);
+    }
     // the groups' states, then the warps', become one
 #pragma unroll
     for (int r = 0; r < R; ++r) {
