@@ -91,8 +91,22 @@ static int make_plan(const chill_cached_args& a, Plan& c) {
   c.min_share = 2;
   c.pad = 0;
   c.tail_shares = 0;
+  const long long keys = (long long)a.table_width * a.page_size;
+  // what a unit can have to do, by the size of the table and the mask
+  long long seen = keys;
+  CHILL_MASK_SWITCH_OR(a.mask.id, (seen = widest<MaskT>(to_mask_args(a.mask, (long long)kMaxLen), (int)keys)), )
+  seen = seen + a.N < keys ? seen + a.N : keys;
+  // A few tiles: one launch and no sum, whatever the lengths (2 requests of 300 cached tokens, fp32: 10 us; cut in shares, with the kernel
+  // that joins them, 23 us)
+  c.whole = seen <= 8 * kKeyTile;
   if (c.kernel == CHILL_CACHED_CUDA_CORES) {
-    c.rows = group_rows <= 2 ? 2 : (group_rows <= 4 ? 4 : (group_rows <= 8 ? 8 : (group_rows <= 16 ? 16 : 32)));
+    // Rows in tiles of 4 where that is faster than larger ones with more work in shared memory.  Whole units: while the SMs have few of them, up
+    // to about six tiles of 4 each (24 rows, 32 / 512 units: 13.5 / 109 us, in tiles of 32 rows 38.8 / 62.8; 8 rows, 408 units: 51 / 75).  Shares: 5 to
+    // 8 rows of 65 to 128 channels, though keys are read twice (one token for 16 requests of 8000, 8 heads a kv head: 118 us, in tiles of 8
+    // rows 148; of 64 channels 70.5 / 68, of 256 55 / 52).
+    const long long fours = (long long)a.B * a.H_kv * ((group_rows + 3) / 4);
+    const bool quads = c.whole ? fours <= 6 * sms : (group_rows <= 8 && a.D > 64 && a.D <= 128);
+    c.rows = group_rows <= 2 ? 2 : (group_rows <= 4 || quads ? 4 : (group_rows <= 8 ? 8 : (group_rows <= 16 ? 16 : 32)));
     c.grid = sms * (c.rows < 8 ? 4 : (a.D <= 64 ? 4 : (a.D <= 128 ? 2 : 1)));
     if (c.rows < 8) c.tail_shares = c.grid;  // 16 rows and more: 1194 us with small shares, 1136 without (500 new tokens for 2 requests)
   } else if (c.kernel == CHILL_CACHED_ROWS) {
@@ -108,17 +122,9 @@ static int make_plan(const chill_cached_args& a, Plan& c) {
     c.grid = sms * (a.D <= 128 ? 2 : 1) / (two ? 2 : 1);
   }
   const long long row_tiles = (group_rows + c.rows - 1) / c.rows, entries = (long long)a.B * row_tiles;
-  const long long keys = (long long)a.table_width * a.page_size;
   if (entries * a.H_kv * (keys / kKeyTile + 8) > 0x7fffffffll) return CHILL_E_TOO_LARGE;
   c.row_tiles = (int)row_tiles;
   auto up = [](size_t x) { return (x + 255) / 256 * 256; };
-  // what a unit can have to do, by the size of the table and the mask
-  long long seen = keys;
-  CHILL_MASK_SWITCH_OR(a.mask.id, (seen = widest<MaskT>(to_mask_args(a.mask, (long long)kMaxLen), (int)keys)), )
-  seen = seen + a.N < keys ? seen + a.N : keys;
-  // A few tiles: one launch and no sum, whatever the lengths (2 requests of 300 cached tokens, fp32: 10 us; cut in shares, with the kernel
-  // that joins them, 23 us)
-  c.whole = seen <= 8 * kKeyTile;
   if (c.whole) {
     c.grid = entries * a.H_kv < c.grid ? (int)(entries * a.H_kv) : c.grid;
     c.tail_shares = 0;

@@ -1,7 +1,7 @@
 // Attention of new tokens over a paged cache on the CUDA cores: fp32 (IEEE arithmetic) and every layout that the tensor-core
 // kernels can not take.  See cache_common.cuh for units and shares.
 //
-// Up to 4 rows (simt_few, tiles of 2 or 4): bound by memory, so nothing goes through shared memory but the weights.  D / 4 lanes (32 at most)
+// Few rows (simt_few, tiles of 2 or 4): bound by memory, so nothing goes through shared memory but the weights.  D / 4 lanes (32 at most)
 // share a key, a warp has 16 keys of every tile of 64; a lane keeps four channels (eight at head dim 256) of Q and O of every row and
 // reads those of K and V of eight steps at once.  The 16 or 32 scores of such a batch are summed over the lanes all together: lanes halve what they
 // hold at each step, each ends up with one or two scores, keeps the maximum and the sum of that row, and takes the exponential once.  Every group
@@ -18,8 +18,7 @@
 // 16-byte boundaries).  Vectors are put at chunk ^ (key mod 8) of a row, so that the reads of a warp fall into different banks.
 // fp32, 500 new tokens for 2 requests of up to 4000, 16 heads on 4 of 128: 1113 us, 25 TFLOP/s (an SM reads as long as it multiplies); 12 drafts
 // for 8 requests of up to 5000 tokens, 16 heads on 8 of 128: 137 us.  (One key and 8 rows a thread, nothing copied ahead: 3016 and 427 us.)
-// One new token for 16 requests of up to 8000, 8 heads of 128 a kv head: 148 us, in tiles of 16 rows 156, as in simt_few 182 (before its
-// sums over the lanes).
+// (make_plan has which rows go where.)
 #pragma once
 #include "cache_common.cuh"
 #include "cache_repair.cuh"

@@ -138,6 +138,14 @@ def test_row_tiles_on_the_cuda_cores(kind, N):
         run_and_check(p, masks()["window_ahead" if N % 2 else "causal"])
 
 
+@pytest.mark.parametrize("N", [6, 12, 20])
+def test_many_whole_units_on_the_cuda_cores(N):
+    """Short tables and more units than the SMs have few of: tiles of 8, 16 and 32 rows, each by one CTA."""
+    lens = [(37 * b) % 90 for b in range(80)]
+    new = [N - b % 3 for b in range(80)]
+    run_and_check(Problem(torch.float32, 8, 8, 32, lens, new, N, 16, tree=True, seed=N), masks()["causal"])
+
+
 @pytest.mark.parametrize("G", [5, 7, 48, 100, 128, 130])
 def test_groups_that_do_not_divide_a_tile(G):
     """Tiles of rows hold whole tokens: 125, 126, 96, 100 and 128 of 128 rows; a token with more goes elsewhere."""
