@@ -103,7 +103,7 @@ size_t chill_cached_workspace_bytes(const chill_cached_args* a);
 int chill_cached_fwd(const chill_cached_args* a, void* stream);
 /* Which kernel chill_cached_fwd would launch (host-only; pointers are looked at for their alignment), or a negative status. */
 #define CHILL_CACHED_CUDA_CORES 0 /* fp32, and what the others can not take */
-#define CHILL_CACHED_ROWS 1       /* 16-bit, up to 32 rows (N * H / H_kv) of a kv head */
+#define CHILL_CACHED_ROWS 1       /* 16-bit, up to 32 rows (N * H / H_kv) of a kv head, and queries that the tiles can not take */
 #define CHILL_CACHED_TILES 2      /* 16-bit, tiles of 128 rows */
 int chill_cached_kernel(const chill_cached_args* a);
 
