@@ -65,7 +65,9 @@ __device__ __forceinline__ void tma_load_5d(uint32_t dst, const CUtensorMap* map
 __device__ __forceinline__ uint64_t ex2_fma(uint64_t x2) {
   float x0, x1;
   tc::upk2(x2, x0, x1);
-  x2 = tc::pk2(fmaxf(x0, -126.f), fmaxf(x1, -126.f));  // below: 2^-126 beside a row's largest weight of 2^-8 or more; not for hidden keys, which need a 0
+  // below: 2^-126 beside a row's largest weight of 2^-8 or more; not for hidden keys, which need a 0, nor for scores that are not finite (NaN
+  // becomes 2^-126 too): whoever calls this looks at the row's maximum
+  x2 = tc::pk2(fmaxf(x0, -126.f), fmaxf(x1, -126.f));
   const uint64_t n2 = tc::fadd2(x2, tc::pk2(12582912.f, 12582912.f));
   const uint64_t f2 = tc::ffma2(tc::fadd2(n2, tc::pk2(-12582912.f, -12582912.f)), tc::pk2(-1.f, -1.f), x2);
   uint64_t p2 = tc::pk2(1.3276472e-3f, 1.3276472e-3f);
@@ -78,6 +80,11 @@ __device__ __forceinline__ uint64_t ex2_fma(uint64_t x2) {
   tc::upk2(p2, a, b);
   tc::upk2(n2, na, nb);
   return tc::pk2u(__float_as_uint(a) + (__float_as_uint(na) << 23), __float_as_uint(b) + (__float_as_uint(nb) << 23));
+}
+__device__ __forceinline__ float fmax3_nan(float a, float b, float c) {  // NaN if any of them is
+  float d;
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
 }
 // Of every sixteen pairs of weights, half as many are worked out so.  The two groups' softmax warps on a scheduler ask its MUFU for 1024
 // of the 2100 clocks of a step, mostly at the same time: 1024 new tokens for each of 4 requests, 507 us with none, 480 with an eighth of
@@ -320,12 +327,13 @@ cached_tiles_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_consta
         float mx0 = -CUDART_INF_F, mx1 = mx0, mx2 = mx0, mx3 = mx0;
 #pragma unroll
         for (int e = 0; e < kKeyTile; e += 8) {
-          mx0 = tc::fmax3(mx0, __uint_as_float(x[e]), __uint_as_float(x[e + 1]));
-          mx1 = tc::fmax3(mx1, __uint_as_float(x[e + 2]), __uint_as_float(x[e + 3]));
-          mx2 = tc::fmax3(mx2, __uint_as_float(x[e + 4]), __uint_as_float(x[e + 5]));
-          mx3 = tc::fmax3(mx3, __uint_as_float(x[e + 6]), __uint_as_float(x[e + 7]));
+          mx0 = fmax3_nan(mx0, __uint_as_float(x[e]), __uint_as_float(x[e + 1]));
+          mx1 = fmax3_nan(mx1, __uint_as_float(x[e + 2]), __uint_as_float(x[e + 3]));
+          mx2 = fmax3_nan(mx2, __uint_as_float(x[e + 4]), __uint_as_float(x[e + 5]));
+          mx3 = fmax3_nan(mx3, __uint_as_float(x[e + 6]), __uint_as_float(x[e + 7]));
         }
-        const float m_cand = fmaxf(m_used, fmaxf(fmaxf(mx0, mx1), fmaxf(mx2, mx3)) * c);
+        const float top = fmax3_nan(fmax3_nan(mx0, mx1, mx2), mx3, mx3);
+        const float m_cand = fmaxf(m_used, top * c);  // passes NaN by
         if (j == 0) {
           m_used = m_cand;
         } else if (__any_sync(0xffffffffu, m_cand - m_used > 8.f)) {  // lazily: O is rescaled when the maximum grew by more than 2^8
@@ -373,6 +381,9 @@ cached_tiles_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_consta
         tc::upk2(l0, a0, a1);
         tc::upk2(l1, a2, a3);
         l += (a0 + a1) + (a2 + a3);
+        // The weights on the FMA pipe know neither NaN nor infinity.  A score of NaN or +inf, or nothing but -inf, shows in the tile's maximum:
+        // 0 times that is NaN, and the sum that holds it sends the piece to repair_piece
+        if (full) l = fmaf(top, 0.f, l);
         tc::tmem_st32(tS, x);
         if (k0 + kKeyTile > total) {  // rows of V behind the last key may hold anything, and 0 * NaN is NaN: they become 0
           ok = __all_sync(0xffffffffu, tc::mbar_wait(v_full + 8 * s, (uint32_t)(n / kStages) & 1u, guard, kStTilesSoftmax));

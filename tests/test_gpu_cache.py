@@ -710,3 +710,51 @@ def test_refusals():
             ca.chill_pages_reserve(*args)
     with pytest.raises(AssertionError):
         ca.chill_pages_trim(pages, step.lens[:1], 16)
+
+
+@pytest.mark.parametrize("value", [float("nan"), float("inf"), float("-inf")], ids=str)
+@pytest.mark.parametrize("room", list(ROOMS))
+@pytest.mark.parametrize("dtype,N,D,page", [(torch.bfloat16, 9, 64, 16), (torch.float16, 9, 128, 16), (torch.bfloat16, 70, 64, 16), (torch.float16, 70, 128, 16),
+                                            (torch.bfloat16, 20, 256, 16), (torch.float32, 1, 64, 16), (torch.float32, 9, 64, 16), (torch.bfloat16, 9, 64, 5)], ids=str)
+def test_a_score_that_is_not_finite_shows(dtype, N, D, page, room, value):
+    """One key, seen by every row and not finite in K alone, at each of the 64 places of a tile: scores of NaN or +inf leave nothing finite in a
+    row of O, one of -inf is a weight of 0, and the rows of the other kv head know nothing of it."""
+    p = Problem(dtype, 4, 2, D, [200] * 64, [N] * 64, N, page, seed=N, room=ROOMS[room])
+    for b in range(64):
+        where, row = int(p.table[b, (64 + b) // page]), (64 + b) % page
+        p.k_cache[where, 1, row, b % D] = value
+    (o, lse), scale = attend(p, masks()["causal"])
+    o_ref = p.oracle(masks()["causal"], scale)[0]
+    finite = torch.isfinite(o_ref).all(-1)  # [batch, head, token]
+    assert finite[:, :2].all() and (value == float("-inf") or not finite[:, 2:].all())
+    gone = ~finite.cuda()
+    assert not torch.isfinite(o[gone]).any() and not torch.isfinite(lse[gone]).any()
+    clean = Clean(p, finite)
+    check_attention(*(torch.where(finite.cuda().view(*finite.shape, *[1] * (x.ndim - 3)), x, 0) for x in (o, lse)), clean, masks()["causal"], scale, dtype != torch.float32)
+
+
+class Clean:
+    """A problem whose rows outside of `finite` [batch, head, token] are zeros on both sides; scores of -inf have no part in the bound."""
+
+    def __init__(self, problem, finite):
+        self.q, self.new, self.N, self.dtype, self.v_cache = problem.q, problem.new, problem.N, problem.dtype, problem.v_cache
+        self.problem, self.finite = problem, finite
+
+    def oracle(self, mask, scale):
+        o, lse, size, _, keys = self.problem.oracle(mask, scale)
+        k = self.problem.k_cache
+        self.problem.k_cache = torch.where(torch.isfinite(k), k, 0)
+        most = self.problem.oracle(mask, scale)[3]
+        self.problem.k_cache = k
+        return tuple(torch.where(self.finite.view(*self.finite.shape, *[1] * (x.ndim - 3)), x, 0) for x in (o, lse, size, most, keys))
+
+
+@pytest.mark.parametrize("dtype,N,D", [(torch.bfloat16, 9, 64), (torch.bfloat16, 70, 64), (torch.float16, 70, 128), (torch.float32, 9, 64)], ids=str)
+def test_scores_of_minus_infinity_everywhere(dtype, N, D):
+    """Every key of a kv head is -inf in a channel in which the rows are positive: nothing is left for these rows, as where nothing is seen."""
+    p = Problem(dtype, 4, 2, D, [200, 130], [N, N], N, 16, seed=N)
+    p.k_cache[:, 1, :, 3] = float("-inf")
+    p.q[:, 2:, :, 3] = p.q[:, 2:, :, 3].abs() + 0.25
+    (o, lse), _ = attend(p, masks()["causal"])
+    assert (o[:, 2:] == 0).all() and torch.isneginf(lse[:, 2:]).all()
+    assert torch.isfinite(o[:, :2]).all() and torch.isfinite(lse[:, :2]).all()
