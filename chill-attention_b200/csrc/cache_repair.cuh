@@ -1,12 +1,38 @@
 // The tensor-core kernels multiply whole tiles: a key that a row does not see has weight 0 there, and 0 * NaN or 0 * inf is NaN.  So
 // whenever a result that is not finite comes out of a piece, its rows are worked out again here, on the CUDA cores and from the
 // visible keys alone.  A NaN that the visible keys do hold comes out again; finite data never gets here.
+// A warp takes its rows key by key, which over a long table can take seconds (32 rows a warp by 173,000 keys: 3), longer than the
+// other warps of the CTA may wait for one another.
 #pragma once
 #include "cache_common.cuh"
 #include "tc_common.cuh"
 
 namespace chill {
 namespace cache {
+
+// The waits of the tensor-core kernels, bounded as tc::mbar_wait's; but warps that repair are at work, not stuck, so how long a waiter waits (units of
+// 2^20 ns) stands in the word behind the abort flag: kWaitLimitNs at first, and who repairs adds the time that it has taken so far.  A repair ends
+// by itself after rows times keys steps, so every wait ends.
+constexpr int kLimitShift = 20;
+constexpr int kFirstLimit = (int)(tc::kWaitLimitNs >> kLimitShift);
+__device__ __forceinline__ bool bounded_wait(uint32_t bar, uint32_t parity, const tc::Guard& g, int code) {
+  if (tc::mbar_try_wait(bar, parity)) return true;
+  uint64_t t0 = 0;
+  for (uint32_t it = 1;; ++it) {
+    if (tc::mbar_try_wait(bar, parity)) return true;
+    if ((it & 7u) == 0u) {
+      if (*g.abort) return false;
+      const uint64_t t = tc::globaltimer_ns();
+      if (t0 == 0) {
+        t0 = t;
+      } else if ((uint32_t)((t - t0) >> kLimitShift) > (uint32_t)g.abort[1]) {
+        atomicCAS(g.status, 0, code);
+        *g.abort = 1;
+        return false;
+      }
+    }
+  }
+}
 
 // Whether any of 128 threads (four warps) says so; also a barrier between their stores before and after it.
 __device__ __forceinline__ bool consumers_any(bool x, int bar = 2) {
@@ -24,12 +50,15 @@ __device__ __forceinline__ bool consumers_any(bool x, int bar = 2) {
   return any != 0;
 }
 
-// Rows row0, row0 + warps, ... below `end` of a piece again, one row a warp, lanes over the channels, key by key.
+// Rows row0, row0 + warps, ... below `end` of a piece again, one row a warp, lanes over the channels, key by key.  `limit`: of the
+// other warps' waits, where there are any.
 template <typename T, int DP, class M, bool kMany = false>
-__device__ __noinline__ void repair_piece(const CachedP& p, const RowTile& t, const Piece& piece, int row0, int warps, int end = 1 << 30) {
+__device__ __noinline__ void repair_piece(const CachedP& p, const RowTile& t, const Piece& piece, int row0, int warps, int end, volatile int* limit) {
   const int lane = threadIdx.x & 31;
   constexpr int kOwn = DP / 32;  // channels of a lane: lane, lane + 32, ...
   const int last = imin(t.k_lo + piece.t1 * kKeyTile, t.total);
+  const uint64_t begun = tc::globaltimer_ns();
+  const int before = limit != nullptr ? *limit : 0;
   for (int r = row0; r < imin(t.rows, end); r += warps) {
     const int i = (t.r0 + r) / p.G, h = piece.head * p.G + (t.r0 + r) % p.G, pos = token_position(p, t, i);
     const T* qr = row_ptr<T>(p.q, t.b, h, i);
@@ -40,6 +69,7 @@ __device__ __noinline__ void repair_piece(const CachedP& p, const RowTile& t, co
       o[c] = 0.f;
     }
     for (int key = t.k_lo + piece.t0 * kKeyTile; key < last; ++key) {
+      if (limit != nullptr && key % kKeyTile == 0 && lane == 0) *limit = imax(*limit, before + (int)((tc::globaltimer_ns() - begun) >> kLimitShift));
       const int page = p.table[t.b * p.table_sb + key / p.page];
       if (page < 0 || page >= p.num_pages || !sees<M>(p, t, i, pos, key)) continue;
       const int row = key % p.page;

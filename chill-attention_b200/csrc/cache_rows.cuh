@@ -44,7 +44,7 @@ struct RowsShape {
   static constexpr int kStat = kQ + 2 * kQBytes + kBetween;    // maximum and sum of each warp's rows
   static constexpr int kBars = kStat + 4 * kRows * 8;          // full[stage], empty[stage], item_full[2], item_empty[2]
   static constexpr int kHoles = kBars + (2 * kStages + 4) * 8; // groups of 8 keys without a page, a word per stage
-  static constexpr int kMisc = kHoles + kStages * 4;
+  static constexpr int kMisc = kHoles + kStages * 4;            // abort flag, limit of the waits
   static constexpr int kItems = (kMisc + 16 + 15) / 16 * 16;
   static constexpr int kCum = kItems + 2 * (int)sizeof(Item);
   static constexpr int kTotal = kCum + (kScanEntries + 1) * 4;
@@ -94,7 +94,8 @@ cached_rows_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constan
   Item* items = reinterpret_cast<Item*>(gen + S::kItems);
   const tc::Guard guard{p.status, abort_flag};
   if (threadIdx.x == 0) {
-    *abort_flag = 0;
+    abort_flag[0] = 0;
+    abort_flag[1] = kFirstLimit;
     for (int s = 0; s < kStages; ++s) {
       tc::mbar_init(full + 8 * s, 1);
       tc::mbar_init(empty + 8 * s, 4);
@@ -128,7 +129,7 @@ cached_rows_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constan
     for (int item = 0;; ++item) {
       const bool more = work.next<M>(p, it);
       const int slot = item & 1;
-      ok = __all_sync(0xffffffffu, tc::mbar_wait(item_empty + 8 * slot, ((uint32_t)(item >> 1) & 1u) ^ 1u, guard, kStRowsProducer));
+      ok = __all_sync(0xffffffffu, bounded_wait(item_empty + 8 * slot, ((uint32_t)(item >> 1) & 1u) ^ 1u, guard, kStRowsProducer));
       if (!ok) break;
       const RowTile& t = it.t;
       const uint32_t sq = base + S::kQ + slot * (S::kQBytes + S::kBetween), bar = item_full + 8 * slot;
@@ -160,7 +161,7 @@ cached_rows_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constan
         there = there_next;
         if (kt + 1 < it.tiles) page_next = tile_page(p, t, k0 + kKeyTile, mine, there_next);
         const unsigned lost = __ballot_sync(0xffffffffu, !there && lane < boxes);
-        ok = __all_sync(0xffffffffu, tc::mbar_wait(empty + 8 * s, ((uint32_t)(n / kStages) & 1u) ^ 1u, guard, kStRowsProducer));
+        ok = __all_sync(0xffffffffu, bounded_wait(empty + 8 * s, ((uint32_t)(n / kStages) & 1u) ^ 1u, guard, kStRowsProducer));
         if (!ok) break;
         if (lane == 0) {
           holes[s] = lost_groups(p, lost, boxes);
@@ -194,7 +195,7 @@ cached_rows_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constan
   for (int item = 0;; ++item) {
     const int slot = item & 1;
     // The four warps leave together: whether there is one more piece, and whether all of them saw it, is settled at a barrier
-    bool leave = !__all_sync(0xffffffffu, tc::mbar_wait(item_full + 8 * slot, (uint32_t)(item >> 1) & 1u, guard, kStRowsConsumer));
+    bool leave = !__all_sync(0xffffffffu, bounded_wait(item_full + 8 * slot, (uint32_t)(item >> 1) & 1u, guard, kStRowsConsumer));
     if (!leave) leave = items[slot].x.entry < 0;
     if (consumers_any(leave)) break;
     const RowTile& t = items[slot].t;
@@ -223,7 +224,7 @@ cached_rows_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constan
     for (int kt = piece.t0; kt < tiles; ++kt) {
       const int s = stage, k0 = k_lo + kt * kKeyTile;
       const uint32_t sk = base + S::kRing + s * 2 * S::kTileBytes, sv = sk + S::kTileBytes;
-      ok = __all_sync(0xffffffffu, tc::mbar_wait(full + 8 * s, phase, guard, kStRowsConsumer));
+      ok = __all_sync(0xffffffffu, bounded_wait(full + 8 * s, phase, guard, kStRowsConsumer));
       if (!ok) break;  // the rest of the piece is skipped; the next one's wait fails at once
       float c[MT][2][4];
 #pragma unroll
@@ -414,7 +415,7 @@ cached_rows_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constan
         else p.part_ml[(long long)piece.slot * p.rows + r] = make_float2(top, sum);
       }
     }
-    if (consumers_any(odd)) repair_piece<T, DP, M>(p, t, piece, warp, 4);
+    if (consumers_any(odd)) repair_piece<T, DP, M>(p, t, piece, warp, 4, S::kRows, abort_flag + 1);
     if (p.D < DP) {  // the channels beyond the head become 0 again
       tc::named_bar_sync(1, 128);
       for (int idx = threadIdx.x; idx < S::kQBytes / 16; idx += 128) *reinterpret_cast<uint4*>(gen + (sq - base) + idx * 16) = make_uint4(0u, 0u, 0u, 0u);

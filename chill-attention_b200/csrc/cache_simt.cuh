@@ -258,7 +258,7 @@ __global__ void __launch_bounds__(kSimtThreads, (SimtSmem<DP, RT>::kCtasPerSm)) 
         else store_lse(p, t.b, h, i, valid, m[n], l[n]);
       }
     }
-    if (consumers_any(odd)) repair_piece<T, DP, M>(p, t, piece, warp, 4);
+    if (consumers_any(odd)) repair_piece<T, DP, M>(p, t, piece, warp, 4, L::kRows, nullptr);
   }
 }
 

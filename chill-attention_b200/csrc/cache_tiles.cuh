@@ -114,7 +114,8 @@ cached_tiles_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_consta
   Item* items = reinterpret_cast<Item*>(gen + S::kItems);
   const tc::Guard guard{p.status, abort_flag};
   if (threadIdx.x == 0) {
-    *abort_flag = 0;
+    abort_flag[0] = 0;
+    abort_flag[1] = kFirstLimit;
     for (int s = 0; s < kStages; ++s) {
       tc::mbar_init(k_full + 8 * s, 1);
       tc::mbar_init(v_full + 8 * s, 1);
@@ -166,7 +167,7 @@ cached_tiles_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_consta
     for (int item = 0;; ++item) {
       const bool more = work.next<M>(p, it);
       const int slot = item & 1;
-      ok = __all_sync(0xffffffffu, tc::mbar_wait(item_empty + 8 * slot, ((uint32_t)(item >> 1) & 1u) ^ 1u, guard, kStTilesProducer));
+      ok = __all_sync(0xffffffffu, bounded_wait(item_empty + 8 * slot, ((uint32_t)(item >> 1) & 1u) ^ 1u, guard, kStTilesProducer));
       if (!ok) break;
       const RowTile& t = it.t;
       if (lane == 0) {
@@ -179,7 +180,7 @@ cached_tiles_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_consta
       bool there = false, there_next = false;
       int page = 0, page_next = tile_page(p, t, t.k_lo + it.x.t0 * kKeyTile, mine, there_next);
       // Q: the last product with the piece before's is done
-      ok = __all_sync(0xffffffffu, tc::mbar_wait(q_empty, ((uint32_t)loads & 1u) ^ 1u, guard, kStTilesProducer));
+      ok = __all_sync(0xffffffffu, bounded_wait(q_empty, ((uint32_t)loads & 1u) ^ 1u, guard, kStTilesProducer));
       if (!ok) break;
       ++loads;
       if (lane == 0) tc::mbar_arrive_expect_tx(q_full, (uint32_t)(NQ * half * S::kChunks * 128));
@@ -194,7 +195,7 @@ cached_tiles_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_consta
         there = there_next;
         if (kt + 1 < it.tiles) page_next = tile_page(p, t, k0 + kKeyTile, mine, there_next);
         const unsigned lost = __ballot_sync(0xffffffffu, !there && lane < boxes);
-        ok = __all_sync(0xffffffffu, tc::mbar_wait(kv_free + 8 * s, ((uint32_t)(n / kStages) & 1u) ^ 1u, guard, kStTilesProducer));
+        ok = __all_sync(0xffffffffu, bounded_wait(kv_free + 8 * s, ((uint32_t)(n / kStages) & 1u) ^ 1u, guard, kStTilesProducer));
         if (!ok) break;
         if (lane == 0) {
           holes[s] = lost_groups(p, lost, boxes);
@@ -229,7 +230,7 @@ cached_tiles_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_consta
     bool ok = true;
     for (int item = 0; ok; ++item) {
       const int slot = item & 1;
-      ok = __all_sync(0xffffffffu, tc::mbar_wait(item_full + 8 * slot, (uint32_t)(item >> 1) & 1u, guard, kStTilesMma));
+      ok = __all_sync(0xffffffffu, bounded_wait(item_full + 8 * slot, (uint32_t)(item >> 1) & 1u, guard, kStTilesMma));
       if (!ok) break;
       const int entry = items[slot].x.entry, count = items[slot].tiles - items[slot].x.t0;
       __syncwarp();
@@ -239,7 +240,7 @@ cached_tiles_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_consta
       if (lane == 0) {
         auto issue_s = [&](uint32_t sb) -> bool {  // S = Q K^T; the buffer's P has been used by a product issued before
           const uint32_t k_lo = tc::desc_lo_sw128(base + S::kK + s_slot * S::kKvBytes, 16);
-          if (!tc::mbar_wait(k_full + 8 * s_slot, s_phase, guard, kStTilesMma)) return false;
+          if (!bounded_wait(k_full + 8 * s_slot, s_phase, guard, kStTilesMma)) return false;
           tc::tc_fence_after();
 #pragma unroll
           for (int kk = 0; kk < DP / 16; ++kk)
@@ -248,16 +249,16 @@ cached_tiles_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_consta
           if (++s_slot == kStages) s_slot = 0, s_phase ^= 1u;
           return true;
         };
-        ok = tc::mbar_wait(q_full, (uint32_t)pieces & 1u, guard, kStTilesMma);
+        ok = bounded_wait(q_full, (uint32_t)pieces & 1u, guard, kStTilesMma);
         if (ok) ok = issue_s(n & 1u);
         for (int j = 0; j < count && ok; ++j, ++n) {
           if (j + 1 < count) ok = issue_s((n + 1) & 1u);
           if (!ok) break;
           const bool first = j == 0;
           const uint32_t sb = n & 1u, v_lo = tc::desc_lo_sw128(base + S::kV + v_slot * S::kKvBytes, S::kKvChunk);  // MN-major: channel blocks one chunk apart
-          if (!(ok = tc::mbar_wait(v_full + 8 * v_slot, v_phase, guard, kStTilesMma))) break;
-          if (first && !(ok = tc::mbar_wait(o_empty, ((uint32_t)pieces & 1u) ^ 1u, guard, kStTilesMma))) break;
-          if (!(ok = tc::mbar_wait(p_full + 8 * sb, (n >> 1) & 1u, guard, kStTilesMma))) break;
+          if (!(ok = bounded_wait(v_full + 8 * v_slot, v_phase, guard, kStTilesMma))) break;
+          if (first && !(ok = bounded_wait(o_empty, ((uint32_t)pieces & 1u) ^ 1u, guard, kStTilesMma))) break;
+          if (!(ok = bounded_wait(p_full + 8 * sb, (n >> 1) & 1u, guard, kStTilesMma))) break;
           tc::tc_fence_after();
 #pragma unroll
           for (int kk = 0; kk < kKeyTile / 16; ++kk)  // O += P V
@@ -289,7 +290,7 @@ cached_tiles_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_consta
     for (int item = 0;; ++item) {
       const int slot = item & 1;
       // The warps leave together: whether there is one more piece, and whether all of them saw it, is settled at a barrier
-      bool leave = !__all_sync(0xffffffffu, tc::mbar_wait(item_full + 8 * slot, (uint32_t)(item >> 1) & 1u, guard, kStTilesSoftmax));
+      bool leave = !__all_sync(0xffffffffu, bounded_wait(item_full + 8 * slot, (uint32_t)(item >> 1) & 1u, guard, kStTilesSoftmax));
       if (!leave) leave = items[slot].x.entry < 0;
       if (consumers_any(leave, 2 + grp)) break;
       const RowTile& t = items[slot].t;
@@ -304,7 +305,7 @@ cached_tiles_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_consta
       for (int j = 0; j < count; ++j, ++n) {
         const int s = n % kStages, sb = n & 1, k0 = k_lo + (t0 + j) * kKeyTile;
         const uint32_t tS = tmem + sb * kKeyTile + lane_sel;
-        ok = __all_sync(0xffffffffu, tc::mbar_wait(s_full + 8 * sb, (uint32_t)(n >> 1) & 1u, guard, kStTilesSoftmax));
+        ok = __all_sync(0xffffffffu, bounded_wait(s_full + 8 * sb, (uint32_t)(n >> 1) & 1u, guard, kStTilesSoftmax));
         if (!ok) break;
         tc::tc_fence_after();
         const int lost = holes[s];
@@ -340,7 +341,7 @@ cached_tiles_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_consta
           // the accumulation of the tile before must be done before O is touched
           const uint32_t done = NQ == 1 ? kv_free + 8 * (uint32_t)((n - 1) % kStages) : s_full + 32 + 8 * (uint32_t)((n - 1) & 1);
           const uint32_t parity = (uint32_t)((n - 1) / (NQ == 1 ? kStages : 2)) & 1u;
-          ok = __all_sync(0xffffffffu, tc::mbar_wait(done, parity, guard, kStTilesSoftmax));
+          ok = __all_sync(0xffffffffu, bounded_wait(done, parity, guard, kStTilesSoftmax));
           if (!ok) break;
           tc::tc_fence_after();
           const bool moves = m_cand - m_used > 8.f;  // a row goes by itself: rows that do not exist hold anything
@@ -386,7 +387,7 @@ cached_tiles_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_consta
         if (full) l = fmaf(top, 0.f, l);
         tc::tmem_st32(tS, x);
         if (k0 + kKeyTile > total) {  // rows of V behind the last key may hold anything, and 0 * NaN is NaN: they become 0
-          ok = __all_sync(0xffffffffu, tc::mbar_wait(v_full + 8 * s, (uint32_t)(n / kStages) & 1u, guard, kStTilesSoftmax));
+          ok = __all_sync(0xffffffffu, bounded_wait(v_full + 8 * s, (uint32_t)(n / kStages) & 1u, guard, kStTilesSoftmax));
           if (!ok) break;
           const int gone = imax(total - k0, 0);
           // both groups write the same zeros: neither's product may start before its own have been written
@@ -401,7 +402,7 @@ cached_tiles_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_consta
         __syncwarp();
         if (lane == 0) tc::mbar_arrive(p_full + 8 * sb);
       }
-      if (ok && count > 0) ok = __all_sync(0xffffffffu, tc::mbar_wait(o_full, (uint32_t)pieces & 1u, guard, kStTilesEpilogue));
+      if (ok && count > 0) ok = __all_sync(0xffffffffu, bounded_wait(o_full, (uint32_t)pieces & 1u, guard, kStTilesEpilogue));
       tc::tc_fence_after();
       const int unit_row = t.r0 + row;
       const bool exists = r < half && unit_row < p.N * p.G;
@@ -455,7 +456,7 @@ cached_tiles_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_consta
         if (lane == 0) tc::mbar_arrive(o_empty);
         ++pieces;
       }
-      if (consumers_any(odd, 2 + grp)) repair_piece<T, DP, M, true>(p, t, piece, grp * half + (warp & 3), 4, (grp + 1) * half);
+      if (consumers_any(odd, 2 + grp)) repair_piece<T, DP, M, true>(p, t, piece, grp * half + (warp & 3), 4, (grp + 1) * half, abort_flag + 1);
       __syncwarp();
       if (lane == 0) tc::mbar_arrive(item_empty + 8 * slot);
     }

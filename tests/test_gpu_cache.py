@@ -758,3 +758,25 @@ def test_scores_of_minus_infinity_everywhere(dtype, N, D):
     (o, lse), _ = attend(p, masks()["causal"])
     assert (o[:, 2:] == 0).all() and torch.isneginf(lse[:, 2:]).all()
     assert torch.isfinite(o[:, :2]).all() and torch.isfinite(lse[:, :2]).all()
+
+
+def test_a_repair_may_take_longer_than_a_wait(_lib):
+    """A key that is not finite, behind 400,000 others: its rows are worked out again key by key for seconds, which the other warps of the CTA
+    have to sit out.  The other request, whose turn comes after it in the same CTA, is served as if nothing had been."""
+    import chill_attention as ca
+
+    H, N, D, page, lens = 64, 256, 64, 64, [400000, 3000]
+    blocks = [-(-(c + N) // page) for c in lens]
+    g = torch.Generator(device="cuda").manual_seed(1)
+    kc, vc = (torch.randn(sum(blocks), 1, page, D, device="cuda", dtype=torch.bfloat16, generator=g) for _ in range(2))
+    table = torch.full((2, max(blocks)), -1, dtype=torch.int32, device="cuda")
+    table[0], table[1, :blocks[1]] = torch.arange(blocks[0]), torch.arange(blocks[0], sum(blocks))
+    q = torch.randn(2, H, N, D, device="cuda", dtype=torch.bfloat16, generator=g)
+    positions = ints(lens)[:, None] + torch.arange(N, device="cuda", dtype=torch.int32)
+    step = ca.ChillStep(ints(lens), ints([N, N]), positions, positions, None)
+    want, want_lse = ca.chill_attention_cached(q, kc, vc, table, step, ca.CausalChillMask(), return_lse=True)
+    kc[399990 // page, 0, 399990 % page] = float("nan")
+    o, lse = ca.chill_attention_cached(q, kc, vc, table, step, ca.CausalChillMask(), return_lse=True)
+    assert torch.equal(o[1], want[1]) and torch.equal(lse[1], want_lse[1])
+    assert torch.isnan(o[0]).all() and torch.isnan(lse[0]).all()
+    assert _lib.chill_cache_read_device_status() == 0
