@@ -14,8 +14,8 @@ ABI_VERSION = 1
 CACHED_CUDA_CORES, CACHED_ROWS, CACHED_TILES = range(3)
 
 EXPORTS = (
-    "chill_pages_reserve", "chill_pages_trim", "chill_cache_append", "chill_cache_commit", "chill_cached_workspace_bytes",
-    "chill_cached_fwd", "chill_cached_kernel", "chill_cache_read_device_status", "chill_cache_launch_count",
+    "chill_pages_reserve", "chill_pages_reserve_stored", "chill_pages_trim", "chill_cache_append", "chill_cache_commit",
+    "chill_cached_workspace_bytes", "chill_cached_fwd", "chill_cached_kernel", "chill_cache_read_device_status", "chill_cache_launch_count",
     "chill_cache_last_cuda_error", "chill_cache_abi_version",
 )
 
@@ -65,6 +65,8 @@ def load_library(path: str | None = None) -> C.CDLL:
                            ("chill_cache_commit", CacheRowsArgs), ("chill_cached_fwd", CachedArgs)):
             getattr(lib, name).argtypes = [C.POINTER(args), C.c_void_p]
             getattr(lib, name).restype = C.c_int
+        lib.chill_pages_reserve_stored.argtypes = [C.POINTER(PagesArgs), C.c_void_p, C.c_void_p]
+        lib.chill_pages_reserve_stored.restype = C.c_int
         lib.chill_cached_workspace_bytes.argtypes = [C.POINTER(CachedArgs)]
         lib.chill_cached_workspace_bytes.restype = C.c_size_t
         lib.chill_cached_kernel.argtypes = [C.POINTER(CachedArgs)]

@@ -11,7 +11,7 @@ for each request, a chunk of a prompt, or a tree of drafted tokens) over the cac
         o = chill_attention_cached(q, k_cache, v_cache, pages.table, step, mask)
         # a tree: choose the path to keep, then
         lens = chill_cache_commit(k_cache, v_cache, pages.table, step, path, accepted)
-        # a chain: lens = lens + new_lens
+        # a chain: lens = lens + step.stored   (new_lens, unless pages ran out: what got no page comes again in a later step)
     chill_pages_trim(pages, lens, page_size)                              # lens[b] = 0: request b is done
 
 Nothing here synchronises or copies to the host, lengths are read on the GPU, and every call can be captured into a CUDA graph and
@@ -33,7 +33,7 @@ from .mask import ChillMask
 _HEAD_DIMS = chill._HEAD_DIMS
 _DTYPES = (torch.float32, torch.float16, torch.bfloat16)
 #: entry points a native CacheLibrary object is made of, in its order
-_ENTRY_POINTS = ("chill_cached_fwd", "chill_cached_workspace_bytes", "chill_pages_reserve", "chill_pages_trim", "chill_cache_append",
+_ENTRY_POINTS = ("chill_cached_fwd", "chill_cached_workspace_bytes", "chill_pages_reserve_stored", "chill_pages_trim", "chill_cache_append",
                  "chill_cache_commit")
 #: library -> its native call object; mask class name -> (call object, functor id, class)
 _NATIVE: dict = {}
@@ -64,13 +64,15 @@ class ChillPages(typing.NamedTuple):
 class ChillStep(typing.NamedTuple):
     """The new tokens of a step, int32 tensors on the GPU: lens [batch] tokens in the cache before, new_lens [batch] new ones,
     slots [batch, max_new] page * page_size + row of each (-1: none), positions [batch, max_new], and for trees ancestors
-    [batch, max_new, (max_new + 31) // 32]: bit j of row i says that token j is token i or above it."""
+    [batch, max_new, (max_new + 31) // 32]: bit j of row i says that token j is token i or above it; stored [batch] how many of the new
+    tokens got a slot, the first so many: all of them unless pages ran out."""
 
     lens: torch.Tensor
     new_lens: torch.Tensor
     slots: torch.Tensor
     positions: torch.Tensor
     ancestors: typing.Optional[torch.Tensor]
+    stored: typing.Optional[torch.Tensor] = None
 
 
 def _native(lib=None):
@@ -163,19 +165,19 @@ def _check_attention(q, k_cache, v_cache, table, lens, new_lens, positions, ance
 @torch.library.custom_op("chill_attention::pages_reserve", mutates_args=("table", "held", "free", "n_free", "missing"), device_types=("cuda",))
 def _reserve_op(table: torch.Tensor, held: torch.Tensor, free: torch.Tensor, n_free: torch.Tensor, missing: torch.Tensor, lens: torch.Tensor,
                 new_lens: torch.Tensor, max_new: int, page_size: int,
-                parents: typing.Optional[torch.Tensor]) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+                parents: typing.Optional[torch.Tensor]) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor]:
     _check_pages(ChillPages(table, held, free, n_free, missing), lens, page_size)
     _check_reserve(ChillPages(table, held, free, n_free, missing), new_lens, max_new, parents)
-    slots, positions, ancestors = _eager.extension().pages_reserve(_native(), table, held, free, n_free, missing, lens, new_lens, max_new,
-                                                                   page_size, parents)
-    return slots, positions, ancestors if ancestors is not None else slots.new_empty(0)
+    slots, positions, ancestors, stored = _eager.extension().pages_reserve(_native(), table, held, free, n_free, missing, lens, new_lens, max_new,
+                                                                           page_size, parents)
+    return slots, positions, ancestors if ancestors is not None else slots.new_empty(0), stored
 
 
 @_reserve_op.register_fake
 def _(table, held, free, n_free, missing, lens, new_lens, max_new, page_size, parents):
     B = table.shape[0]
     shape = (B, max_new, (max_new + 31) // 32) if parents is not None else (0,)
-    return table.new_empty(B, max_new), table.new_empty(B, max_new), table.new_empty(shape)
+    return table.new_empty(B, max_new), table.new_empty(B, max_new), table.new_empty(shape), table.new_empty(B)
 
 
 @torch.library.custom_op("chill_attention::pages_trim", mutates_args=("table", "held", "free", "n_free"), device_types=("cuda",))
@@ -243,7 +245,9 @@ def chill_pages_reserve(pages: ChillPages, lens: torch.Tensor, new_lens: torch.T
     Args:
         pages: changed in place.  Pages are taken from the top of the stack, requests in order; a request keeps what it holds
             already.  Where the stack runs out, or a table is full, the tokens left without a page get slot -1 (they are not
-            stored, and nobody sees them) and ``pages.missing`` says how many pages the stack was short of.
+            stored, and nobody sees them) and ``pages.missing`` says how many pages the stack was short of.  Only the ``step.stored[b]``
+            others may be counted in lens afterwards: a page that a later step finds for a token that was never stored holds what its
+            former owner left there.
         lens, new_lens: int32 [batch]; new_lens is clamped to [0, max_new].
         max_new: second dimension of the step's tensors.
         page_size: rows of a page of the caches.
@@ -259,8 +263,8 @@ def chill_pages_reserve(pages: ChillPages, lens: torch.Tensor, new_lens: torch.T
             return ChillStep(lens, new_lens, *out)
     _check_pages(pages, lens, page_size)
     _check_reserve(pages, new_lens, max_new, parents)
-    slots, positions, ancestors = _reserve_op(*pages, lens, new_lens, max_new, page_size, parents)
-    return ChillStep(lens, new_lens, slots, positions, ancestors if parents is not None else None)
+    slots, positions, ancestors, stored = _reserve_op(*pages, lens, new_lens, max_new, page_size, parents)
+    return ChillStep(lens, new_lens, slots, positions, ancestors if parents is not None else None, stored)
 
 
 def chill_pages_trim(pages: ChillPages, lens: torch.Tensor, page_size: int) -> None:
@@ -291,7 +295,7 @@ def chill_cache_commit(k_cache: torch.Tensor, v_cache: torch.Tensor, table: torc
         path: int32 [batch, longest path], numbers of the accepted tokens from the root on (increasing).
         accepted: int32 [batch], how many of them; clamped to [0, min(longest path, new_lens[b])].
 
-    Returns: int32 [batch], the new lengths ``lens + accepted``.  Pages stay reserved; ``chill_pages_trim`` gives spare ones back.
+    Returns: int32 [batch], the new lengths ``lens + accepted``, without the accepted tokens from the first one without a page on.  Pages stay reserved; ``chill_pages_trim`` gives spare ones back.
     """
     N = step.slots.shape[1]
     if _direct():
@@ -355,7 +359,7 @@ def _attention(q, k_cache, v_cache, table, step, mask, sm_scale, return_lse, fla
         _mask_functor(mask)
     elif not _is_compiling() and _MASKS[mask.name][2] is not type(mask):
         _check_same_name(mask)
-    lens, new_lens, _, positions, ancestors = step
+    lens, new_lens, _, positions, ancestors = step[:5]
     if _direct():
         native, functor_id, _ = _MASKS[mask.name]
         out = _eager._extension.cached_attention(native, functor_id, q, k_cache, v_cache, table, lens, new_lens, positions, ancestors,

@@ -38,6 +38,7 @@ struct PagesP {
   int *held, *free_pages, *n_free, *missing;
   const int *lens, *new_lens, *parents;
   int *slots, *positions, *ancestors;
+  int* stored;  // may be null
 };
 
 __device__ __forceinline__ void cluster_sync() {
@@ -137,7 +138,7 @@ __global__ void __launch_bounds__(kPageThreads) pages_kernel(PagesP p, int ctas)
     pages_of<kTrim>(p, b, held, need);
     const int off = before[b - b0];
     int* row = p.table + b * p.table_sb;
-    __syncwarp();  // all lanes have read held[b]
+    __syncwarp();  // all lanes have read held[b] and off
     if (kTrim) {
       for (int j = lane; j < held - need; j += 32) {
         const int at = n_free + sum - 1 - (off + j);
@@ -148,7 +149,10 @@ __global__ void __launch_bounds__(kPageThreads) pages_kernel(PagesP p, int ctas)
     } else {
       const int got = imin(imax(need - held, 0), imax(n_free - off, 0));
       for (int j = lane; j < got; j += 32) row[held + j] = p.free_pages[n_free - 1 - (off + j)];
-      if (lane == 0) p.held[b] = held + got;
+      if (lane == 0) {
+        p.held[b] = held + got;
+        before[b - b0] = p.N;  // from here on: number of the first new token without a slot (all lanes have read `off`)
+      }
     }
   }
   if (rank == ctas - 1 && threadIdx.x == 0) {
@@ -173,6 +177,11 @@ __global__ void __launch_bounds__(kPageThreads) pages_kernel(PagesP p, int ctas)
       if (page >= 0 && page < p.num_pages) slot = page * p.page + (t - block * p.page);
     }
     p.slots[(long long)b * p.N + i] = slot;
+    if (slot < 0 && i <= fresh) atomicMin(&before[own], i);
+  }
+  if (p.stored != nullptr) {
+    __syncthreads();
+    for (int own = threadIdx.x; own < b1 - b0; own += kPageThreads) p.stored[b0 + own] = before[own];
   }
   if ((int)gridDim.x == ctas) place_tokens(p, (long long)rank * kPageThreads + threadIdx.x, (long long)ctas * kPageThreads);
 }
@@ -213,7 +222,7 @@ static int check_pages(const chill_pages_args* a, bool trim) {
   return CHILL_OK;
 }
 
-static PagesP pages_params(const chill_pages_args& a) {
+static PagesP pages_params(const chill_pages_args& a, int32_t* stored) {
   PagesP p{};
   p.B = a.B; p.N = a.N; p.page = a.page_size; p.num_pages = a.num_pages; p.width = a.table_width;
   p.words = (a.N + 31) / 32;
@@ -221,6 +230,7 @@ static PagesP pages_params(const chill_pages_args& a) {
   p.held = a.held; p.free_pages = a.free_pages; p.n_free = a.n_free; p.missing = a.missing;
   p.lens = a.lens; p.new_lens = a.new_lens; p.parents = a.parents;
   p.slots = a.slots; p.positions = a.positions; p.ancestors = a.ancestors;
+  p.stored = stored;
   return p;
 }
 
@@ -266,6 +276,8 @@ __global__ void __launch_bounds__(256) append_kernel(RowsP p) {
 // Row lens[b] + path[b][j] -> row lens[b] + j for j < accepted[b].  The path increases, so path[j] >= j: no row is written before
 // the rows that it is the source of have been read, as long as j runs upwards.  A thread owns one vector of every row (of K or of
 // V), so no two threads meet; it reads kBatch rows before it writes them, which only reads rows earlier than the order asks for.
+// A row without a page was never stored, so the path ends there: a CTA of its own, a lane for each token of the path, works out how long it is
+// (by the thread of the first vector, on its way, it took the call 2 us longer: 9 of 64 drafts for 128 requests, 22.6 us with the append).
 constexpr int kBatch = 8;
 
 template <typename V>
@@ -273,21 +285,35 @@ __global__ void __launch_bounds__(128) commit_kernel(RowsP p) {
   for (int b = blockIdx.y; b < p.B; b += gridDim.y) {
     const int cached = clamp_len(p.lens[b]), fresh = imin(imax(p.new_lens[b], 0), p.N);
     const int take = imin(imin(imax(p.accepted[b], 0), p.A), fresh);
-    if (blockIdx.x == 0 && threadIdx.x == 0) p.out_lens[b] = cached + take;
+    const int* table = p.table + b * p.table_sb;
+    const int* path = p.path + (long long)b * p.A;
+    auto page_of = [&](int t) -> int {  // -1 where there is none
+      const int block = t / p.page, page = block < p.width ? table[block] : -1;
+      return page < p.num_pages ? imax(page, -1) : -1;
+    };
+    if (blockIdx.x == gridDim.x - 1) {
+      if (threadIdx.x >= 32) continue;
+      int kept = take;
+      for (int j0 = 0; j0 < take; j0 += 32) {
+        const int j = j0 + (int)threadIdx.x, from = j < take ? path[j] : 0;
+        const bool moves = from > j && from < fresh;
+        const unsigned lost = __ballot_sync(0xffffffffu, j < take && (page_of(cached + j) < 0 || (moves && page_of(cached + from) < 0)));
+        if (lost == 0) continue;
+        kept = j0 + __ffs(lost) - 1;
+        break;
+      }
+      if (threadIdx.x == 0) p.out_lens[b] = cached + kept;
+      continue;
+    }
     const int idx = blockIdx.x * 128 + threadIdx.x;
     if (idx >= 2 * p.per_token) continue;
     const bool is_v = idx >= p.per_token;
     const int rem = is_v ? idx - p.per_token : idx, h = rem / p.per_row, c = rem - h * p.per_row;
     const long long* st = is_v ? p.vcs : p.kcs;
     char* base = (is_v ? p.vc : p.kc) + h * st[1] + c * st[3];
-    const int* table = p.table + b * p.table_sb;
-    const int* path = p.path + (long long)b * p.A;
     auto row_of = [&](int t) -> char* {  // nullptr where there is no page
-      const int block = t / p.page;
-      if (block >= p.width) return nullptr;
-      const int page = table[block];
-      if (page < 0 || page >= p.num_pages) return nullptr;
-      return base + page * st[0] + (t - block * p.page) * st[2];
+      const int page = page_of(t);
+      return page < 0 ? nullptr : base + page * st[0] + t % p.page * st[2];
     };
     int from[kBatch];  // asked for before it is known how many count: one trip to memory less
 #pragma unroll
@@ -344,14 +370,16 @@ using namespace chill::cache;
 
 extern "C" {
 
-int chill_pages_reserve(const chill_pages_args* a, void* stream) {
+int chill_pages_reserve_stored(const chill_pages_args* a, int32_t* stored, void* stream) {
   const int st = check_pages(a, false);
-  return st != CHILL_OK ? st : launch_pages<false>(pages_params(*a), (cudaStream_t)stream);
+  return st != CHILL_OK ? st : launch_pages<false>(pages_params(*a, stored), (cudaStream_t)stream);
 }
+
+int chill_pages_reserve(const chill_pages_args* a, void* stream) { return chill_pages_reserve_stored(a, nullptr, stream); }
 
 int chill_pages_trim(const chill_pages_args* a, void* stream) {
   const int st = check_pages(a, true);
-  return st != CHILL_OK ? st : launch_pages<true>(pages_params(*a), (cudaStream_t)stream);
+  return st != CHILL_OK ? st : launch_pages<true>(pages_params(*a, nullptr), (cudaStream_t)stream);
 }
 
 int chill_cache_append(const chill_cache_rows_args* a, void* stream) {
@@ -398,7 +426,7 @@ int chill_cache_commit(const chill_cache_rows_args* a, void* stream) {
   byte_strides(p.kcs, a->k_cache_strides, es, vec); byte_strides(p.vcs, a->v_cache_strides, es, vec);
   p.table = a->table; p.table_sb = a->table_stride; p.width = a->table_width;
   p.lens = a->lens; p.new_lens = a->new_lens; p.path = a->path; p.accepted = a->accepted; p.A = a->A; p.out_lens = a->out_lens;
-  const dim3 grid((unsigned)((2 * p.per_token + 127) / 128), (unsigned)imin(a->B, 65535));
+  const dim3 grid((unsigned)((2 * p.per_token + 127) / 128 + 1), (unsigned)imin(a->B, 65535));
   if (wide) commit_kernel<uint4><<<grid, 128, 0, (cudaStream_t)stream>>>(p);
   else if (es == 4) commit_kernel<uint32_t><<<grid, 128, 0, (cudaStream_t)stream>>>(p);
   else commit_kernel<uint16_t><<<grid, 128, 0, (cudaStream_t)stream>>>(p);

@@ -24,7 +24,7 @@ namespace {
 struct CacheLibrary {
   decltype(&chill_cached_fwd) fwd;
   decltype(&chill_cached_workspace_bytes) workspace_bytes;
-  decltype(&chill_pages_reserve) reserve;
+  decltype(&chill_pages_reserve_stored) reserve;
   decltype(&chill_pages_trim) trim;
   decltype(&chill_cache_append) append;
   decltype(&chill_cache_commit) commit;
@@ -95,7 +95,7 @@ py::object reserve(const CacheLibrary& lib, const Tensor& table, const Tensor& h
       !ints(missing, {1}, table) || !ints(lens, {B}, table) || !ints(new_lens, {B}, table) || (parents.has_value() && !ints(*parents, {B, N}, table)))
     return py::none();
   c10::cuda::CUDAGuard guard(table.device());
-  Tensor slots = empty({B, N}, at::kInt, table), positions = empty({B, N}, at::kInt, table), ancestors;
+  Tensor slots = empty({B, N}, at::kInt, table), positions = empty({B, N}, at::kInt, table), stored = empty({B}, at::kInt, table), ancestors;
   if (parents.has_value()) ancestors = empty({B, N, (N + 31) / 32}, at::kInt, table);
   chill_pages_args a{};
   a.B = (int32_t)B; a.N = (int32_t)N; a.page_size = (int32_t)page; a.num_pages = (int32_t)free.size(0); a.table_width = (int32_t)table.size(1);
@@ -105,8 +105,8 @@ py::object reserve(const CacheLibrary& lib, const Tensor& table, const Tensor& h
   a.lens = lens.const_data_ptr<int32_t>(); a.new_lens = new_lens.const_data_ptr<int32_t>(); a.parents = optional_ints(parents);
   a.slots = slots.mutable_data_ptr<int32_t>(); a.positions = positions.mutable_data_ptr<int32_t>();
   a.ancestors = parents.has_value() ? ancestors.mutable_data_ptr<int32_t>() : nullptr;
-  check(lib, lib.reserve(&a, current_stream(table)), "chill_pages_reserve");
-  return py::make_tuple(slots, positions, parents.has_value() ? py::cast(ancestors) : py::none());
+  check(lib, lib.reserve(&a, stored.mutable_data_ptr<int32_t>(), current_stream(table)), "chill_pages_reserve");
+  return py::make_tuple(slots, positions, parents.has_value() ? py::cast(ancestors) : py::none(), stored);
 }
 
 bool trim(const CacheLibrary& lib, const Tensor& table, const Tensor& held, const Tensor& free, const Tensor& n_free, const Tensor& lens, int64_t page) {
@@ -216,7 +216,7 @@ void bind_cache(py::module_& m) {
   py::class_<CacheLibrary, std::shared_ptr<CacheLibrary>>(m, "CacheLibrary").def(py::init([](const std::vector<uint64_t>& fn) {
     if (fn.size() != 8) throw py::value_error("eight entry points");
     return std::make_shared<CacheLibrary>(CacheLibrary{pointer<decltype(&chill_cached_fwd)>(fn[0]), pointer<decltype(&chill_cached_workspace_bytes)>(fn[1]),
-                          pointer<decltype(&chill_pages_reserve)>(fn[2]), pointer<decltype(&chill_pages_trim)>(fn[3]),
+                          pointer<decltype(&chill_pages_reserve_stored)>(fn[2]), pointer<decltype(&chill_pages_trim)>(fn[3]),
                           pointer<decltype(&chill_cache_append)>(fn[4]), pointer<decltype(&chill_cache_commit)>(fn[5]),
                           pointer<decltype(&chill_status_string)>(fn[6]), pointer<decltype(&chill_cache_last_cuda_error)>(fn[7])});
   }));

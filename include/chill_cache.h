@@ -48,6 +48,9 @@ typedef struct chill_pages_args {
  * (lens[b] + depth; without parents lens[b] + number) and ancestors of the new tokens.  Pages that a request holds beyond
  * that stay its own.  Where pages run out, or a table is full, the tokens without one get slot -1. */
 int chill_pages_reserve(const chill_pages_args* a, void* stream);
+/* The same, and in stored[b] (may be NULL) how many of a request's new tokens got a slot: the first so many.  Where there was a shortage only these
+ * may be counted in lens afterwards; the others' rows are never written, and a page that turns up for them later holds its former owner's. */
+int chill_pages_reserve_stored(const chill_pages_args* a, int32_t* stored, void* stream);
 /* Pages behind lens[b] tokens go back to the stack (lens[b] = 0: all), their table entries become -1.  The inverse of reserve: the
  * pages come back in the order in which reserving them again takes them. */
 int chill_pages_trim(const chill_pages_args* a, void* stream);
@@ -66,13 +69,13 @@ typedef struct chill_cache_rows_args {
   const int32_t *lens, *new_lens; /* [B] */
   const int32_t* path;            /* [B][A]: numbers of the accepted tokens, increasing */
   const int32_t* accepted;        /* [B]: how many of them, clamped to [0, min(A, new_lens[b])] */
-  int32_t* out_lens;              /* [B]: lens[b] + accepted[b]; not lens itself */
+  int32_t* out_lens;              /* [B]: lens[b] + accepted[b], as far as these have a page; not lens itself */
 } chill_cache_rows_args;
 
 /* Row (b, head, i) of k and v goes to slot slots[b][i] of the caches; slots outside the cache are skipped. */
 int chill_cache_append(const chill_cache_rows_args* a, void* stream);
 /* The accepted path of every tree becomes contiguous: for j < accepted[b], row lens[b] + path[b][j] is copied to row lens[b] + j
- * (path[b][j] <= j: it stays as it is). */
+ * (path[b][j] <= j: it stays as it is).  The path ends before the first token without a page. */
 int chill_cache_commit(const chill_cache_rows_args* a, void* stream);
 
 /* O = softmax(mask(Q K^T * sm_scale)) V of the new tokens over the cached and the new keys, and its LSE (log2 units).  The rows of

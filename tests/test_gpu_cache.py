@@ -780,3 +780,69 @@ def test_a_repair_may_take_longer_than_a_wait(_lib):
     assert torch.equal(o[1], want[1]) and torch.equal(lse[1], want_lse[1])
     assert torch.isnan(o[0]).all() and torch.isnan(lse[0]).all()
     assert _lib.chill_cache_read_device_status() == 0
+
+
+def test_a_session_that_runs_short_of_pages():
+    """Request 1 gets too few pages, request 0 leaves, request 1 goes on with what it was short of: its rows are those of a session that never
+    ran short, and nothing of request 0 is among its keys."""
+    import chill_attention as ca
+    from helpers import O_ATOL
+
+    page, D, total = 16, 64, 40
+    g = torch.Generator(device="cuda").manual_seed(2)
+    q, k, v = (torch.randn(2, h, total, D, device="cuda", generator=g) for h in (4, 2, 2))
+    want = ca.chill_attention(q, k, v, mask=ca.CausalChillMask())
+    pages = ca.ChillPages.empty(2, 64, 4, page)
+    kc, vc = (torch.full((4, 2, page, D), 50.0, device="cuda") for _ in range(2))
+    lens, done = ints([0, 0]), [0, 0]
+    stored = []
+    for turn, new in enumerate([(20, 10), (12, 30), (0, 8)]):
+        N = max(new)
+        row = lambda t: torch.stack([torch.nn.functional.pad(t[b, :, done[b]:done[b] + new[b]], (0, 0, 0, N - t[b, :, done[b]:done[b] + new[b]].shape[1])) for b in range(2)])  # noqa: E731
+        step = ca.chill_pages_reserve(pages, lens, ints(new), N, page)
+        stored.append(step.stored.tolist())
+        assert step.stored.tolist() == (step.slots >= 0).sum(1).tolist()
+        ca.chill_cache_append(kc, vc, row(k), row(v), step.slots)
+        o = ca.chill_attention_cached(row(q), kc, vc, pages.table, step, ca.CausalChillMask())
+        for b, n in enumerate(step.stored.tolist()):
+            if n > 0:  # both are within the operator's bar of the exact result
+                assert (o[b, :, :n] - want[b, :, done[b]:done[b] + n]).abs().max() <= 2 * O_ATOL[torch.float32]
+            done[b] += n
+        lens = lens + step.stored
+        assert lens.tolist() == done
+        if turn == 1:
+            assert pages.missing.item() == 1
+            lens, done = lens * ints([0, 1]), [0, done[1]]
+            ca.chill_pages_trim(pages, lens, page)
+    assert stored == [[20, 10], [12, 22], [0, 8]] and done == [0, total]
+
+
+@pytest.mark.parametrize("B,N,page", [(3, 5, 1), (70, 33, 7), (300, 40, 16)])
+def test_stored_counts_the_slots(B, N, page):
+    import chill_attention as ca
+
+    g = torch.Generator().manual_seed(B)
+    draw = lambda hi: torch.randint(0, hi + 1, (B,), generator=g).tolist()  # noqa: E731
+    for num in (1, B * (20 + N) // page // 2 + 1, B * (-(-(20 + N) // page))):
+        pages = ca.ChillPages.empty(B, 10 + N, num, page)  # some tables are full too
+        for parents in (None, torch.full((B, N), -1, dtype=torch.int32, device="cuda")):
+            step = ca.chill_pages_reserve(pages, ints(draw(20)), ints(draw(N)), N, page, parents)
+            assert step.stored.tolist() == (step.slots >= 0).sum(1).tolist()
+
+
+def test_commit_ends_before_the_first_token_without_a_page():
+    import chill_attention as ca
+
+    page, D = 16, 64
+    pages = ca.ChillPages.empty(3, 64, 3, page)
+    kc, vc = (torch.full((3, 1, page, D), 9.0, device="cuda") for _ in range(2))
+    first = ca.chill_pages_reserve(pages, ints([0, 0, 0]), ints([10, 14, 14]), 14, page)
+    assert first.stored.tolist() == [10, 14, 14]
+    step = ca.chill_pages_reserve(pages, ints([10, 14, 14]), ints([4, 6, 6]), 6, page, ints([[-1] * 6] * 3))
+    assert step.stored.tolist() == [4, 2, 2] and pages.missing.item() == 2
+    k = torch.arange(18, device="cuda", dtype=torch.float32).view(3, 1, 6, 1).expand(3, 1, 6, D)
+    ca.chill_cache_append(kc, vc, k, -k, step.slots)
+    lens = ca.chill_cache_commit(kc, vc, pages.table, step, ints([[1, 3, 5], [0, 1, 2], [1, 4, 5]]), ints([2, 3, 3]))
+    assert lens.tolist() == [12, 16, 15]
+    rows = lambda b, t: kc[int(pages.table[b, t // page]), 0, t % page, 0].item()  # noqa: E731
+    assert [rows(0, 10), rows(0, 11)] == [1, 3] and [rows(1, 14), rows(1, 15)] == [6, 7] and rows(2, 14) == 13
