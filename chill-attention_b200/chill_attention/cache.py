@@ -357,7 +357,7 @@ def _attention(q, k_cache, v_cache, table, step, mask, sm_scale, return_lse, fla
         sm_scale = q.shape[-1] ** -0.5
     if mask.name not in _MASKS:
         _mask_functor(mask)
-    elif not _is_compiling() and _MASKS[mask.name][2] is not type(mask):
+    elif _MASKS[mask.name][2] is not type(mask):
         _check_same_name(mask)
     lens, new_lens, _, positions, ancestors = step[:5]
     if _direct():

@@ -150,6 +150,33 @@ def test_two_mask_classes_of_one_name():
         del cache._MASKS["OneName"]
 
 
+@pytest.mark.parametrize("fullgraph", [False, True])
+def test_two_mask_classes_of_one_name_under_compile(lib, fullgraph):
+    """A graph finds its kernel by the class name, so the second class is refused while it is traced too."""
+    from chill_attention import CausalChillMask, cache
+
+    def make(functor, **more):
+        return type("OneName", (CausalChillMask,), {"cuda_functor": functor, **more})()
+
+    def run(mask):
+        torch._dynamo.reset()
+        call = lambda q: cache._attention(q, q, q, q, (q,) * 5, mask, None, False, 0)  # noqa: E731
+        return torch.compile(call, backend="eager", fullgraph=fullgraph)(torch.zeros(1, 1, 1, 64))
+
+    first = make("CausalMask")
+    cache._MASKS["OneName"] = (cache._native(), 1, type(first))
+    try:
+        for other in (make("FullMask"), make("CausalMask", cuda_functor_header="/tmp/x.h")):
+            with pytest.raises(Exception, match="two mask classes"):
+                run(other)
+        for same in (first, make("CausalMask")):  # goes on, to the next check
+            with pytest.raises(Exception, match="CUDA tensors"):
+                run(same)
+    finally:
+        del cache._MASKS["OneName"]
+        torch._dynamo.reset()
+
+
 def test_oracle_trim_undoes_reserve():
     table, held, free = [[5, -1, -1, -1], [-1] * 4, [7, 2, -1, -1]], [1, 0, 2], [9, 8, 6, 4, 3, 1, 0]
     lens, new = [10, 0, 20], [30, 16, 0]
