@@ -419,8 +419,8 @@ cached_rows_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constan
     if (p.D < DP) {  // the channels beyond the head become 0 again
       tc::named_bar_sync(1, 128);
       for (int idx = threadIdx.x; idx < S::kQBytes / 16; idx += 128) *reinterpret_cast<uint4*>(gen + (sq - base) + idx * 16) = make_uint4(0u, 0u, 0u, 0u);
-      tc::fence_proxy_async_smem();
     }
+    tc::fence_proxy_async_smem();  // the merge buffer and these zeros lie where the next copy of Q goes
     __syncwarp();
     if (lane == 0) tc::mbar_arrive(item_empty + 8 * slot);
   }

@@ -846,3 +846,18 @@ def test_commit_ends_before_the_first_token_without_a_page():
     assert lens.tolist() == [12, 16, 15]
     rows = lambda b, t: kc[int(pages.table[b, t // page]), 0, t % page, 0].item()  # noqa: E731
     assert [rows(0, 10), rows(0, 11)] == [1, 3] and [rows(1, 14), rows(1, 15)] == [6, 7] and rows(2, 14) == 13
+
+
+@pytest.mark.parametrize("room", list(ROOMS))
+@pytest.mark.parametrize("D,N", [(32, 2), (64, 2), (64, 13), (128, 2), (128, 13), (256, 2)])
+def test_many_pieces_one_after_the_other(D, N, room):
+    """Every CTA of the kernel for few rows joins its warps' states where the Q of the piece after the next one goes."""
+    from chill_attention import _cache_abi
+
+    B = 1000
+    p = Problem(torch.bfloat16, 2, 1, D, [(11 * b) % 70 for b in range(B)], [N - b % 2 for b in range(B)], N, 16, tree=N > 2, seed=D, room=ROOMS[room])
+    assert kernel_of(p) == _cache_abi.CACHED_ROWS
+    o, lse = run_and_check(p, masks()["causal"])
+    for _ in range(3):
+        (again, lse_again), _ = attend(p, masks()["causal"])
+        assert torch.equal(o, again) and torch.equal(lse, lse_again)
