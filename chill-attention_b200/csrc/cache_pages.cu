@@ -141,7 +141,7 @@ __global__ void __launch_bounds__(kPageThreads) pages_kernel(PagesP p, int ctas)
     __syncwarp();  // all lanes have read held[b] and off
     if (kTrim) {
       for (int j = lane; j < held - need; j += 32) {
-        const int at = n_free + sum - 1 - (off + j);
+        const long long at = (long long)n_free + sum - 1 - (off + j);  // `held` can be nonsense
         if (at >= 0 && at < p.num_pages) p.free_pages[at] = row[need + j];
         row[need + j] = -1;
       }
@@ -157,7 +157,7 @@ __global__ void __launch_bounds__(kPageThreads) pages_kernel(PagesP p, int ctas)
   }
   if (rank == ctas - 1 && threadIdx.x == 0) {
     if (kTrim) {
-      *p.n_free = imin(n_free + sum, p.num_pages);
+      *p.n_free = imin(sum, p.num_pages - n_free) + n_free;
     } else {
       *p.n_free = n_free - imin(sum, n_free);
       *p.missing = imax(sum - n_free, 0);
@@ -211,7 +211,8 @@ static int launch_pages(const PagesP& p, cudaStream_t st) {
 static int check_pages(const chill_pages_args* a, bool trim) {
   if (a == nullptr || a->B <= 0 || a->page_size <= 0 || a->num_pages <= 0 || a->table_width <= 0) return CHILL_E_INVALID;
   if (a->B > kMaxRequests || (long long)a->num_pages * a->page_size > 0x7fffffffll ||
-      (long long)a->table_width * a->page_size > kMaxLen)
+      (long long)a->table_width * a->page_size > kMaxLen ||
+      (long long)a->B * a->table_width > 0x7fffffffll)  // what the requests can hold, take or give back is summed up in 32 bits
     return CHILL_E_TOO_LARGE;
   if (!a->table || !a->held || !a->free_pages || !a->n_free || !a->lens) return CHILL_E_INVALID;
   if (a->table_stride < a->table_width && a->B > 1) return CHILL_E_INVALID;

@@ -25,7 +25,8 @@ extern "C" {
  * (clamped to [0, N]) behind the lens[b] that are cached: one each, a chunk, or a tree of drafted tokens.  All of it is read on the
  * GPU, nothing here synchronises, and every call can be captured into a graph and replayed with other lengths.  Calls that use
  * the same pages are ordered by the caller (one stream, or events).  All integer arrays are int32, device, contiguous unless a stride
- * is given.  Sizes: B <= 65535, num_pages * page_size < 2^31, table_width * page_size <= 2^29 (CHILL_E_TOO_LARGE). */
+ * is given.  Sizes: B <= 65535, num_pages * page_size < 2^31, table_width * page_size <= 2^29, for reserve and trim
+ * B * table_width < 2^31 (CHILL_E_TOO_LARGE). */
 
 typedef struct chill_pages_args {
   int32_t B, N;  /* requests; most new tokens of a request */

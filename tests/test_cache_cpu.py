@@ -91,6 +91,11 @@ def test_page_and_row_refusals(lib):
     assert lib.chill_pages_reserve(pages(B=65536), None) == lib.chill_pages_reserve(pages(num_pages=2 ** 27), None) == -4
     assert lib.chill_pages_trim(pages(table_width=2 ** 26), None) == -4
 
+    # sums of pages over the requests are 32 bits wide: tables with more entries than that
+    for B, width in ((65535, 2 ** 16), (8, 2 ** 28), (5, 2 ** 29)):
+        big = pages(B=B, page_size=1, num_pages=2 ** 30, table_width=width, table_stride=width)
+        assert lib.chill_pages_reserve(big, None) == lib.chill_pages_reserve_stored(big, None, None) == lib.chill_pages_trim(big, None) == -4
+
     def rows(**changes):
         a = _cache_abi.CacheRowsArgs()
         a.B, a.H_kv, a.N, a.D, a.dtype, a.page_size, a.num_pages, a.table_width, a.A = 4, 2, 3, 64, 2, 16, 100, 20, 2
