@@ -103,7 +103,13 @@ def _check_ints(like, **named):
         assert t.device == like.device, f"{name} must be on {like.device}"
 
 
+def _check_sizes(**named):
+    for name, t in named.items():
+        assert max(t.shape, default=0) < 2 ** 31, f"the sizes of {name} must fit 32 bits"
+
+
 def _check_table(table):
+    _check_sizes(table=table)
     assert table.is_cuda, "the paged cache runs on CUDA tensors only"
     assert table.dtype == torch.int32 and table.ndim == 2 and table.numel() > 0, "table must be an int32 tensor [batch, blocks]"
     assert table.stride(1) == 1 and (table.shape[0] == 1 or table.stride(0) >= table.shape[1]), "the rows of table must be contiguous"
@@ -112,11 +118,13 @@ def _check_table(table):
 def _check_pages(pages, lens, page_size):
     _check_table(pages.table)
     B = pages.table.shape[0]
-    assert page_size >= 1 and pages.free.ndim == 1 and pages.free.numel() >= 1
+    assert 1 <= page_size < 2 ** 31 and pages.free.ndim == 1 and pages.free.numel() >= 1
+    _check_sizes(free=pages.free)
     _check_ints(pages.table, held=(pages.held, (B,)), free=(pages.free, pages.free.shape), n_free=(pages.n_free, (1,)), lens=(lens, (B,)))
 
 
 def _check_caches(k_cache, v_cache):
+    _check_sizes(k_cache=k_cache)
     assert k_cache.is_cuda and k_cache.device == v_cache.device, "the caches must be CUDA tensors on one device"
     assert k_cache.ndim == 4 and k_cache.shape == v_cache.shape and k_cache.numel() > 0, \
         "k_cache and v_cache must have one shape [num_pages, kv_heads, page_size, head_dim]"
@@ -130,6 +138,7 @@ def _check_grad(*tensors):
 
 def _check_rows(k_cache, v_cache, k, v, slots):
     _check_caches(k_cache, v_cache)
+    _check_sizes(k=k)
     assert k.ndim == 4 and k.shape == v.shape and k.numel() > 0, "k and v must have one shape [batch, kv_heads, max_new, head_dim]"
     assert k.shape[1] == k_cache.shape[1] and k.shape[3] == k_cache.shape[3], "kv heads and head dim must be those of the caches"
     assert k.dtype == v.dtype == k_cache.dtype and k.device == v.device == k_cache.device
@@ -142,6 +151,7 @@ def _check_commit(k_cache, v_cache, table, lens, new_lens, path, accepted):
     _check_table(table)
     assert table.device == k_cache.device
     B = table.shape[0]
+    _check_sizes(path=path)
     assert path.ndim == 2 and path.shape[1] >= 1, "path must be [batch, longest path]"
     _check_ints(k_cache, lens=(lens, (B,)), new_lens=(new_lens, (B,)), path=(path, (B, path.shape[1])), accepted=(accepted, (B,)))
     _check_grad(k_cache, v_cache)
@@ -150,6 +160,7 @@ def _check_commit(k_cache, v_cache, table, lens, new_lens, path, accepted):
 def _check_attention(q, k_cache, v_cache, table, lens, new_lens, positions, ancestors):
     _check_caches(k_cache, v_cache)
     _check_table(table)
+    _check_sizes(q=q)
     assert q.ndim == 4 and q.numel() > 0, "q must be [batch, heads, max_new, head_dim]"
     B, H, N, D = q.shape
     assert D in _HEAD_DIMS, f"head dim must be one of {sorted(_HEAD_DIMS)}"
@@ -232,7 +243,7 @@ def _(q, k_cache, v_cache, table, lens, new_lens, positions, ancestors, mask_nam
 # ------------------------------------------------------------------------------------------------------------ public calls
 def _check_reserve(pages, new_lens, max_new, parents):
     B = pages.table.shape[0]
-    assert max_new >= 1
+    assert 1 <= max_new < 2 ** 31
     _check_ints(pages.table, missing=(pages.missing, (1,)), new_lens=(new_lens, (B,)))
     if parents is not None:
         _check_ints(pages.table, parents=(parents, (B, max_new)))

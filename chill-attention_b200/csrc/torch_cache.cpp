@@ -69,13 +69,20 @@ bool ints(const Tensor& t, std::initializer_list<int64_t> sizes, const Tensor& l
   return t.scalar_type() == at::kInt && t.sizes() == at::IntArrayRef(sizes) && t.is_contiguous() && t.device() == like.device();
 }
 
+// The C ABI takes 32-bit sizes.
+bool fit(const Tensor& t) {
+  for (const int64_t n : t.sizes())
+    if (n > INT32_MAX) return false;
+  return true;
+}
+
 bool table_ok(const Tensor& table) {
-  return table.scalar_type() == at::kInt && table.dim() == 2 && table.size(0) > 0 && table.size(1) > 0 && table.is_cuda() && table.stride(1) == 1 &&
+  return fit(table) && table.scalar_type() == at::kInt && table.dim() == 2 && table.size(0) > 0 && table.size(1) > 0 && table.is_cuda() && table.stride(1) == 1 &&
          (table.size(0) == 1 || table.stride(0) >= table.size(1));
 }
 
 bool pools_ok(const Tensor& k, const Tensor& v) {
-  return k.dim() == 4 && k.sizes() == v.sizes() && k.numel() > 0 && k.scalar_type() == v.scalar_type() && dtype_of(k) >= 0 && k.is_cuda() && v.device() == k.device();
+  return k.dim() == 4 && fit(k) && k.sizes() == v.sizes() && k.numel() > 0 && k.scalar_type() == v.scalar_type() && dtype_of(k) >= 0 && k.is_cuda() && v.device() == k.device();
 }
 
 bool wants_grad(std::initializer_list<const Tensor*> tensors) {
@@ -91,7 +98,7 @@ py::object reserve(const CacheLibrary& lib, const Tensor& table, const Tensor& h
                    const Tensor& lens, const Tensor& new_lens, int64_t N, int64_t page, const std::optional<Tensor>& parents) {
   if (watched({&table, &held, &free, &n_free, &missing, &lens, &new_lens}) || !table_ok(table) || N < 1 || N > INT32_MAX || page < 1 || page > INT32_MAX) return py::none();
   const int64_t B = table.size(0);
-  if (!ints(held, {B}, table) || free.dim() != 1 || free.size(0) < 1 || !ints(free, {free.size(0)}, table) || !ints(n_free, {1}, table) ||
+  if (!ints(held, {B}, table) || free.dim() != 1 || free.size(0) < 1 || !fit(free) || !ints(free, {free.size(0)}, table) || !ints(n_free, {1}, table) ||
       !ints(missing, {1}, table) || !ints(lens, {B}, table) || !ints(new_lens, {B}, table) || (parents.has_value() && !ints(*parents, {B, N}, table)))
     return py::none();
   c10::cuda::CUDAGuard guard(table.device());
@@ -112,7 +119,7 @@ py::object reserve(const CacheLibrary& lib, const Tensor& table, const Tensor& h
 bool trim(const CacheLibrary& lib, const Tensor& table, const Tensor& held, const Tensor& free, const Tensor& n_free, const Tensor& lens, int64_t page) {
   if (watched({&table, &held, &free, &n_free, &lens}) || !table_ok(table) || page < 1 || page > INT32_MAX) return false;
   const int64_t B = table.size(0);
-  if (!ints(held, {B}, table) || free.dim() != 1 || free.size(0) < 1 || !ints(free, {free.size(0)}, table) || !ints(n_free, {1}, table) || !ints(lens, {B}, table))
+  if (!ints(held, {B}, table) || free.dim() != 1 || free.size(0) < 1 || !fit(free) || !ints(free, {free.size(0)}, table) || !ints(n_free, {1}, table) || !ints(lens, {B}, table))
     return false;
   c10::cuda::CUDAGuard guard(table.device());
   chill_pages_args a{};
@@ -135,7 +142,7 @@ chill_cache_rows_args rows_args(const Tensor& kc, const Tensor& vc) {
 }
 
 bool append(const CacheLibrary& lib, const Tensor& kc, const Tensor& vc, const Tensor& k, const Tensor& v, const Tensor& slots) {
-  if (watched({&kc, &vc, &k, &v, &slots}) || !pools_ok(kc, vc) || k.dim() != 4 || k.numel() == 0 || k.sizes() != v.sizes() || k.size(1) != kc.size(1) || k.size(3) != kc.size(3)) return false;
+  if (watched({&kc, &vc, &k, &v, &slots}) || !pools_ok(kc, vc) || k.dim() != 4 || k.numel() == 0 || !fit(k) || k.sizes() != v.sizes() || k.size(1) != kc.size(1) || k.size(3) != kc.size(3)) return false;
   if (k.scalar_type() != kc.scalar_type() || v.scalar_type() != kc.scalar_type() || k.device() != kc.device() || v.device() != kc.device()) return false;
   if (!ints(slots, {k.size(0), k.size(2)}, kc) || wants_grad({&kc, &vc, &k, &v})) return false;
   c10::cuda::CUDAGuard guard(kc.device());
@@ -150,7 +157,7 @@ bool append(const CacheLibrary& lib, const Tensor& kc, const Tensor& vc, const T
 
 py::object commit(const CacheLibrary& lib, const Tensor& kc, const Tensor& vc, const Tensor& table, const Tensor& lens, const Tensor& new_lens,
                   int64_t N, const Tensor& path, const Tensor& accepted) {
-  if (watched({&kc, &vc, &table, &lens, &new_lens, &path, &accepted}) || !pools_ok(kc, vc) || !table_ok(table) || table.device() != kc.device() || path.dim() != 2 || path.size(1) < 1 || N < 1 || N > INT32_MAX) return py::none();
+  if (watched({&kc, &vc, &table, &lens, &new_lens, &path, &accepted}) || !pools_ok(kc, vc) || !table_ok(table) || table.device() != kc.device() || path.dim() != 2 || path.size(1) < 1 || !fit(path) || N < 1 || N > INT32_MAX) return py::none();
   const int64_t B = table.size(0);
   if (!ints(lens, {B}, kc) || !ints(new_lens, {B}, kc) || !ints(path, {B, path.size(1)}, kc) || !ints(accepted, {B}, kc) || wants_grad({&kc, &vc})) return py::none();
   c10::cuda::CUDAGuard guard(kc.device());
@@ -169,7 +176,7 @@ py::object commit(const CacheLibrary& lib, const Tensor& kc, const Tensor& vc, c
 py::object attention(const CacheLibrary& lib, int32_t functor_id, const Tensor& q, const Tensor& kc, const Tensor& vc, const Tensor& table,
                      const Tensor& lens, const Tensor& new_lens, const Tensor& positions, const std::optional<Tensor>& ancestors,
                      const py::tuple& mask_args, double sm_scale, bool return_lse, uint32_t flags) {
-  if (watched({&q, &kc, &vc, &table, &lens, &new_lens, &positions}) || !pools_ok(kc, vc) || !table_ok(table) || table.device() != kc.device() || q.dim() != 4 || q.numel() == 0) return py::none();
+  if (watched({&q, &kc, &vc, &table, &lens, &new_lens, &positions}) || !pools_ok(kc, vc) || !table_ok(table) || table.device() != kc.device() || q.dim() != 4 || q.numel() == 0 || !fit(q)) return py::none();
   const int64_t B = q.size(0), H = q.size(1), N = q.size(2), D = q.size(3);
   if (table.size(0) != B || kc.size(3) != D || H % kc.size(1) != 0 || q.scalar_type() != kc.scalar_type() || q.device() != kc.device()) return py::none();
   if (D != 16 && D != 32 && D != 64 && D != 128 && D != 256) return py::none();

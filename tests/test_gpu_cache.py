@@ -861,3 +861,24 @@ def test_many_pieces_one_after_the_other(D, N, room):
     for _ in range(3):
         (again, lse_again), _ = attend(p, masks()["causal"])
         assert torch.equal(o, again) and torch.equal(lse, lse_again)
+
+
+def test_sizes_beyond_32_bits_are_refused():
+    """Not cut to their low bits: one page of memory that stands for 2^32 + 1 of them, and so on."""
+    import chill_attention as ca
+
+    p = Problem(torch.bfloat16, 4, 2, 64, [40, 20], [3, 3], 3, 16, tree=True, seed=1)
+    q, kc, vc, table, step = p.q.cuda(), p.k_cache.cuda(), p.v_cache.cuda(), p.table.cuda(), p.step()
+    pages, lens, far = ca.ChillPages.empty(2, 100, 8, 16), ints([0, 0]), 2 ** 32 + 1
+    many = kc[:1].expand(far, -1, -1, -1)
+    path = torch.zeros(1, 1, dtype=torch.int32, device="cuda")
+    for call in (lambda: ca.chill_attention_cached(q, many, many, table, step, ca.CausalChillMask()),
+                 lambda: ca.chill_cache_append(many, many, kc[:2, :, :3], kc[:2, :, :3], step.slots),
+                 lambda: ca.chill_cache_commit(many, many, table, step, ints([[0], [0]]), ints([1, 1])),
+                 lambda: ca.chill_cache_commit(kc, vc, table, step, path.expand(2, far), ints([1, 1])),
+                 lambda: ca.chill_attention_cached(q[:, :, :1].expand(-1, -1, far, -1), kc, vc, table, step, ca.CausalChillMask()),
+                 lambda: ca.chill_pages_reserve(pages, lens, lens, far, 16), lambda: ca.chill_pages_reserve(pages, lens, lens, 1, far),
+                 lambda: ca.chill_pages_trim(pages, lens, far), lambda: ca.chill_pages_trim(pages._replace(free=path[0].expand(far)), lens, 16),
+                 lambda: ca.chill_pages_trim(pages._replace(table=path.expand(2, far)), lens, 16)):
+        with pytest.raises(AssertionError):
+            call()
