@@ -92,6 +92,12 @@ bool wants_grad(std::initializer_list<const Tensor*> tensors) {
   return false;
 }
 
+// Changed in place: autograd looks at a tensor's version where it saved one.  (Inference tensors have none.)
+void changed(std::initializer_list<const Tensor*> tensors) {
+  for (const Tensor* t : tensors)
+    if (!t->is_inference()) t->unsafeGetTensorImpl()->bump_version();
+}
+
 const int32_t* optional_ints(const std::optional<Tensor>& t) { return t.has_value() ? t->const_data_ptr<int32_t>() : nullptr; }
 
 py::object reserve(const CacheLibrary& lib, const Tensor& table, const Tensor& held, const Tensor& free, const Tensor& n_free, const Tensor& missing,
@@ -113,6 +119,7 @@ py::object reserve(const CacheLibrary& lib, const Tensor& table, const Tensor& h
   a.slots = slots.mutable_data_ptr<int32_t>(); a.positions = positions.mutable_data_ptr<int32_t>();
   a.ancestors = parents.has_value() ? ancestors.mutable_data_ptr<int32_t>() : nullptr;
   check(lib, lib.reserve(&a, stored.mutable_data_ptr<int32_t>(), current_stream(table)), "chill_pages_reserve");
+  changed({&table, &held, &free, &n_free, &missing});
   return py::make_tuple(slots, positions, parents.has_value() ? py::cast(ancestors) : py::none(), stored);
 }
 
@@ -128,6 +135,7 @@ bool trim(const CacheLibrary& lib, const Tensor& table, const Tensor& held, cons
   a.held = held.mutable_data_ptr<int32_t>(); a.free_pages = free.mutable_data_ptr<int32_t>(); a.n_free = n_free.mutable_data_ptr<int32_t>();
   a.lens = lens.const_data_ptr<int32_t>();
   check(lib, lib.trim(&a, current_stream(table)), "chill_pages_trim");
+  changed({&table, &held, &free, &n_free});
   return true;
 }
 
@@ -152,6 +160,7 @@ bool append(const CacheLibrary& lib, const Tensor& kc, const Tensor& vc, const T
   set_strides(a.k_strides, k); set_strides(a.v_strides, v);
   a.slots = slots.const_data_ptr<int32_t>();
   check(lib, lib.append(&a, current_stream(kc)), "chill_cache_append");
+  changed({&kc, &vc});
   return true;
 }
 
@@ -168,6 +177,7 @@ py::object commit(const CacheLibrary& lib, const Tensor& kc, const Tensor& vc, c
   a.lens = lens.const_data_ptr<int32_t>(); a.new_lens = new_lens.const_data_ptr<int32_t>();
   a.path = path.const_data_ptr<int32_t>(); a.accepted = accepted.const_data_ptr<int32_t>(); a.out_lens = out.mutable_data_ptr<int32_t>();
   check(lib, lib.commit(&a, current_stream(kc)), "chill_cache_commit");
+  changed({&kc, &vc});
   return py::cast(out);
 }
 

@@ -882,3 +882,35 @@ def test_sizes_beyond_32_bits_are_refused():
                  lambda: ca.chill_pages_trim(pages._replace(table=path.expand(2, far)), lens, 16)):
         with pytest.raises(AssertionError):
             call()
+
+
+def test_autograd_notices_what_is_changed_in_place():
+    import chill_attention as ca
+
+    kc, vc = (torch.zeros(4, 1, 16, 64, device="cuda") for _ in range(2))
+    w = torch.ones(64, device="cuda", requires_grad=True)
+    new = torch.randn(1, 1, 3, 64, device="cuda")
+    pages, lens = ca.ChillPages.empty(1, 64, 4, 16), ints([0])
+
+    def versions():
+        return [t._version for t in (*pages, kc, vc)]
+
+    before = versions()
+    step = ca.chill_pages_reserve(pages, lens, ints([3]), 3, 16, ints([[-1, 0, 0]]))
+    reserved = versions()
+    assert all(a > b for a, b in zip(reserved[:5], before[:5])) and reserved[5:] == before[5:]
+    y = (kc * w).sum()  # saves kc
+    ca.chill_cache_append(kc, vc, new, new, step.slots)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.backward()
+    appended = versions()
+    assert appended[:5] == reserved[:5] and all(a > b for a, b in zip(appended[5:], reserved[5:]))
+    lens = ca.chill_cache_commit(kc, vc, pages.table, step, ints([[0, 2]]), ints([2]))
+    committed = versions()
+    assert all(a > b for a, b in zip(committed[5:], appended[5:]))
+    ca.chill_pages_trim(pages, lens, 16)
+    assert all(a > b for a, b in zip(versions()[:4], committed[:4]))
+    with torch.inference_mode():  # tensors without a version
+        kc, vc = torch.zeros_like(kc), torch.zeros_like(vc)
+    ca.chill_cache_append(kc, vc, new, new, step.slots)
+    assert torch.equal(kc[int(pages.table[0, 0]), 0, :3], new[0, 0])
