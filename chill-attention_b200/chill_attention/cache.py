@@ -26,6 +26,7 @@ import ctypes as C
 import typing
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _cabi, _cache_abi, _eager, chill
 from .mask import ChillMask
@@ -134,6 +135,8 @@ def _check_caches(k_cache, v_cache):
 def _check_grad(*tensors):
     assert not (torch.is_grad_enabled() and any(t.requires_grad for t in tensors)), \
         "the paged cache has no gradients: call it under torch.no_grad() or with detached tensors"
+    if not _is_compiling():
+        assert all(forward_ad.unpack_dual(t).tangent is None for t in tensors), "the paged cache has no gradients: the tensors carry tangents"
 
 
 def _check_rows(k_cache, v_cache, k, v, slots):

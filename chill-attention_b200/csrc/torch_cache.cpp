@@ -3,6 +3,7 @@
 // repeats the checks in Python for the message.
 #include <ATen/core/grad_mode.h>
 #include <ATen/cuda/EmptyTensor.h>
+#include <c10/core/AutogradState.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/Exceptions.h>
@@ -85,10 +86,11 @@ bool pools_ok(const Tensor& k, const Tensor& v) {
   return k.dim() == 4 && fit(k) && k.sizes() == v.sizes() && k.numel() > 0 && k.scalar_type() == v.scalar_type() && dtype_of(k) >= 0 && k.is_cuda() && v.device() == k.device();
 }
 
+// Gradients asked for, or a tangent carried along (forward mode, which no_grad leaves on).
 bool wants_grad(std::initializer_list<const Tensor*> tensors) {
-  if (!at::GradMode::is_enabled()) return false;
+  const bool backward = at::GradMode::is_enabled(), forward = c10::AutogradState::get_tls_state().get_fw_grad_mode();
   for (const Tensor* t : tensors)
-    if (t->requires_grad()) return true;
+    if ((backward && t->requires_grad()) || (forward && t->_fw_grad(/*level=*/0).defined())) return true;
   return false;
 }
 

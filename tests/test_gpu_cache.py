@@ -914,3 +914,23 @@ def test_autograd_notices_what_is_changed_in_place():
         kc, vc = torch.zeros_like(kc), torch.zeros_like(vc)
     ca.chill_cache_append(kc, vc, new, new, step.slots)
     assert torch.equal(kc[int(pages.table[0, 0]), 0, :3], new[0, 0])
+
+
+@pytest.mark.parametrize("grad", [True, False])
+def test_tangents_are_refused(grad):
+    """Forward-mode derivatives are not dropped without a word, not under no_grad either."""
+    import chill_attention as ca
+    from torch.autograd import forward_ad
+
+    p = Problem(torch.float32, 4, 2, 64, [40, 20], [3, 3], 3, 16, tree=True, seed=1)
+    q, kc, vc, table, step = p.q.cuda(), p.k_cache.cuda(), p.v_cache.cuda(), p.table.cuda(), p.step()
+    k, path, accepted = torch.randn(2, 2, 3, 64, device="cuda"), ints([[0, 1], [0, 2]]), ints([1, 2])
+    with forward_ad.dual_level(), torch.set_grad_enabled(grad):
+        dual = lambda t: forward_ad.make_dual(t.clone(), torch.ones_like(t))  # noqa: E731
+        for call in (lambda: ca.chill_attention_cached(dual(q), kc, vc, table, step, ca.CausalChillMask()),
+                     lambda: ca.chill_attention_cached(q, kc, dual(vc), table, step, ca.CausalChillMask()),
+                     lambda: ca.chill_cache_append(kc, vc, dual(k), k, step.slots), lambda: ca.chill_cache_append(dual(kc), vc, k, k, step.slots),
+                     lambda: ca.chill_cache_commit(kc, dual(vc), table, step, path, accepted)):
+            with pytest.raises(AssertionError, match="tangents"):
+                call()
+        ca.chill_attention_cached(q, kc, vc, table, step, ca.CausalChillMask())
