@@ -44,10 +44,11 @@ void check(const CacheLibrary& lib, int status, const char* what) {
 Tensor empty(at::IntArrayRef sizes, at::ScalarType type, const Tensor& like) { return at::detail::empty_cuda(sizes, type, like.device(), std::nullopt); }
 
 // A tensor that something looks in on (a subclass with its own dispatch, a transform): the dispatcher ops serve it.
-bool watched(std::initializer_list<const Tensor*> tensors) {
+bool watched(std::initializer_list<const Tensor*> tensors, const std::optional<Tensor>& one_more = std::nullopt) {
+  auto looked_at = [](const Tensor& t) { return t.unsafeGetTensorImpl()->key_set().has_any(c10::python_ks | c10::functorch_transforms_ks); };
   for (const Tensor* t : tensors)
-    if (t->unsafeGetTensorImpl()->key_set().has_any(c10::python_ks | c10::functorch_transforms_ks)) return true;
-  return false;
+    if (looked_at(*t)) return true;
+  return one_more.has_value() && looked_at(*one_more);
 }
 
 void* current_stream(const Tensor& t) { return (void*)c10::cuda::getCurrentCUDAStream(t.get_device()).stream(); }
@@ -104,7 +105,7 @@ const int32_t* optional_ints(const std::optional<Tensor>& t) { return t.has_valu
 
 py::object reserve(const CacheLibrary& lib, const Tensor& table, const Tensor& held, const Tensor& free, const Tensor& n_free, const Tensor& missing,
                    const Tensor& lens, const Tensor& new_lens, int64_t N, int64_t page, const std::optional<Tensor>& parents) {
-  if (watched({&table, &held, &free, &n_free, &missing, &lens, &new_lens}) || !table_ok(table) || N < 1 || N > INT32_MAX || page < 1 || page > INT32_MAX) return py::none();
+  if (watched({&table, &held, &free, &n_free, &missing, &lens, &new_lens}, parents) || !table_ok(table) || N < 1 || N > INT32_MAX || page < 1 || page > INT32_MAX) return py::none();
   const int64_t B = table.size(0);
   if (!ints(held, {B}, table) || free.dim() != 1 || free.size(0) < 1 || !fit(free) || !ints(free, {free.size(0)}, table) || !ints(n_free, {1}, table) ||
       !ints(missing, {1}, table) || !ints(lens, {B}, table) || !ints(new_lens, {B}, table) || (parents.has_value() && !ints(*parents, {B, N}, table)))
@@ -188,7 +189,7 @@ py::object commit(const CacheLibrary& lib, const Tensor& kc, const Tensor& vc, c
 py::object attention(const CacheLibrary& lib, int32_t functor_id, const Tensor& q, const Tensor& kc, const Tensor& vc, const Tensor& table,
                      const Tensor& lens, const Tensor& new_lens, const Tensor& positions, const std::optional<Tensor>& ancestors,
                      const py::tuple& mask_args, double sm_scale, bool return_lse, uint32_t flags) {
-  if (watched({&q, &kc, &vc, &table, &lens, &new_lens, &positions}) || !pools_ok(kc, vc) || !table_ok(table) || table.device() != kc.device() || q.dim() != 4 || q.numel() == 0 || !fit(q)) return py::none();
+  if (watched({&q, &kc, &vc, &table, &lens, &new_lens, &positions}, ancestors) || !pools_ok(kc, vc) || !table_ok(table) || table.device() != kc.device() || q.dim() != 4 || q.numel() == 0 || !fit(q)) return py::none();
   const int64_t B = q.size(0), H = q.size(1), N = q.size(2), D = q.size(3);
   if (table.size(0) != B || kc.size(3) != D || H % kc.size(1) != 0 || q.scalar_type() != kc.scalar_type() || q.device() != kc.device()) return py::none();
   if (D != 16 && D != 32 && D != 64 && D != 128 && D != 256) return py::none();

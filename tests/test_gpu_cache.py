@@ -934,3 +934,34 @@ def test_tangents_are_refused(grad):
             with pytest.raises(AssertionError, match="tangents"):
                 call()
         ca.chill_attention_cached(q, kc, vc, table, step, ca.CausalChillMask())
+
+
+def test_a_tensor_that_watches_its_operators():
+    """A subclass sees the dispatcher op whichever argument it is."""
+    import chill_attention as ca
+
+    class Watching(torch.Tensor):
+        seen = []
+
+        @staticmethod
+        def __new__(cls, held):
+            t = torch.Tensor._make_subclass(cls, held)
+            t.held = held
+            return t
+
+        @classmethod
+        def __torch_dispatch__(cls, func, types, args=(), kwargs=None):
+            cls.seen.append(str(func))
+            return func(*(a.held if isinstance(a, cls) else a for a in args), **(kwargs or {}))
+
+    p = Problem(torch.bfloat16, 4, 2, 64, [40, 20], [3, 3], 3, 16, tree=True, seed=1)
+    q, kc, vc, table, step = p.q.cuda(), p.k_cache.cuda(), p.v_cache.cuda(), p.table.cuda(), p.step()
+    want = ca.chill_attention_cached(q, kc, vc, table, step, ca.CausalChillMask())
+    for changed in ((Watching(q), step), (q, step._replace(positions=Watching(step.positions))), (q, step._replace(ancestors=Watching(step.ancestors)))):
+        Watching.seen.clear()
+        o = ca.chill_attention_cached(changed[0], kc, vc, table, changed[1], ca.CausalChillMask())
+        assert any("cached_forward" in name for name in Watching.seen) and torch.equal(o, want)
+    for lens, parents in ((Watching(ints([0, 0])), ints(p.parents)), (ints([0, 0]), Watching(ints(p.parents)))):
+        Watching.seen.clear()
+        got = ca.chill_pages_reserve(ca.ChillPages.empty(2, 100, 8, 16), lens, step.new_lens, 3, 16, parents)
+        assert any("pages_reserve" in name for name in Watching.seen) and (got.slots >= 0).all()
