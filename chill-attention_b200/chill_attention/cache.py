@@ -91,9 +91,9 @@ _dispatch_depth, _function_depth, _functorch_top = _eager._dispatch_depth, _eage
 
 
 def _direct() -> bool:
-    """Whether a call can go to the native module: nothing watches the dispatcher.  (The module itself turns away tensors that are
-    watched, or not on a GPU.)"""
-    return not _is_compiling() and _eager._PROBES_OK and _dispatch_depth() == 0 and _function_depth() == 0 and _functorch_top() is None
+    """Whether a call can go to the native module: the eager path is on (CHILL_ATTENTION_EAGER_FAST), nothing watches the dispatcher.
+    (The module itself turns away tensors that are watched, or not on a GPU.)"""
+    return not _is_compiling() and _eager.ENABLED and _eager._PROBES_OK and _dispatch_depth() == 0 and _function_depth() == 0 and _functorch_top() is None
 
 
 # --------------------------------------------------------------------------------------------- argument checks, with messages

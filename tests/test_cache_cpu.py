@@ -182,6 +182,16 @@ def test_two_mask_classes_of_one_name_under_compile(lib, fullgraph):
         torch._dynamo.reset()
 
 
+def test_the_switch_of_the_eager_path(monkeypatch):
+    """CHILL_ATTENTION_EAGER_FAST=0 sends these calls to the dispatcher ops too."""
+    from chill_attention import _eager, cache
+
+    monkeypatch.setattr(_eager, "ENABLED", True)
+    assert cache._direct()
+    monkeypatch.setattr(_eager, "ENABLED", False)
+    assert not cache._direct()
+
+
 def test_oracle_trim_undoes_reserve():
     table, held, free = [[5, -1, -1, -1], [-1] * 4, [7, 2, -1, -1]], [1, 0, 2], [9, 8, 6, 4, 3, 1, 0]
     lens, new = [10, 0, 20], [30, 16, 0]
