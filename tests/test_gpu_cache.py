@@ -965,3 +965,26 @@ def test_a_tensor_that_watches_its_operators():
         Watching.seen.clear()
         got = ca.chill_pages_reserve(ca.ChillPages.empty(2, 100, 8, 16), lens, step.new_lens, 3, 16, parents)
         assert any("pages_reserve" in name for name in Watching.seen) and (got.slots >= 0).all()
+
+
+@pytest.mark.parametrize("name,status", [("libchill_cache_b200.so", "chill_cache_read_device_status"), ("libchill_b200.so", "chill_read_device_status")])
+def test_the_status_word_after_a_reset_of_the_device(name, status):
+    """A process that resets its device (its own context alone) finds the word again."""
+    import glob
+    import os
+    import subprocess
+    import sys
+
+    from chill_attention import _cabi
+
+    runtime = glob.glob(os.path.join(os.path.dirname(os.path.dirname(torch.__file__)), "nvidia", "cuda_runtime", "lib", "libcudart.so.*"))
+    if not runtime:
+        pytest.skip("no shared CUDA runtime")
+    code = f"""
+import ctypes
+read = getattr(ctypes.CDLL({os.path.join(_cabi.LIB_DIR, name)!r}), {status!r})
+runtime = ctypes.CDLL({runtime[0]!r})
+print(read(), runtime.cudaDeviceReset(), read(), read())
+"""
+    r = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=240)
+    assert r.stdout.split() == ["0"] * 4, r.stdout + r.stderr[-2000:]
