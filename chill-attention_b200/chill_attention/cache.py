@@ -309,7 +309,8 @@ def chill_cache_commit(k_cache: torch.Tensor, v_cache: torch.Tensor, table: torc
         path: int32 [batch, longest path], numbers of the accepted tokens from the root on (increasing).
         accepted: int32 [batch], how many of them; clamped to [0, min(longest path, new_lens[b])].
 
-    Returns: int32 [batch], the new lengths ``lens + accepted``, without the accepted tokens from the first one without a page on.  Pages stay reserved; ``chill_pages_trim`` gives spare ones back.
+    Returns: int32 [batch], the new lengths ``lens + accepted``, without the accepted tokens from the first one without a page on.  k_cache and
+    v_cache may be the same tensor, but not overlap otherwise.  Pages stay reserved; ``chill_pages_trim`` gives spare ones back.
     """
     N = step.slots.shape[1]
     if _direct():

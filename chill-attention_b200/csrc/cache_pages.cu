@@ -250,6 +250,7 @@ struct RowsP {
   const int *table, *lens, *new_lens, *path, *accepted;
   long long table_sb;
   int width, A;
+  int moved;  // vectors of a token that move: those of K and V, or where both are one tensor those of it
   int* out_lens;
 };
 
@@ -307,7 +308,7 @@ __global__ void __launch_bounds__(128) commit_kernel(RowsP p) {
       continue;
     }
     const int idx = blockIdx.x * 128 + threadIdx.x;
-    if (idx >= 2 * p.per_token) continue;
+    if (idx >= p.moved) continue;
     const bool is_v = idx >= p.per_token;
     const int rem = is_v ? idx - p.per_token : idx, h = rem / p.per_row, c = rem - h * p.per_row;
     const long long* st = is_v ? p.vcs : p.kcs;
@@ -427,7 +428,12 @@ int chill_cache_commit(const chill_cache_rows_args* a, void* stream) {
   byte_strides(p.kcs, a->k_cache_strides, es, vec); byte_strides(p.vcs, a->v_cache_strides, es, vec);
   p.table = a->table; p.table_sb = a->table_stride; p.width = a->table_width;
   p.lens = a->lens; p.new_lens = a->new_lens; p.path = a->path; p.accepted = a->accepted; p.A = a->A; p.out_lens = a->out_lens;
-  const dim3 grid((unsigned)((2 * p.per_token + 127) / 128 + 1), (unsigned)imin(a->B, 65535));
+  // K and V in one tensor: each row moves once (two threads that move it one after the other would read what the other has written)
+  bool one = a->k_cache == a->v_cache;
+  for (int d = 0; d < 4 && one; ++d)
+    if (a->k_cache_strides[d] != a->v_cache_strides[d]) return CHILL_E_INVALID;
+  p.moved = (one ? 1 : 2) * p.per_token;
+  const dim3 grid((unsigned)((p.moved + 127) / 128 + 1), (unsigned)imin(a->B, 65535));
   if (wide) commit_kernel<uint4><<<grid, 128, 0, (cudaStream_t)stream>>>(p);
   else if (es == 4) commit_kernel<uint32_t><<<grid, 128, 0, (cudaStream_t)stream>>>(p);
   else commit_kernel<uint16_t><<<grid, 128, 0, (cudaStream_t)stream>>>(p);

@@ -76,7 +76,8 @@ typedef struct chill_cache_rows_args {
 /* Row (b, head, i) of k and v goes to slot slots[b][i] of the caches; slots outside the cache are skipped. */
 int chill_cache_append(const chill_cache_rows_args* a, void* stream);
 /* The accepted path of every tree becomes contiguous: for j < accepted[b], row lens[b] + path[b][j] is copied to row lens[b] + j
- * (path[b][j] <= j: it stays as it is).  The path ends before the first token without a page. */
+ * (path[b][j] <= j: it stays as it is).  The path ends before the first token without a page.  k_cache and v_cache may be one tensor (then with
+ * one set of strides), but not overlap in another way. */
 int chill_cache_commit(const chill_cache_rows_args* a, void* stream);
 
 /* O = softmax(mask(Q K^T * sm_scale)) V of the new tokens over the cached and the new keys, and its LSE (log2 units).  The rows of

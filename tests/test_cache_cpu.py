@@ -115,6 +115,9 @@ def test_page_and_row_refusals(lib):
     for name in ("table", "lens", "new_lens", "path", "accepted", "out_lens"):
         assert lib.chill_cache_commit(rows(**{name: None}), None) == -1
     assert lib.chill_cache_commit(rows(), None) == -1  # out_lens is lens: the CTAs of a request all read its length
+    strides = (ctypes.c_int64 * 4)(2048, 1024, 64, 1)
+    apart = dict(out_lens=8192, k_cache_strides=strides)  # one tensor for K and V, in two layouts
+    assert lib.chill_cache_commit(rows(**apart), None) == -1
     assert lib.chill_cache_commit(rows(A=0), None) == -1 and lib.chill_cache_commit(rows(table_width=0), None) == -1
 
 

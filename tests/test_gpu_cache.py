@@ -988,3 +988,21 @@ print(read(), runtime.cudaDeviceReset(), read(), read())
 """
     r = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=240)
     assert r.stdout.split() == ["0"] * 4, r.stdout + r.stderr[-2000:]
+
+
+@pytest.mark.parametrize("layout", ["plain", "odd"])
+def test_commit_of_one_tensor_for_keys_and_values(layout):
+    """Each row moves once, also along a path whose rows are sources after they were targets."""
+    import chill_attention as ca
+
+    N, D, lens = 40, 256, [10, 0, 77]
+    paths, accepted = [list(range(1, 21)), list(range(0, 40, 2)), list(range(20, 40))], [20, 20, 20]
+    p = Problem(torch.bfloat16, 2, 2, D, lens, [N] * 3, N, 16, tree=True, seed=1)
+    want = p.k_cache.clone()
+    for b, c in enumerate(lens):
+        for j, f in enumerate(paths[b]):
+            want[p.table[b, (c + j) // 16], :, (c + j) % 16] = p.k_cache[p.table[b, (c + f) // 16], :, (c + f) % 16]
+    for _ in range(5):
+        cache = strided(p.k_cache, layout).clone() if layout == "plain" else strided(p.k_cache, layout)
+        assert ca.chill_cache_commit(cache, cache, p.table.cuda(), p.step(), ints(paths), ints(accepted)).tolist() == [30, 20, 97]
+        assert torch.equal(cache.cpu().nan_to_num(7), want.nan_to_num(7))
