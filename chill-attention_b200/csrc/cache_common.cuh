@@ -285,10 +285,8 @@ struct Work {
   __device__ __forceinline__ void close(const CachedP& p) {
     if ((threadIdx.x & 31) == 0) {
       p.seams[share] = seam;
-      if (cut.shares > cut.large) {
-        pdl_wait();
-        ahead = cut.large + atomicAdd(p.queue, 1);
-      }
+      if (p.tail_shares > 0) pdl_wait();  // prepare_kernel has cleared the counter; also where nobody asks it, or the call could end before that kernel
+      if (cut.shares > cut.large) ahead = cut.large + atomicAdd(p.queue, 1);
     }
     __syncwarp();
   }

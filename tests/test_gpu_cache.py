@@ -1006,3 +1006,29 @@ def test_commit_of_one_tensor_for_keys_and_values(layout):
         cache = strided(p.k_cache, layout).clone() if layout == "plain" else strided(p.k_cache, layout)
         assert ca.chill_cache_commit(cache, cache, p.table.cuda(), p.step(), ints(paths), ints(accepted)).tolist() == [30, 20, 97]
         assert torch.equal(cache.cpu().nan_to_num(7), want.nan_to_num(7))
+
+
+def test_nothing_of_a_call_comes_after_it():
+    """A table with room for small shares and few keys there: the kernel that clears their counter is waited for, so what takes the
+    workspace's memory next keeps its bytes."""
+    import ctypes
+
+    from chill_attention import _cabi, _cache_abi
+
+    p = Problem(torch.bfloat16, 4, 4, 64, [300, 20], [2] * 2, 2, 64, tree=True, seed=5, room=400000)
+    a = _cache_abi.CachedArgs()
+    a.mask = _cabi.mask_desc(_cabi.MASK_CAUSAL, ())
+    a.B, a.H, a.H_kv, a.N, a.D, a.dtype, a.page_size, a.num_pages, a.table_width, a.sm_scale = 2, 4, 4, 2, 64, 2, 64, p.k_cache.shape[0], p.table.shape[1], 1.0
+    for name, t in (("q_strides", p.q), ("k_cache_strides", p.k_cache), ("v_cache_strides", p.v_cache)):
+        setattr(a, name, (ctypes.c_int64 * 4)(*t.stride()))
+    size = _cache_abi.load_library().chill_cached_workspace_bytes(ctypes.byref(a))
+    assert size > 0
+    args = p.q.cuda(), p.k_cache.cuda(), p.v_cache.cuda(), p.table.cuda(), p.step(), masks()["causal"]
+    import chill_attention as ca
+
+    want = ca.chill_attention_cached(*args)
+    for _ in range(50):
+        o = ca.chill_attention_cached(*args)
+        behind = torch.full((size,), 7, dtype=torch.uint8, device="cuda")
+        assert (behind == 7).all() and torch.equal(o, want)
+        del behind
