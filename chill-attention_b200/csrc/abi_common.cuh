@@ -24,28 +24,10 @@ static int cuda_fail(cudaError_t e, const char* what) {
 }
 
 static int* device_status_ptr() {
-  // One word per device (the symbol is instantiated in every device's module image).  Asking for its address takes time (one new token for two
-  // requests of 300: 12.8 us a call, 10.5 without), so a thread keeps it by the context's id: after a reset of the device the context is
-  // another one, and so may the address be.
-  typedef CUresult (*CtxGetIdFn)(CUcontext, unsigned long long*);
-  static const CtxGetIdFn ctx_id = [] {
-    void* f = nullptr;
-    cudaDriverEntryPointQueryResult found;
-    return cudaGetDriverEntryPoint("cuCtxGetId", &f, cudaEnableDefault, &found) == cudaSuccess && found == cudaDriverEntryPointSuccess ? (CtxGetIdFn)f : nullptr;
-  }();
-  struct Known {
-    bool is;
-    unsigned long long id;
-    int* p;
-  };
-  static thread_local Known known[8] = {};
-  unsigned long long id = 0;
-  const bool has_id = ctx_id != nullptr && ctx_id(nullptr, &id) == CUDA_SUCCESS;
-  Known& k = known[id % 8];
-  if (has_id && k.is && k.id == id) return k.p;
+  // one word per device (the symbol is instantiated in every device's module image), asked for each time (33 ns): an address that is kept is
+  // a stale one after a reset of the device
   int* p = nullptr;
   if (cudaGetSymbolAddress((void**)&p, g_device_status) != cudaSuccess) return nullptr;
-  if (has_id) k = Known{true, id, p};
   return p;
 }
 
