@@ -4,14 +4,15 @@ for each request, a chunk of a prompt, or a tree of drafted tokens) over the cac
     pages = ChillPages.empty(batch, max_len, num_pages, page_size)        # integer tensors, on the GPU
     k_cache = torch.empty(num_pages, kv_heads, page_size, head_dim, dtype=..., device="cuda")   # v_cache alike
     lens = torch.zeros(batch, dtype=torch.int32, device="cuda")           # tokens in the cache
+    stored = torch.empty_like(lens)
     while ...:                                                            # one step, for every layer its own caches
-        step = chill_pages_reserve(pages, lens, new_lens, max_new, page_size, parents)
+        step = chill_pages_reserve(pages, lens, new_lens, max_new, page_size, parents, stored)
         # project; rotate q and k to step.positions
         chill_cache_append(k_cache, v_cache, k, v, step.slots)            # k, v: [batch, kv_heads, max_new, head_dim]
         o = chill_attention_cached(q, k_cache, v_cache, pages.table, step, mask)
         # a tree: choose the path to keep, then
         lens = chill_cache_commit(k_cache, v_cache, pages.table, step, path, accepted)
-        # a chain: lens = lens + step.stored   (new_lens, unless pages ran out: what got no page comes again in a later step)
+        # a chain: lens = lens + stored   (new_lens, unless pages ran out: what got no page comes again in a later step)
     chill_pages_trim(pages, lens, page_size)                              # lens[b] = 0: request b is done
 
 Nothing here synchronises or copies to the host, lengths are read on the GPU, and every call can be captured into a CUDA graph and
@@ -65,15 +66,13 @@ class ChillPages(typing.NamedTuple):
 class ChillStep(typing.NamedTuple):
     """The new tokens of a step, int32 tensors on the GPU: lens [batch] tokens in the cache before, new_lens [batch] new ones,
     slots [batch, max_new] page * page_size + row of each (-1: none), positions [batch, max_new], and for trees ancestors
-    [batch, max_new, (max_new + 31) // 32]: bit j of row i says that token j is token i or above it; stored [batch] how many of the new
-    tokens got a slot, the first so many: all of them unless pages ran out."""
+    [batch, max_new, (max_new + 31) // 32]: bit j of row i says that token j is token i or above it."""
 
     lens: torch.Tensor
     new_lens: torch.Tensor
     slots: torch.Tensor
     positions: torch.Tensor
     ancestors: typing.Optional[torch.Tensor]
-    stored: typing.Optional[torch.Tensor] = None
 
 
 def _native(lib=None):
@@ -176,22 +175,34 @@ def _check_attention(q, k_cache, v_cache, table, lens, new_lens, positions, ance
 
 
 # ------------------------------------------------------------------------- dispatcher ops: torch.compile, modes, subclasses
+def _reserve(pages, lens, new_lens, max_new, page_size, parents, stored):
+    _check_pages(pages, lens, page_size)
+    _check_reserve(pages, new_lens, max_new, parents, stored)
+    slots, positions, ancestors = _eager.extension().pages_reserve(_native(), *pages, lens, new_lens, max_new, page_size, parents, stored)
+    return slots, positions, ancestors if ancestors is not None else slots.new_empty(0)
+
+
 @torch.library.custom_op("chill_attention::pages_reserve", mutates_args=("table", "held", "free", "n_free", "missing"), device_types=("cuda",))
 def _reserve_op(table: torch.Tensor, held: torch.Tensor, free: torch.Tensor, n_free: torch.Tensor, missing: torch.Tensor, lens: torch.Tensor,
                 new_lens: torch.Tensor, max_new: int, page_size: int,
-                parents: typing.Optional[torch.Tensor]) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor]:
-    _check_pages(ChillPages(table, held, free, n_free, missing), lens, page_size)
-    _check_reserve(ChillPages(table, held, free, n_free, missing), new_lens, max_new, parents)
-    slots, positions, ancestors, stored = _eager.extension().pages_reserve(_native(), table, held, free, n_free, missing, lens, new_lens, max_new,
-                                                                           page_size, parents)
-    return slots, positions, ancestors if ancestors is not None else slots.new_empty(0), stored
+                parents: typing.Optional[torch.Tensor]) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    return _reserve(ChillPages(table, held, free, n_free, missing), lens, new_lens, max_new, page_size, parents, None)
 
 
+@torch.library.custom_op("chill_attention::pages_reserve_stored", mutates_args=("table", "held", "free", "n_free", "missing", "stored"),
+                         device_types=("cuda",))
+def _reserve_stored_op(table: torch.Tensor, held: torch.Tensor, free: torch.Tensor, n_free: torch.Tensor, missing: torch.Tensor, lens: torch.Tensor,
+                       new_lens: torch.Tensor, max_new: int, page_size: int, parents: typing.Optional[torch.Tensor],
+                       stored: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    return _reserve(ChillPages(table, held, free, n_free, missing), lens, new_lens, max_new, page_size, parents, stored)
+
+
+@_reserve_stored_op.register_fake
 @_reserve_op.register_fake
-def _(table, held, free, n_free, missing, lens, new_lens, max_new, page_size, parents):
+def _(table, held, free, n_free, missing, lens, new_lens, max_new, page_size, parents, stored=None):
     B = table.shape[0]
     shape = (B, max_new, (max_new + 31) // 32) if parents is not None else (0,)
-    return table.new_empty(B, max_new), table.new_empty(B, max_new), table.new_empty(shape), table.new_empty(B)
+    return table.new_empty(B, max_new), table.new_empty(B, max_new), table.new_empty(shape)
 
 
 @torch.library.custom_op("chill_attention::pages_trim", mutates_args=("table", "held", "free", "n_free"), device_types=("cuda",))
@@ -244,41 +255,47 @@ def _(q, k_cache, v_cache, table, lens, new_lens, positions, ancestors, mask_nam
 
 
 # ------------------------------------------------------------------------------------------------------------ public calls
-def _check_reserve(pages, new_lens, max_new, parents):
+def _check_reserve(pages, new_lens, max_new, parents, stored):
     B = pages.table.shape[0]
     assert 1 <= max_new < 2 ** 31
     _check_ints(pages.table, missing=(pages.missing, (1,)), new_lens=(new_lens, (B,)))
     if parents is not None:
         _check_ints(pages.table, parents=(parents, (B, max_new)))
+    if stored is not None:
+        _check_ints(pages.table, stored=(stored, (B,)))
 
 
 def chill_pages_reserve(pages: ChillPages, lens: torch.Tensor, new_lens: torch.Tensor, max_new: int, page_size: int,
-                        parents: torch.Tensor | None = None) -> ChillStep:
+                        parents: torch.Tensor | None = None, stored: torch.Tensor | None = None) -> ChillStep:
     """Pages for ``new_lens[b]`` tokens behind the ``lens[b]`` that request b has, and where they go.
 
     Args:
         pages: changed in place.  Pages are taken from the top of the stack, requests in order; a request keeps what it holds
             already.  Where the stack runs out, or a table is full, the tokens left without a page get slot -1 (they are not
-            stored, and nobody sees them) and ``pages.missing`` says how many pages the stack was short of.  Only the ``step.stored[b]``
-            others may be counted in lens afterwards: a page that a later step finds for a token that was never stored holds what its
-            former owner left there.
+            stored, and nobody sees them) and ``pages.missing`` says how many pages the stack was short of.  Only the others may
+            be counted in lens afterwards (see stored): a page that a later step finds for a token that was never stored holds what
+            its former owner left there.
         lens, new_lens: int32 [batch]; new_lens is clamped to [0, max_new].
         max_new: second dimension of the step's tensors.
         page_size: rows of a page of the caches.
         parents: int32 [batch, max_new] for trees of drafted tokens: number of each token's parent among the new ones, smaller than its
             own; anything else (-1) makes it a child of the last cached token.  Without it the new tokens are a chain.
+        stored: int32 [batch], written where given (a tensor of its own): how many of a request's new tokens got a slot, the first so many.
 
     Returns: the step's ChillStep; positions are lens[b] + depth (chain: lens[b] + number).
     """
     if _direct():
         native = _NATIVE.get(None) or _native()
-        out = _eager._extension.pages_reserve(native, *pages, lens, new_lens, max_new, page_size, parents)
+        out = _eager._extension.pages_reserve(native, *pages, lens, new_lens, max_new, page_size, parents, stored)
         if out is not None:
             return ChillStep(lens, new_lens, *out)
     _check_pages(pages, lens, page_size)
-    _check_reserve(pages, new_lens, max_new, parents)
-    slots, positions, ancestors, stored = _reserve_op(*pages, lens, new_lens, max_new, page_size, parents)
-    return ChillStep(lens, new_lens, slots, positions, ancestors if parents is not None else None, stored)
+    _check_reserve(pages, new_lens, max_new, parents, stored)
+    if stored is None:
+        slots, positions, ancestors = _reserve_op(*pages, lens, new_lens, max_new, page_size, parents)
+    else:
+        slots, positions, ancestors = _reserve_stored_op(*pages, lens, new_lens, max_new, page_size, parents, stored)
+    return ChillStep(lens, new_lens, slots, positions, ancestors if parents is not None else None)
 
 
 def chill_pages_trim(pages: ChillPages, lens: torch.Tensor, page_size: int) -> None:
@@ -374,7 +391,7 @@ def _attention(q, k_cache, v_cache, table, step, mask, sm_scale, return_lse, fla
         _mask_functor(mask)
     elif _MASKS[mask.name][2] is not type(mask):
         _check_same_name(mask)
-    lens, new_lens, _, positions, ancestors = step[:5]
+    lens, new_lens, _, positions, ancestors = step
     if _direct():
         native, functor_id, _ = _MASKS[mask.name]
         out = _eager._extension.cached_attention(native, functor_id, q, k_cache, v_cache, table, lens, new_lens, positions, ancestors,

@@ -373,7 +373,11 @@ using namespace chill::cache;
 extern "C" {
 
 int chill_pages_reserve_stored(const chill_pages_args* a, int32_t* stored, void* stream) {
-  const int st = check_pages(a, false);
+  int st = check_pages(a, false);
+  if (st == CHILL_OK && stored != nullptr)  // written while CTAs read and write the others
+    for (const int32_t* other : {a->lens, a->new_lens, a->parents, (const int32_t*)a->table, (const int32_t*)a->held, (const int32_t*)a->free_pages, (const int32_t*)a->n_free,
+                                 (const int32_t*)a->missing, (const int32_t*)a->slots, (const int32_t*)a->positions, (const int32_t*)a->ancestors})
+      if (stored == other) st = CHILL_E_INVALID;
   return st != CHILL_OK ? st : launch_pages<false>(pages_params(*a, stored), (cudaStream_t)stream);
 }
 

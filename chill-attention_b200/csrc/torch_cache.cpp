@@ -44,11 +44,11 @@ void check(const CacheLibrary& lib, int status, const char* what) {
 Tensor empty(at::IntArrayRef sizes, at::ScalarType type, const Tensor& like) { return at::detail::empty_cuda(sizes, type, like.device(), std::nullopt); }
 
 // A tensor that something looks in on (a subclass with its own dispatch, a transform): the dispatcher ops serve it.
-bool watched(std::initializer_list<const Tensor*> tensors, const std::optional<Tensor>& one_more = std::nullopt) {
+bool watched(std::initializer_list<const Tensor*> tensors, const std::optional<Tensor>& one_more = std::nullopt, const std::optional<Tensor>& another = std::nullopt) {
   auto looked_at = [](const Tensor& t) { return t.unsafeGetTensorImpl()->key_set().has_any(c10::python_ks | c10::functorch_transforms_ks); };
   for (const Tensor* t : tensors)
     if (looked_at(*t)) return true;
-  return one_more.has_value() && looked_at(*one_more);
+  return (one_more.has_value() && looked_at(*one_more)) || (another.has_value() && looked_at(*another));
 }
 
 void* current_stream(const Tensor& t) { return (void*)c10::cuda::getCurrentCUDAStream(t.get_device()).stream(); }
@@ -104,14 +104,14 @@ void changed(std::initializer_list<const Tensor*> tensors) {
 const int32_t* optional_ints(const std::optional<Tensor>& t) { return t.has_value() ? t->const_data_ptr<int32_t>() : nullptr; }
 
 py::object reserve(const CacheLibrary& lib, const Tensor& table, const Tensor& held, const Tensor& free, const Tensor& n_free, const Tensor& missing,
-                   const Tensor& lens, const Tensor& new_lens, int64_t N, int64_t page, const std::optional<Tensor>& parents) {
-  if (watched({&table, &held, &free, &n_free, &missing, &lens, &new_lens}, parents) || !table_ok(table) || N < 1 || N > INT32_MAX || page < 1 || page > INT32_MAX) return py::none();
+                   const Tensor& lens, const Tensor& new_lens, int64_t N, int64_t page, const std::optional<Tensor>& parents, const std::optional<Tensor>& stored) {
+  if (watched({&table, &held, &free, &n_free, &missing, &lens, &new_lens}, parents, stored) || !table_ok(table) || N < 1 || N > INT32_MAX || page < 1 || page > INT32_MAX) return py::none();
   const int64_t B = table.size(0);
   if (!ints(held, {B}, table) || free.dim() != 1 || free.size(0) < 1 || !fit(free) || !ints(free, {free.size(0)}, table) || !ints(n_free, {1}, table) ||
-      !ints(missing, {1}, table) || !ints(lens, {B}, table) || !ints(new_lens, {B}, table) || (parents.has_value() && !ints(*parents, {B, N}, table)))
+      !ints(missing, {1}, table) || !ints(lens, {B}, table) || !ints(new_lens, {B}, table) || (parents.has_value() && !ints(*parents, {B, N}, table)) || (stored.has_value() && !ints(*stored, {B}, table)))
     return py::none();
   c10::cuda::CUDAGuard guard(table.device());
-  Tensor slots = empty({B, N}, at::kInt, table), positions = empty({B, N}, at::kInt, table), stored = empty({B}, at::kInt, table), ancestors;
+  Tensor slots = empty({B, N}, at::kInt, table), positions = empty({B, N}, at::kInt, table), ancestors;
   if (parents.has_value()) ancestors = empty({B, N, (N + 31) / 32}, at::kInt, table);
   chill_pages_args a{};
   a.B = (int32_t)B; a.N = (int32_t)N; a.page_size = (int32_t)page; a.num_pages = (int32_t)free.size(0); a.table_width = (int32_t)table.size(1);
@@ -121,9 +121,10 @@ py::object reserve(const CacheLibrary& lib, const Tensor& table, const Tensor& h
   a.lens = lens.const_data_ptr<int32_t>(); a.new_lens = new_lens.const_data_ptr<int32_t>(); a.parents = optional_ints(parents);
   a.slots = slots.mutable_data_ptr<int32_t>(); a.positions = positions.mutable_data_ptr<int32_t>();
   a.ancestors = parents.has_value() ? ancestors.mutable_data_ptr<int32_t>() : nullptr;
-  check(lib, lib.reserve(&a, stored.mutable_data_ptr<int32_t>(), current_stream(table)), "chill_pages_reserve");
+  check(lib, lib.reserve(&a, stored.has_value() ? stored->mutable_data_ptr<int32_t>() : nullptr, current_stream(table)), "chill_pages_reserve");
   changed({&table, &held, &free, &n_free, &missing});
-  return py::make_tuple(slots, positions, parents.has_value() ? py::cast(ancestors) : py::none(), stored);
+  if (stored.has_value()) changed({&*stored});
+  return py::make_tuple(slots, positions, parents.has_value() ? py::cast(ancestors) : py::none());
 }
 
 bool trim(const CacheLibrary& lib, const Tensor& table, const Tensor& held, const Tensor& free, const Tensor& n_free, const Tensor& lens, int64_t page) {

@@ -49,7 +49,7 @@ typedef struct chill_pages_args {
  * (lens[b] + depth; without parents lens[b] + number) and ancestors of the new tokens.  Pages that a request holds beyond
  * that stay its own.  Where pages run out, or a table is full, the tokens without one get slot -1. */
 int chill_pages_reserve(const chill_pages_args* a, void* stream);
-/* The same, and in stored[b] (may be NULL) how many of a request's new tokens got a slot: the first so many.  Where there was a shortage only these
+/* The same, and in stored[b] (may be NULL; an array of its own) how many of a request's new tokens got a slot: the first so many.  Where there was a shortage only these
  * may be counted in lens afterwards; the others' rows are never written, and a page that turns up for them later holds its former owner's. */
 int chill_pages_reserve_stored(const chill_pages_args* a, int32_t* stored, void* stream);
 /* Pages behind lens[b] tokens go back to the stack (lens[b] = 0: all), their table entries become -1.  The inverse of reserve: the

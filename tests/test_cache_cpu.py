@@ -91,6 +91,8 @@ def test_page_and_row_refusals(lib):
     assert lib.chill_pages_reserve(pages(B=65536), None) == lib.chill_pages_reserve(pages(num_pages=2 ** 27), None) == -4
     assert lib.chill_pages_trim(pages(table_width=2 ** 26), None) == -4
 
+    for name in ("lens", "new_lens", "held", "table", "slots"):  # stored is an array of its own
+        assert lib.chill_pages_reserve_stored(pages(**{name: 8192}), 8192, None) == -1
     # sums of pages over the requests are 32 bits wide: tables with more entries than that
     for B, width in ((65535, 2 ** 16), (8, 2 ** 28), (5, 2 ** 29)):
         big = pages(B=B, page_size=1, num_pages=2 ** 30, table_width=width, table_stride=width)

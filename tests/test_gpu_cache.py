@@ -795,20 +795,20 @@ def test_a_session_that_runs_short_of_pages():
     pages = ca.ChillPages.empty(2, 64, 4, page)
     kc, vc = (torch.full((4, 2, page, D), 50.0, device="cuda") for _ in range(2))
     lens, done = ints([0, 0]), [0, 0]
-    stored = []
+    stored, got = [], ints([-9, -9])
     for turn, new in enumerate([(20, 10), (12, 30), (0, 8)]):
         N = max(new)
         row = lambda t: torch.stack([torch.nn.functional.pad(t[b, :, done[b]:done[b] + new[b]], (0, 0, 0, N - t[b, :, done[b]:done[b] + new[b]].shape[1])) for b in range(2)])  # noqa: E731
-        step = ca.chill_pages_reserve(pages, lens, ints(new), N, page)
-        stored.append(step.stored.tolist())
-        assert step.stored.tolist() == (step.slots >= 0).sum(1).tolist()
+        step = ca.chill_pages_reserve(pages, lens, ints(new), N, page, stored=got)
+        stored.append(got.tolist())
+        assert stored[-1] == (step.slots >= 0).sum(1).tolist()
         ca.chill_cache_append(kc, vc, row(k), row(v), step.slots)
         o = ca.chill_attention_cached(row(q), kc, vc, pages.table, step, ca.CausalChillMask())
-        for b, n in enumerate(step.stored.tolist()):
+        for b, n in enumerate(stored[-1]):
             if n > 0:  # both are within the operator's bar of the exact result
                 assert (o[b, :, :n] - want[b, :, done[b]:done[b] + n]).abs().max() <= 2 * O_ATOL[torch.float32]
             done[b] += n
-        lens = lens + step.stored
+        lens = lens + got
         assert lens.tolist() == done
         if turn == 1:
             assert pages.missing.item() == 1
@@ -826,8 +826,9 @@ def test_stored_counts_the_slots(B, N, page):
     for num in (1, B * (20 + N) // page // 2 + 1, B * (-(-(20 + N) // page))):
         pages = ca.ChillPages.empty(B, 10 + N, num, page)  # some tables are full too
         for parents in (None, torch.full((B, N), -1, dtype=torch.int32, device="cuda")):
-            step = ca.chill_pages_reserve(pages, ints(draw(20)), ints(draw(N)), N, page, parents)
-            assert step.stored.tolist() == (step.slots >= 0).sum(1).tolist()
+            stored = torch.full((B,), -9, dtype=torch.int32, device="cuda")
+            step = ca.chill_pages_reserve(pages, ints(draw(20)), ints(draw(N)), N, page, parents, stored)
+            assert stored.tolist() == (step.slots >= 0).sum(1).tolist()
 
 
 def test_commit_ends_before_the_first_token_without_a_page():
@@ -836,10 +837,11 @@ def test_commit_ends_before_the_first_token_without_a_page():
     page, D = 16, 64
     pages = ca.ChillPages.empty(3, 64, 3, page)
     kc, vc = (torch.full((3, 1, page, D), 9.0, device="cuda") for _ in range(2))
-    first = ca.chill_pages_reserve(pages, ints([0, 0, 0]), ints([10, 14, 14]), 14, page)
-    assert first.stored.tolist() == [10, 14, 14]
-    step = ca.chill_pages_reserve(pages, ints([10, 14, 14]), ints([4, 6, 6]), 6, page, ints([[-1] * 6] * 3))
-    assert step.stored.tolist() == [4, 2, 2] and pages.missing.item() == 2
+    stored = ints([0, 0, 0])
+    ca.chill_pages_reserve(pages, ints([0, 0, 0]), ints([10, 14, 14]), 14, page, stored=stored)
+    assert stored.tolist() == [10, 14, 14]
+    step = ca.chill_pages_reserve(pages, ints([10, 14, 14]), ints([4, 6, 6]), 6, page, ints([[-1] * 6] * 3), stored)
+    assert stored.tolist() == [4, 2, 2] and pages.missing.item() == 2
     k = torch.arange(18, device="cuda", dtype=torch.float32).view(3, 1, 6, 1).expand(3, 1, 6, D)
     ca.chill_cache_append(kc, vc, k, -k, step.slots)
     lens = ca.chill_cache_commit(kc, vc, pages.table, step, ints([[1, 3, 5], [0, 1, 2], [1, 4, 5]]), ints([2, 3, 3]))
@@ -1032,3 +1034,30 @@ def test_nothing_of_a_call_comes_after_it():
         behind = torch.full((size,), 7, dtype=torch.uint8, device="cuda")
         assert (behind == 7).all() and torch.equal(o, want)
         del behind
+
+
+def test_stored_through_the_dispatcher_and_its_refusals():
+    import chill_attention as ca
+
+    lens, new, parents = ints([0, 5]), ints([20, 30]), ints([[-1] * 30] * 2)
+
+    def reserve(pages, stored):
+        return ca.chill_pages_reserve(pages, lens, new, 30, 16, parents, stored).slots
+
+    results = []
+    for call in (reserve, torch.compile(reserve, fullgraph=True), lambda pages, stored: torch.ops.chill_attention.pages_reserve_stored(
+            *pages, lens, new, 30, 16, parents, stored)[0]):
+        pages, stored = ca.ChillPages.empty(2, 100, 3, 16), ints([-9, -9])
+        version = stored._version
+        slots = call(pages, stored)
+        assert stored.tolist() == (slots >= 0).sum(1).tolist() == [20, 11] and stored._version > version
+        results.append((slots, *pages))
+    assert all(torch.equal(x, y) for other in results[1:] for x, y in zip(results[0], other))
+    pages = ca.ChillPages.empty(2, 100, 3, 16)
+    for bad in (ints([0]), torch.zeros(2, device="cuda"), torch.zeros(2, dtype=torch.int32), ints([0, 0, 0, 0])[::2]):
+        with pytest.raises(AssertionError):
+            reserve(pages, bad)
+    for taken in (lens, new, pages.held):
+        with pytest.raises(RuntimeError, match="invalid argument"):
+            reserve(pages, taken)
+    assert pages.n_free.item() == 3
