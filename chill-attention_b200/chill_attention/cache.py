@@ -367,7 +367,8 @@ def chill_attention_cached(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torc
                            sm_scale: float | None = None, return_lse: bool = False):
     """Exact softmax attention of the step's new tokens over the cached and the new keys that ``mask`` allows.
 
-    Token i of request b stands at position ``step.positions[b, i]`` and sees cached key t (position t) iff the mask allows the pair, and
+    Token i of request b stands at position ``step.positions[b, i]`` in a tree and at ``step.lens[b] + i`` in a chain (whatever
+    ``step.positions`` holds; ``chill_pages_reserve`` puts the same there), and sees cached key t (position t) iff the mask allows the pair, and
     new key j iff the mask allows their positions and, in a tree, j is an ancestor of i or i itself.  In a chain a mask that looks ahead (full,
     chunkwise) lets a token see the new ones behind it.  Keys without a page are not there.
 
@@ -380,6 +381,11 @@ def chill_attention_cached(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torc
         return_lse: also return the log-sum-exp of every row in log2 units, shape [batch, heads, max_new].
 
     Returns: O, or (O, LSE).  A token that sees nothing: O = 0, LSE = -inf; rows at or behind new_lens[b]: zeros, LSE 0.
+
+    Scores, sums and O are kept in fp32.  16-bit caches on the tensor cores: the softmax weights go into the second product rounded once to
+    the caches' type (as in ``chill_attention``), with up to 16 rows (tokens times the heads that share a kv head) as two such numbers; so a
+    token's last bits depend on how many stand beside it.  A key that is not finite shows in the rows that see it and in no others; these are
+    worked out key by key, which over long tables takes seconds.
     """
     return _attention(q, k_cache, v_cache, table, step, mask, sm_scale, return_lse, 0)
 

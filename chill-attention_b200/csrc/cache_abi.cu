@@ -66,8 +66,8 @@ struct Plan {
 
 // What a CTA spends on a unit beside its tiles (Q, the parts of O, the next piece's start), in tiles.  Kernel for few rows: 0 / 2 / 4 tiles
 // 184.5 / 182.3 / 183.4 us (64 requests of up to 8192 tokens, one new each), 48.5 / 46.9 / 54.5 us (24 drafts each for 32 requests, window
-// of 1024).  Kernel for many rows: 0 / 3 / 5 / 7 / 10 tiles 110 / 96.3 / 92.4 / 90.1 / 92.9 us (64 drafts for 16 requests), 453 / 463 / 449 / 450 / 454
-// us (1024 new tokens for 4 requests).
+// of 1024).  Kernel for many rows: 0 / 3 / 5 / 6 / 7 / 10 tiles 106.4 / 99.1 / 94.2 / 92.3 / 92.7 / 94.6 us (64 drafts for 16 requests), 437 / 418 /
+// 411 / 407 / 403 to 428 / 408 to 438 us (1024 new tokens for 4 requests).
 constexpr int kRowsPad = 2, kTilesPad = 6;
 
 // Keys a token can see at most in a table of `keys` (looked at for 32 positions: what is chosen by it is a matter of time alone).

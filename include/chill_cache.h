@@ -108,11 +108,11 @@ size_t chill_cached_workspace_bytes(const chill_cached_args* a);
 int chill_cached_fwd(const chill_cached_args* a, void* stream);
 /* Which kernel chill_cached_fwd would launch (host-only; pointers are looked at for their alignment), or a negative status. */
 #define CHILL_CACHED_CUDA_CORES 0 /* fp32, and what the others can not take */
-#define CHILL_CACHED_ROWS 1       /* 16-bit, up to 32 rows (N * H / H_kv) of a kv head, and queries that the tiles can not take */
+#define CHILL_CACHED_ROWS 1       /* 16-bit, up to 32 rows (N * H / H_kv) of a kv head, 16 above head dim 128, and queries that the tiles can not take */
 #define CHILL_CACHED_TILES 2      /* 16-bit, tiles of 128 rows */
 int chill_cached_kernel(const chill_cached_args* a);
 
-/* As chill_read_device_status, chill_launch_count and chill_last_cuda_error, for this library. */
+/* As chill_read_device_status (0: no kernel of this library gave up a wait since the last look; a call whose kernel did has incomplete results), chill_launch_count and chill_last_cuda_error, for this library. */
 int chill_cache_read_device_status(void);
 unsigned long long chill_cache_launch_count(void);
 const char* chill_cache_last_cuda_error(void);
