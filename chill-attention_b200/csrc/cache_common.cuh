@@ -490,15 +490,15 @@ __global__ void __launch_bounds__(kJoinThreads, QUADS == 1 ? 4 : 2) join_few_ker
       float top = m;
 #pragma unroll
       for (int u = 0; u < 8; ++u) top = fmaxf(top, ml[u].x);
-      if (top == -CUDART_INF_F) continue;
-      const float a = exp2f(m - top);
+      const float safe = top == -CUDART_INF_F ? 0.f : top;  // nothing was seen, or nothing but NaN: the sums know
+      const float a = exp2f(m - safe);
       m = top;
       l *= a;
 #pragma unroll
       for (int v = 0; v < QUADS; ++v) o[v].x *= a, o[v].y *= a, o[v].z *= a, o[v].w *= a;
 #pragma unroll
       for (int u = 0; u < 8; ++u) {
-        const float w = exp2f(ml[u].x - top);
+        const float w = exp2f(ml[u].x - safe);
         l = fmaf(w, ml[u].y, l);
 #pragma unroll
         for (int v = 0; v < QUADS; ++v) {
@@ -518,16 +518,15 @@ __global__ void __launch_bounds__(kJoinThreads, QUADS == 1 ? 4 : 2) join_few_ker
       l = 0.f;
 #pragma unroll
       for (int w = 0; w < 8; ++w) m = fmaxf(m, stat[w].x);
-      if (m != -CUDART_INF_F) {
+      const float safe = m == -CUDART_INF_F ? 0.f : m;
 #pragma unroll
-        for (int w = 0; w < 8; ++w) {
-          const float a = exp2f(stat[w].x - m);
-          l = fmaf(a, stat[w].y, l);
+      for (int w = 0; w < 8; ++w) {
+        const float a = exp2f(stat[w].x - safe);
+        l = fmaf(a, stat[w].y, l);
 #pragma unroll
-          for (int v = 0; v < QUADS; ++v) {
-            const float4 y = sums[w][lane + 32 * v];
-            o[v].x = fmaf(a, y.x, o[v].x); o[v].y = fmaf(a, y.y, o[v].y); o[v].z = fmaf(a, y.z, o[v].z); o[v].w = fmaf(a, y.w, o[v].w);
-          }
+        for (int v = 0; v < QUADS; ++v) {
+          const float4 y = sums[w][lane + 32 * v];
+          o[v].x = fmaf(a, y.x, o[v].x); o[v].y = fmaf(a, y.y, o[v].y); o[v].z = fmaf(a, y.z, o[v].z); o[v].w = fmaf(a, y.w, o[v].w);
         }
       }
     }

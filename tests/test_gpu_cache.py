@@ -1061,3 +1061,19 @@ def test_stored_through_the_dispatcher_and_its_refusals():
         with pytest.raises(RuntimeError, match="invalid argument"):
             reserve(pages, taken)
     assert pages.n_free.item() == 3
+
+
+@pytest.mark.parametrize("dtype,N,G,page", [(torch.bfloat16, 2, 4, 16), (torch.float16, 9, 2, 16), (torch.bfloat16, 70, 2, 16), (torch.float32, 1, 1, 16),
+                                            (torch.float32, 9, 1, 16), (torch.float16, 3, 2, 5)], ids=str)
+@pytest.mark.parametrize("length", [200, 1500, 30000])
+def test_a_query_that_is_not_finite_shows(dtype, N, G, page, length):
+    """Rows that have nothing but NaN for scores, over whole units, a few parts and many of them; the other rows are as without these."""
+    p = Problem(dtype, 2 * G, 2, 64, [length, 40], [N, N], N, page, tree=N > 3, seed=N)
+    (want, want_lse), scale = attend(p, masks()["causal"])
+    was = p.q[0, 1, N - 1, 5].clone()
+    p.q[0, 1, N - 1, 5] = float("nan")
+    (o, lse), _ = attend(p, masks()["causal"])
+    assert torch.isnan(o[0, 1, N - 1]).all() and torch.isnan(lse[0, 1, N - 1])
+    p.q[0, 1, N - 1, 5] = was
+    o[0, 1, N - 1], lse[0, 1, N - 1] = want[0, 1, N - 1], want_lse[0, 1, N - 1]
+    check_attention(o, lse, p, masks()["causal"], scale, dtype != torch.float32)
