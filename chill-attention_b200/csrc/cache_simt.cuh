@@ -397,9 +397,11 @@ __global__ void __launch_bounds__(WARPS * 32, 16 / WARPS) cached_simt_few_kernel
         my_l *= a;
 #pragma unroll
         for (int i = 0; i < kOwn; ++i) {
+          const int s = first + i;
+          const bool is = ((there >> s) & (seen >> ((s0 + s) * kKeys + group)) & 1u) != 0;
           const float w = tc::ex2(x[i] - safe);
           my_l += w;
-          if (sub % kSame == 0) reinterpret_cast<float*>(weights[warp][group])[sub * kVals / kLanes + i] = w;
+          if (sub % kSame == 0) reinterpret_cast<float*>(weights[warp][group])[sub * kVals / kLanes + i] = is ? w : -1.f;
         }
         if (sub % kRowLanes == 0) alpha[warp][group][my_r] = a;
         const bool moved = __any_sync(0xffffffffu, a != 1.f);
@@ -417,7 +419,7 @@ __global__ void __launch_bounds__(WARPS * 32, 16 / WARPS) cached_simt_few_kernel
 #pragma unroll
             for (int u = 0; u < 4; ++u) {
               const float w = u == 0 ? w4.x : (u == 1 ? w4.y : (u == 2 ? w4.z : w4.w));
-              if (w != 0.f) {  // a hidden key may hold anything
+              if (!(w < 0.f)) {  // a hidden key may hold anything; what a visible one holds counts whatever its weight
 #pragma unroll
                 for (int v = 0; v < kVecs; ++v) {
                   o[r][v].x = fmaf(w, vx[s4 + u][v].x, o[r][v].x); o[r][v].y = fmaf(w, vx[s4 + u][v].y, o[r][v].y);

@@ -1077,3 +1077,21 @@ def test_a_query_that_is_not_finite_shows(dtype, N, G, page, length):
     p.q[0, 1, N - 1, 5] = was
     o[0, 1, N - 1], lse[0, 1, N - 1] = want[0, 1, N - 1], want_lse[0, 1, N - 1]
     check_attention(o, lse, p, masks()["causal"], scale, dtype != torch.float32)
+
+
+@pytest.mark.parametrize("room", list(ROOMS))
+@pytest.mark.parametrize("dtype,N,G,page", [(torch.float32, 1, 1, 16), (torch.float32, 2, 2, 16), (torch.float32, 9, 1, 16), (torch.float16, 2, 1, 5),
+                                            (torch.bfloat16, 2, 4, 16), (torch.bfloat16, 70, 2, 16)], ids=str)
+def test_a_value_that_is_not_finite_shows_whatever_its_weight(dtype, N, G, page, room):
+    """A visible key far below the others (its weight is 0 in 32 bits) or at -inf: 0 times what it holds is NaN, in that channel alone."""
+    for k in (-1000.0, float("-inf")):
+        p = Problem(dtype, 2 * G, 2, 64, [200, 40], [N, N], N, page, tree=N > 2, seed=N, room=ROOMS[room])
+        p.q[..., 0] = p.q[..., 0].abs() + 1.0
+        where, row = int(p.table[0, 70 // page]), 70 % page
+        p.k_cache[where, 0, row] = 0
+        p.k_cache[where, 0, row, 0] = k
+        p.v_cache[where, 0, row, 3] = float("nan")
+        (o, lse), _ = attend(p, masks()["causal"])
+        assert torch.isnan(o[0, :G, :, 3]).all() and torch.isfinite(lse).all()
+        o[0, :G, :, 3] = 0
+        assert torch.isfinite(o).all()
