@@ -105,7 +105,8 @@ def _check_ints(like, **named):
 
 def _check_sizes(**named):
     for name, t in named.items():
-        assert max(t.shape, default=0) < 2 ** 31, f"the sizes of {name} must fit 32 bits"
+        for size in t.shape:
+            assert size < 2 ** 31, f"the sizes of {name} must fit 32 bits"
 
 
 def _check_table(table):

@@ -1095,3 +1095,37 @@ def test_a_value_that_is_not_finite_shows_whatever_its_weight(dtype, N, G, page,
         assert torch.isnan(o[0, :G, :, 3]).all() and torch.isfinite(lse).all()
         o[0, :G, :, 3] = 0
         assert torch.isfinite(o).all()
+
+
+@pytest.mark.parametrize("dynamic", [None, True])
+def test_a_compiled_step_with_other_sizes(dynamic):
+    """Graphs of one traced step for batches and steps of other sizes."""
+    import chill_attention as ca
+
+    mask = masks()["window"]
+
+    def step(pages, kc, vc, lens, new, q, k, v, parents, path, accepted):
+        s = ca.chill_pages_reserve(pages, lens, new, q.shape[2], 16, parents)
+        ca.chill_cache_append(kc, vc, k, v, s.slots)
+        o, lse = ca.chill_attention_cached(q, kc, vc, pages.table, s, mask, return_lse=True)
+        lens = ca.chill_cache_commit(kc, vc, pages.table, s, path, accepted)
+        ca.chill_pages_trim(pages, lens, 16)
+        return o, lse, lens
+
+    torch._dynamo.reset()
+    compiled = torch.compile(step, fullgraph=True, dynamic=dynamic)
+    for lens, N in (([250, 90], 6), ([30, 200], 9), ([77, 5, 300], 4), ([1] * 5, 33)):
+        B = len(lens)
+        p = Problem(torch.bfloat16, 8, 2, 64, lens, [N] * B, N, 16, tree=True, seed=N, room=600)
+        k, v = (torch.randn(B, 2, N, 64, device="cuda", dtype=torch.bfloat16) for _ in range(2))
+
+        def state():
+            free = ints(p.spare_pages + [-1] * (p.k_cache.shape[0] - len(p.spare_pages)))
+            pages = ca.ChillPages(p.table.cuda(), ints(p.held), free, ints([len(p.spare_pages)]), ints([0]))
+            return pages, p.k_cache.nan_to_num(0.25).cuda(), p.v_cache.nan_to_num(0.25).cuda(), ints(p.lens), ints(p.new)
+
+        a, b = state(), state()
+        args = p.q.cuda(), k, v, ints(p.parents), ints([[0, 2, 3]] * B), ints([2] * B)
+        want, got = step(*a, *args), compiled(*b, *args)
+        assert all(torch.equal(x, y) for x, y in zip([*want, *a[0], a[1], a[2]], [*got, *b[0], b[1], b[2]]))
+    torch._dynamo.reset()
