@@ -81,11 +81,6 @@ __device__ __forceinline__ uint64_t ex2_fma(uint64_t x2) {
   tc::upk2(n2, na, nb);
   return tc::pk2u(__float_as_uint(a) + (__float_as_uint(na) << 23), __float_as_uint(b) + (__float_as_uint(nb) << 23));
 }
-__device__ __forceinline__ float fmax3_nan(float a, float b, float c) {  // NaN if any of them is
-  float d;
-  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
-  return d;
-}
 // Of every sixteen pairs of weights, half as many are worked out so.  The two groups' softmax warps on a scheduler ask its MUFU for 1024
 // of the 2100 clocks of a step, mostly at the same time: 1024 new tokens for each of 4 requests, 507 us with none, 480 with an eighth of
 // the pairs, 467 with a quarter, 512 with half of them.
@@ -328,12 +323,12 @@ cached_tiles_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_consta
         float mx0 = -CUDART_INF_F, mx1 = mx0, mx2 = mx0, mx3 = mx0;
 #pragma unroll
         for (int e = 0; e < kKeyTile; e += 8) {
-          mx0 = fmax3_nan(mx0, __uint_as_float(x[e]), __uint_as_float(x[e + 1]));
-          mx1 = fmax3_nan(mx1, __uint_as_float(x[e + 2]), __uint_as_float(x[e + 3]));
-          mx2 = fmax3_nan(mx2, __uint_as_float(x[e + 4]), __uint_as_float(x[e + 5]));
-          mx3 = fmax3_nan(mx3, __uint_as_float(x[e + 6]), __uint_as_float(x[e + 7]));
+          mx0 = tc::fmax3_nan(mx0, __uint_as_float(x[e]), __uint_as_float(x[e + 1]));
+          mx1 = tc::fmax3_nan(mx1, __uint_as_float(x[e + 2]), __uint_as_float(x[e + 3]));
+          mx2 = tc::fmax3_nan(mx2, __uint_as_float(x[e + 4]), __uint_as_float(x[e + 5]));
+          mx3 = tc::fmax3_nan(mx3, __uint_as_float(x[e + 6]), __uint_as_float(x[e + 7]));
         }
-        const float top = fmax3_nan(fmax3_nan(mx0, mx1, mx2), mx3, mx3);
+        const float top = tc::fmax3_nan(tc::fmax3_nan(mx0, mx1, mx2), mx3, mx3);
         const float m_cand = fmaxf(m_used, top * c);  // passes NaN by
         if (j == 0) {
           m_used = m_cand;

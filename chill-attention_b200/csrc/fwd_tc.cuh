@@ -158,14 +158,23 @@ __device__ __forceinline__ void softmax_tile(uint32_t tS, uint32_t tO, uint32_t 
       }
     }
   }
+  // Share of the pairs whose 2^x is the polynomial on the FMA pipe instead of MUFU.  Head dim 256 runs one CTA per
+  // SM, i.e. one softmax warp per scheduler with nothing to hide its MUFU latency behind: a quarter there measured
+  // 1.155 vs 1.211 ms (causal L = 4096); every share made head dims 64 / 128 slower (see tc_common.cuh).
+  constexpr int kPolyNum = (D == 256 && CHILL_FWD_POLY_NUM == 0) ? 1 : CHILL_FWD_POLY_NUM;
+  constexpr int kPolyDen = (D == 256 && CHILL_FWD_POLY_NUM == 0) ? 4 : CHILL_FWD_POLY_DEN;
   float mx0 = -CUDART_INF_F, mx1 = -CUDART_INF_F, mx2 = -CUDART_INF_F, mx3 = -CUDART_INF_F;
+  auto max3 = [](float a, float b, float x) { return kPolyNum > 0 ? fmax3_nan(a, b, x) : fmax3(a, b, x); };
 #pragma unroll
   for (int i = 0; i < KT; i += 8) {
-    mx0 = fmax3(mx0, __uint_as_float(sreg[i]), __uint_as_float(sreg[i + 1]));
-    mx1 = fmax3(mx1, __uint_as_float(sreg[i + 2]), __uint_as_float(sreg[i + 3]));
-    mx2 = fmax3(mx2, __uint_as_float(sreg[i + 4]), __uint_as_float(sreg[i + 5]));
-    mx3 = fmax3(mx3, __uint_as_float(sreg[i + 6]), __uint_as_float(sreg[i + 7]));
+    mx0 = max3(mx0, __uint_as_float(sreg[i]), __uint_as_float(sreg[i + 1]));
+    mx1 = max3(mx1, __uint_as_float(sreg[i + 2]), __uint_as_float(sreg[i + 3]));
+    mx2 = max3(mx2, __uint_as_float(sreg[i + 4]), __uint_as_float(sreg[i + 5]));
+    mx3 = max3(mx3, __uint_as_float(sreg[i + 6]), __uint_as_float(sreg[i + 7]));
   }
+  // The polynomial knows neither NaN nor infinity (both would become 2^-126): a score of NaN or +inf goes into the sum here, as 0 times
+  // the row's maximum
+  if (kPolyNum > 0) l = fmaf(fmax3_nan(fmax3_nan(mx0, mx1, mx2), mx3, -3.4028235e38f), 0.f, l);
   const float m_tile = fmaxf(fmaxf(mx0, mx1), fmaxf(mx2, mx3)) * c;  // c > 0 (checked by the host)
   const float m_cand = fmaxf(m_used, m_tile);
   if (first) {
@@ -195,11 +204,6 @@ __device__ __forceinline__ void softmax_tile(uint32_t tS, uint32_t tO, uint32_t 
   const float m_safe = (m_used == -CUDART_INF_F) ? 0.f : m_used;
   const uint64_t c2 = pk2(c, c), nm2 = pk2(-m_safe, -m_safe);
   uint64_t l0 = 0ull, l1 = 0ull;  // two packed partial row sums (+0.0f, +0.0f)
-  // Share of the pairs whose 2^x is the polynomial on the FMA pipe instead of MUFU.  Head dim 256 runs one CTA per
-  // SM, i.e. one softmax warp per scheduler with nothing to hide its MUFU latency behind: a quarter there measured
-  // 1.155 vs 1.211 ms (causal L = 4096); every share made head dims 64 / 128 slower (see tc_common.cuh).
-  constexpr int kPolyNum = (D == 256 && CHILL_FWD_POLY_NUM == 0) ? 1 : CHILL_FWD_POLY_NUM;
-  constexpr int kPolyDen = (D == 256 && CHILL_FWD_POLY_NUM == 0) ? 4 : CHILL_FWD_POLY_DEN;
 #pragma unroll
   for (int i = 0; i < KT / 2; i += 2) {
     // two pairs per step

@@ -309,6 +309,11 @@ __device__ __forceinline__ float fmax3(float a, float b, float c) {
   asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
   return d;
 }
+__device__ __forceinline__ float fmax3_nan(float a, float b, float c) {  // NaN if any of them is
+  float d;
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
 
 
 // 2^x for a packed pair on the FMA pipe instead of the MUFU unit (which delivers only 16 ex2 per
@@ -316,7 +321,8 @@ __device__ __forceinline__ float fmax3(float a, float b, float c) {
 // x = n + f with n = round(x) via the 1.5 * 2^23 trick, f in [-0.5, 0.5]; 2^f by a degree-3
 // minimax polynomial (max relative error 7.5e-5, below fp16/bf16 resolution of the P operand it
 // feeds); the exponent is patched in with one integer multiply-add per element.  x is clamped to
-// [-126, ...) so that -inf (masked) and very negative arguments give ~0 instead of garbage.
+// [-126, ...) so that -inf (masked) and very negative arguments give ~0 instead of garbage; NaN becomes ~0 too, so whoever calls
+// this looks at the row's maximum.
 __device__ __forceinline__ uint64_t ex2_poly2(uint64_t x2) {
   float x0, x1;
   upk2(x2, x0, x1);

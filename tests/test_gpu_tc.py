@@ -485,3 +485,28 @@ def test_forward_and_backward_replay_from_a_cuda_graph():
     assert torch.equal(outs[2], eager[2]) and torch.equal(outs[3], eager[3])  # dK, dV are deterministic
     rel = ((outs[1].double() - eager[1].double()).norm() / eager[1].double().norm()).item()
     assert rel <= 1e-2  # dQ: fp32 reductions in an order that is not fixed
+
+
+@pytest.mark.parametrize("value", [float("nan"), float("inf")], ids=str)
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16], ids=["fp16", "bf16"])
+@pytest.mark.parametrize("D", [64, 128, 256])
+@pytest.mark.parametrize("name", ["causal", "window"])
+def test_a_score_that_is_not_finite_shows(name, D, dtype, value):
+    """One key, not finite in K alone, at each of 64 places: every row that sees it has nothing finite in O and LSE, every row before it
+    is what it is without the key, both within the operator's bar of the exact result.  (A part of the exponentials of head dim 256 is a polynomial that knows neither NaN nor infinity.)"""
+    import chill_attention as ca
+
+    L, reach = 512, 150
+    mask = ca.CausalChillMask() if name == "causal" else ca.SlidingWindowChillMask(reach, 0)
+    q, k, v, _ = make_inputs(64, 1, 1, L, D, dtype, seed=D)
+    q[..., 0] = q[..., 0].abs() + 0.5
+    q, k, v = q.cuda(), k.cuda(), v.cuda()
+    want, want_lse = ca.chill_attention(q, k, v, mask=mask, return_lse=True)
+    for j in range(64):
+        k[j, 0, 128 + j, 0] = value
+    o, lse = ca.chill_attention(q, k, v, mask=mask, return_lse=True)
+    for j in range(64):
+        end = L if name == "causal" else 128 + j + reach + 1
+        assert not torch.isfinite(o[j, 0, 128 + j:end]).any() and not torch.isfinite(lse[j, 0, 128 + j:end]).any()
+        assert (o[j, 0, :128 + j].float() - want[j, 0, :128 + j].float()).abs().max().item() <= 2 * O_ATOL[dtype]
+        assert (lse[j, 0, :128 + j] - want_lse[j, 0, :128 + j]).abs().max().item() <= 2e-3
