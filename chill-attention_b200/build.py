@@ -1,12 +1,14 @@
 """Build the CUDA library for sm_100a with nvcc (no other toolchain needed).
 
-    python chill-attention_b200/build.py            # -> chill_attention/_lib/libchill_b200.so, libchill_cache_b200.so, _chill_torch.so
+    python chill-attention_b200/build.py            # -> chill_attention/_lib/libchill_b200.so, libchill_cache_b200.so,
+                                                    #    libchill_decode_b200.so, _chill_torch.so
 
 Each mask functor's tensor-core kernels and its CUDA-core kernels are translation units of their own
 (csrc/tc_inst.cu, csrc/simt_inst.cu with -DCHILL_INST_MASK=<functor>), compiled in parallel.
 ``build_library`` is also what ``chill_attention.custom`` calls to produce a private
 library for a user-defined mask functor.  The objects of the built-in functors, nine tenths of a build, are kept beside the
-library and linked into such private libraries as they are.  The paged cache is a library of its own (csrc/cache_*.cu).
+library and linked into such private libraries as they are.  The paged cache is a library of its own (csrc/cache_*.cu), and so are
+rotary positions, the selection of a beam search and shared pages (csrc/decode_*.cu), which no mask has a part in.
 """
 from __future__ import annotations
 
@@ -43,7 +45,8 @@ def _sources_digest(extra=(), cache=False):
     """Of the kernel library's sources, or of those of the paged cache's library (csrc/cache_* and what they include)."""
     h = hashlib.sha256()
     headers = ("abi_common.cuh", "generic.cuh", "masks.cuh", "tc_common.cuh", "tc_launch.h")
-    names = sorted(n for n in os.listdir(CSRC) if not n.startswith("torch_") and (n.startswith("cache_") or n in headers if cache else not n.startswith("cache_")))
+    others = ("torch_", "decode_")
+    names = sorted(n for n in os.listdir(CSRC) if not n.startswith(others) and (n.startswith("cache_") or n in headers if cache else not n.startswith("cache_")))
     names += [os.path.join(INCLUDE, n) for n in (("chill_b200.h", "chill_cache.h") if cache else ("chill_b200.h",))]
     for name in names:
         path = name if os.path.isabs(name) else os.path.join(CSRC, name)
@@ -149,17 +152,46 @@ def build_cache_library(out_path=None, custom_header=None, custom_functor=None, 
     return out_path
 
 
+def build_decode_library(verbose=False, force=False):
+    """The library of csrc/decode_*.cu.  Returns its path; skips work when sources are unchanged."""
+    out_path = os.path.join(LIB_DIR, "libchill_decode_b200.so")
+    os.makedirs(LIB_DIR, exist_ok=True)
+    defines = os.environ.get("CHILL_B200_NVCC_FLAGS", "").split()
+    h = hashlib.sha256(" ".join(defines).encode())
+    names = sorted(n for n in os.listdir(CSRC) if n.startswith("decode_"))
+    for path in [os.path.join(CSRC, n) for n in names] + [os.path.join(INCLUDE, n) for n in ("chill_b200.h", "chill_decode.h")]:
+        h.update(os.path.basename(path).encode())
+        with open(path, "rb") as f:
+            h.update(f.read())
+    stamp = out_path + ".stamp"
+    if not force and os.path.exists(out_path) and os.path.exists(stamp) and open(stamp).read() == h.hexdigest():
+        return out_path
+    obj_dir = os.path.join(LIB_DIR, "obj_" + os.path.basename(out_path))
+    os.makedirs(obj_dir, exist_ok=True)
+    nvcc = [_nvcc()] + (["-Xptxas", "-v"] if verbose else []) + NVCC_FLAGS + defines
+    units = [(os.path.join(CSRC, n), os.path.join(obj_dir, n + ".o")) for n in names if n.endswith(".cu")]
+    with cf.ThreadPoolExecutor(max_workers=8) as ex:
+        outs = list(ex.map(lambda u: _run(nvcc + ["-c", u[0], "-o", u[1]]), units))
+    if verbose:
+        print("\n".join(outs))
+    _run([_nvcc(), "-shared", "-gencode", "arch=compute_100a,code=sm_100a", "-o", out_path] + [obj for _, obj in units])
+    with open(stamp, "w") as f:
+        f.write(h.hexdigest())
+    shutil.rmtree(obj_dir, ignore_errors=True)
+    return out_path
+
+
 def build_extension(force=False):
-    """Compile the native eager-mode call path (csrc/torch_ext.cpp, csrc/torch_cache.cpp) against the installed torch; returns its path."""
+    """Compile the native eager-mode call path (csrc/torch_ext.cpp, torch_cache.cpp, torch_decode.cpp) against the installed torch; returns its path."""
     import sysconfig
 
     import torch
     from torch.utils.cpp_extension import include_paths, library_paths
 
     out = os.path.join(LIB_DIR, "_chill_torch.so")
-    sources = [os.path.join(CSRC, name) for name in ("torch_ext.cpp", "torch_cache.cpp")]
+    sources = [os.path.join(CSRC, name) for name in ("torch_ext.cpp", "torch_cache.cpp", "torch_decode.cpp")]
     h = hashlib.sha256((torch.__version__ + sys.version).encode())
-    for path in sources + [os.path.join(CSRC, "torch_ext.h")] + [os.path.join(INCLUDE, n) for n in ("chill_b200.h", "chill_cache.h")]:
+    for path in sources + [os.path.join(CSRC, n) for n in ("torch_ext.h", "torch_call.h")] + [os.path.join(INCLUDE, n) for n in ("chill_b200.h", "chill_cache.h", "chill_decode.h")]:
         with open(path, "rb") as f:
             h.update(f.read())
     stamp = out + ".stamp"
@@ -180,4 +212,5 @@ if __name__ == "__main__":
     path = build_library(verbose="-v" in sys.argv, force="-f" in sys.argv)
     print(path)
     print(build_cache_library(verbose="-v" in sys.argv, force="-f" in sys.argv))
+    print(build_decode_library(verbose="-v" in sys.argv, force="-f" in sys.argv))
     print(build_extension(force="-f" in sys.argv))

@@ -46,7 +46,7 @@ class ChillPages(typing.NamedTuple):
     """Which pages a batch of requests holds and which are free; int32 tensors on the GPU, changed in place.
 
     table: [batch, blocks], page of every block of page_size tokens (-1: none); held: [batch], blocks with a page;
-    free: [num_pages], a stack, n_free: [1], its height; missing: [1], pages that the last reservation wanted and did not get."""
+    free: [num_pages], a stack, n_free: [1], its height; missing: [1], pages that the last reservation or fork wanted and did not get."""
 
     table: torch.Tensor
     held: torch.Tensor
@@ -61,6 +61,15 @@ class ChillPages(typing.NamedTuple):
         ints = {"dtype": torch.int32, "device": device}
         return cls(torch.full((batch, -(-max_len // page_size)), -1, **ints), torch.zeros(batch, **ints),
                    torch.arange(num_pages - 1, -1, -1, **ints), torch.full((1,), num_pages, **ints), torch.zeros(1, **ints))
+
+
+class ChillCopies(typing.NamedTuple):
+    """Pages to be copied, int32 tensors on the GPU: the first rows[i] rows of page source[i] go to page target[i], for i < count ([1])."""
+
+    source: torch.Tensor
+    target: torch.Tensor
+    rows: torch.Tensor
+    count: torch.Tensor
 
 
 class ChillStep(typing.NamedTuple):
@@ -255,6 +264,93 @@ def _(q, k_cache, v_cache, table, lens, new_lens, positions, ancestors, mask_nam
     return torch.empty_like(q, memory_format=torch.contiguous_format), q.new_empty(q.shape[:3], dtype=torch.float32)
 
 
+# The operators of pages that several requests share (libchill_decode_b200.so)
+def _decode():
+    from . import rotary
+
+    return rotary._NATIVE or rotary._native()
+
+
+def _places(pages):
+    return pages.table, pages.held, pages.free, pages.n_free
+
+
+def _check_fork(pages, shared, lens, parents, page_size):
+    _check_pages(pages, lens, page_size)
+    B = pages.table.shape[0]
+    assert B <= 8192, "a fork takes at most 8192 requests"
+    _check_ints(pages.table, missing=(pages.missing, (1,)), shared=(shared, pages.free.shape), parents=(parents, (B,)))
+
+
+def _check_compact(pages, page_size, shared):
+    _check_pages(pages, pages.held, page_size)
+    if shared is not None:
+        _check_ints(pages.table, shared=(shared, pages.free.shape))
+
+
+def _check_copy(k_cache, v_cache, copies):
+    _check_sizes(k_cache=k_cache)
+    assert k_cache.is_cuda and k_cache.device == v_cache.device, "the caches must be CUDA tensors on one device"
+    assert k_cache.ndim in (4, 5) and k_cache.shape == v_cache.shape and k_cache.numel() > 0, \
+        "k_cache and v_cache must have one shape [num_pages, kv_heads, page_size, head_dim], or [layers, ...]"
+    assert k_cache.dtype == v_cache.dtype and k_cache.dtype in _DTYPES
+    source, target, rows, count = copies
+    assert isinstance(source, torch.Tensor) and source.ndim == 1 and source.numel() > 0
+    _check_sizes(source=source)
+    _check_ints(k_cache, source=(source, source.shape), target=(target, source.shape), rows=(rows, source.shape), count=(count, (1,)))
+    _check_grad(k_cache, v_cache)
+
+
+@torch.library.custom_op("chill_attention::pages_trim_shared", mutates_args=("table", "held", "free", "n_free", "shared"), device_types=("cuda",))
+def _trim_shared_op(table: torch.Tensor, held: torch.Tensor, free: torch.Tensor, n_free: torch.Tensor, shared: torch.Tensor, lens: torch.Tensor,
+                    page_size: int) -> None:
+    _check_pages(ChillPages(table, held, free, n_free, n_free), lens, page_size)
+    _check_ints(table, shared=(shared, free.shape))
+    _eager.extension().pages_trim_shared(_decode(), table, held, free, n_free, shared, lens, page_size)
+
+
+@_trim_shared_op.register_fake
+def _(table, held, free, n_free, shared, lens, page_size):
+    return None
+
+
+@torch.library.custom_op("chill_attention::pages_fork", mutates_args=("table", "held", "free", "n_free", "missing", "shared"), device_types=("cuda",))
+def _fork_op(table: torch.Tensor, held: torch.Tensor, free: torch.Tensor, n_free: torch.Tensor, missing: torch.Tensor, shared: torch.Tensor, lens: torch.Tensor,
+             parents: torch.Tensor, page_size: int) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor]:
+    _check_fork(ChillPages(table, held, free, n_free, missing), shared, lens, parents, page_size)
+    return _eager.extension().pages_fork(_decode(), table, held, free, n_free, missing, shared, lens, parents, page_size)
+
+
+@_fork_op.register_fake
+def _(table, held, free, n_free, missing, shared, lens, parents, page_size):
+    B = table.shape[0]
+    return (*(table.new_empty(B) for _ in range(4)), table.new_empty(1))
+
+
+@torch.library.custom_op("chill_attention::pages_compact", mutates_args=("table", "free", "n_free", "shared"), device_types=("cuda",))
+def _compact_op(table: torch.Tensor, held: torch.Tensor, free: torch.Tensor, n_free: torch.Tensor, shared: typing.Optional[torch.Tensor],
+                page_size: int) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor]:
+    _check_compact(ChillPages(table, held, free, n_free, n_free), page_size, shared)
+    return _eager.extension().pages_compact(_decode(), table, held, free, n_free, shared, page_size)
+
+
+@_compact_op.register_fake
+def _(table, held, free, n_free, shared, page_size):
+    n = max(free.shape[0] // 2, 1)
+    return (*(table.new_empty(n) for _ in range(3)), table.new_empty(1))
+
+
+@torch.library.custom_op("chill_attention::cache_copy", mutates_args=("k_cache", "v_cache"), device_types=("cuda",))
+def _copy_op(k_cache: torch.Tensor, v_cache: torch.Tensor, source: torch.Tensor, target: torch.Tensor, rows: torch.Tensor, count: torch.Tensor) -> None:
+    _check_copy(k_cache, v_cache, (source, target, rows, count))
+    _eager.extension().cache_copy(_decode(), k_cache, v_cache, source, target, rows, count)
+
+
+@_copy_op.register_fake
+def _(k_cache, v_cache, source, target, rows, count):
+    return None
+
+
 # ------------------------------------------------------------------------------------------------------------ public calls
 def _check_reserve(pages, new_lens, max_new, parents, stored):
     B = pages.table.shape[0]
@@ -299,14 +395,81 @@ def chill_pages_reserve(pages: ChillPages, lens: torch.Tensor, new_lens: torch.T
     return ChillStep(lens, new_lens, slots, positions, ancestors if parents is not None else None)
 
 
-def chill_pages_trim(pages: ChillPages, lens: torch.Tensor, page_size: int) -> None:
+def chill_pages_trim(pages: ChillPages, lens: torch.Tensor, page_size: int, shared: torch.Tensor | None = None) -> None:
     """Gives the pages behind ``lens[b]`` tokens of every request back (``lens[b] = 0``: all of them), in place.
 
-    The exact inverse of a reservation: what it gives back is what the same reservation takes again, in the same order."""
+    The exact inverse of a reservation: what it gives back is what the same reservation takes again, in the same order.
+
+    ``shared``, int32 [num_pages], changed in place: how many requests beyond one hold a page (``chill_pages_fork``).  Given that, a page goes back when the last of its
+    holders lets go of it.  Without it pages must have one holder each.  A request that is cut back inside a page that others hold, and grows again, would write into it:
+    ``chill_pages_fork`` with its own number as parent gives it a page of its own first."""
+    if shared is not None:
+        if _direct() and _eager.extension().pages_trim_shared(_decode(), *_places(pages), shared, lens, page_size):
+            return
+        _check_pages(pages, lens, page_size)
+        _check_ints(pages.table, shared=(shared, pages.free.shape))
+        _trim_shared_op(*_places(pages), shared, lens, page_size)
+        return
     if _direct() and _eager.extension().pages_trim(_NATIVE.get(None) or _native(), pages.table, pages.held, pages.free, pages.n_free, lens, page_size):
         return
     _check_pages(pages, lens, page_size)
     _trim_op(pages.table, pages.held, pages.free, pages.n_free, lens, page_size)
+
+
+def chill_pages_fork(pages: ChillPages, shared: torch.Tensor, lens: torch.Tensor, parents: torch.Tensor, page_size: int) -> tuple[torch.Tensor, ChillCopies]:
+    """Request b goes on from where request ``parents[b]`` is: it takes over that one's ``lens[parents[b]]`` tokens, all requests at once and in place.
+
+    Whole pages are shared between the children of a request.  A page that is only begun is written to next, so it has one holder: the first child keeps it (if no other
+    request holds it), every other one gets a page from the stack, into which ``chill_cache_copy`` has to copy what is written.  Pages that nobody holds any more, those
+    of requests without children and those behind the tokens among them, go back to the stack, in the order of the requests and blocks that held them first, the first on top.
+
+    Args:
+        pages: changed in place.
+        shared: int32 [num_pages], changed in place: how many requests beyond one hold a page; zeros to begin with (``chill_pages_reserve`` hands out pages with one holder).
+        lens: int32 [batch], tokens of each request.
+        parents: int32 [batch]; itself to stay as it is, anything outside [0, batch): the request is empty afterwards.
+
+    Returns: (tokens of each request now, int32 [batch]; the copies to be made in every layer's caches before anything else is written there).  Where the stack runs
+    out of pages (``pages.missing`` says of how many) a request keeps whole pages only, and its tokens say so.  At most 8192 requests.
+    """
+    if _direct():
+        out = _eager.extension().pages_fork(_decode(), *pages, shared, lens, parents, page_size)
+        if out is not None:
+            return out[0], ChillCopies(*out[1:])
+    _check_fork(pages, shared, lens, parents, page_size)
+    out = _fork_op(*pages, shared, lens, parents, page_size)
+    return out[0], ChillCopies(*out[1:])
+
+
+def chill_pages_compact(pages: ChillPages, page_size: int, shared: torch.Tensor | None = None) -> ChillCopies:
+    """Moves the pages in use to the bottom of the pool, in place: with U of them, the highest one goes to the lowest free page below U, and so on; afterwards pages
+    0 ... U - 1 are in use and the stack has the lowest free page on top.
+
+    Every page that is not on the stack counts as used, whether a table names it or not; tables and ``shared`` follow.
+
+    Returns: the copies to be made in every layer's caches (whole pages; sources and targets have none in common) before anything else is read or written there.
+    """
+    if _direct():
+        out = _eager.extension().pages_compact(_decode(), *_places(pages), shared, page_size)
+        if out is not None:
+            return ChillCopies(*out)
+    _check_compact(pages, page_size, shared)
+    return ChillCopies(*_compact_op(*_places(pages), shared, page_size))
+
+
+def chill_cache_copy(k_cache: torch.Tensor, v_cache: torch.Tensor, copies: ChillCopies) -> None:
+    """Copies pages, in place: the first ``rows[i]`` rows of page ``source[i]`` to page ``target[i]``, for i < count.
+
+    Args:
+        k_cache, v_cache: [num_pages, kv_heads, page_size, head_dim], or those of all layers [layers, num_pages, ...]; any strides.  They may be the same tensor, but not
+            overlap otherwise.
+        copies: of ``chill_pages_fork`` or ``chill_pages_compact``, or the caller's own; orders with a page outside the cache are left out, a target must not be source or
+            target of another order.
+    """
+    if _direct() and _eager.extension().cache_copy(_decode(), k_cache, v_cache, *copies):
+        return
+    _check_copy(k_cache, v_cache, copies)
+    _copy_op(k_cache, v_cache, *copies)
 
 
 def chill_cache_append(k_cache: torch.Tensor, v_cache: torch.Tensor, k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor) -> None:

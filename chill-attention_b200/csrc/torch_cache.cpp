@@ -1,11 +1,7 @@
 // Eager-mode call path of the paged-cache operators (chill_attention/cache.py): argument checks, outputs and workspace from torch's
 // allocator, C-ABI calls.  Part of the native module that torch_ext.cpp defines.  A check that fails returns None; the caller
 // repeats the checks in Python for the message.
-#include <ATen/core/grad_mode.h>
-#include <ATen/cuda/EmptyTensor.h>
-#include <c10/core/AutogradState.h>
 #include <c10/cuda/CUDAGuard.h>
-#include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/utils/pybind.h>
 
@@ -15,10 +11,12 @@
 #include <vector>
 
 #include "chill_cache.h"
+#include "torch_call.h"
 #include "torch_ext.h"
 
 namespace py = pybind11;
 using at::Tensor;
+using namespace chill_torch;
 
 namespace {
 
@@ -40,68 +38,9 @@ void check(const CacheLibrary& lib, int status, const char* what) {
   throw_chill_error(msg);
 }
 
-// Without the dispatcher: 0.7 us instead of 1.1, and a call makes up to three.
-Tensor empty(at::IntArrayRef sizes, at::ScalarType type, const Tensor& like) { return at::detail::empty_cuda(sizes, type, like.device(), std::nullopt); }
-
-// A tensor that something looks in on (a subclass with its own dispatch, a transform): the dispatcher ops serve it.
-bool watched(std::initializer_list<const Tensor*> tensors, const std::optional<Tensor>& one_more = std::nullopt, const std::optional<Tensor>& another = std::nullopt) {
-  auto looked_at = [](const Tensor& t) { return t.unsafeGetTensorImpl()->key_set().has_any(c10::python_ks | c10::functorch_transforms_ks); };
-  for (const Tensor* t : tensors)
-    if (looked_at(*t)) return true;
-  return (one_more.has_value() && looked_at(*one_more)) || (another.has_value() && looked_at(*another));
-}
-
-void* current_stream(const Tensor& t) { return (void*)c10::cuda::getCurrentCUDAStream(t.get_device()).stream(); }
-
-void set_strides(int64_t* dst, const Tensor& t) {
-  for (int64_t d = 0; d < t.dim(); ++d) dst[d] = t.stride(d);
-}
-
-int dtype_of(const Tensor& t) {
-  switch (t.scalar_type()) {
-    case at::kFloat: return CHILL_F32;
-    case at::kHalf: return CHILL_F16;
-    case at::kBFloat16: return CHILL_BF16;
-    default: return -1;
-  }
-}
-
-// An int32 tensor of these sizes on the device of `like`, contiguous.
-bool ints(const Tensor& t, std::initializer_list<int64_t> sizes, const Tensor& like) {
-  return t.scalar_type() == at::kInt && t.sizes() == at::IntArrayRef(sizes) && t.is_contiguous() && t.device() == like.device();
-}
-
-// The C ABI takes 32-bit sizes.
-bool fit(const Tensor& t) {
-  for (const int64_t n : t.sizes())
-    if (n > INT32_MAX) return false;
-  return true;
-}
-
-bool table_ok(const Tensor& table) {
-  return fit(table) && table.scalar_type() == at::kInt && table.dim() == 2 && table.size(0) > 0 && table.size(1) > 0 && table.is_cuda() && table.stride(1) == 1 &&
-         (table.size(0) == 1 || table.stride(0) >= table.size(1));
-}
-
 bool pools_ok(const Tensor& k, const Tensor& v) {
   return k.dim() == 4 && fit(k) && k.sizes() == v.sizes() && k.numel() > 0 && k.scalar_type() == v.scalar_type() && dtype_of(k) >= 0 && k.is_cuda() && v.device() == k.device();
 }
-
-// Gradients asked for, or a tangent carried along (forward mode, which no_grad leaves on).
-bool wants_grad(std::initializer_list<const Tensor*> tensors) {
-  const bool backward = at::GradMode::is_enabled(), forward = c10::AutogradState::get_tls_state().get_fw_grad_mode();
-  for (const Tensor* t : tensors)
-    if ((backward && t->requires_grad()) || (forward && t->_fw_grad(/*level=*/0).defined())) return true;
-  return false;
-}
-
-// Changed in place: autograd looks at a tensor's version where it saved one.  (Inference tensors have none.)
-void changed(std::initializer_list<const Tensor*> tensors) {
-  for (const Tensor* t : tensors)
-    if (!t->is_inference()) t->unsafeGetTensorImpl()->bump_version();
-}
-
-const int32_t* optional_ints(const std::optional<Tensor>& t) { return t.has_value() ? t->const_data_ptr<int32_t>() : nullptr; }
 
 py::object reserve(const CacheLibrary& lib, const Tensor& table, const Tensor& held, const Tensor& free, const Tensor& n_free, const Tensor& missing,
                    const Tensor& lens, const Tensor& new_lens, int64_t N, int64_t page, const std::optional<Tensor>& parents, const std::optional<Tensor>& stored) {
@@ -224,11 +163,6 @@ py::object attention(const CacheLibrary& lib, int32_t functor_id, const Tensor& 
   check(lib, lib.fwd(&a, current_stream(q)), "chill_cached_fwd");
   if (!return_lse) return py::cast(o);
   return py::make_tuple(o, lse);
-}
-
-template <class F>
-F pointer(uint64_t address) {
-  return reinterpret_cast<F>(static_cast<uintptr_t>(address));
 }
 
 }  // namespace

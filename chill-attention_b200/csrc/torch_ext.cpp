@@ -265,5 +265,6 @@ PYBIND11_MODULE(_chill_torch, m) {
   m.def("set_deterministic", [](bool flag) { g_deterministic = flag; });
   m.def("backward_counts", [] { return std::make_pair(g_bwd_tc.load(), g_bwd_generic.load()); });
   bind_cache(m);
+  bind_decode(m);
   m.attr("abi_version") = CHILL_ABI_VERSION;
 }

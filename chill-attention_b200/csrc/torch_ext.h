@@ -1,4 +1,4 @@
-// What the two halves of the native torch module share (torch_ext.cpp, torch_cache.cpp).
+// What the parts of the native torch module share (torch_ext.cpp, torch_cache.cpp, torch_decode.cpp).
 #pragma once
 #include <torch/csrc/utils/pybind.h>
 
@@ -11,3 +11,4 @@ void set_mask_constants(chill_mask_desc& desc, const pybind11::tuple& mask_args)
 // Throws what Python sees as chill_attention._cabi.ChillLibraryError.
 [[noreturn]] void throw_chill_error(const std::string& message);
 void bind_cache(pybind11::module_& m);
+void bind_decode(pybind11::module_& m);
