@@ -16,8 +16,8 @@ SELECT_MAX = 64
 FORK_MAX = 8192
 
 EXPORTS = (
-    "chill_rotate", "chill_rotate_append", "chill_beam_select", "chill_pages_fork", "chill_pages_trim_shared", "chill_pages_compact",
-    "chill_share_workspace_bytes", "chill_cache_copy", "chill_decode_launch_count", "chill_decode_last_cuda_error", "chill_decode_abi_version",
+    "chill_rotate", "chill_rotate_append", "chill_beam_select", "chill_select_workspace_bytes", "chill_pages_fork", "chill_pages_trim_shared",
+    "chill_pages_compact", "chill_share_workspace_bytes", "chill_cache_copy", "chill_decode_launch_count", "chill_decode_last_cuda_error", "chill_decode_abi_version",
 )
 
 _S5 = C.c_int64 * 5
@@ -35,7 +35,8 @@ class RotateArgs(C.Structure):
 class SelectArgs(C.Structure):
     _fields_ = [(n, C.c_int32) for n in ("G", "K", "M", "dtype")] + \
                [("V", C.c_int64), ("logits", C.c_void_p), ("row_stride", C.c_int64), ("scores", C.c_void_p), ("finished", C.c_void_p),
-                ("end_token", C.c_int64), ("out_scores", C.c_void_p), ("out_rows", C.c_void_p), ("out_tokens", C.c_void_p)]
+                ("end_token", C.c_int64), ("out_scores", C.c_void_p), ("out_rows", C.c_void_p), ("out_tokens", C.c_void_p),
+                ("workspace", C.c_void_p), ("workspace_bytes", C.c_size_t)]
 
 
 class ShareArgs(C.Structure):
@@ -70,8 +71,9 @@ def load_library(path: str | None = None) -> C.CDLL:
                            ("chill_cache_copy", CopyArgs)):
             getattr(lib, name).argtypes = [C.POINTER(args), C.c_void_p]
             getattr(lib, name).restype = C.c_int
-        lib.chill_share_workspace_bytes.argtypes = [C.POINTER(ShareArgs)]
-        lib.chill_share_workspace_bytes.restype = C.c_size_t
+        for name, args in (("chill_share_workspace_bytes", ShareArgs), ("chill_select_workspace_bytes", SelectArgs)):
+            getattr(lib, name).argtypes = [C.POINTER(args)]
+            getattr(lib, name).restype = C.c_size_t
         lib.chill_decode_launch_count.restype = C.c_ulonglong
         lib.chill_decode_last_cuda_error.restype = C.c_char_p
         lib.chill_decode_abi_version.restype = C.c_int

@@ -20,8 +20,8 @@ from . import _cabi, _decode_abi, _eager, cache
 
 _DTYPES = (torch.float32, torch.float16, torch.bfloat16)
 #: entry points the native DecodeLibrary object is made of, in its order
-_ENTRY_POINTS = ("chill_rotate", "chill_rotate_append", "chill_beam_select", "chill_pages_fork", "chill_pages_trim_shared", "chill_pages_compact",
-                 "chill_share_workspace_bytes", "chill_cache_copy")
+_ENTRY_POINTS = ("chill_rotate", "chill_rotate_append", "chill_beam_select", "chill_select_workspace_bytes", "chill_pages_fork", "chill_pages_trim_shared",
+                 "chill_pages_compact", "chill_share_workspace_bytes", "chill_cache_copy")
 _NATIVE = None
 
 

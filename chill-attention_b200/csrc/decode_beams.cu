@@ -1,42 +1,50 @@
 // Selection of a beam search (chill_beam_select, include/chill_decode.h): candidates c = s_k + x_kv - lse_k of the K beams of a group over a vocabulary of V,
 // the M largest of them.
 //
-// The logits are read once, and that is the floor.  Within a row the order is that of x, so while a warp streams its segment of a row it keeps the M
-// largest x beside the running maximum and sum of the softmax, without knowing lse yet.  A cluster has a group: its warps share the rows, exchange maxima and
-// sums through distributed shared memory, and only then turn their lists into candidates, which are merged by warps, CTAs and at last by the
-// cluster's first CTA.  One launch, no workspace.
+// The logits are read once, and that is the floor.  Within a row the order is that of x, so a CTA that streams a segment of a row keeps the M largest x beside the
+// maximum and sum of the softmax, without knowing lse yet; a second kernel, a CTA for each group, turns the segments' lists into candidates and merges them.  (One
+// kernel with a group in a cluster of 16 CTAs, exchanging sums and lists through distributed shared memory: 62 us where this takes 20, 32 groups of 8 beams over
+// 128000 tokens in bf16, and 75 us where this takes 16, 4 groups of 32 beams over 50021 in fp32: 64 CTAs do not fill the GPU.)
 //
-// A list is sorted and lies across the lanes of a warp (64 entries: two a lane).  What beats its last entry is collected in shared memory and merged in 32
-// or 64 at a time by a bitonic network: the threshold lags behind by a batch, but a batch costs about 150 instructions where single insertions cost 25
-// each, and a threshold of the M-th largest of t values lets about M of the next t through, so a segment of n values has log2(n / M) batches.
-#include <cooperative_groups.h>
-
+// What is kept is not sorted while it grows.  The first batch of a segment gives a lower limit: a number that M of the 256 threads' maxima reach.  That
+// lets about 1.5 M of 8192 values through; they wait in shared memory, and at the end each counts how many are larger than
+// itself.  Where more come than there is room for (sorted rows, constant ones) the M-th largest of all 256 thread maxima is a limit that leaves values of M threads.
 #include <type_traits>
 
 #include "decode_common.cuh"
 
 namespace chill {
 namespace decode {
-namespace cg = cooperative_groups;
+
+constexpr int kThreads = 256;
+constexpr int kWarps = kThreads / 32;
+constexpr int kMost = CHILL_SELECT_MAX;
+constexpr int kBatch = 4;       // vectors of 16 bytes that a thread has at a time
+constexpr int kMaxParts = 64;   // segments of a row
+constexpr int kRoom = 2304;     // values that wait: those of M threads and more, a whole number for each thread
+constexpr int kQueue = 256;      // vectors of a warp that wait to be looked at
+constexpr int kRound = 16;       // batches until they are
+constexpr float kLog2e = 1.4426950408889634f;
+
+struct Sum {
+  double sum;
+  float top;
+  int unused;
+};
 
 struct SelectP {
-  int K, M, V, per_row;  // per_row: warps (segments) of a row
-  int segment;           // values of a segment, whole vectors
+  int K, M, V, parts;
+  int segment;  // values of a segment, whole vectors
   const void* logits;
   long long row_stride;
   const float* scores;
   const uint8_t* finished;
   int end_token;
+  uint64_t* lists;  // [row][part][M], descending
+  Sum* sums;        // [row][part]
   float* out_scores;
   int *out_rows, *out_tokens;
 };
-
-constexpr int kWarps = 8;
-constexpr int kMaxCluster = 16;
-constexpr int kMost = CHILL_SELECT_MAX;
-constexpr float kLog2e = 1.4426950408889634f;
-
-__device__ __forceinline__ long long imin64(long long a, long long b) { return a < b ? a : b; }
 
 // A value and its place as one number: larger values first, of equal ones the lower place.  0: nothing (NaN never gets in).
 __device__ __forceinline__ uint64_t key_of(float x, int v) {
@@ -50,10 +58,13 @@ __device__ __forceinline__ float value_of(uint64_t key) {
 }
 __device__ __forceinline__ int place_of(uint64_t key) { return (int)~(uint32_t)key; }
 
-// A candidate: its 64-bit value mapped to a whole number in the same order (NaN on top), then the place among the group's K * V.  rank 0: nothing.
-struct Candidate {
-  uint64_t rank, place;  // place: inverted, larger is earlier
-};
+// So many of what may be among the M largest are not worth another look at it.
+__host__ __device__ constexpr int enough(int M) { return M + M / 4 + 1; }
+
+// The order of numbers as 32 bits; nothing (-inf) is 0.
+__device__ __forceinline__ uint32_t order_of(float x) { return x > -INFINITY ? (uint32_t)(key_of(x, 0) >> 32) : 0; }
+
+// 64-bit scores in their order as whole numbers, NaN on top; 0: nothing.
 __device__ __forceinline__ uint64_t rank_of(double c) {
   if (c != c) return ~0ull;
   const uint64_t bits = (uint64_t)__double_as_longlong(c + 0.0);
@@ -64,9 +75,359 @@ __device__ __forceinline__ double value_of_rank(uint64_t rank) {
   return __longlong_as_double((long long)(rank & 0x8000000000000000ull ? rank ^ 0x8000000000000000ull : ~rank));
 }
 
-__device__ __forceinline__ bool before(uint64_t a, uint64_t b) { return a > b; }
+__device__ __forceinline__ float exp2_of(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+// The largest of 16 bytes of values; without NaN, these show in the sum.
+template <class T>
+__device__ __forceinline__ float vector_max(const uint4& raw) {
+  if constexpr (std::is_same<T, float>::value) {
+    return fmaxf(fmaxf(__uint_as_float(raw.x), __uint_as_float(raw.y)), fmaxf(__uint_as_float(raw.z), __uint_as_float(raw.w)));
+  } else {
+    using T2 = typename std::conditional<std::is_same<T, __half>::value, __half2, __nv_bfloat162>::type;
+    const T2* p = reinterpret_cast<const T2*>(&raw);
+    const T2 most = __hmax2(__hmax2(p[0], p[1]), __hmax2(p[2], p[3]));
+    return fmaxf(Elem<T>::up(most.x), Elem<T>::up(most.y));
+  }
+}
+
+// Two fp32 numbers in one register pair: Blackwell adds and multiplies both in one instruction.
+__device__ __forceinline__ uint64_t pair_of(float a, float b) {
+  uint64_t d;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(d) : "f"(a), "f"(b));
+  return d;
+}
+__device__ __forceinline__ void split(uint64_t d, float& a, float& b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(d)); }
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t d;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+  uint64_t d;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
+
+// A segment's values that may be among its M largest, in shared memory.
+struct alignas(16) Kept {
+  uint64_t waiting[kRoom + 4];
+  uint64_t maxima[kThreads];
+  uint64_t nth;
+  uint32_t least[kWarps], most[kWarps];
+  int count;
+  int queued[kWarps];
+  int queue[kWarps][kQueue];  // numbers of the vectors in which a warp met something to keep
+};
+
+// Every thread has a key, all that are not 0 are different: the M-th largest (0: there are fewer).
+__device__ __forceinline__ uint64_t nth_of_threads(Kept& kept, uint64_t key, int M) {
+  __syncthreads();
+  kept.maxima[threadIdx.x] = key;
+  if (threadIdx.x == 0) kept.nth = 0;
+  __syncthreads();
+  if (key != 0) {
+    const ulonglong2* others = reinterpret_cast<const ulonglong2*>(kept.maxima);
+    int larger = 0;
+#pragma unroll 4
+    for (int i = 0; i < kThreads / 2; ++i) larger += (others[i].x > key) + (others[i].y > key);
+    if (larger == M - 1) kept.nth = key;
+  }
+  __syncthreads();
+  return kept.nth;
+}
+
+// A number that at least M of the threads' numbers reach, and not many more, by halving (0: fewer than M are not 0; all alike: that one).  Some 8 barriers.
+__device__ __forceinline__ uint32_t reached(Kept& kept, uint32_t own, int M) {
+  const uint32_t least = __reduce_min_sync(0xffffffffu, own), largest = __reduce_max_sync(0xffffffffu, own);
+  __syncthreads();  // what lies there has been read
+  if ((threadIdx.x & 31) == 0) {
+    kept.least[threadIdx.x >> 5] = least;
+    kept.most[threadIdx.x >> 5] = largest;
+  }
+  __syncthreads();
+  uint32_t lo = 0xffffffffu, hi = 0;
+#pragma unroll
+  for (int w = 0; w < kWarps; ++w) {
+    lo = min(lo, kept.least[w]);
+    hi = max(hi, kept.most[w]);
+  }
+  for (int i = 0; i < 20 && lo < hi; ++i) {
+    const uint32_t middle = lo + (hi - lo) / 2 + 1;
+    const int reach = __syncthreads_count(own >= middle);
+    if (reach < M) {
+      hi = middle - 1;
+    } else {
+      lo = middle;
+      if (reach <= enough(M)) break;
+    }
+  }
+  return lo > 0x007fffffu ? lo : 0;  // that is -inf
+}
+
+// Drops what is not among the M largest of those that wait until few more are left, a thread has one at most.  Returns how many; `limit` rises.
+__device__ __forceinline__ int shrink(Kept& kept, int count, int M, uint64_t& limit) {
+  bool exact = false;
+  while (count > enough(M)) {
+    uint64_t key[kRoom / kThreads], most = 0;
+#pragma unroll
+    for (int i = 0; i < kRoom / kThreads; ++i) {
+      const int at = i * kThreads + (int)threadIdx.x;
+      key[i] = at < count ? kept.waiting[at] : 0;
+      most = key[i] > most ? key[i] : most;
+    }
+    const uint64_t lowest = exact ? nth_of_threads(kept, most, M) : (uint64_t)reached(kept, (uint32_t)(most >> 32), M) << 32;
+    limit = lowest > limit ? lowest : limit;
+    __syncthreads();
+    if (threadIdx.x == 0) kept.count = 0;
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < kRoom / kThreads; ++i)
+      if (key[i] != 0 && key[i] >= lowest) kept.waiting[atomicAdd(&kept.count, 1)] = key[i];
+    __syncthreads();
+    const int left = kept.count;
+    __syncthreads();
+    if (left == count) {  // many are alike: places decide
+      if (count <= kThreads) break;
+      exact = true;
+    }
+    count = left;
+  }
+  return count;
+}
+
+// Which value is whose depends on its number alone, not on where the row lies in memory: equal rows have equal sums to the last bit, so that equal beams are ties.
+// A thread has vectors of 16 bytes; kShifted, where rows do not begin at multiples of 16 bytes: words of 4 bytes, 256 apart, of which rows that begin in the middle of one
+// put theirs together from two.
+//
+// Warps stream on their own: sums in registers, numbers of vectors that reach the limit in a queue of their own.  After a round (16 batches) the CTA looks at the queued
+// vectors' values again, which are in L2.  32 groups of 8 beams, 128000 tokens, bf16: loads and maxima alone take 14 us of the 19, exponentials 4.
+template <class T, bool kShifted>
+__global__ void __launch_bounds__(kThreads, 4) scan_kernel(const __grid_constant__ SelectP p) {
+  constexpr int V = 16 / sizeof(T), kWord = 4 / sizeof(T), kStep = kThreads * kBatch;
+  __shared__ Kept kept;
+  __shared__ Sum of_warps[kWarps];
+  asm volatile("griddepcontrol.launch_dependents;");
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int beam = (int)blockIdx.x / p.parts, part = (int)blockIdx.x - beam * p.parts;
+  const int from = (int)((long long)part * p.segment < p.V ? (long long)part * p.segment : p.V);
+  const int to = (int)((long long)from + p.segment < p.V ? from + p.segment : p.V);
+  const T* row = reinterpret_cast<const T*>(p.logits) + beam * p.row_stride + from;
+  const int size = to - from;
+  if (p.scores[beam] == -INFINITY || (p.finished != nullptr && p.finished[beam] != 0)) return;  // nothing of it is looked at
+  const uint32_t none = sizeof(T) == 4 ? 0xff800000u : (std::is_same<T, __half>::value ? 0xfc00fc00u : 0xff80ff80u);  // -inf in every element
+  if (threadIdx.x == 0) kept.count = 0;
+  float top = -INFINITY;  // of this thread's values; the sum of exponentials relative to it is kept in 64 bits, a batch's terms are added up before
+  double sum = 0.0;
+  uint64_t limit = 0;
+
+  // kWord values from number v on, as far as they are there, the others -inf
+  auto word_of = [&](int v) {
+    uint32_t word = none;
+    T* x = reinterpret_cast<T*>(&word);
+#pragma unroll
+    for (int e = 0; e < kWord; ++e)
+      if (v + e < size) x[e] = row[v + e];
+    return word;
+  };
+  // Number of element e of vector `id`: the first one of the batch + 256 u + thread
+  auto number_of = [&](int id, int e) {
+    if (!kShifted) return id * V + e;
+    return (id / kStep * kStep * 4 + (id % kStep / kThreads * 4 + e / kWord) * kThreads + id % kThreads) * kWord + e % kWord;
+  };
+  auto load = [&](int n0, uint4 (&raw)[kBatch]) {
+    const bool whole = n0 + kStep < size / V;  // every vector of the batch is there, and one more value
+    if constexpr (kShifted) {
+      uint32_t* words = reinterpret_cast<uint32_t*>(raw);
+      const bool odd = reinterpret_cast<uintptr_t>(row) % 4 != 0;
+      const uint32_t* at = reinterpret_cast<const uint32_t*>(reinterpret_cast<uintptr_t>(row) / 4 * 4) + n0 * 4 + threadIdx.x;
+      if (whole && n0 > 0 && sizeof(T) == 2 && odd) {
+#pragma unroll
+        for (int i = 0; i < 4 * kBatch; ++i) words[i] = __funnelshift_r(__ldg(at + i * kThreads), __ldg(at + i * kThreads + 1), 16);
+      } else if (whole && !(sizeof(T) == 2 && odd)) {
+#pragma unroll
+        for (int i = 0; i < 4 * kBatch; ++i) words[i] = __ldg(at + i * kThreads);
+      } else {
+#pragma unroll
+        for (int i = 0; i < 4 * kBatch; ++i) words[i] = word_of((n0 * 4 + i * kThreads + (int)threadIdx.x) * kWord);
+      }
+    } else {
+      const uint4* at = reinterpret_cast<const uint4*>(row) + n0 + threadIdx.x;
+      if (whole) {
+#pragma unroll
+        for (int u = 0; u < kBatch; ++u) raw[u] = __ldg(at + u * kThreads);
+      } else {
+#pragma unroll
+        for (int u = 0; u < kBatch; ++u) {
+          const int v = (n0 + u * kThreads + (int)threadIdx.x) * V;
+          if (v + V <= size) raw[u] = __ldg(at + u * kThreads);
+          else raw[u] = make_uint4(word_of(v), word_of(v + kWord), word_of(v + 2 * kWord), word_of(v + 3 * kWord));
+        }
+      }
+    }
+  };
+
+  for (int round = 0; round * V < size; round += kRound * kStep) {
+    int queued = 0;
+    const int end = imin(round + kRound * kStep, (size + V - 1) / V);
+    for (int n0 = round; n0 < end; n0 += kStep) {
+      uint4 raw[kBatch];
+      load(n0, raw);
+      float most[kBatch], all = -INFINITY;
+#pragma unroll
+      for (int u = 0; u < kBatch; ++u) {
+        most[u] = vector_max<T>(raw[u]);
+        all = fmaxf(all, most[u]);
+      }
+      if (all > top) {
+        sum *= (double)exp2_of((top - all) * kLog2e);  // 0 * 0 the first time
+        top = all;
+      }
+      const float base = top == -INFINITY ? 0.f : -top;  // nothing but -inf so far
+      const uint64_t base2 = pair_of(base, base), log2e2 = pair_of(kLog2e, kLog2e);
+      uint64_t terms = 0;
+#pragma unroll
+      for (int u = 0; u < kBatch; ++u) {
+        const T* x = reinterpret_cast<const T*>(&raw[u]);
+#pragma unroll
+        for (int e = 0; e < V; e += 2) {
+          float a, b;
+          split(mul2(add2(pair_of(Elem<T>::up(x[e]), Elem<T>::up(x[e + 1])), base2), log2e2), a, b);
+          terms = add2(terms, pair_of(exp2_of(a), exp2_of(b)));
+        }
+      }
+      float even, uneven;
+      split(terms, even, uneven);
+      sum += (double)(even + uneven);
+
+      if (n0 == 0) {
+        limit = (uint64_t)reached(kept, order_of(all), p.M) << 32;
+      }
+      const float lowest = limit == 0 ? -INFINITY : value_of(limit);
+      if (!__any_sync(0xffffffffu, all > -INFINITY && all >= lowest)) continue;
+#pragma unroll
+      for (int u = 0; u < kBatch; ++u) {
+        const unsigned who = __ballot_sync(0xffffffffu, most[u] > -INFINITY && most[u] >= lowest);
+        const int at = queued + __popc(who & ((1u << lane) - 1));
+        if ((who >> lane & 1) && at < kQueue) kept.queue[warp][at] = n0 + u * kThreads + (int)threadIdx.x;
+        queued += __popc(who);
+      }
+    }
+    if (lane == 0) kept.queued[warp] = queued;
+    __syncthreads();
+    const int before = kept.count;
+    int fullest = 0;
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) fullest = imax(fullest, kept.queued[w]);
+    __syncthreads();
+    if (fullest <= kQueue) {
+      const float lowest = limit == 0 ? -INFINITY : value_of(limit);
+      for (int i = lane; i < queued; i += 32) {
+        const int id = kept.queue[warp][i];
+        uint4 raw;
+        if (!kShifted && (id + 1) * V <= size) raw = __ldg(reinterpret_cast<const uint4*>(row) + id);
+        else raw = make_uint4(word_of(number_of(id, 0)), word_of(number_of(id, kWord)), word_of(number_of(id, 2 * kWord)), word_of(number_of(id, 3 * kWord)));
+        const T* x = reinterpret_cast<const T*>(&raw);
+#pragma unroll
+        for (int e = 0; e < V; ++e) {
+          const float value = Elem<T>::up(x[e]);
+          if (value > -INFINITY && value >= lowest) {
+            const uint64_t key = key_of(value, from + number_of(id, e));
+            if (key >= limit) {
+              const int at = atomicAdd(&kept.count, 1);
+              if (at < kRoom) kept.waiting[at] = key;
+            }
+          }
+        }
+      }
+      __syncthreads();
+    }
+    if (fullest > kQueue || kept.count > kRoom) {
+      // Sorted or constant values, or very many that are alike: batch by batch, with the M-th largest of the threads' maxima as the limit, which leaves values of M threads
+      __syncthreads();
+      if (threadIdx.x == 0) kept.count = before;
+      for (int n0 = round; n0 < end; n0 += kStep) {
+        __syncthreads();
+        shrink(kept, kept.count, p.M, limit);  // 256 wait at most
+        uint4 raw[kBatch];
+        load(n0, raw);
+        uint64_t first = 0;
+#pragma unroll
+        for (int u = 0; u < kBatch; ++u) {
+          const T* x = reinterpret_cast<const T*>(&raw[u]);
+#pragma unroll
+          for (int e = 0; e < V; ++e) {
+            const float value = Elem<T>::up(x[e]);
+            const uint64_t key = value > -INFINITY ? key_of(value, from + number_of(n0 + u * kThreads + (int)threadIdx.x, e)) : 0;
+            first = key > first ? key : first;
+          }
+        }
+        const uint64_t nth = nth_of_threads(kept, first, p.M);
+        limit = nth > limit ? nth : limit;
+        if (first == 0 || first < limit) continue;
+#pragma unroll
+        for (int u = 0; u < kBatch; ++u) {
+          const T* x = reinterpret_cast<const T*>(&raw[u]);
+#pragma unroll
+          for (int e = 0; e < V; ++e) {
+            const float value = Elem<T>::up(x[e]);
+            const uint64_t key = value > -INFINITY ? key_of(value, from + number_of(n0 + u * kThreads + (int)threadIdx.x, e)) : 0;
+            if (key != 0 && key >= limit) kept.waiting[atomicAdd(&kept.count, 1)] = key;
+          }
+        }
+      }
+    }
+    if (end * V < size) {  // another round: its limit is about the M-th largest of those that wait
+      __syncthreads();
+      shrink(kept, kept.count, p.M, limit);
+    }
+  }
+
+  // The segment's sum
+  float highest = top;
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) highest = fmaxf(highest, __shfl_xor_sync(0xffffffffu, highest, o));
+  if (top != -INFINITY) sum *= (double)exp2_of((top - highest) * kLog2e);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+  if (lane == 0) of_warps[warp] = {sum, highest, 0};
+  __syncthreads();
+  if (warp == 0) {
+    const Sum s = of_warps[lane % kWarps];
+    highest = s.top;
+#pragma unroll
+    for (int o = kWarps / 2; o > 0; o >>= 1) highest = fmaxf(highest, __shfl_xor_sync(0xffffffffu, highest, o));
+    sum = s.top != -INFINITY ? s.sum * exp((double)s.top - (double)highest) : s.sum;
+#pragma unroll
+    for (int o = kWarps / 2; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    if (lane == 0) p.sums[blockIdx.x] = {sum, highest, 0};
+  }
+  // Its list: every value that waits counts the larger ones
+  const int count = shrink(kept, kept.count, p.M, limit);
+  uint64_t* list = p.lists + (long long)blockIdx.x * p.M;
+  if ((int)threadIdx.x < (-count & 3)) kept.waiting[count + threadIdx.x] = 0;
+  __syncthreads();
+  if ((int)threadIdx.x < count) {
+    const uint64_t key = kept.waiting[threadIdx.x];
+    const ulonglong2* others = reinterpret_cast<const ulonglong2*>(kept.waiting);
+    int larger = 0;
+    for (int i = 0; i < (count + 3) / 4; ++i) {
+      const ulonglong2 a = others[2 * i], b = others[2 * i + 1];
+      larger += (a.x > key) + (a.y > key) + (b.x > key) + (b.y > key);
+    }
+    if (larger < p.M) list[larger] = key;
+  }
+  if ((int)threadIdx.x >= count && (int)threadIdx.x < p.M) list[threadIdx.x] = 0;
+}
+
+// A candidate in the order of its 64-bit score, then of its place among the group's K * V (inverted: larger is earlier).
+struct Candidate {
+  uint64_t rank, place;
+};
 __device__ __forceinline__ bool before(const Candidate& a, const Candidate& b) { return a.rank != b.rank ? a.rank > b.rank : a.place > b.place; }
-__device__ __forceinline__ uint64_t from_lane(uint64_t x, int mask) { return __shfl_xor_sync(0xffffffffu, x, mask); }
+
 __device__ __forceinline__ Candidate from_lane(const Candidate& x, int mask) {
   return {__shfl_xor_sync(0xffffffffu, x.rank, mask), __shfl_xor_sync(0xffffffffu, x.place, mask)};
 }
@@ -115,318 +476,144 @@ struct List {
   }
 };
 
+// One CTA for a group.  Its warps go over the lists in turn; a warp keeps the M first of those it has met, sorted across its lanes, and merges a list of which the
+// first entry comes before its last one (a bitonic network; most lists are passed over).  At the end the warps' lists are merged two and two.
+constexpr int kMergeWarps = 32;  // at most: one for every list, and 4 at least
 
-__device__ __forceinline__ float exp2_of(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
-// The largest number below x (x finite); what is above it is at least x.
-__device__ __forceinline__ float just_below(float x) {
-  const int bits = __float_as_int(x);
-  return x == 0.f ? __int_as_float((int)0x80000001u) : __int_as_float(x > 0.f ? bits - 1 : bits + 1);
-}
+template <class T, int R>
+__global__ void __launch_bounds__(kMergeWarps * 32) merge_kernel(const __grid_constant__ SelectP p) {
+  constexpr int kList = 32 * R;
+  __shared__ double lse[kMost];
+  __shared__ float score[kMost];
+  __shared__ bool over[kMost], flat[kMost];  // finished beams; rows whose candidates are all alike: NaN or +inf
+  __shared__ Candidate exchange[kMergeWarps / 2][kList];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, group = (int)blockIdx.x, warps = (int)blockDim.x >> 5;
+  const int lists = p.K * p.parts;
+  const uint64_t* const entries = p.lists + (long long)group * lists * p.M;
+  asm volatile("griddepcontrol.wait;" ::: "memory");  // the lists are there
+  // This warp's first list is on its way while the sums are worked out (nonsense where nothing was written)
+  uint64_t first[R];
+#pragma unroll
+  for (int r = 0; r < R; ++r) first[r] = warp < lists && lane + 32 * r < p.M ? __ldcg(&entries[(long long)warp * p.M + lane + 32 * r]) : 0;
 
-// What a warp knows of the segment that it streams.
-template <int R>
-struct Stream {
-  List<uint64_t, R> best;
-  float top;   // of this lane's values; their sum of exponentials relative to it, in 64 bits (a vector's terms are added up before)
-  double sum;
-  uint64_t* waiting;
-  int count;    // of those that wait
-  float limit;  // what is not above it is not among the M largest
-  int last;     // M - 1
-
-  __device__ __forceinline__ void begin(uint64_t* buffer, int M) {
+  for (int k = warp; k < p.K; k += warps) {
+    const long long beam = (long long)group * p.K + k;
+    const float s = p.scores[beam];
+    const bool ended = p.finished != nullptr && p.finished[beam] != 0;
+    Sum mine[kMaxParts / 32];  // nonsense for beams that were not looked at
 #pragma unroll
-    for (int r = 0; r < R; ++r) best.x[r] = 0;
-    top = -INFINITY;
-    sum = 0.0;
-    waiting = buffer;
-    count = 0;
-    limit = -INFINITY;
-    last = M - 1;
-  }
-
-  // Merges the first 32 * R that wait (what is missing of them is nothing) and moves the rest to the front.
-  __device__ __forceinline__ void flush() {
-    const int lane = threadIdx.x & 31;
-    __syncwarp();
-    List<uint64_t, R> more, reversed;
+    for (int i = 0; i < kMaxParts / 32; ++i) mine[i] = lane + 32 * i < p.parts ? p.sums[beam * p.parts + lane + 32 * i] : Sum{0.0, -INFINITY, 0};
+    float top = -INFINITY;
 #pragma unroll
-    for (int r = 0; r < R; ++r) more.x[r] = lane + 32 * r < count ? waiting[lane + 32 * r] : 0;
-    more.sort();
+    for (int i = 0; i < kMaxParts / 32; ++i) top = fmaxf(top, mine[i].top);
 #pragma unroll
-    for (int r = 0; r < R; ++r) reversed.x[r] = __shfl_sync(0xffffffffu, more.x[R - 1 - r], 31 - lane);
-    best.merge(reversed);
-    const uint64_t key = __shfl_sync(0xffffffffu, last >= 32 ? best.x[R - 1] : best.x[0], last & 31);
-    if (key != 0) limit = value_of(key);
-    const int rest = count - 32 * R;
-    for (int e0 = 0; e0 < rest; e0 += 32) {
-      const uint64_t x = e0 + lane < rest ? waiting[32 * R + e0 + lane] : 0;
-      __syncwarp();
-      if (e0 + lane < rest) waiting[e0 + lane] = x;
-      __syncwarp();
-    }
-    count = imax(rest, 0);
-  }
-
-  // A lower limit to begin with: the M-th largest of 32 * R values, each the maximum of values of its own.
-  __device__ __forceinline__ void first_limit(const float (&maxima)[R]) {
-    List<uint64_t, R> sample;
+    for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+    double sum = 0.0;
 #pragma unroll
-    for (int r = 0; r < R; ++r) sample.x[r] = key_of(maxima[r], 0);
-    sample.sort();
-    const float found = value_of(__shfl_sync(0xffffffffu, last >= 32 ? sample.x[R - 1] : sample.x[0], last & 31));
-    if (found > -INFINITY) limit = just_below(found);
-  }
-
-  // N values of each lane, the first of them number v of the row; -inf where there is none.
-  template <int N>
-  __device__ __forceinline__ void add(const float (&x)[N], float most) {
-    if (most > top) {
-      sum *= (double)exp2_of((top - most) * kLog2e);  // 0 * 0 the first time
-      top = most;
-    }
-    const float base = top == -INFINITY ? 0.f : top;  // nothing but -inf so far
-    float terms = 0.f;
+    for (int i = 0; i < kMaxParts / 32; ++i)
+      if (lane + 32 * i < p.parts) sum += mine[i].top == -INFINITY ? mine[i].sum : mine[i].sum * exp((double)mine[i].top - (double)top);
 #pragma unroll
-    for (int e = 0; e < N; ++e) terms += exp2_of((x[e] - base) * kLog2e);
-    sum += (double)terms;
-  }
-  // Those above the limit wait; flush() has to follow where 32 * R do.
-  template <int N>
-  __device__ __forceinline__ void keep(const float (&x)[N], int v) {
-    const unsigned below = (1u << (threadIdx.x & 31)) - 1;
-#pragma unroll
-    for (int e = 0; e < N; ++e) {
-      const bool in = x[e] > limit;
-      const unsigned who = __ballot_sync(0xffffffffu, in);
-      if (in) waiting[count + __popc(who & below)] = key_of(x[e], v + e);
-      count += __popc(who);
+    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    if (lane == 0) {
+      const double l = (double)top + log(sum);  // a row without values has empty lists
+      lse[k] = l;
+      score[k] = s;
+      over[k] = ended;
+      flat[k] = s != -INFINITY && !ended && (l != l || !(s < INFINITY));
     }
   }
-};
-
-template <class T, int V>
-__device__ __forceinline__ float unpack(const uint4& raw, float (&x)[V]) {
-  const T* p = reinterpret_cast<const T*>(&raw);
-  float most = -INFINITY;
-#pragma unroll
-  for (int e = 0; e < V; ++e) {
-    x[e] = Elem<T>::up(p[e]);
-    most = fmaxf(most, x[e]);  // without NaN; these show in the sum
-  }
-  return most;
-}
-
-// 16 bytes from `byte` bytes into the first of two adjacent vectors on (a multiple of the element size).
-__device__ __forceinline__ uint4 straddle(const uint4& a, const uint4& b, int byte) {
-  const uint32_t w[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
-  uint32_t x[5];  // from the word on that the byte lies in
-#pragma unroll
-  for (int i = 0; i < 5; ++i) x[i] = byte < 4 ? w[i] : (byte < 8 ? w[i + 1] : (byte < 12 ? w[i + 2] : w[i + 3]));
-  const int bits = 8 * (byte & 3);
-  return make_uint4(__funnelshift_r(x[0], x[1], bits), __funnelshift_r(x[1], x[2], bits), __funnelshift_r(x[2], x[3], bits), __funnelshift_r(x[3], x[4], bits));
-}
-
-// Values [from, to) of a row, `from` a whole number of vectors of 16 bytes: a lane has a vector at a time, the last few values come at the end.  Which value is whose
-// depends on its number alone, not on where the row lies in memory: equal rows have equal sums to the last bit, so that equal beams are ties.
-// kShifted: rows do not begin at multiples of 16 bytes; a vector is put together from the two that it lies in, the first and the last one of a segment, whose
-// neighbours are another's, value by value.
-template <class T, int R, bool kShifted>
-__device__ __forceinline__ void stream_row(Stream<R>& s, const T* row, int from, int to) {
-  constexpr int V = 16 / sizeof(T), kBatch = kShifted ? 2 : 4;
-  const int lane = threadIdx.x & 31, vectors = (to - from) / V;
-  const int byte = kShifted ? (int)(reinterpret_cast<uintptr_t>(row) % 16) : 0;
-  const uint4* at = reinterpret_cast<const uint4*>(reinterpret_cast<const char*>(row + from) - byte);
-  // -inf in every element, where there is no vector
-  const uint32_t none = sizeof(T) == 4 ? 0xff800000u : (std::is_same<T, __half>::value ? 0xfc00fc00u : 0xff80ff80u);
-  for (int n0 = 0; n0 < vectors; n0 += 32 * kBatch) {
-    uint4 raw[kBatch];
-    float most[kBatch], x[V];
-    if constexpr (kShifted) {
-      uint4 next[kBatch];
-#pragma unroll
-      for (int u = 0; u < kBatch; ++u) {
-        const int n = n0 + 32 * u + lane;
-        raw[u] = next[u] = make_uint4(none, none, none, none);
-        if (n > 0 && n < vectors - 1) {
-          raw[u] = __ldg(at + n);
-          next[u] = __ldg(at + n + 1);
-        }
-      }
-#pragma unroll
-      for (int u = 0; u < kBatch; ++u) {
-        const int n = n0 + 32 * u + lane;
-        raw[u] = straddle(raw[u], next[u], byte);
-        if (n == 0 || n == vectors - 1) {
-          T* to_raw = reinterpret_cast<T*>(&raw[u]);
-#pragma unroll
-          for (int e = 0; e < V; ++e) to_raw[e] = row[from + n * V + e];
-        }
-      }
-    } else {
-#pragma unroll
-      for (int u = 0; u < kBatch; ++u) {
-        const int n = n0 + 32 * u + lane;
-        raw[u] = n < vectors ? __ldcs(at + n) : make_uint4(none, none, none, none);
-      }
-    }
-    float block = -INFINITY;
-#pragma unroll
-    for (int u = 0; u < kBatch; ++u) {
-      most[u] = unpack<T, V>(raw[u], x);
-      s.add(x, most[u]);
-      block = fmaxf(block, most[u]);
-    }
-    if (n0 == 0) {
-      float maxima[R];
-#pragma unroll
-      for (int r = 0; r < R; ++r) maxima[r] = -INFINITY;
-#pragma unroll
-      for (int u = 0; u < kBatch; ++u) maxima[u % R] = fmaxf(maxima[u % R], most[u]);
-      s.first_limit(maxima);
-    }
-    if (!__any_sync(0xffffffffu, block > s.limit)) continue;
-#pragma unroll 1
-    for (int u = 0; u < kBatch; ++u) {
-      uint4 one = raw[0];
-#pragma unroll
-      for (int i = 1; i < kBatch; ++i) one = u == i ? raw[i] : one;
-      if (!__any_sync(0xffffffffu, unpack<T, V>(one, x) > s.limit)) continue;
-      s.keep(x, from + (n0 + 32 * u + lane) * V);
-      while (s.count >= 32 * R) s.flush();
-    }
-  }
-  const int v = from + vectors * V + lane;
-  const float x[1] = {v < to ? Elem<T>::up(row[v]) : -INFINITY};
-  s.add(x, fmaxf(x[0], -INFINITY));
-  s.keep(x, v);
-  while (s.count > 0) s.flush();
-}
-
-template <class T, int R, bool kShifted>
-__global__ void __launch_bounds__(kWarps * 32) select_kernel(const __grid_constant__ SelectP p) {
-  constexpr int kList = 32 * R, kBuffer = kList + 32 * (16 / (int)sizeof(T));
-  union Room {  // of a warp: what waits while it streams, its list of candidates later
-    uint64_t waiting[kBuffer];
-    Candidate list[kList];
+  __syncthreads();
+  auto candidate = [&](int k, float x, int v) {
+    return Candidate{rank_of((double)score[k] + ((double)x - lse[k])), ~(uint64_t)((long long)k * p.V + v)};
   };
-  __shared__ __align__(16) unsigned char room_bytes[kWarps * sizeof(Room)];
-  __shared__ __align__(16) unsigned char list_bytes[kMaxCluster * kList * sizeof(Candidate)];  // first CTA: the lists of all
-  __shared__ float tops[kWarps];
-  __shared__ double sums[kWarps];
-  Room* const room = reinterpret_cast<Room*>(room_bytes);
-  Candidate(*const lists)[kList] = reinterpret_cast<Candidate(*)[kList]>(list_bytes);
-  cg::cluster_group cluster = cg::this_cluster();
-  const int ctas = (int)cluster.num_blocks(), cta = (int)cluster.block_rank(), group = (int)blockIdx.x / ctas;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  auto usable = [&](int k) { return score[k] != -INFINITY && !over[k] && !flat[k]; };
 
-  // Unit u of the cluster, segment u % per_row of beam u / per_row, is warp u / ctas of CTA u % ctas
-  const int unit = warp * ctas + cta, k = unit / p.per_row, part = unit - k * p.per_row;
-  const bool works = k < p.K;
-  const float base = works ? p.scores[group * p.K + k] : -INFINITY;
-  const bool over = works && p.finished != nullptr && p.finished[group * p.K + k] != 0;
-  const bool reads = works && !over && base != -INFINITY;
-  const T* row = reinterpret_cast<const T*>(p.logits) + (long long)(group * p.K + k) * p.row_stride;
-  Stream<R> s;
-  s.begin(room[warp].waiting, p.M);
-  if (reads) {
-    const int from = (int)imin64((long long)part * p.segment, p.V), to = (int)imin64((long long)(part + 1) * p.segment, p.V);
-    if (from < to) stream_row<T, R, kShifted>(s, row, from, to);
-  }
-  float top = s.top;
+  List<Candidate, R> best;
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-  double sum = s.top == -INFINITY ? s.sum : s.sum * exp((double)s.top - (double)top);
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-  if (lane == 0) {
-    tops[warp] = top;
-    sums[warp] = sum;
-  }
-  cluster.sync();
-
-  // log sum exp of the row, from all its segments
-  List<Candidate, R> mine;
-#pragma unroll
-  for (int r = 0; r < R; ++r) mine.x[r] = {0, 0};
-  if (reads) {
-    float all = -INFINITY;
-    double total = 0.0;
-    for (int u = k * p.per_row + lane; u < (k + 1) * p.per_row; u += 32) all = fmaxf(all, *cluster.map_shared_rank(&tops[u / ctas], u % ctas));
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) all = fmaxf(all, __shfl_xor_sync(0xffffffffu, all, o));
-    for (int u = k * p.per_row + lane; u < (k + 1) * p.per_row; u += 32) {
-      const float t = *cluster.map_shared_rank(&tops[u / ctas], u % ctas);
-      const double x = *cluster.map_shared_rank(&sums[u / ctas], u % ctas);
-      total += t == -INFINITY ? x : x * exp((double)t - (double)all);
-    }
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
-    const double lse = (double)all + log(total);
-    const long long first = (long long)k * p.V;
-    auto candidate = [&](float x, int v) { return Candidate{rank_of((double)base + ((double)x - lse)), ~(uint64_t)(first + v)}; };
-    if (lse != lse || base != base || base == INFINITY) {
-      // All candidates are equal (NaN, or +inf): the first ones count
-      if (part == 0) {
-        int found = 0;
-        for (int v0 = 0; v0 < p.V && found < p.M; v0 += 32) {
-          const float x = v0 + lane < p.V ? Elem<T>::up(row[v0 + lane]) : -INFINITY;
-          const unsigned who = __ballot_sync(0xffffffffu, x != -INFINITY);
-          const int e = found + __popc(who & ((1u << lane) - 1));
-          if (x != -INFINITY && e < kList) room[warp].list[e] = candidate(x, v0 + lane);
-          found += __popc(who);
-        }
-        __syncwarp();
-#pragma unroll
-        for (int r = 0; r < R; ++r)
-          if (lane + 32 * r < found) mine.x[r] = room[warp].list[lane + 32 * r];
-        __syncwarp();
+  for (int r = 0; r < R; ++r) best.x[r] = {0, 0};
+  if (warp < 2) {  // rows of NaN, rows of +inf: the first values of the first ones
+    int n = 0;
+    for (int k = 0; k < p.K; ++k) {
+      if (!flat[k] || (score[k] == INFINITY && lse[k] == lse[k]) != (warp == 1)) continue;
+      const T* row = reinterpret_cast<const T*>(p.logits) + ((long long)group * p.K + k) * p.row_stride;
+      for (int v0 = 0; v0 < p.V && n < p.M; v0 += 32) {
+        const float x = v0 + lane < p.V ? Elem<T>::up(row[v0 + lane]) : -INFINITY;
+        const unsigned who = __ballot_sync(0xffffffffu, x != -INFINITY);
+        const int e = n + __popc(who & ((1u << lane) - 1));
+        if (x != -INFINITY && e < kList) exchange[warp][e] = candidate(k, x, v0 + lane);
+        n += __popc(who);
       }
-    } else {
+    }
+    __syncwarp();
+#pragma unroll
+    for (int r = 0; r < R; ++r)
+      if (lane + 32 * r < n) best.x[r] = exchange[warp][lane + 32 * r];
+  }
+
+  auto nth = [&]() {  // the M-th; with all lanes
+    return Candidate{__shfl_sync(0xffffffffu, p.M > 32 ? best.x[R - 1].rank : best.x[0].rank, (p.M - 1) & 31),
+                     __shfl_sync(0xffffffffu, p.M > 32 ? best.x[R - 1].place : best.x[0].place, (p.M - 1) & 31)};
+  };
+  // Entry e of list l
+  auto entry = [&](int l, int e, uint64_t key) {
+    const int k = l / p.parts;
+    if (usable(k)) return key != 0 ? candidate(k, value_of(key), place_of(key)) : Candidate{0, 0};
+    if (over[k] && e == 0 && l == k * p.parts && score[k] != -INFINITY)  // a finished beam: a list of one
+      return Candidate{rank_of((double)score[k]), ~(uint64_t)((long long)k * p.V + p.end_token)};
+    return Candidate{0, 0};
+  };
+  if (warp < lists) {
+    List<Candidate, R> own;
+#pragma unroll
+    for (int r = 0; r < R; ++r) own.x[r] = entry(warp, lane + 32 * r, first[r]);
+    if (warp < 2) {  // there may be something already: the list's entries from the last one to the first
+      List<Candidate, R> reversed;
 #pragma unroll
       for (int r = 0; r < R; ++r)
-        if (s.best.x[r] != 0) mine.x[r] = candidate(value_of(s.best.x[r]), place_of(s.best.x[r]));
+        reversed.x[r] = {__shfl_sync(0xffffffffu, own.x[R - 1 - r].rank, 31 - lane), __shfl_sync(0xffffffffu, own.x[R - 1 - r].place, 31 - lane)};
+      best.merge(reversed);
+    } else {
+      best = own;
     }
-  } else if (over && part == 0 && base != -INFINITY && lane == 0) {
-    mine.x[0] = {rank_of((double)base), ~(uint64_t)((long long)k * p.V + p.end_token)};
   }
-
-  // The lists of the warps, two and two
-  auto merge_with = [&](const Candidate* list) {
-    List<Candidate, R> reversed;
+  for (int l0 = warp + warps; l0 < lists; l0 += 32 * warps) {  // of the others a lane looks at the first entry
+    const int own = l0 + lane * warps;
+    const Candidate head = own < lists ? entry(own, 0, entries[(long long)own * p.M]) : Candidate{0, 0};
+    bool waits = head.rank != 0;
+    while (true) {
+      const Candidate last = nth();  // with all lanes
+      waits = waits && before(head, last);
+      // the one with the best first entry (or next to it), after which more are passed over
+      const uint32_t top = waits ? (uint32_t)(head.rank >> 32) : 0, most = __reduce_max_sync(0xffffffffu, top);
+      if (most == 0) break;
+      const int next = __ffs(__ballot_sync(0xffffffffu, top == most)) - 1, l = l0 + next * warps;
+      if (lane == next) waits = false;
+      List<Candidate, R> reversed;
 #pragma unroll
-    for (int r = 0; r < R; ++r) reversed.x[r] = list[kList - 1 - lane - 32 * r];
-    mine.merge(reversed);
-  };
-  auto merge_warps = [&]() {
-#pragma unroll
-    for (int apart = 1; apart < kWarps; apart <<= 1) {
-      if ((warp & (2 * apart - 1)) == apart) {
-#pragma unroll
-        for (int r = 0; r < R; ++r) room[warp].list[lane + 32 * r] = mine.x[r];
+      for (int r = 0; r < R; ++r) {
+        const int e = kList - 1 - lane - 32 * r;
+        reversed.x[r] = e < p.M ? entry(l, e, entries[(long long)l * p.M + e]) : Candidate{0, 0};
       }
-      __syncthreads();
-      if ((warp & (2 * apart - 1)) == 0) merge_with(room[warp + apart].list);
+      best.merge(reversed);
     }
-  };
-  merge_warps();
-  if (ctas > 1) {
-    if (warp == 0) {
-      Candidate* to = cluster.map_shared_rank(&lists[cta][0], 0);
+  }
+#pragma unroll 1
+  for (int apart = warps / 2; apart > 0; apart >>= 1) {
+    __syncthreads();  // what lies in `exchange` has been read
+    if (warp >= apart && warp < 2 * apart) {
 #pragma unroll
-      for (int r = 0; r < R; ++r) to[lane + 32 * r] = mine.x[r];
+      for (int r = 0; r < R; ++r) exchange[warp - apart][lane + 32 * r] = best.x[r];
     }
-    cluster.sync();
-    if (cta != 0) return;
+    __syncthreads();
+    if (warp < apart) {
+      const Candidate last = nth();
+      if (before(exchange[warp][0], last)) {
+        List<Candidate, R> reversed;
 #pragma unroll
-    for (int r = 0; r < R; ++r) mine.x[r] = warp < ctas ? lists[warp][lane + 32 * r] : Candidate{0, 0};
-    if (warp + kWarps < ctas) merge_with(lists[warp + kWarps]);
-    __syncthreads();  // room is written again
-    merge_warps();
+        for (int r = 0; r < R; ++r) reversed.x[r] = exchange[warp][kList - 1 - lane - 32 * r];
+        best.merge(reversed);
+      }
+    }
   }
   if (warp != 0) return;
 
@@ -434,90 +621,117 @@ __global__ void __launch_bounds__(kWarps * 32) select_kernel(const __grid_consta
   int found = 0;
 #pragma unroll
   for (int r = 0; r < R; ++r) {
-    found += __popc(__ballot_sync(0xffffffffu, mine.x[r].rank != 0));
-    room[0].list[lane + 32 * r] = mine.x[r];
+    found += __popc(__ballot_sync(0xffffffffu, best.x[r].rank != 0));
+    exchange[1][lane + 32 * r] = best.x[r];  // read by warp 1 in the last round but one
   }
   __syncwarp();
 #pragma unroll
   for (int r = 0; r < R; ++r) {
     const int e = lane + 32 * r;
     if (e >= p.M) continue;
-    long long place = (long long)~mine.x[r].place;
+    long long place = (long long)~best.x[r].place;
     double value = -INFINITY;
     if (e < found) {
-      value = value_of_rank(mine.x[r].rank);
+      value = value_of_rank(best.x[r].rank);
     } else {
-      long long before_it = -1, places = 0;  // of those found
-      while (places != before_it) {
-        before_it = places;
-        places = 0;
-        for (int n = 0; n < found; ++n) places += (long long)~room[0].list[n].place <= e - found + before_it;
+      long long so_far = -1, skipped = 0;  // of those found
+      while (skipped != so_far) {
+        so_far = skipped;
+        skipped = 0;
+        for (int i = 0; i < found; ++i) skipped += (long long)~exchange[1][i].place <= e - found + so_far;
       }
-      place = e - found + places;
+      place = e - found + skipped;
     }
-    const long long at = (long long)group * p.M + e;
-    const int beam = (int)(place / p.V);
-    p.out_scores[at] = (float)value;
-    p.out_rows[at] = group * p.K + beam;
-    p.out_tokens[at] = (int)(place - (long long)beam * p.V);
+    const long long to = (long long)group * p.M + e;
+    const int k = (int)(place / p.V);
+    p.out_scores[to] = (float)value;
+    p.out_rows[to] = group * p.K + k;
+    p.out_tokens[to] = (int)(place - (long long)k * p.V);
   }
 }
 
-template <class T, int R, bool kShifted>
-static cudaError_t launch_kernel(const SelectP& p, int groups, int ctas, cudaStream_t st) {
-  cudaLaunchConfig_t cfg{};
-  cudaLaunchAttribute attr[1];
-  if (ctas > 8) {
-    const cudaError_t e = cudaFuncSetAttribute(select_kernel<T, R, kShifted>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
-    if (e != cudaSuccess) return e;
-  }
-  cfg.gridDim = dim3((unsigned)(groups * ctas));
-  cfg.blockDim = dim3(kWarps * 32);
-  cfg.stream = st;
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = (unsigned)ctas;
-  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, select_kernel<T, R, kShifted>, p);
+// Segments of a row, and their length: whole batches, as many as the GPU has room for CTAs (four an SM).
+static int parts_of(const chill_select_args& a, int& segment) {
+  const int vec = 16 / elem_size(a.dtype), batch = kThreads * kBatch * vec;
+  const long long batches = (a.V + batch - 1) / batch, rows = (long long)a.G * a.K, slots = 4ll * sm_count();
+  long long parts = rows < slots ? slots / rows : 1;
+  if (parts > kMaxParts) parts = kMaxParts;
+  const long long each = (batches + parts - 1) / parts;
+  segment = (int)(each * batch);
+  return (int)((batches + each - 1) / each);
 }
 
-template <class T>
-static cudaError_t launch_select(const SelectP& p, int groups, int ctas, cudaStream_t st) {
-  const bool shifted = reinterpret_cast<uintptr_t>(p.logits) % 16 != 0 || (groups * p.K > 1 && p.row_stride * (long long)sizeof(T) % 16 != 0);
-  if (p.M <= 32) return shifted ? launch_kernel<T, 1, true>(p, groups, ctas, st) : launch_kernel<T, 1, false>(p, groups, ctas, st);
-  return shifted ? launch_kernel<T, 2, true>(p, groups, ctas, st) : launch_kernel<T, 2, false>(p, groups, ctas, st);
+static size_t workspace_of(const chill_select_args& a) {
+  int segment;
+  const size_t lists = (size_t)a.G * a.K * parts_of(a, segment);
+  return lists * (a.M * sizeof(uint64_t) + sizeof(Sum));
 }
 
-static int select(const chill_select_args* a, cudaStream_t st) {
+static int check_select(const chill_select_args* a, bool pointers) {
   if (a == nullptr || a->G <= 0 || a->K <= 0 || a->M <= 0 || a->V <= 0) return CHILL_E_INVALID;
   if (!known_dtype(a->dtype)) return CHILL_E_UNSUPPORTED;
   if (a->K > kMost || a->M > kMost || a->V > (1ll << 30) || (long long)a->G * a->K > kMaxRequests) return CHILL_E_TOO_LARGE;
-  if (a->M > a->K * a->V || !a->logits || !a->scores || !a->out_scores || !a->out_rows || !a->out_tokens) return CHILL_E_INVALID;
+  if (a->M > a->K * a->V) return CHILL_E_INVALID;
+  if (!pointers) return CHILL_OK;
+  if (!a->logits || !a->scores || !a->out_scores || !a->out_rows || !a->out_tokens) return CHILL_E_INVALID;
   if (a->finished != nullptr && (a->end_token < 0 || a->end_token >= a->V)) return CHILL_E_INVALID;
+  if (a->workspace == nullptr || a->workspace_bytes < workspace_of(*a) || reinterpret_cast<uintptr_t>(a->workspace) % 16 != 0) return CHILL_E_INVALID;
+  return CHILL_OK;
+}
+
+template <class T>
+static cudaError_t launch_select(const SelectP& p, int groups, cudaStream_t st) {
+  const bool shifted = reinterpret_cast<uintptr_t>(p.logits) % 16 != 0 || (groups * p.K > 1 && p.row_stride * (long long)sizeof(T) % 16 != 0);
+  const unsigned units = (unsigned)(groups * p.K * p.parts);
+  if (shifted) scan_kernel<T, true><<<units, kThreads, 0, st>>>(p);
+  else scan_kernel<T, false><<<units, kThreads, 0, st>>>(p);
+  const cudaError_t e = cudaGetLastError();
+  if (e != cudaSuccess) return e;
+  // The second kernel is brought up beside the first one's last CTAs, and waits for their end (griddepcontrol)
+  cudaLaunchConfig_t cfg{};
+  cudaLaunchAttribute attr[1];
+  cfg.gridDim = dim3((unsigned)groups);
+  int warps = 4;
+  while (warps < kMergeWarps && warps < p.K * p.parts) warps *= 2;
+  cfg.blockDim = dim3((unsigned)warps * 32);
+  cfg.stream = st;
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return p.M <= 32 ? cudaLaunchKernelEx(&cfg, merge_kernel<T, 1>, p) : cudaLaunchKernelEx(&cfg, merge_kernel<T, 2>, p);
+}
+
+static int select(const chill_select_args& a, cudaStream_t st) {
   SelectP p{};
-  p.K = a->K; p.M = a->M; p.V = (int)a->V;
-  p.logits = a->logits; p.row_stride = a->row_stride;
-  p.scores = a->scores; p.finished = a->finished; p.end_token = (int)a->end_token;
-  p.out_scores = a->out_scores; p.out_rows = a->out_rows; p.out_tokens = a->out_tokens;
-  // A warp for every beam at least; more CTAs while they fit the GPU, four an SM, and a warp has a thousand values
-  int ctas = 1;
-  while (ctas * kWarps < a->K) ctas *= 2;
-  while (ctas < kMaxCluster && 2ll * ctas * a->G <= 4ll * sm_count() && (long long)a->K * a->V >= 2ll * ctas * kWarps * 1024) ctas *= 2;
-  p.per_row = ctas * kWarps / a->K;
-  const int vec = 16 / elem_size(a->dtype);
-  const long long segment = (a->V + p.per_row - 1) / p.per_row;
-  p.segment = (int)((segment + vec - 1) / vec * vec);
+  p.K = a.K; p.M = a.M; p.V = (int)a.V;
+  p.parts = parts_of(a, p.segment);
+  p.logits = a.logits; p.row_stride = a.row_stride;
+  p.scores = a.scores; p.finished = a.finished; p.end_token = (int)a.end_token;
+  p.sums = (Sum*)a.workspace;
+  p.lists = (uint64_t*)(p.sums + (size_t)a.G * a.K * p.parts);
+  p.out_scores = a.out_scores; p.out_rows = a.out_rows; p.out_tokens = a.out_tokens;
   cudaError_t e;
-  if (a->dtype == CHILL_F32) e = launch_select<float>(p, a->G, ctas, st);
-  else if (a->dtype == CHILL_F16) e = launch_select<__half>(p, a->G, ctas, st);
-  else e = launch_select<__nv_bfloat16>(p, a->G, ctas, st);
+  if (a.dtype == CHILL_F32) e = launch_select<float>(p, a.G, st);
+  else if (a.dtype == CHILL_F16) e = launch_select<__half>(p, a.G, st);
+  else e = launch_select<__nv_bfloat16>(p, a.G, st);
   if (e != cudaSuccess) return record_cuda_failure(e, "select launch");
-  count_launches(1);
+  count_launches(2);
   return CHILL_OK;
 }
 
 }  // namespace decode
 }  // namespace chill
 
-extern "C" int chill_beam_select(const chill_select_args* a, void* stream) { return chill::decode::select(a, (cudaStream_t)stream); }
+extern "C" {
+
+size_t chill_select_workspace_bytes(const chill_select_args* a) {
+  return chill::decode::check_select(a, false) == CHILL_OK ? chill::decode::workspace_of(*a) : 0;
+}
+
+int chill_beam_select(const chill_select_args* a, void* stream) {
+  const int st = chill::decode::check_select(a, true);
+  return st != CHILL_OK ? st : chill::decode::select(*a, (cudaStream_t)stream);
+}
+
+}  // extern "C"

@@ -29,6 +29,7 @@ struct DecodeLibrary {
   decltype(&chill_rotate) rotate;
   decltype(&chill_rotate_append) rotate_append;
   decltype(&chill_beam_select) select;
+  decltype(&chill_select_workspace_bytes) select_bytes;
   decltype(&chill_pages_fork) fork;
   decltype(&chill_pages_trim_shared) trim;
   decltype(&chill_pages_compact) compact;
@@ -218,6 +219,9 @@ py::object beam_select(const DecodeLibrary& lib, const Tensor& logits, const Ten
   a.finished = finished.has_value() ? reinterpret_cast<const uint8_t*>(finished->const_data_ptr<bool>()) : nullptr;
   a.end_token = end_token;
   a.out_scores = out.mutable_data_ptr<float>(); a.out_rows = parents.mutable_data_ptr<int32_t>(); a.out_tokens = tokens.mutable_data_ptr<int32_t>();
+  a.workspace_bytes = lib.select_bytes(&a);
+  Tensor work = empty({(int64_t)a.workspace_bytes}, at::kByte, logits);
+  a.workspace = work.mutable_data_ptr();
   check(lib, lib.select(&a, current_stream(logits)), "chill_beam_select");
   return py::make_tuple(out, parents, tokens);
 }
@@ -320,12 +324,13 @@ bool cache_copy(const DecodeLibrary& lib, const Tensor& kc, const Tensor& vc, co
 
 void bind_decode(py::module_& m) {
   py::class_<DecodeLibrary, std::shared_ptr<DecodeLibrary>>(m, "DecodeLibrary").def(py::init([](const std::vector<uint64_t>& fn) {
-    if (fn.size() != 10) throw py::value_error("ten entry points");
+    if (fn.size() != 11) throw py::value_error("eleven entry points");
     return std::make_shared<DecodeLibrary>(DecodeLibrary{pointer<decltype(&chill_rotate)>(fn[0]), pointer<decltype(&chill_rotate_append)>(fn[1]),
-                           pointer<decltype(&chill_beam_select)>(fn[2]), pointer<decltype(&chill_pages_fork)>(fn[3]),
-                           pointer<decltype(&chill_pages_trim_shared)>(fn[4]), pointer<decltype(&chill_pages_compact)>(fn[5]),
-                           pointer<decltype(&chill_share_workspace_bytes)>(fn[6]), pointer<decltype(&chill_cache_copy)>(fn[7]),
-                           pointer<decltype(&chill_status_string)>(fn[8]), pointer<decltype(&chill_decode_last_cuda_error)>(fn[9])});
+                           pointer<decltype(&chill_beam_select)>(fn[2]), pointer<decltype(&chill_select_workspace_bytes)>(fn[3]),
+                           pointer<decltype(&chill_pages_fork)>(fn[4]), pointer<decltype(&chill_pages_trim_shared)>(fn[5]),
+                           pointer<decltype(&chill_pages_compact)>(fn[6]), pointer<decltype(&chill_share_workspace_bytes)>(fn[7]),
+                           pointer<decltype(&chill_cache_copy)>(fn[8]), pointer<decltype(&chill_status_string)>(fn[9]),
+                           pointer<decltype(&chill_decode_last_cuda_error)>(fn[10])});
   }));
   m.def("rotate", &rotate);
   m.def("rotate_append", &rotate_append);

@@ -67,8 +67,11 @@ typedef struct chill_select_args {
   float* out_scores;       /* [G][M] */
   int32_t* out_rows;       /* [G][M], g * K + k */
   int32_t* out_tokens;     /* [G][M] */
+  void* workspace;         /* chill_select_workspace_bytes() bytes, 16-byte aligned; one for each call that can overlap */
+  size_t workspace_bytes;
 } chill_select_args;
 /* 1 <= K, M <= CHILL_SELECT_MAX, M <= K * V, G * K <= 65535. */
+size_t chill_select_workspace_bytes(const chill_select_args* a); /* from G, K, M, V and dtype alone */
 int chill_beam_select(const chill_select_args* a, void* stream);
 
 /* ------------------------------------------------------------------------------------------------------------------

@@ -24,7 +24,7 @@ def test_struct_sizes_match_header():
     from chill_attention import _decode_abi as abi
 
     assert ctypes.sizeof(abi.RotateArgs) == 40 + 24 + 24 + 16 + 64 + 16 + 64 + 8 + 32 + 16 + 64 + 8 + 8
-    assert ctypes.sizeof(abi.SelectArgs) == 16 + 8 * 9
+    assert ctypes.sizeof(abi.SelectArgs) == 16 + 8 * 11
     assert ctypes.sizeof(abi.ShareArgs) == 16 + 16 + 8 * 13 + 8
     assert ctypes.sizeof(abi.CopyArgs) == 24 + 16 + 80 + 32 + 8
 
@@ -91,8 +91,8 @@ def test_selection_refusals(lib):
     from chill_attention import _decode_abi as abi
 
     def call(**changes):
-        return lib.chill_beam_select(made(abi.SelectArgs, ("logits", "scores", "out_scores", "out_rows", "out_tokens"),
-                                          **{**dict(G=2, K=4, M=4, dtype=0, V=100, row_stride=100), **changes}), None)
+        return lib.chill_beam_select(made(abi.SelectArgs, ("logits", "scores", "out_scores", "out_rows", "out_tokens", "workspace"),
+                                          **{**dict(G=2, K=4, M=4, dtype=0, V=100, row_stride=100, workspace_bytes=1 << 20), **changes}), None)
 
     assert lib.chill_beam_select(None, None) == -1
     for name in ("G", "K", "M", "V"):
@@ -100,8 +100,9 @@ def test_selection_refusals(lib):
     assert call(dtype=3) == -2
     assert call(K=65) == call(M=65) == call(V=2 ** 30 + 1) == call(G=20000) == -4
     assert call(K=1, V=3) == -1  # fewer candidates than are asked for
-    for name in ("logits", "scores", "out_scores", "out_rows", "out_tokens"):
+    for name in ("logits", "scores", "out_scores", "out_rows", "out_tokens", "workspace"):
         assert call(**{name: None}) == -1
+    assert call(workspace=4104) == call(workspace_bytes=100) == -1
     assert call(finished=4096, end_token=100) == call(finished=4096, end_token=-1) == -1
 
 

@@ -194,9 +194,9 @@ def test_rotate_append(ca, dtype, H, Hkv, N, D, page, channels, axes, interleave
 
 # ------------------------------------------------------------------------------------------------------------ selection
 def score_bound(x, c):
-    """x: a row of logits, c: scores, in 64 bits.  A term of the sum: difference to the maximum and its product with log2 e (2 u of d each way), exponential 2^-22, a vector's sum
-    of up to 8 terms 7 u, rescaled up to 16 times at 2^-22 each; d counts by its weight, E[d] <= log V + spread, taken as 40.  The result is rounded to fp32."""
-    return 17 * 2.0 ** -22 + 7 * U + 2 * 40 * U + U * c.abs()
+    """x: a row of logits, c: scores, in 64 bits.  A term of the sum: difference to the maximum and its product with log2 e (2 u of d each way), exponential 2^-22, a thread's
+    32 terms in two sums 17 u, rescaled up to 16 times at 2^-22 each; d counts by its weight, E[d] <= log V + spread, taken as 40.  The result is rounded to fp32."""
+    return 17 * 2.0 ** -22 + 17 * U + 2 * 40 * U + U * c.abs()
 
 
 def check_select(out, logits, scores, count, finished=None, end=0):
@@ -297,6 +297,34 @@ def test_select_extremes(ca, dtype):
         out = ca.chill_beam_select(x[[7, 7]].cuda(), scores.cuda(), 5, finished=over.cuda(), end_token=3)
         want, parents, tokens = orc.select(x[[7, 7]], scores, 5, over, 3)
         assert torch.equal(out.parents.cpu().long(), parents) and torch.equal(out.tokens.cpu().long(), tokens)
+
+
+@pytest.mark.parametrize("dtype,V,M", [(torch.float32, 40000, 64), (torch.bfloat16, 70001, 5), (torch.float16, 33000, 33)])
+def test_select_of_rows_in_order(ca, dtype, V, M):
+    """Ascending, descending and constant rows and steps: what is kept runs over again and again."""
+    up = torch.arange(V, dtype=torch.float64) / V * 8 - 4
+    rows = torch.stack([up, up.flip(0), torch.zeros(V, dtype=torch.float64), (up * 3).floor(), torch.where(torch.arange(V) % 7 == 0, up, -math.inf)]).to(dtype)
+    for beams in ([0], [1], [2], [3], [4], [0, 1, 2, 3, 4]):
+        scores = torch.zeros(1, len(beams))
+        out = ca.chill_beam_select(rows[beams].cuda(), scores.cuda(), M)
+        want, parents, tokens = orc.select(rows[beams], scores, M)
+        if len(beams) == 1:
+            assert torch.equal(out.tokens.cpu().long(), tokens)
+        check_select(out, rows[beams], scores, M)
+
+
+@pytest.mark.parametrize("dtype,V", [(torch.bfloat16, 140000), (torch.float32, 70001)])
+def test_select_of_many_long_rows(ca, dtype, V):
+    """More rows than the GPU has room for at once: a row is one segment, and that of several rounds."""
+    g = torch.Generator(device="cuda").manual_seed(V)
+    G, K, M = 11, 60, 7
+    logits = (torch.randn(G * K, V, generator=g, device="cuda") * 2.5).to(dtype)
+    logits[3 * K + 1] = logits[3 * K + 1].sort().values
+    scores = -5 * torch.rand(G, K, generator=g, device="cuda")
+    out = ca.chill_beam_select(logits, scores, M)
+    for group in (0, 3, 10):
+        part = ca.ChillBeams(out.scores[group:group + 1], out.parents[group:group + 1] - group * K, out.tokens[group:group + 1])
+        check_select(part, logits[group * K:(group + 1) * K], scores[group:group + 1], M)
 
 
 def test_select_of_strided_rows(ca):
