@@ -11,6 +11,7 @@ namespace cg = cooperative_groups;
 constexpr int kPageThreads = 1024;
 constexpr int kPageWarps = kPageThreads / 32;
 constexpr int kPageCtas = 8;
+constexpr int kMaxCtas = 16;
 constexpr int kForkRequests = 8192;
 
 struct ShareP {
@@ -24,7 +25,8 @@ struct ShareP {
   int* out_lens;
   int *source, *target, *rows, *count;
   int orders;
-  int *before, *state;  // workspace: fork: the tables as they were, [B][2] what rows held; compact: [num_pages] where a page goes
+  int *before, *bits, *state;  // workspace: the tables as they were and a bit for every entry, where they are too large for shared memory; fork: [B][2] what rows held; compact:
+                               // [num_pages] where a page goes
 };
 
 // Exclusive prefix sum of one value per thread; `total` is the block's sum.
@@ -40,7 +42,7 @@ __device__ __forceinline__ int block_scan(int v, int& total) {
   __syncthreads();  // the sums of the call before this one have been read
   if (lane == 31) sums[warp] = x;
   __syncthreads();
-  const int s = sums[lane];
+  const int s = lane < (int)(blockDim.x >> 5) ? sums[lane] : 0;
   int y = s;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
@@ -61,180 +63,228 @@ __device__ __forceinline__ int block_scan(int v, int& total) {
 // that nobody holds the page, and then every row that let go of it writes the number of its entry, the first (lowest) one stays.  The word of
 // shared[] takes both: -1 for a page without holders, -2 - (entries - 1 - entry) for the claims, of which the minimum is the lowest entry.
 //
-// Latency is all there is: one cluster, whose barriers separate the steps.  Every CTA has a share of the rows, a warp goes over a row.
-struct Row {
-  int held, len, whole, rest, page;  // page: of the begun block, -1 where there is none
-};
+// Latency is all there is: one cluster, whose barriers separate the steps, and few trips to memory one after the other.  Every CTA has a share of the rows and keeps them as they
+// were in shared memory, where children in other CTAs find them too (in the workspace where they are too large: kInside false); what goes back is noted there in bits.
+// Rows that a warp has at a time, 32 blocks of each: what neighbouring rows share (the beams of a request, nearly everything) is counted in registers before it is
+// counted in memory.
+constexpr int kRows = 8;
 
-__device__ __forceinline__ Row row_of(const ShareP& p, int r) {
-  Row x;
-  x.held = imin(imax(p.held[r], 0), p.width);
-  x.len = (int)imin((long long)clamp_len(p.lens[r]) < (long long)x.held * p.page ? clamp_len(p.lens[r]) : x.held * p.page, kMaxLen);
-  x.whole = x.len / p.page;
-  x.rest = x.len - x.whole * p.page;
-  x.page = -1;
-  if (x.rest > 0) {
-    const int q = p.table[r * p.table_sb + x.whole];
-    if (q >= 0 && q < p.num_pages) x.page = q;
-  }
-  return x;
-}
-
-// What children need to know of a row, in two words: its tokens, and its begun page: stays with the first child (page), goes (-2 - page), none (-1).
-// Tokens of a begun block without a page are not there.
-__device__ __forceinline__ int2 summary_of(const ShareP& p, const Row& x) {
-  if (x.page < 0) return make_int2(x.whole * p.page, -1);
-  return make_int2(x.len, p.shared[x.page] == 0 ? x.page : -2 - x.page);
-}
-
-// Blocks of a row that a lane has at a time: as many loads on their way.
-constexpr int kUnroll = 8;
-
-template <bool kTrim>
+template <bool kTrim, bool kInside>
 __global__ void __launch_bounds__(kPageThreads) share_kernel(const __grid_constant__ ShareP p) {
   extern __shared__ int dynamic[];
+  __shared__ int own_total;
   cg::cluster_group cluster = cg::this_cluster();
   const int ctas = (int)cluster.num_blocks(), cta = (int)cluster.block_rank();
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int per = (p.B + ctas - 1) / ctas, r0 = imin(cta * per, p.B), r1 = imin(r0 + per, p.B);
-  int* const number = dynamic;                 // [per]: of this CTA's rows, see below
-  int* const children = dynamic + per;         // [B], fork
-  int* const first = dynamic + per + p.B;      // [B], fork: the first child
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, threads = (int)blockDim.x, warps = threads >> 5;
+  const int per = ((p.B + ctas - 1) / ctas + kRows - 1) / kRows * kRows, r0 = imin(cta * per, p.B), r1 = imin(r0 + per, p.B);
+  const int words = (p.width + 31) / 32;  // of 32 blocks
+  // Of this CTA's rows as they were: blocks they hold, those of the run that they let go of begin where, how many go back to the stack (later: before them)
+  int *const held = dynamic, *const begin = held + per, *const number = begin + per;
+  // fork: blocks that a row's children share; of a row as it will be: the parent (-1: none), its whole blocks, all blocks, the page of the last one
+  int *const whole = number + per, *const parent = whole + per, *const taken_over = parent + per, *const now = taken_over + per, *const begun = now + per;
+  int *const children = begun + per, *const first = children + p.B;  // fork, [B]: of every row, how many and the first
+  int* const rows_inside = kTrim ? whole : first + p.B;              // [per][width]
+  int* const back = kInside ? rows_inside + (size_t)per * p.width : p.bits + (size_t)r0 * words;  // [per][words]: bits of the blocks whose pages go back
   const long long entries = (long long)p.B * p.width;
   int2* const summary = reinterpret_cast<int2*>(p.state);
-  int* const totals = p.state + (kTrim ? 0 : 2 * p.B);
   const int n_free = imin(imax(*p.n_free, 0), p.num_pages);
-  // Warps go over pieces of rows: 32 * kUnroll blocks
-  const int pieces = (p.width + 32 * kUnroll - 1) / (32 * kUnroll);
   auto is_page = [&](int q) { return q >= 0 && q < p.num_pages; };
-  auto held_of = [&](int r) { return imin(imax(p.held[r], 0), p.width); };
-  auto table_before = [&](int r) { return kTrim ? p.table + r * p.table_sb : p.before + (long long)r * p.width; };
+  auto before = [&](int r) -> int* {  // of this CTA's rows
+    return kInside ? rows_inside + (size_t)(r - r0) * p.width : (kTrim ? p.table + r * p.table_sb : p.before + (long long)r * p.width);
+  };
+  // A warp has a block of kRows rows and some of their words of 32 blocks, every `stride`-th from `word` on
+  const int row_blocks = (r1 - r0 + kRows - 1) / kRows, stride = row_blocks > 0 ? imax(warps / row_blocks, 1) : 1;
+  auto sweep = [&](auto body) {
+    for (int unit = warp; unit < row_blocks * stride; unit += warps) body(r0 + unit % row_blocks * kRows, unit / row_blocks);
+  };
 
+  // The rows as they are
+  if constexpr (!kTrim || kInside) {
+    sweep([&](int rows, int word) {
+      for (int j = word * 32 + lane; j < p.width; j += stride * 32) {
+        int q[kRows];
+#pragma unroll
+        for (int u = 0; u < kRows; ++u) q[u] = rows + u < r1 ? p.table[(rows + u) * p.table_sb + j] : -1;
+#pragma unroll
+        for (int u = 0; u < kRows; ++u)
+          if (rows + u < r1) before(rows + u)[j] = q[u];
+      }
+    });
+  }
   if constexpr (!kTrim) {
-    for (int r = threadIdx.x; r < p.B; r += kPageThreads) {
+    for (int r = threadIdx.x; r < p.B; r += threads) {
       children[r] = 0;
       first[r] = p.B;
     }
-    for (int r = r0 + threadIdx.x; r < r1; r += kPageThreads) summary[r] = summary_of(p, row_of(p, r));
-    for (int item = warp; item < (r1 - r0) * pieces; item += kPageWarps) {
-      const int r = r0 + item / pieces, j0 = item % pieces * 32 * kUnroll + lane, held = held_of(r);
-      int q[kUnroll];
-#pragma unroll
-      for (int u = 0; u < kUnroll; ++u) q[u] = j0 + 32 * u < held ? p.table[r * p.table_sb + j0 + 32 * u] : -1;
-#pragma unroll
-      for (int u = 0; u < kUnroll; ++u)
-        if (j0 + 32 * u < held) p.before[(long long)r * p.width + j0 + 32 * u] = q[u];
+  }
+  for (int r = r0 + threadIdx.x; r < r1; r += threads) {
+    const int i = r - r0, len = clamp_len(p.lens[r]);
+    held[i] = imin(imax(p.held[r], 0), p.width);
+    if constexpr (kTrim) {
+      begin[i] = imin((len + p.page - 1) / p.page, held[i]);
+    } else {
+      begin[i] = imin(len, held[i] * p.page);  // for now: its tokens
     }
-    __syncthreads();
-    for (int b = threadIdx.x; b < p.B; b += kPageThreads) {
+    number[i] = 0;
+  }
+  __syncthreads();
+  if constexpr (!kTrim) {
+    for (int b = threadIdx.x; b < p.B; b += threads) {
       const int r = p.parents[b];
       if (r < 0 || r >= p.B) continue;
       atomicAdd(&children[r], 1);
       atomicMin(&first[r], b);
     }
-    cluster.sync();  // what rows held is written down
-  }
-
-  // Row r: `whole` blocks that its children share, the run [begin, held) that it lets go of.
-  auto run_of = [&](int r, int& whole, int& begin, int& held) {
-    held = held_of(r);
-    if constexpr (kTrim) {
-      whole = 0;
-      begin = imin((clamp_len(p.lens[r]) + p.page - 1) / p.page, held);
-    } else {
-      const int2 s = summary[r];
-      const bool begun = s.x % p.page != 0;
-      whole = children[r] > 0 ? s.x / p.page : 0;
-      begin = children[r] > 0 ? whole + (begun && s.y >= 0 ? 1 : 0) : 0;
+    // What children need to know of a row, in two words: its tokens, and its begun page: stays with the first child (page), goes (-2 - page), none (-1).  Tokens of
+    // a begun block without a page are not there.
+    for (int r = r0 + threadIdx.x; r < r1; r += threads) {
+      const int i = r - r0, len = begin[i], full = len / p.page;
+      int2 s = make_int2(full * p.page, -1);
+      if (len != s.x) {
+        const int q = before(r)[full];
+        if (is_page(q)) s = make_int2(len, p.shared[q] == 0 ? q : -2 - q);
+      }
+      summary[r] = s;
     }
-  };
+    cluster.sync();  // what rows held is written down
+    for (int r = r0 + threadIdx.x; r < r1; r += threads) {
+      const int i = r - r0;
+      const int2 s = summary[r];
+      whole[i] = children[r] > 0 ? s.x / p.page : 0;
+      begin[i] = children[r] > 0 && s.x % p.page != 0 && s.y >= 0 ? whole[i] + 1 : whole[i];
+    }
+    __syncthreads();
+  }
 
   // Counts of holders
-  for (int item = warp; item < (r1 - r0) * pieces; item += kPageWarps) {
-    const int r = r0 + item / pieces, j0 = item % pieces * 32 * kUnroll + lane;
-    int whole, begin, held;
-    run_of(r, whole, begin, held);
-    const int more = kTrim ? 0 : children[r] - 1;
-    if (more <= 0) whole = 0;
-    int q[kUnroll];
+  sweep([&](int rows, int word) {
+    // of the rows: children beyond one and for how many blocks they count, the run
+    int more[kRows], until[kRows], lo[kRows], hi[kRows], top = 0;
 #pragma unroll
-    for (int u = 0; u < kUnroll; ++u) {
-      const int j = j0 + 32 * u;
-      q[u] = j < whole || (j >= begin && j < held) ? table_before(r)[j] : -1;
+    for (int u = 0; u < kRows; ++u) {
+      const int i = rows + u - r0;
+      const bool is_row = rows + u < r1;
+      more[u] = !kTrim && is_row ? children[rows + u] - 1 : 0;
+      until[u] = more[u] > 0 ? whole[i] : 0;
+      lo[u] = is_row ? begin[i] : 0;
+      hi[u] = is_row ? held[i] : 0;
+      top = imax(top, imax(until[u], lo[u] < hi[u] ? hi[u] : 0));
     }
+    for (int j = word * 32 + lane; j < top; j += stride * 32) {
+      int page = -1, sum = 0;
 #pragma unroll
-    for (int u = 0; u < kUnroll; ++u)
-      if (is_page(q[u])) atomicAdd(&p.shared[q[u]], j0 + 32 * u < whole ? more : -1);
-  }
+      for (int u = 0; u < kRows; ++u) {
+        const bool goes = j >= lo[u] && j < hi[u];
+        if (j >= until[u] && !goes) continue;
+        const int q = before(rows + u)[j];
+        if (!is_page(q)) continue;
+        if (q != page) {
+          if (sum != 0) atomicAdd(&p.shared[page], sum);
+          page = q;
+          sum = 0;
+        }
+        sum += goes ? -1 : more[u];
+      }
+      if (sum != 0) atomicAdd(&p.shared[page], sum);
+    }
+  });
   // New pages: for every child but the first, or for all where the page is somebody else's too; requests in order
   int taken = 0;
-  auto parent_of = [&](int b) {
-    const int r = p.parents[b];
-    return r >= 0 && r < p.B ? r : -1;
-  };
-  auto wants = [&](int b, int r) {
-    if (r < 0) return false;
-    const int2 s = summary[r];
-    return s.x % p.page != 0 && !(s.y >= 0 && first[r] == b);
-  };
   if constexpr (!kTrim) {
-    for (int base = 0; base < p.B; base += kPageThreads) {
+    for (int base = 0; base < p.B; base += threads) {
       const int b = base + (int)threadIdx.x;
-      int total;
-      const int x = block_scan(b < p.B && wants(b, parent_of(b)) ? 1 : 0, total);
-      if (b >= r0 && b < r1) number[b - r0] = taken + x;  // pages that the rows before b want
+      int r = b < p.B ? p.parents[b] : -1, rest = 0, total;
+      if (r >= p.B) r = -1;
+      int2 s = make_int2(0, -1);
+      if (r >= 0) {
+        s = summary[r];
+        rest = s.x % p.page;
+      }
+      const bool asks = rest != 0 && !(s.y >= 0 && first[r] == b);
+      const int off = taken + block_scan(asks ? 1 : 0, total);  // pages that the rows before b want
       taken += total;
+      if (b < r0 || b >= r1) continue;
+      // row b as it will be
+      const bool gets = asks && off < n_free, here = rest != 0 && (!asks || gets);
+      const int blocks = s.x / p.page, page = gets ? p.free_pages[n_free - 1 - off] : s.y;
+      parent[b - r0] = r;
+      taken_over[b - r0] = blocks;
+      now[b - r0] = blocks + (here ? 1 : 0);
+      begun[b - r0] = page;
+      p.out_lens[b] = here ? s.x : blocks * p.page;
+      if (gets) {
+        p.source[off] = s.y >= 0 ? s.y : -2 - s.y;
+        p.target[off] = page;
+        p.rows[off] = rest;
+      }
     }
   }
   cluster.sync();  // the counts are complete
 
-  // Claims to the pages that nobody holds
+  // Claims to the pages that nobody holds.  `back` notes for whose
   auto claim_of = [&](int r, int j) { return (int)(-1 - entries + ((long long)r * p.width + j)); };
-  for (int item = warp; item < (r1 - r0) * pieces; item += kPageWarps) {
-    const int r = r0 + item / pieces, j0 = item % pieces * 32 * kUnroll + lane;
-    int whole, begin, held;
-    run_of(r, whole, begin, held);
-    int q[kUnroll], left[kUnroll];
+  sweep([&](int rows, int first_word) {
+    int lo[kRows], hi[kRows], bottom = p.width, top = 0;
 #pragma unroll
-    for (int u = 0; u < kUnroll; ++u) q[u] = j0 + 32 * u >= begin && j0 + 32 * u < held ? table_before(r)[j0 + 32 * u] : -1;
+    for (int u = 0; u < kRows; ++u) {
+      const int i = rows + u - r0;
+      lo[u] = rows + u < r1 ? begin[i] : 0;
+      hi[u] = rows + u < r1 ? held[i] : 0;
+      if (lo[u] >= hi[u]) continue;
+      bottom = imin(bottom, lo[u]);
+      top = imax(top, hi[u]);
+    }
+    for (int word = first_word; word < words; word += stride) {
+      const int j = word * 32 + lane;
+      const bool any = word * 32 < top && word * 32 + 32 > bottom;
+      int q[kRows], left[kRows];
 #pragma unroll
-    for (int u = 0; u < kUnroll; ++u) left[u] = is_page(q[u]) ? __ldcg(&p.shared[q[u]]) : 0;
+      for (int u = 0; u < kRows; ++u) q[u] = any && j >= lo[u] && j < hi[u] ? before(rows + u)[j] : -1;
 #pragma unroll
-    for (int u = 0; u < kUnroll; ++u)
-      if (left[u] < 0) atomicMin(&p.shared[q[u]], claim_of(r, j0 + 32 * u));
-  }
+      for (int u = 0; u < kRows; ++u) left[u] = is_page(q[u]) && (u == 0 || q[u] != q[u - 1]) ? __ldcg(&p.shared[q[u]]) : 0;  // of equal ones the first is the lowest
+#pragma unroll
+      for (int u = 0; u < kRows; ++u) {
+        if (left[u] < 0) atomicMin(&p.shared[q[u]], claim_of(rows + u, j));
+        const unsigned who = any ? __ballot_sync(0xffffffffu, left[u] < 0) : 0;
+        if (lane == 0 && rows + u < r1) back[(size_t)(rows + u - r0) * words + word] = (int)who;
+      }
+    }
+  });
   // The new tables
   if constexpr (!kTrim) {
     const int got = imin(taken, n_free);
-    for (int item = warp; item < (r1 - r0) * pieces; item += kPageWarps) {
-      const int b = r0 + item / pieces, j0 = item % pieces * 32 * kUnroll + lane, held = held_of(b), r = parent_of(b);
-      const int2 s = r >= 0 ? summary[r] : make_int2(0, -1);
-      const int whole = s.x / p.page, rest = s.x - whole * p.page, off = number[b - r0];
-      const bool asks = wants(b, r), here = rest > 0 && (!asks || off < got);
-      const int begun = asks && here ? p.free_pages[n_free - 1 - off] : s.y, now = whole + (here ? 1 : 0);
-      int* to = p.table + b * p.table_sb;
-      int q[kUnroll];
+    sweep([&](int rows, int word) {
+      const int* from[kRows];  // the parent's row, nullptr: its blocks stay as they are
+      int until[kRows], end[kRows], hi[kRows], last[kRows], top = 0;
 #pragma unroll
-      for (int u = 0; u < kUnroll; ++u) q[u] = j0 + 32 * u < whole && r != b ? p.before[(long long)r * p.width + j0 + 32 * u] : begun;
+      for (int u = 0; u < kRows; ++u) {
+        const int i = rows + u - r0;
+        const bool is_row = rows + u < r1;
+        const int r = is_row ? parent[i] : -1, owner = r >= 0 ? r / per : 0;
+        from[u] = nullptr;
+        if (r >= 0 && r != rows + u)
+          from[u] = kInside ? cluster.map_shared_rank(rows_inside, owner) + (size_t)(r - owner * per) * p.width : p.before + (long long)r * p.width;
+        until[u] = is_row ? taken_over[i] : 0;
+        end[u] = is_row ? now[i] : 0;
+        hi[u] = is_row ? held[i] : 0;
+        last[u] = is_row ? begun[i] : 0;
+        top = imax(top, imax(end[u], hi[u]));
+      }
+      for (int j = word * 32 + lane; j < top; j += stride * 32) {
+        int q[kRows];
 #pragma unroll
-      for (int u = 0; u < kUnroll; ++u) {
-        const int j = j0 + 32 * u;
-        if (j < now) {
-          if (j >= whole || r != b) to[j] = q[u];
-        } else if (j < held) {
-          to[j] = -1;
+        for (int u = 0; u < kRows; ++u) {
+          q[u] = -2;  // stays as it is
+          if (j < until[u]) q[u] = from[u] != nullptr ? from[u][j] : -2;
+          else if (j < end[u]) q[u] = last[u];
+          else if (j < hi[u]) q[u] = -1;
         }
+#pragma unroll
+        for (int u = 0; u < kRows; ++u)
+          if (q[u] != -2) p.table[(rows + u) * p.table_sb + j] = q[u];
       }
-      if (item % pieces == 0 && lane == 0) {
-        p.out_lens[b] = here ? s.x : whole * p.page;
-        if (asks && here) {
-          p.source[off] = -2 - (s.y >= 0 ? -2 - s.y : s.y);
-          p.target[off] = begun;
-          p.rows[off] = rest;
-        }
-      }
-    }
-    for (int i = got + cta * kPageThreads + (int)threadIdx.x; i < p.B; i += ctas * kPageThreads) {
+    });
+    for (int i = got + cta * threads + (int)threadIdx.x; i < p.B; i += ctas * threads) {
       p.source[i] = p.target[i] = -1;
       p.rows[i] = 0;
     }
@@ -243,65 +293,64 @@ __global__ void __launch_bounds__(kPageThreads) share_kernel(const __grid_consta
       *p.missing = imax(taken - n_free, 0);
     }
   }
-  cluster.sync();  // the lowest claims are there; what was taken from the stack has been read
+  cluster.sync();  // the lowest claims are there; what was taken from the stack, and other CTAs' rows, have been read
 
-  // How many pages every row puts on the stack
-  auto goes_back = [&](int r, int j, int q) { return is_page(q) && __ldcg(&p.shared[q]) == claim_of(r, j); };
-  for (int r = r0 + warp; r < r1; r += kPageWarps) {
-    int whole, begin, held, n = 0;
-    run_of(r, whole, begin, held);
-    for (int j = begin + lane; j < held; j += 32) n += goes_back(r, j, table_before(r)[j]) ? 1 : 0;
-    n = __reduce_add_sync(0xffffffffu, n);
-    __syncwarp();
-    if (lane == 0) number[r - r0] = n;
+  // How many pages every row puts on the stack: those of which its claim is the lowest
+  for (int item = warp; item < (r1 - r0) * words; item += warps) {
+    const unsigned claims = (unsigned)back[item];
+    if (claims == 0) continue;
+    const int i = item / words, j = item % words * 32 + lane;
+    const bool mine = (claims >> lane & 1) && __ldcg(&p.shared[before(r0 + i)[j]]) == claim_of(r0 + i, j);
+    const unsigned who = __ballot_sync(0xffffffffu, mine);
+    if (lane == 0) {
+      back[item] = (int)who;
+      if (who != 0) atomicAdd(&number[i], __popc(who));
+    }
   }
   __syncthreads();
   int own = 0;
-  for (int base = 0; base < r1 - r0; base += kPageThreads) {
+  for (int base = 0; base < r1 - r0; base += threads) {
     const int i = base + (int)threadIdx.x;
     int total;
     const int n = i < r1 - r0 ? number[i] : 0, x = block_scan(n, total);
-    if (i < r1 - r0) number[i] = n == 0 ? -1 : own + x;  // pages of this CTA's rows before it, -1: none of its own
+    if (i < r1 - r0) number[i] = n == 0 ? -1 : own + x;  // pages of this CTA's rows before it; -1: it has none itself
     own += total;
   }
-  if (threadIdx.x == 0) totals[cta] = own;
+  if (threadIdx.x == 0) own_total = own;
   cluster.sync();
   int earlier = 0, all = 0;
   for (int c = 0; c < ctas; ++c) {
-    const int n = __ldcg(&totals[c]);
+    const int n = *cluster.map_shared_rank(&own_total, c);
     if (c < cta) earlier += n;
     all += n;
   }
   const int left = n_free - imin(taken, n_free);
-  for (int r = r0 + warp; r < r1; r += kPageWarps) {
-    int whole, begin, held;
-    run_of(r, whole, begin, held);
-    int at = number[r - r0];
-    if (at < 0 && !kTrim) begin = held;
-    at += earlier;
-    const int* old = table_before(r);
-    for (int j0 = begin; j0 < held; j0 += 32) {
-      const int j = j0 + lane, q = j < held ? old[j] : -1;
-      const bool back = goes_back(r, j, q);
-      const unsigned who = __ballot_sync(0xffffffffu, back);
-      if (back) {
-        const long long to = (long long)left + all - 1 - (at + __popc(who & ((1u << lane) - 1)));
+  for (int r = r0 + warp; r < r1; r += warps) {
+    const int i = r - r0;
+    for (int w0 = 0, at = number[i]; number[i] >= 0 && w0 < words; w0 += 32) {
+      unsigned who = w0 + lane < words ? (unsigned)back[(size_t)i * words + w0 + lane] : 0;
+      int n = __popc(who), x = n;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int y = __shfl_up_sync(0xffffffffu, x, o);
+        if (lane >= o) x += y;
+      }
+      for (int rank = at + x - n; who != 0; who &= who - 1, ++rank) {
+        const int q = before(r)[(w0 + lane) * 32 + __ffs(who) - 1];
+        const long long to = (long long)left + all - 1 - (earlier + rank);
         if (to >= 0 && to < p.num_pages) p.free_pages[to] = q;  // `held` can be nonsense
         p.shared[q] = 0;
       }
-      at += __popc(who);
-      if (kTrim && j < held) p.table[r * p.table_sb + j] = -1;
+      at += __shfl_sync(0xffffffffu, x, 31);
+    }
+    if (kTrim) {
+      __syncwarp();
+      for (int j = begin[i] + lane; j < held[i]; j += 32) p.table[r * p.table_sb + j] = -1;
     }
   }
-  __syncthreads();  // `held` has been read
-  for (int b = r0 + threadIdx.x; b < r1; b += kPageThreads) {
-    if constexpr (kTrim) {
-      p.held[b] = imin(held_of(b), (clamp_len(p.lens[b]) + p.page - 1) / p.page);
-    } else {
-      p.held[b] = (p.out_lens[b] + p.page - 1) / p.page;
-    }
-  }
+  for (int b = r0 + threadIdx.x; b < r1; b += threads) p.held[b] = kTrim ? begin[b - r0] : now[b - r0];
   if (cta == 0 && threadIdx.x == 0) *p.n_free = imin(all, p.num_pages - left) + left;
+  if (ctas > 1) cluster.sync();  // own_total has been read
 }
 
 // ------------------------------------------------------------------------------------------------------------ compact
@@ -374,6 +423,7 @@ __global__ void __launch_bounds__(kPageThreads) compact_kernel(const __grid_cons
     *p.n_free = all;
   }
   cluster.sync();
+  constexpr int kUnroll = 8;
   const int warp = thread >> 5, warps = threads >> 5, lane = threadIdx.x & 31, pieces = (p.width + 32 * kUnroll - 1) / (32 * kUnroll);
   for (long long item = warp; item < (long long)p.B * pieces; item += warps) {
     const int b = (int)(item / pieces), j0 = (int)(item % pieces) * 32 * kUnroll + lane, held = imin(imax(p.held[b], 0), p.width);
@@ -391,7 +441,7 @@ __global__ void __launch_bounds__(kPageThreads) compact_kernel(const __grid_cons
 }
 
 static size_t workspace_of(const chill_share_args& a) {
-  const size_t ints = (size_t)a.B * a.table_width + 2 * (size_t)a.B + 2 + (size_t)a.num_pages + 64;
+  const size_t ints = (size_t)a.B * a.table_width + (size_t)a.B * ((a.table_width + 31) / 32) + 2 * (size_t)a.B + (size_t)a.num_pages + 64;
   return (ints * 4 + 255) / 256 * 256;
 }
 
@@ -414,20 +464,25 @@ static ShareP share_params(const chill_share_args& a) {
   p.lens = a.lens; p.missing = a.missing; p.parents = a.parents; p.out_lens = a.out_lens;
   p.source = a.source; p.target = a.target; p.rows = a.rows; p.count = a.count;
   p.state = (int*)a.workspace;
-  p.before = p.state + 2 * ((size_t)a.B + 1) + 62;
+  p.before = p.state + 2 * (size_t)a.B;  // fork and trim; compact has the whole of it
+  p.bits = p.before + (size_t)a.B * a.table_width;
   return p;
 }
 
 template <class F>
-static int launch_cluster(F kernel, const ShareP& p, int ctas, size_t smem, cudaStream_t st, const char* what) {
+static int launch_cluster(F kernel, const ShareP& p, int ctas, int threads, size_t smem, cudaStream_t st, const char* what) {
   cudaLaunchConfig_t cfg{};
   cudaLaunchAttribute attr[1];
   if (smem > 48 * 1024) {
     const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
     if (e != cudaSuccess) return record_cuda_failure(e, what);
   }
+  if (ctas > 8) {
+    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+    if (e != cudaSuccess) return record_cuda_failure(e, what);
+  }
   cfg.gridDim = dim3((unsigned)ctas);
-  cfg.blockDim = dim3(kPageThreads);
+  cfg.blockDim = dim3((unsigned)threads);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = st;
   attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -441,16 +496,24 @@ static int launch_cluster(F kernel, const ShareP& p, int ctas, size_t smem, cuda
   return CHILL_OK;
 }
 
-// One CTA where a warp has a piece of a row each, a cluster for more.
-static int ctas_for(const ShareP& p) {
-  const long long pieces = (long long)p.B * ((p.width + 32 * kUnroll - 1) / (32 * kUnroll));
-  return pieces <= kPageWarps ? 1 : kPageCtas;
+// What a call has to look at: words of 32 blocks of kRows rows.  One CTA of 256 threads for little of it, a cluster of 8 or 16 for more.
+struct Shape {
+  int ctas, threads;
+};
+static Shape shape_for(const ShareP& p) {
+  const long long items = (long long)((p.B + kRows - 1) / kRows) * ((p.width + 31) / 32);
+  if (items <= 16) return {1, 256};
+  return {items <= 256 ? kPageCtas : kMaxCtas, kPageThreads};
 }
 
 template <bool kTrim>
 static int launch_share(const ShareP& p, cudaStream_t st) {
-  const int ctas = ctas_for(p), per = (p.B + ctas - 1) / ctas;
-  return launch_cluster(share_kernel<kTrim>, p, ctas, ((size_t)per + (kTrim ? 0 : 2 * (size_t)p.B)) * 4, st, kTrim ? "trim launch" : "fork launch");
+  const Shape s = shape_for(p);
+  const int per = ((p.B + s.ctas - 1) / s.ctas + kRows - 1) / kRows * kRows;
+  const size_t bytes = (kTrim ? 3 * (size_t)per : 8 * (size_t)per + 2 * (size_t)p.B) * 4, rows = (size_t)per * (p.width + (p.width + 31) / 32) * 4;
+  const char* what = kTrim ? "trim launch" : "fork launch";
+  if (bytes + rows <= 200 * 1024) return launch_cluster(share_kernel<kTrim, true>, p, s.ctas, s.threads, bytes + rows, st, what);
+  return launch_cluster(share_kernel<kTrim, false>, p, s.ctas, s.threads, bytes, st, what);
 }
 
 // ------------------------------------------------------------------------------------------------------------ copy
@@ -465,39 +528,49 @@ struct CopyP {
 };
 
 template <class V>
-__global__ void __launch_bounds__(256) copy_kernel(const __grid_constant__ CopyP p) {
+__device__ __forceinline__ V load_once(const char* p) {
+  if constexpr (sizeof(V) == 16) return __ldcs(reinterpret_cast<const V*>(p));
+  else return *reinterpret_cast<const V*>(p);
+}
+template <class V>
+__device__ __forceinline__ void store_once(char* p, const V& v) {
+  if constexpr (sizeof(V) == 16) __stcs(reinterpret_cast<V*>(p), v);
+  else *reinterpret_cast<V*>(p) = v;
+}
+
+constexpr int kCopyThreads = 256, kCopyEach = 4;
+
+template <class V>
+__global__ void __launch_bounds__(kCopyThreads) copy_kernel(const __grid_constant__ CopyP p) {
+  constexpr int kChunk = kCopyThreads * kCopyEach;  // vectors that a block moves at a time, of one page, layer and tensor
   const int count = imin(imax(*p.count, 0), p.orders);
-  const long long per_head = (long long)p.page * p.per_row;               // vectors of a kv head's part of a page
-  const long long chunks = (per_head + 1023) / 1024;                      // a block moves 1024 of them
-  const long long items = (long long)count * p.layers * p.Hkv * chunks * (p.both ? 2 : 1);
+  const long long chunks = ((long long)p.Hkv * p.page * p.per_row + kChunk - 1) / kChunk, items = (long long)count * p.layers * chunks * (p.both ? 2 : 1);
   for (long long item = blockIdx.x; item < items; item += gridDim.x) {
-    long long at = item;
-    const int chunk = (int)(at % chunks);
-    at /= chunks;
-    const int h = (int)(at % p.Hkv);
-    at /= p.Hkv;
-    const int layer = (int)(at % p.layers);
-    at /= p.layers;
-    const int order = (int)(at % count);
-    const bool is_v = at >= count;
+    const long long at = item / chunks;
+    const int chunk = (int)(item - at * chunks), order = (int)(at / p.layers % count), layer = (int)(at % p.layers);
+    const bool is_v = at >= (long long)count * p.layers;
     const int from = p.source[order], to = p.target[order], rows = imin(imax(p.rows[order], 0), p.page);
     if (from < 0 || from >= p.num_pages || to < 0 || to >= p.num_pages || from == to) continue;
     const long long* st = is_v ? p.vs : p.ks;
-    char* base = (is_v ? p.v : p.k) + layer * st[0] + h * st[2];
+    char* base = (is_v ? p.v : p.k) + layer * st[0];
     const char* src = base + from * st[1];
     char* dst = base + to * st[1];
-    const int end = rows * p.per_row;
-    V x[4];
+    const unsigned per_head = (unsigned)rows * (unsigned)p.per_row;
+    const unsigned end = (unsigned)p.Hkv * per_head;
+    V x[kCopyEach];
+    long long offset[kCopyEach];
 #pragma unroll
-    for (int u = 0; u < 4; ++u) {
-      const int i = chunk * 1024 + u * 256 + (int)threadIdx.x, row = i / p.per_row, c = i - row * p.per_row;
-      if (i < end) x[u] = *reinterpret_cast<const V*>(src + row * st[3] + c * st[4]);
+    for (int u = 0; u < kCopyEach; ++u) {
+      const unsigned i = (unsigned)chunk * kChunk + u * kCopyThreads + threadIdx.x;
+      offset[u] = -1;
+      if (i >= end) continue;
+      const unsigned h = i / per_head, in_head = i - h * per_head, row = in_head / (unsigned)p.per_row, c = in_head - row * (unsigned)p.per_row;
+      offset[u] = h * st[2] + row * st[3] + c * st[4];
+      x[u] = load_once<V>(src + offset[u]);
     }
 #pragma unroll
-    for (int u = 0; u < 4; ++u) {
-      const int i = chunk * 1024 + u * 256 + (int)threadIdx.x, row = i / p.per_row, c = i - row * p.per_row;
-      if (i < end) *reinterpret_cast<V*>(dst + row * st[3] + c * st[4]) = x[u];
-    }
+    for (int u = 0; u < kCopyEach; ++u)
+      if (offset[u] >= 0) store_once(dst + offset[u], x[u]);
   }
 }
 
@@ -532,13 +605,15 @@ int chill_pages_compact(const chill_share_args* a, void* stream) {
   if (!a->source || !a->target || !a->rows || !a->count) return CHILL_E_INVALID;
   ShareP p = share_params(*a);
   p.orders = imax(a->num_pages / 2, 1);
-  return launch_cluster(compact_kernel, p, a->num_pages <= 2 * kPageThreads && ctas_for(p) == 1 ? 1 : kPageCtas, 0, (cudaStream_t)stream, "compact launch");
+  return launch_cluster(compact_kernel, p, a->num_pages <= 2 * kPageThreads && shape_for(p).ctas == 1 ? 1 : kPageCtas, kPageThreads, 0, (cudaStream_t)stream, "compact launch");
 }
 
 int chill_cache_copy(const chill_copy_args* a, void* stream) {
   if (a == nullptr || a->layers <= 0 || a->num_pages <= 0 || a->H_kv <= 0 || a->page_size <= 0 || a->D <= 0 || a->orders <= 0) return CHILL_E_INVALID;
   if (!known_dtype(a->dtype)) return CHILL_E_UNSUPPORTED;
-  if ((long long)a->num_pages * a->page_size > 0x7fffffffll || (long long)a->page_size * a->D > (1 << 30)) return CHILL_E_TOO_LARGE;
+  if ((long long)a->num_pages * a->page_size > 0x7fffffffll || (long long)a->page_size * a->D > (1 << 30) ||
+      (long long)a->page_size * a->D * a->H_kv > (1 << 30))
+    return CHILL_E_TOO_LARGE;
   if (!a->k_cache || !a->v_cache || !a->source || !a->target || !a->rows || !a->count) return CHILL_E_INVALID;
   const int es = elem_size(a->dtype);
   CopyP p{};
@@ -558,9 +633,9 @@ int chill_cache_copy(const chill_copy_args* a, void* stream) {
   }
   if (vec == 16) p.ks[4] = p.vs[4] = 16;
   const dim3 grid((unsigned)(8 * sm_count()));
-  if (vec == 16) copy_kernel<uint4><<<grid, 256, 0, (cudaStream_t)stream>>>(p);
-  else if (es == 4) copy_kernel<uint32_t><<<grid, 256, 0, (cudaStream_t)stream>>>(p);
-  else copy_kernel<uint16_t><<<grid, 256, 0, (cudaStream_t)stream>>>(p);
+  if (vec == 16) copy_kernel<uint4><<<grid, kCopyThreads, 0, (cudaStream_t)stream>>>(p);
+  else if (es == 4) copy_kernel<uint32_t><<<grid, kCopyThreads, 0, (cudaStream_t)stream>>>(p);
+  else copy_kernel<uint16_t><<<grid, kCopyThreads, 0, (cudaStream_t)stream>>>(p);
   const cudaError_t e = cudaGetLastError();
   if (e != cudaSuccess) return record_cuda_failure(e, "copy launch");
   count_launches(1);

@@ -8,6 +8,8 @@
 namespace chill {
 namespace decode {
 
+constexpr int kThreads = 128;
+
 struct RotateP {
   int B, L, H, Hkv, pairs, D, n_axes, inverse;
   int per_row;        // threads of a row: vectors of pairs, then vectors of channels that stay
@@ -34,11 +36,27 @@ __device__ __forceinline__ float2 turn(int position, float freq) {
   return cs;
 }
 
+// Nobody reads these again here: with plain loads and stores 106 us instead of 87 (q and k of (8, 16, 4096, 128) in bf16).
+template <class VecT>
+__device__ __forceinline__ VecT load_once(const char* p) {
+  if constexpr (sizeof(VecT) == 16) {
+    const uint4 raw = __ldcs(reinterpret_cast<const uint4*>(p));
+    return *reinterpret_cast<const VecT*>(&raw);
+  } else {
+    return *reinterpret_cast<const VecT*>(p);
+  }
+}
+template <class VecT>
+__device__ __forceinline__ void store_once(char* p, const VecT& v) {
+  if constexpr (sizeof(VecT) == 16) __stcs(reinterpret_cast<uint4*>(p), *reinterpret_cast<const uint4*>(&v));
+  else *reinterpret_cast<VecT*>(p) = v;
+}
+
 // kPaired: pairs (2 i, 2 i + 1); a vector of V channels is V / 2 pairs (V = 1: a thread moves a pair as two elements).  Otherwise pairs (i, i + pairs): two
 // vectors.  kAdjacent: channels lie beside each other (V > 1 needs it).
 template <class T, int V, bool kPaired, bool kAppend>
-__global__ void __launch_bounds__(256) rotate_kernel(const __grid_constant__ RotateP p) {
-  const unsigned at = blockIdx.x * 256u + threadIdx.x;
+__global__ void __launch_bounds__(kThreads, 8) rotate_kernel(const __grid_constant__ RotateP p) {
+  const unsigned at = blockIdx.x * (unsigned)kThreads + threadIdx.x;
   if (at >= p.items) return;
   const unsigned token = at / (unsigned)p.per_row;
   const int part = (int)(at - token * (unsigned)p.per_row);
@@ -72,14 +90,14 @@ __global__ void __launch_bounds__(256) rotate_kernel(const __grid_constant__ Rot
   using VecT = Vec<T, V>;
   // Heads [from, to) of one tensor, kBatch at a time: as many loads on their way before the first store.
   auto go = [&](const char* src, long long src_head, char* dst, long long dst_head, long long src_chan, long long dst_chan, int count, bool rotate) {
-    constexpr int kBatch = 4;
+    constexpr int kBatch = kTwo && V * sizeof(T) == 16 ? 2 : 4;
     for (int n0 = 0; n0 < count; n0 += kBatch) {
       VecT x[kBatch], y[kBatch];
 #pragma unroll
       for (int u = 0; u < kBatch; ++u)
         if (n0 + u < count) {
-          x[u] = *reinterpret_cast<const VecT*>(src + (n0 + u) * src_head);
-          if (kTwo && turns) y[u] = *reinterpret_cast<const VecT*>(src + (n0 + u) * src_head + apart * src_chan);
+          x[u] = load_once<VecT>(src + (n0 + u) * src_head);
+          if (kTwo && turns) y[u] = load_once<VecT>(src + (n0 + u) * src_head + apart * src_chan);
         }
 #pragma unroll
       for (int u = 0; u < kBatch; ++u)
@@ -94,8 +112,8 @@ __global__ void __launch_bounds__(256) rotate_kernel(const __grid_constant__ Rot
               *hi = Elem<T>::down(c * cs[n].x + a * cs[n].y);
             }
           }
-          *reinterpret_cast<VecT*>(dst + (n0 + u) * dst_head) = x[u];
-          if (kTwo && turns) *reinterpret_cast<VecT*>(dst + (n0 + u) * dst_head + apart * dst_chan) = y[u];
+          store_once(dst + (n0 + u) * dst_head, x[u]);
+          if (kTwo && turns) store_once(dst + (n0 + u) * dst_head + apart * dst_chan, y[u]);
         }
     }
   };
@@ -132,17 +150,17 @@ static cudaError_t launch_rotate(RotateP& p, int vec, bool paired, cudaStream_t 
   p.per_row = p.turning + (p.D - 2 * p.pairs) / vec;
   const long long items = (long long)p.B * p.L * p.per_row;
   p.items = (unsigned)items;
-  const long long blocks = (items + 255) / 256;
-  // Heads in as many slices as fill the SMs with 8 blocks each
-  const long long want = 8ll * sm_count();
+  const long long blocks = (items + kThreads - 1) / kThreads;
+  // Heads in as many slices as fill the SMs with 16 blocks each (8: 89 us instead of 87, and 32: 123)
+  const long long want = 16ll * sm_count();
   p.slices = (int)(blocks >= want ? 1 : (want + blocks - 1) / blocks);
   p.slices = imax(1, imin(p.slices, p.heads));
   const dim3 grid((unsigned)blocks, (unsigned)imin(p.slices, 65535));
   p.slices = (int)grid.y;
 #define CHILL_ROTATE(VEC)                                                     \
   case VEC:                                                                   \
-    if (paired) rotate_kernel<T, VEC, true, kAppend><<<grid, 256, 0, st>>>(p); \
-    else rotate_kernel<T, VEC, false, kAppend><<<grid, 256, 0, st>>>(p);       \
+    if (paired) rotate_kernel<T, VEC, true, kAppend><<<grid, kThreads, 0, st>>>(p); \
+    else rotate_kernel<T, VEC, false, kAppend><<<grid, kThreads, 0, st>>>(p);       \
     break
   switch (vec) {
     CHILL_ROTATE(1);
@@ -150,8 +168,8 @@ static cudaError_t launch_rotate(RotateP& p, int vec, bool paired, cudaStream_t 
     CHILL_ROTATE(4);
     default:
       if constexpr (sizeof(T) == 2) {
-        if (paired) rotate_kernel<T, 8, true, kAppend><<<grid, 256, 0, st>>>(p);
-        else rotate_kernel<T, 8, false, kAppend><<<grid, 256, 0, st>>>(p);
+        if (paired) rotate_kernel<T, 8, true, kAppend><<<grid, kThreads, 0, st>>>(p);
+        else rotate_kernel<T, 8, false, kAppend><<<grid, kThreads, 0, st>>>(p);
       }
   }
 #undef CHILL_ROTATE

@@ -357,7 +357,7 @@ def state_of(pages, shared):
 
 @pytest.mark.parametrize("B,ctx,page,num_pages,seed", [
     (1, 40, 16, 10, 0), (4, 700, 16, 260, 1), (6, 100, 5, 160, 2), (3, 30, 1, 100, 3), (40, 200, 8, 1200, 4), (70, 3000, 16, 14000, 5), (600, 20, 4, 4000, 6),
-    (4, 60, 16, 17, 7), (12, 90, 8, 70, 8),
+    (4, 60, 16, 17, 7), (12, 90, 8, 70, 8), (24, 5000, 1, 40000, 9), (9, 20000, 2, 60000, 10),
 ])
 def test_fork_trim_and_compact(ca, B, ctx, page, num_pages, seed):
     """A run of forks with tokens in between, cuts and compactions; where there are few pages some rows get none."""
