@@ -22,8 +22,7 @@ constexpr int kMost = CHILL_SELECT_MAX;
 constexpr int kBatch = 4;       // vectors of 16 bytes that a thread has at a time
 constexpr int kMaxParts = 64;   // segments of a row
 constexpr int kRoom = 2304;     // values that wait: those of M threads and more, a whole number for each thread
-constexpr int kQueue = 256;      // vectors of a warp that wait to be looked at
-constexpr int kRound = 16;       // batches until they are
+constexpr int kQueue = 64;       // vectors of a warp that wait to be looked at, after so many batches that 30 are to be expected
 constexpr float kLog2e = 1.4426950408889634f;
 
 struct Sum {
@@ -111,6 +110,65 @@ __device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
   return d;
 }
 
+// A candidate in the order of its 64-bit score, then of its place: beam and token, side by side and inverted (larger is earlier).
+struct Candidate {
+  uint64_t rank, place;
+};
+constexpr int kTokenBits = 31;
+__device__ __forceinline__ uint64_t place_at(int beam, int token) { return ~((uint64_t)beam << kTokenBits | (uint64_t)token); }
+__device__ __forceinline__ bool before(const Candidate& a, const Candidate& b) { return a.rank != b.rank ? a.rank > b.rank : a.place > b.place; }
+
+__device__ __forceinline__ bool before(uint64_t a, uint64_t b) { return a > b; }
+
+__device__ __forceinline__ uint64_t from_lane(uint64_t x, int mask) { return __shfl_xor_sync(0xffffffffu, x, mask); }
+__device__ __forceinline__ Candidate from_lane(const Candidate& x, int mask) {
+  return {__shfl_xor_sync(0xffffffffu, x.rank, mask), __shfl_xor_sync(0xffffffffu, x.place, mask)};
+}
+
+// Lists of 32 * R entries over a warp: entry e is in register e / 32 of lane e % 32.  Sorted: entry 0 comes first.
+template <class T, int R>
+struct List {
+  T x[R];
+
+  // Entry e takes the earlier of e and e ^ distance where `keep_first` says so of it, else the later.
+  __device__ __forceinline__ void step(int distance, int block) {
+    const int lane = threadIdx.x & 31;
+    if (R == 2 && distance == 32) {  // only for block 64, which is one direction
+      const bool swap = before(x[R - 1], x[0]);
+      const T a = x[0], b = x[R - 1];
+      x[0] = swap ? b : a;
+      x[R - 1] = swap ? a : b;
+      return;
+    }
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      const int e = lane + 32 * r;
+      const T other = from_lane(x[r], distance);
+      const bool first = ((e & distance) == 0) == ((e & block) == 0);
+      if (before(other, x[r]) == first) x[r] = other;
+    }
+  }
+  // A bitonic sequence becomes sorted.
+  __device__ __forceinline__ void settle() {
+#pragma unroll
+    for (int distance = 16 * R; distance > 0; distance >>= 1) step(distance, 0);
+  }
+  __device__ __forceinline__ void sort() {
+#pragma unroll
+    for (int block = 2; block < 32 * R; block <<= 1)
+#pragma unroll
+      for (int distance = block >> 1; distance > 0; distance >>= 1) step(distance, block);
+    settle();
+  }
+  // The 32 * R first of this list and of another one, given from its last entry to its first (entry e of `reversed` is entry 32 * R - 1 - e).
+  __device__ __forceinline__ void merge(const List& reversed) {
+#pragma unroll
+    for (int r = 0; r < R; ++r)
+      if (before(reversed.x[r], x[r])) x[r] = reversed.x[r];
+    settle();
+  }
+};
+
 // A segment's values that may be among its M largest, in shared memory.
 struct alignas(16) Kept {
   uint64_t waiting[kRoom + 4];
@@ -119,7 +177,8 @@ struct alignas(16) Kept {
   uint32_t least[kWarps], most[kWarps];
   int count;
   int queued[kWarps];
-  int queue[kWarps][kQueue];  // numbers of the vectors in which a warp met something to keep
+  uint4 queue[kWarps][kQueue];  // vectors in which a warp met something to keep, and their numbers
+  int numbers[kWarps][kQueue];
 };
 
 // Every thread has a key, all that are not 0 are different: the M-th largest (0: there are fewer).
@@ -202,8 +261,8 @@ __device__ __forceinline__ int shrink(Kept& kept, int count, int M, uint64_t& li
 // A thread has vectors of 16 bytes; kShifted, where rows do not begin at multiples of 16 bytes: words of 4 bytes, 256 apart, of which rows that begin in the middle of one
 // put theirs together from two.
 //
-// Warps stream on their own: sums in registers, numbers of vectors that reach the limit in a queue of their own.  After a round (16 batches) the CTA looks at the queued
-// vectors' values again, which are in L2.  32 groups of 8 beams, 128000 tokens, bf16: loads and maxima alone take 14 us of the 19, exponentials 4.
+// Warps stream on their own: sums in registers, vectors that reach the limit in a queue of their own, which are looked at value by value
+// after a round of some batches.  32 groups of 8 beams, 128000 tokens, bf16: loads and maxima alone take 14 us of the 19, exponentials 4.
 template <class T, bool kShifted>
 __global__ void __launch_bounds__(kThreads, 4) scan_kernel(const __grid_constant__ SelectP p) {
   constexpr int V = 16 / sizeof(T), kWord = 4 / sizeof(T), kStep = kThreads * kBatch;
@@ -269,9 +328,20 @@ __global__ void __launch_bounds__(kThreads, 4) scan_kernel(const __grid_constant
     }
   };
 
-  for (int round = 0; round * V < size; round += kRound * kStep) {
+  auto add_up = [&]() {  // a warp's sum, once it has streamed its part
+    float highest = top;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) highest = fmaxf(highest, __shfl_xor_sync(0xffffffffu, highest, o));
+    if (top != -INFINITY) sum *= (double)exp2_of((top - highest) * kLog2e);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    if (lane == 0) of_warps[warp] = {sum, highest, 0};
+  };
+  if (size == 0) add_up();
+  const int round_step = imin(imax(192 / p.M, 1), 16) * kStep;
+  for (int round = 0; round * V < size; round += round_step) {
     int queued = 0;
-    const int end = imin(round + kRound * kStep, (size + V - 1) / V);
+    const int end = imin(round + round_step, (size + V - 1) / V);
     for (int n0 = round; n0 < end; n0 += kStep) {
       uint4 raw[kBatch];
       load(n0, raw);
@@ -311,11 +381,15 @@ __global__ void __launch_bounds__(kThreads, 4) scan_kernel(const __grid_constant
       for (int u = 0; u < kBatch; ++u) {
         const unsigned who = __ballot_sync(0xffffffffu, most[u] > -INFINITY && most[u] >= lowest);
         const int at = queued + __popc(who & ((1u << lane) - 1));
-        if ((who >> lane & 1) && at < kQueue) kept.queue[warp][at] = n0 + u * kThreads + (int)threadIdx.x;
+        if ((who >> lane & 1) && at < kQueue) {
+          kept.queue[warp][at] = raw[u];
+          kept.numbers[warp][at] = n0 + u * kThreads + (int)threadIdx.x;
+        }
         queued += __popc(who);
       }
     }
     if (lane == 0) kept.queued[warp] = queued;
+    if (end * V >= size) add_up();
     __syncthreads();
     const int before = kept.count;
     int fullest = 0;
@@ -324,21 +398,14 @@ __global__ void __launch_bounds__(kThreads, 4) scan_kernel(const __grid_constant
     __syncthreads();
     if (fullest <= kQueue) {
       const float lowest = limit == 0 ? -INFINITY : value_of(limit);
-      for (int i = lane; i < queued; i += 32) {
-        const int id = kept.queue[warp][i];
-        uint4 raw;
-        if (!kShifted && (id + 1) * V <= size) raw = __ldg(reinterpret_cast<const uint4*>(row) + id);
-        else raw = make_uint4(word_of(number_of(id, 0)), word_of(number_of(id, kWord)), word_of(number_of(id, 2 * kWord)), word_of(number_of(id, 3 * kWord)));
-        const T* x = reinterpret_cast<const T*>(&raw);
-#pragma unroll
-        for (int e = 0; e < V; ++e) {
-          const float value = Elem<T>::up(x[e]);
-          if (value > -INFINITY && value >= lowest) {
-            const uint64_t key = key_of(value, from + number_of(id, e));
-            if (key >= limit) {
-              const int at = atomicAdd(&kept.count, 1);
-              if (at < kRoom) kept.waiting[at] = key;
-            }
+      const T* values = reinterpret_cast<const T*>(kept.queue[warp]);
+      for (int i = lane; i < queued * V; i += 32) {
+        const float value = Elem<T>::up(values[i]);
+        if (value > -INFINITY && value >= lowest) {
+          const uint64_t key = key_of(value, from + number_of(kept.numbers[warp][i / V], i % V));
+          if (key >= limit) {
+            const int at = atomicAdd(&kept.count, 1);
+            if (at < kRoom) kept.waiting[at] = key;
           }
         }
       }
@@ -385,18 +452,10 @@ __global__ void __launch_bounds__(kThreads, 4) scan_kernel(const __grid_constant
     }
   }
 
-  // The segment's sum
-  float highest = top;
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) highest = fmaxf(highest, __shfl_xor_sync(0xffffffffu, highest, o));
-  if (top != -INFINITY) sum *= (double)exp2_of((top - highest) * kLog2e);
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-  if (lane == 0) of_warps[warp] = {sum, highest, 0};
   __syncthreads();
   if (warp == 0) {
     const Sum s = of_warps[lane % kWarps];
-    highest = s.top;
+    float highest = s.top;
 #pragma unroll
     for (int o = kWarps / 2; o > 0; o >>= 1) highest = fmaxf(highest, __shfl_xor_sync(0xffffffffu, highest, o));
     sum = s.top != -INFINITY ? s.sum * exp((double)s.top - (double)highest) : s.sum;
@@ -404,81 +463,37 @@ __global__ void __launch_bounds__(kThreads, 4) scan_kernel(const __grid_constant
     for (int o = kWarps / 2; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
     if (lane == 0) p.sums[blockIdx.x] = {sum, highest, 0};
   }
-  // Its list: every value that waits counts the larger ones
-  const int count = shrink(kept, kept.count, p.M, limit);
+  // Its list.  A thread has a value at most: warps sort theirs, and a value's place is the sum of its places in all 8 sorted runs
+  const int count = kept.count > kThreads ? shrink(kept, kept.count, p.M, limit) : kept.count;
   uint64_t* list = p.lists + (long long)blockIdx.x * p.M;
-  if ((int)threadIdx.x < (-count & 3)) kept.waiting[count + threadIdx.x] = 0;
+  List<uint64_t, 1> run;
+  run.x[0] = (int)threadIdx.x < count ? kept.waiting[threadIdx.x] : 0;
+  if (warp * 32 < count) run.sort();
+  kept.maxima[threadIdx.x] = run.x[0];
   __syncthreads();
-  if ((int)threadIdx.x < count) {
-    const uint64_t key = kept.waiting[threadIdx.x];
-    const ulonglong2* others = reinterpret_cast<const ulonglong2*>(kept.waiting);
-    int larger = 0;
-    for (int i = 0; i < (count + 3) / 4; ++i) {
-      const ulonglong2 a = others[2 * i], b = others[2 * i + 1];
-      larger += (a.x > key) + (a.y > key) + (b.x > key) + (b.y > key);
+  const uint64_t key = run.x[0];
+  if (key != 0) {
+    int larger = lane;
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) {
+      const uint64_t* other = kept.maxima + w * 32;
+      if (w == warp || w * 32 >= count || other[0] <= key) continue;
+      int n = 0;  // how many of them are larger: between 1 and 32
+#pragma unroll
+      for (int step = 16; step > 0; step >>= 1) n += other[n + step - 1] > key ? step : 0;
+      larger += n + (other[n] > key);
     }
     if (larger < p.M) list[larger] = key;
   }
   if ((int)threadIdx.x >= count && (int)threadIdx.x < p.M) list[threadIdx.x] = 0;
 }
 
-// A candidate in the order of its 64-bit score, then of its place among the group's K * V (inverted: larger is earlier).
-struct Candidate {
-  uint64_t rank, place;
-};
-__device__ __forceinline__ bool before(const Candidate& a, const Candidate& b) { return a.rank != b.rank ? a.rank > b.rank : a.place > b.place; }
-
-__device__ __forceinline__ Candidate from_lane(const Candidate& x, int mask) {
-  return {__shfl_xor_sync(0xffffffffu, x.rank, mask), __shfl_xor_sync(0xffffffffu, x.place, mask)};
-}
-
-// Lists of 32 * R entries over a warp: entry e is in register e / 32 of lane e % 32.  Sorted: entry 0 comes first.
-template <class T, int R>
-struct List {
-  T x[R];
-
-  // Entry e takes the earlier of e and e ^ distance where `keep_first` says so of it, else the later.
-  __device__ __forceinline__ void step(int distance, int block) {
-    const int lane = threadIdx.x & 31;
-    if (R == 2 && distance == 32) {  // only for block 64, which is one direction
-      const bool swap = before(x[R - 1], x[0]);
-      const T a = x[0], b = x[R - 1];
-      x[0] = swap ? b : a;
-      x[R - 1] = swap ? a : b;
-      return;
-    }
-#pragma unroll
-    for (int r = 0; r < R; ++r) {
-      const int e = lane + 32 * r;
-      const T other = from_lane(x[r], distance);
-      const bool first = ((e & distance) == 0) == ((e & block) == 0);
-      if (before(other, x[r]) == first) x[r] = other;
-    }
-  }
-  // A bitonic sequence becomes sorted.
-  __device__ __forceinline__ void settle() {
-#pragma unroll
-    for (int distance = 16 * R; distance > 0; distance >>= 1) step(distance, 0);
-  }
-  __device__ __forceinline__ void sort() {
-#pragma unroll
-    for (int block = 2; block < 32 * R; block <<= 1)
-#pragma unroll
-      for (int distance = block >> 1; distance > 0; distance >>= 1) step(distance, block);
-    settle();
-  }
-  // The 32 * R first of this list and of another one, given from its last entry to its first (entry e of `reversed` is entry 32 * R - 1 - e).
-  __device__ __forceinline__ void merge(const List& reversed) {
-#pragma unroll
-    for (int r = 0; r < R; ++r)
-      if (before(reversed.x[r], x[r])) x[r] = reversed.x[r];
-    settle();
-  }
-};
-
-// One CTA for a group.  Its warps go over the lists in turn; a warp keeps the M first of those it has met, sorted across its lanes, and merges a list of which the
-// first entry comes before its last one (a bitonic network; most lists are passed over).  At the end the warps' lists are merged two and two.
+// One CTA for a group.  Up to 32 lists are merged two and two, by warps (bitonic networks).  Of more lists a lower limit, from their entries at some depths, leaves few candidates, which
+// are sorted (4 groups of 32 beams in 4 segments, 64 candidates: 9 us, by merging 15; 32 groups of 8 beams in 2 segments, 16 candidates: 6 us, by merging 3).  Where very many are
+// alike, or rows are NaN, many lists are merged too: a warp keeps the M first of those it has met, and merges a list of which the first entry comes before its last one.
 constexpr int kMergeWarps = 32;  // at most: one for every list, and 4 at least
+constexpr int kDepths = 7;       // 1, 2, 4, ... 64 entries
+constexpr int kFound = 512;
 
 template <class T, int R>
 __global__ void __launch_bounds__(kMergeWarps * 32) merge_kernel(const __grid_constant__ SelectP p) {
@@ -486,16 +501,19 @@ __global__ void __launch_bounds__(kMergeWarps * 32) merge_kernel(const __grid_co
   __shared__ double lse[kMost];
   __shared__ float score[kMost];
   __shared__ bool over[kMost], flat[kMost];  // finished beams; rows whose candidates are all alike: NaN or +inf
-  __shared__ Candidate exchange[kMergeWarps / 2][kList];
+  __shared__ Candidate exchange[kMergeWarps / 2][kList], found[kFound];
+  __shared__ uint32_t bounds[kDepths];
+  __shared__ int n_found;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, group = (int)blockIdx.x, warps = (int)blockDim.x >> 5;
   const int lists = p.K * p.parts;
   const uint64_t* const entries = p.lists + (long long)group * lists * p.M;
   asm volatile("griddepcontrol.wait;" ::: "memory");  // the lists are there
-  // This warp's first list is on its way while the sums are worked out (nonsense where nothing was written)
+  // Few lists: a warp has one, which is on its way while the sums are worked out (nonsense where nothing was written)
+  const bool few = lists <= warps;
   uint64_t first[R];
 #pragma unroll
-  for (int r = 0; r < R; ++r) first[r] = warp < lists && lane + 32 * r < p.M ? __ldcg(&entries[(long long)warp * p.M + lane + 32 * r]) : 0;
-
+  for (int r = 0; r < R; ++r) first[r] = few && warp < lists && lane + 32 * r < p.M ? __ldcg(&entries[(long long)warp * p.M + lane + 32 * r]) : 0;
+  bool any_flat = false;
   for (int k = warp; k < p.K; k += warps) {
     const long long beam = (long long)group * p.K + k;
     const float s = p.scores[beam];
@@ -514,24 +532,26 @@ __global__ void __launch_bounds__(kMergeWarps * 32) merge_kernel(const __grid_co
       if (lane + 32 * i < p.parts) sum += mine[i].top == -INFINITY ? mine[i].sum : mine[i].sum * exp((double)mine[i].top - (double)top);
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    const double l = (double)top + log(sum);  // a row without values has empty lists
+    const bool alike = s != -INFINITY && !ended && (l != l || !(s < INFINITY));
+    any_flat = any_flat || alike;
     if (lane == 0) {
-      const double l = (double)top + log(sum);  // a row without values has empty lists
       lse[k] = l;
       score[k] = s;
       over[k] = ended;
-      flat[k] = s != -INFINITY && !ended && (l != l || !(s < INFINITY));
+      flat[k] = alike;
     }
   }
-  __syncthreads();
+  any_flat = __syncthreads_or(any_flat) != 0;
   auto candidate = [&](int k, float x, int v) {
-    return Candidate{rank_of((double)score[k] + ((double)x - lse[k])), ~(uint64_t)((long long)k * p.V + v)};
+    return Candidate{rank_of((double)score[k] + ((double)x - lse[k])), place_at(k, v)};
   };
   auto usable = [&](int k) { return score[k] != -INFINITY && !over[k] && !flat[k]; };
 
   List<Candidate, R> best;
 #pragma unroll
   for (int r = 0; r < R; ++r) best.x[r] = {0, 0};
-  if (warp < 2) {  // rows of NaN, rows of +inf: the first values of the first ones
+  if (any_flat && warp < 2) {  // rows of NaN, rows of +inf: the first values of the first ones
     int n = 0;
     for (int k = 0; k < p.K; ++k) {
       if (!flat[k] || (score[k] == INFINITY && lse[k] == lse[k]) != (warp == 1)) continue;
@@ -550,78 +570,181 @@ __global__ void __launch_bounds__(kMergeWarps * 32) merge_kernel(const __grid_co
       if (lane + 32 * r < n) best.x[r] = exchange[warp][lane + 32 * r];
   }
 
-  auto nth = [&]() {  // the M-th; with all lanes
-    return Candidate{__shfl_sync(0xffffffffu, p.M > 32 ? best.x[R - 1].rank : best.x[0].rank, (p.M - 1) & 31),
-                     __shfl_sync(0xffffffffu, p.M > 32 ? best.x[R - 1].place : best.x[0].place, (p.M - 1) & 31)};
-  };
   // Entry e of list l
   auto entry = [&](int l, int e, uint64_t key) {
     const int k = l / p.parts;
     if (usable(k)) return key != 0 ? candidate(k, value_of(key), place_of(key)) : Candidate{0, 0};
     if (over[k] && e == 0 && l == k * p.parts && score[k] != -INFINITY)  // a finished beam: a list of one
-      return Candidate{rank_of((double)score[k]), ~(uint64_t)((long long)k * p.V + p.end_token)};
+      return Candidate{rank_of((double)score[k]), place_at(k, p.end_token)};
     return Candidate{0, 0};
   };
-  if (warp < lists) {
-    List<Candidate, R> own;
+  auto merge_all = [&]() {
+    auto nth = [&]() {  // the M-th; with all lanes
+      return Candidate{__shfl_sync(0xffffffffu, p.M > 32 ? best.x[R - 1].rank : best.x[0].rank, (p.M - 1) & 31),
+                       __shfl_sync(0xffffffffu, p.M > 32 ? best.x[R - 1].place : best.x[0].place, (p.M - 1) & 31)};
+    };
+    if (warp < lists) {
+      List<Candidate, R> own;
 #pragma unroll
-    for (int r = 0; r < R; ++r) own.x[r] = entry(warp, lane + 32 * r, first[r]);
-    if (warp < 2) {  // there may be something already: the list's entries from the last one to the first
-      List<Candidate, R> reversed;
-#pragma unroll
-      for (int r = 0; r < R; ++r)
-        reversed.x[r] = {__shfl_sync(0xffffffffu, own.x[R - 1 - r].rank, 31 - lane), __shfl_sync(0xffffffffu, own.x[R - 1 - r].place, 31 - lane)};
-      best.merge(reversed);
-    } else {
-      best = own;
-    }
-  }
-  for (int l0 = warp + warps; l0 < lists; l0 += 32 * warps) {  // of the others a lane looks at the first entry
-    const int own = l0 + lane * warps;
-    const Candidate head = own < lists ? entry(own, 0, entries[(long long)own * p.M]) : Candidate{0, 0};
-    bool waits = head.rank != 0;
-    while (true) {
-      const Candidate last = nth();  // with all lanes
-      waits = waits && before(head, last);
-      // the one with the best first entry (or next to it), after which more are passed over
-      const uint32_t top = waits ? (uint32_t)(head.rank >> 32) : 0, most = __reduce_max_sync(0xffffffffu, top);
-      if (most == 0) break;
-      const int next = __ffs(__ballot_sync(0xffffffffu, top == most)) - 1, l = l0 + next * warps;
-      if (lane == next) waits = false;
-      List<Candidate, R> reversed;
-#pragma unroll
-      for (int r = 0; r < R; ++r) {
-        const int e = kList - 1 - lane - 32 * r;
-        reversed.x[r] = e < p.M ? entry(l, e, entries[(long long)l * p.M + e]) : Candidate{0, 0};
-      }
-      best.merge(reversed);
-    }
-  }
-#pragma unroll 1
-  for (int apart = warps / 2; apart > 0; apart >>= 1) {
-    __syncthreads();  // what lies in `exchange` has been read
-    if (warp >= apart && warp < 2 * apart) {
-#pragma unroll
-      for (int r = 0; r < R; ++r) exchange[warp - apart][lane + 32 * r] = best.x[r];
-    }
-    __syncthreads();
-    if (warp < apart) {
-      const Candidate last = nth();
-      if (before(exchange[warp][0], last)) {
+      for (int r = 0; r < R; ++r) own.x[r] = lane + 32 * r < p.M ? entry(warp, lane + 32 * r, few ? first[r] : entries[(long long)warp * p.M + lane + 32 * r]) : Candidate{0, 0};
+      if (any_flat && warp < 2) {  // there may be something already: the list's entries from the last one to the first
         List<Candidate, R> reversed;
 #pragma unroll
-        for (int r = 0; r < R; ++r) reversed.x[r] = exchange[warp][kList - 1 - lane - 32 * r];
+        for (int r = 0; r < R; ++r)
+          reversed.x[r] = {__shfl_sync(0xffffffffu, own.x[R - 1 - r].rank, 31 - lane), __shfl_sync(0xffffffffu, own.x[R - 1 - r].place, 31 - lane)};
+        best.merge(reversed);
+      } else {
+        best = own;
+      }
+    }
+    for (int l0 = warp + warps; l0 < lists; l0 += 32 * warps) {  // of the others a lane looks at the first entry
+      const int own = l0 + lane * warps;
+      const Candidate head = own < lists ? entry(own, 0, entries[(long long)own * p.M]) : Candidate{0, 0};
+      bool waits = head.rank != 0;
+      while (true) {
+        const Candidate last = nth();  // with all lanes
+        waits = waits && before(head, last);
+        // the one with the best first entry (or next to it), after which more are passed over
+        const uint32_t top = waits ? (uint32_t)(head.rank >> 32) : 0, most = __reduce_max_sync(0xffffffffu, top);
+        if (most == 0) break;
+        const int next = __ffs(__ballot_sync(0xffffffffu, top == most)) - 1, l = l0 + next * warps;
+        if (lane == next) waits = false;
+        List<Candidate, R> reversed;
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+          const int e = kList - 1 - lane - 32 * r;
+          reversed.x[r] = e < p.M ? entry(l, e, entries[(long long)l * p.M + e]) : Candidate{0, 0};
+        }
         best.merge(reversed);
       }
     }
+#pragma unroll 1
+    for (int apart = warps / 2; apart > 0; apart >>= 1) {
+      __syncthreads();  // what lies in `exchange` has been read
+      if (warp >= apart && warp < 2 * apart) {
+#pragma unroll
+        for (int r = 0; r < R; ++r) exchange[warp - apart][lane + 32 * r] = best.x[r];
+      }
+      __syncthreads();
+      if (warp < apart) {
+        const Candidate last = nth();
+        if (before(exchange[warp][0], last)) {
+          List<Candidate, R> reversed;
+#pragma unroll
+          for (int r = 0; r < R; ++r) reversed.x[r] = exchange[warp][kList - 1 - lane - 32 * r];
+          best.merge(reversed);
+        }
+      }
+    }
+  };
+  // A lower limit.  Of n lists that have d entries each that reach a number, n d candidates do: for d = 1, 2, 4, ... the (M / d)-th largest of the lists' d-th entries, by their
+  // leading 32 bits and by halving, and the largest of these numbers.  Some 1.3 M candidates reach it.
+  bool by_limit = !few && !any_flat;
+  if (by_limit && warp < kDepths) {
+    const int depth = imin(1 << warp, p.M), need = (p.M + depth - 1) / depth;
+    constexpr int kEach = 4;
+    uint32_t x[kEach] = {};
+    for (int l0 = lane; l0 < lists; l0 += 32 * kEach) {  // of more than 128 lists the largest of several
+      uint64_t key[kEach];
+#pragma unroll
+      for (int i = 0; i < kEach; ++i) key[i] = l0 + 32 * i < lists ? __ldcg(&entries[(long long)(l0 + 32 * i) * p.M + depth - 1]) : 0;
+#pragma unroll
+      for (int i = 0; i < kEach; ++i)
+        if (l0 + 32 * i < lists) x[i] = max(x[i], (uint32_t)(entry(l0 + 32 * i, depth - 1, key[i]).rank >> 32));
+    }
+    auto reach = [&](uint32_t number) {
+      int n = 0;
+#pragma unroll
+      for (int i = 0; i < kEach; ++i) n += __popc(__ballot_sync(0xffffffffu, x[i] >= number));
+      return n;
+    };
+    uint32_t some = 0xffffffffu;
+#pragma unroll
+    for (int i = 0; i < kEach; ++i) some = x[i] != 0 ? min(some, x[i]) : some;
+    uint32_t lo = __reduce_min_sync(0xffffffffu, some), hi = __reduce_max_sync(0xffffffffu, max(max(x[0], x[1]), max(x[2], x[3])));
+    if (hi == 0 || reach(lo) < need) lo = hi = 0;  // fewer lists than that have so many entries
+    while (lo < hi) {
+      const uint32_t middle = lo + (hi - lo) / 2 + 1;
+      const int n = reach(middle);
+      if (n >= need) lo = middle;
+      else hi = middle - 1;
+      if (n >= need && n <= need + need / 8) break;
+    }
+    if (lane == 0) bounds[warp] = lo;
   }
-  if (warp != 0) return;
+  if (threadIdx.x == 0) n_found = 0;
+  __syncthreads();
+  uint32_t bound = 0;
+#pragma unroll
+  for (int i = 0; i < kDepths; ++i) bound = max(bound, bounds[i]);
+  if (by_limit) {
+    // A warp has a list at a time, a lane an entry (two); within a row the limit is one for the logits, rounded down
+    const double least = value_of_rank((uint64_t)bound << 32);
+    constexpr int kEach = 4;
+    for (int l0 = warp; l0 < lists; l0 += warps * kEach) {
+      uint64_t key[kEach][R];
+#pragma unroll
+      for (int i = 0; i < kEach; ++i)
+#pragma unroll
+        for (int r = 0; r < R; ++r)
+          key[i][r] = l0 + i * warps < lists && lane + 32 * r < p.M ? __ldcg(&entries[(long long)(l0 + i * warps) * p.M + lane + 32 * r]) : 0;
+#pragma unroll
+      for (int i = 0; i < kEach; ++i) {
+        const int l = l0 + i * warps, k = l / p.parts;
+        if (l >= lists) break;
+        const float floor = bound == 0 ? -INFINITY : __double2float_rd(least - (double)score[k] + lse[k] - 1e-6);
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+          const bool may = over[k] ? l == k * p.parts && lane == 0 && r == 0 : key[i][r] != 0 && !(value_of(key[i][r]) < floor);
+          if (!may) continue;
+          const Candidate c = entry(l, lane + 32 * r, key[i][r]);
+          if (c.rank == 0 || (uint32_t)(c.rank >> 32) < bound) continue;
+          const int at = atomicAdd(&n_found, 1);
+          if (at < kFound) found[at] = c;
+        }
+      }
+    }
+  }
+  __syncthreads();
+  const int n = n_found;
+  by_limit = by_limit && n <= kFound;
+  if (by_limit) {
+    // Runs of 32 are sorted; a candidate's place is the sum of its places in all of them
+    for (int i0 = warp * 32; i0 < n; i0 += warps * 32) {
+      List<Candidate, 1> run;
+      run.x[0] = i0 + lane < n ? found[i0 + lane] : Candidate{0, 0};
+      run.sort();
+      found[i0 + lane] = run.x[0];
+    }
+    __syncthreads();
+    for (int i = threadIdx.x; i < n; i += blockDim.x) {
+      const Candidate c = found[i];
+      int place = i & 31;
+      if (c.rank == 0) continue;
+      for (int run = 0; run < n; run += 32) {
+        if (run == (i & ~31) || !before(found[run], c)) continue;
+        int larger = 0;
+#pragma unroll
+        for (int step = 16; step > 0; step >>= 1) larger += before(found[run + larger + step - 1], c) ? step : 0;
+        place += larger + (before(found[run + larger], c) ? 1 : 0);
+      }
+      if (place < kList) exchange[1][place] = c;
+    }
+    __syncthreads();
+    if (warp != 0) return;
+#pragma unroll
+    for (int r = 0; r < R; ++r) best.x[r] = lane + 32 * r < n ? exchange[1][lane + 32 * r] : Candidate{0, 0};
+  } else {
+    // The lists are merged, two and two
+    merge_all();
+    if (warp != 0) return;
+  }
 
   // Fewer than M that are not -inf: these are all there are, and the others follow in the order of their places
-  int found = 0;
+  int total = 0;
 #pragma unroll
   for (int r = 0; r < R; ++r) {
-    found += __popc(__ballot_sync(0xffffffffu, best.x[r].rank != 0));
+    total += __popc(__ballot_sync(0xffffffffu, best.x[r].rank != 0));
     exchange[1][lane + 32 * r] = best.x[r];  // read by warp 1 in the last round but one
   }
   __syncwarp();
@@ -629,24 +752,27 @@ __global__ void __launch_bounds__(kMergeWarps * 32) merge_kernel(const __grid_co
   for (int r = 0; r < R; ++r) {
     const int e = lane + 32 * r;
     if (e >= p.M) continue;
-    long long place = (long long)~best.x[r].place;
+    const long long to = (long long)group * p.M + e;
+    int k = (int)(~best.x[r].place >> kTokenBits), v = (int)(~best.x[r].place & ((1u << kTokenBits) - 1));
     double value = -INFINITY;
-    if (e < found) {
+    if (e < total) {
       value = value_of_rank(best.x[r].rank);
     } else {
       long long so_far = -1, skipped = 0;  // of those found
       while (skipped != so_far) {
         so_far = skipped;
         skipped = 0;
-        for (int i = 0; i < found; ++i) skipped += (long long)~exchange[1][i].place <= e - found + so_far;
+        for (int i = 0; i < total; ++i) {
+          const uint64_t place = ~exchange[1][i].place;
+          skipped += (long long)(place >> kTokenBits) * p.V + (long long)(place & ((1u << kTokenBits) - 1)) <= e - total + so_far;
+        }
       }
-      place = e - found + skipped;
+      k = (int)((e - total + skipped) / p.V);
+      v = (int)(e - total + skipped - (long long)k * p.V);
     }
-    const long long to = (long long)group * p.M + e;
-    const int k = (int)(place / p.V);
     p.out_scores[to] = (float)value;
     p.out_rows[to] = group * p.K + k;
-    p.out_tokens[to] = (int)(place - (long long)k * p.V);
+    p.out_tokens[to] = v;
   }
 }
 
@@ -693,7 +819,7 @@ static cudaError_t launch_select(const SelectP& p, int groups, cudaStream_t st) 
   cfg.gridDim = dim3((unsigned)groups);
   int warps = 4;
   while (warps < kMergeWarps && warps < p.K * p.parts) warps *= 2;
-  cfg.blockDim = dim3((unsigned)warps * 32);
+  cfg.blockDim = dim3(32u * (unsigned)warps);
   cfg.stream = st;
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
