@@ -67,8 +67,8 @@ def chill_beam_select(logits: torch.Tensor, scores: torch.Tensor, count: int | N
     """The ``count`` best continuations of every group of beams.
 
     Candidate (beam, token) of a group has ``scores[group, beam] + log_softmax(logits[row])[token]``, row = group * beams + beam; -inf where the logit or the beam's score
-    is -inf (a row of nothing but -inf has no candidates).  They are ranked by that value before it is rounded (sums of a row are kept in 64 bits); of equal ones the lowest
-    beam, then the lowest token comes first.  A NaN or +inf among a row's logits makes its candidates NaN, which rank first: they show.
+    is -inf (a row of nothing but -inf has no candidates).  They are ranked by that value in 64 bits, and it is rounded to fp32 at the end; of equal ones the lowest
+    beam, then the lowest token comes first.  (Scores beyond 1e13, where 64 bits do not tell the candidates of a beam apart: its largest logits stand for them.)  A NaN or +inf among a row's logits makes its candidates NaN, which rank first: they show.
 
     Args:
         logits: [groups * beams, vocab], fp16 / bf16 / fp32; rows any stride apart.

@@ -13,6 +13,7 @@ constexpr int kPageWarps = kPageThreads / 32;
 constexpr int kPageCtas = 8;
 constexpr int kMaxCtas = 16;
 constexpr int kForkRequests = 8192;
+constexpr int kMostShared = 200 * 1024;
 
 struct ShareP {
   int B, page, num_pages, width;
@@ -473,8 +474,8 @@ template <class F>
 static int launch_cluster(F kernel, const ShareP& p, int ctas, int threads, size_t smem, cudaStream_t st, const char* what) {
   cudaLaunchConfig_t cfg{};
   cudaLaunchAttribute attr[1];
-  if (smem > 48 * 1024) {
-    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+  if (smem > 48 * 1024) {  // always to the same limit: host threads may be here at once
+    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kMostShared);
     if (e != cudaSuccess) return record_cuda_failure(e, what);
   }
   if (ctas > 8) {
@@ -512,7 +513,7 @@ static int launch_share(const ShareP& p, cudaStream_t st) {
   const int per = ((p.B + s.ctas - 1) / s.ctas + kRows - 1) / kRows * kRows;
   const size_t bytes = (kTrim ? 3 * (size_t)per : 8 * (size_t)per + 2 * (size_t)p.B) * 4, rows = (size_t)per * (p.width + (p.width + 31) / 32) * 4;
   const char* what = kTrim ? "trim launch" : "fork launch";
-  if (bytes + rows <= 200 * 1024) return launch_cluster(share_kernel<kTrim, true>, p, s.ctas, s.threads, bytes + rows, st, what);
+  if (bytes + rows <= (size_t)kMostShared) return launch_cluster(share_kernel<kTrim, true>, p, s.ctas, s.threads, bytes + rows, st, what);
   return launch_cluster(share_kernel<kTrim, false>, p, s.ctas, s.threads, bytes, st, what);
 }
 

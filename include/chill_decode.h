@@ -53,8 +53,9 @@ int chill_rotate_append(const chill_rotate_args* a, void* stream);
 /* ------------------------------------------------------------------------------------------------------------------
  * Selection over beams and vocabulary.  Candidate (k, v) of group g: c = scores[g][k] + x - log sum exp x', x = logits[g * K + k][v], the sum over the
  * row; -inf where the logit or the beam's score is -inf.  A finished beam has one candidate, (k, end_token) with c = scores[g][k], and its
- * logits are not looked at.  The M candidates that are largest before c is rounded, in descending order, ties to the lowest k * V + v; NaN counts as
- * largest (a NaN or +inf among a row's logits makes all its candidates NaN, but for those of -inf). */
+ * logits are not looked at.  The M candidates of the largest c, worked out in 64 bits, in descending order, ties to the lowest k * V + v; NaN counts as
+ * largest (a NaN or +inf among a row's logits makes all its candidates NaN, but for those of -inf).  Where 64 bits do not tell the candidates of one beam apart
+ * (scores beyond 1e13) those of its M largest logits stand for them. */
 #define CHILL_SELECT_MAX 64 /* beams of a group, and candidates that are kept */
 typedef struct chill_select_args {
   int32_t G, K, M, dtype;

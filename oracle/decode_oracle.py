@@ -48,13 +48,10 @@ def select(logits, scores, count, finished=None, end_token=0):
 def _let_go(entries, shared, stack):
     """entries: pages whose holder lets go of them, in the order of rows and blocks; `shared`: counts beyond one before anything is let go of.  The pages that nobody holds
     then go on the stack, the first on top."""
-    back = []
     left = dict()
     for q in entries:
         left[q] = left.get(q, shared[q] + 1) - 1
-    for q in entries:
-        if left[q] == 0 and q not in back:
-            back.append(q)
+    back = [q for q in dict.fromkeys(entries) if left[q] == 0]
     for q, n in left.items():
         shared[q] = max(n - 1, 0)
     return stack + back[::-1]
@@ -81,6 +78,10 @@ def fork(table, held, free, n_free, shared, lens, parents, page):
     shared, before = list(shared), list(shared)
     new, now, out, copies, missing = [], [], [], [], 0
     kept = set()  # rows whose begun page stays with the first child
+    first, count = {}, {}
+    for b, r in enumerate(parents):
+        first.setdefault(r, b)
+        count[r] = count.get(r, 0) + 1
     for b, r in enumerate(parents):
         if not 0 <= r < B:
             new.append([])
@@ -93,7 +94,7 @@ def fork(table, held, free, n_free, shared, lens, parents, page):
             q = old[r][whole]
             if q < 0:
                 tokens = whole * page
-            elif before[q] == 0 and r not in kept and parents.index(r) == b:
+            elif before[q] == 0 and r not in kept and first[r] == b:
                 kept.add(r)
                 row.append(q)
             elif stack:
@@ -107,7 +108,7 @@ def fork(table, held, free, n_free, shared, lens, parents, page):
         out.append(tokens)
     entries = []
     for r in range(B):
-        children = sum(p == r for p in parents)
+        children = count.get(r, 0)
         whole = lens[r] // page if children else 0
         for q in old[r][:whole]:
             if q >= 0:

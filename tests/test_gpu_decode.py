@@ -473,3 +473,29 @@ def test_cache_copy_of_one_tensor(ca):
     expected[7, :, :5] = expected[2, :, :5]
     ca.chill_cache_copy(cache, cache, ca.ChillCopies(ints([2]), ints([7]), ints([5]), ints([1])))
     assert torch.equal(cache, expected)
+
+
+@pytest.mark.parametrize("mark", [-1e9, torch.finfo(torch.float32).min])
+def test_select_with_marks_for_missing_beams(ca, mark):
+    """The first step with a low score instead of -inf for the beams that are not there yet."""
+    g = torch.Generator().manual_seed(4)
+    logits = (torch.randn(8, 3001, generator=g) * 2).bfloat16()
+    scores = torch.full((2, 4), mark)
+    scores[:, 0] = 0
+    out = ca.chill_beam_select(logits.cuda(), scores.cuda(), 8)
+    check_select(out, logits, scores, 8)
+    assert (out.parents.cpu() == torch.tensor([[0], [4]])).all()
+
+
+def test_fork_of_the_largest_batch(ca):
+    """8192 requests, every other one twice, in a cluster; shared memory beyond the default limit."""
+    B, page = 8192, 4
+    pages, shared = ca.ChillPages.empty(B, 24, 5 * B, page), torch.zeros(5 * B, dtype=torch.int32, device="cuda")
+    lens = torch.arange(B, dtype=torch.int32, device="cuda") % 14 + 1
+    ca.chill_pages_reserve(pages, torch.zeros_like(lens), lens, 14, page)
+    before = state_of(pages, shared)
+    parents = torch.arange(B, dtype=torch.int32, device="cuda") // 2 * 2
+    table, held, stack, counts, missing, out, orders = orc.fork(*before, lens.tolist(), parents.tolist(), page)
+    lens, copies = ca.chill_pages_fork(pages, shared, lens, parents, page)
+    check_pages(pages, shared, table, held, stack, counts)
+    assert lens.tolist() == out and copies_of(copies) == orders and missing == pages.missing.item() == 0
