@@ -2,13 +2,14 @@
 // the M largest of them.
 //
 // The logits are read once, and that is the floor.  Within a row the order is that of x, so a CTA that streams a segment of a row keeps the M largest x beside the
-// maximum and sum of the softmax, without knowing lse yet; a second kernel, a CTA for each group, turns the segments' lists into candidates and merges them.  (One
-// kernel with a group in a cluster of 16 CTAs, exchanging sums and lists through distributed shared memory: 62 us where this takes 20, 32 groups of 8 beams over
-// 128000 tokens in bf16, and 75 us where this takes 16, 4 groups of 32 beams over 50021 in fp32: 64 CTAs do not fill the GPU.)
+// maximum and sum of the softmax, without knowing lse yet; a second kernel, a CTA for each group, turns the segments' lists into candidates and merges them.  Replayed from a
+// graph: 32 groups of 8 beams over 128000 tokens in bf16, 16 candidates 30 us (floor 9), 4 groups of 32 beams over 50021 in fp32, 64 candidates 26 us (floor 4), one group of 4 beams
+// over 32000 in fp32 10 us (floor: two launches).  One kernel with a group in a cluster of 16 CTAs, which exchange sums and lists through distributed shared memory, takes
+// 62, 75 and 14 us: 64 CTAs do not fill the GPU, and lists that are kept sorted while they grow cost more than the logits.
 //
 // What is kept is not sorted while it grows.  The first batch of a segment gives a lower limit: a number that M of the 256 threads' maxima reach.  That
-// lets about 1.5 M of 8192 values through; they wait in shared memory, and at the end each counts how many are larger than
-// itself.  Where more come than there is room for (sorted rows, constant ones) the M-th largest of all 256 thread maxima is a limit that leaves values of M threads.
+// lets about 1.5 M of 8192 values through; they wait in shared memory, where the limit is raised if they become many, and are sorted at the end.  Where more come than there is room
+// for (sorted rows, constant ones) the M-th largest of all 256 thread maxima is a limit that leaves values of M threads.
 #include <type_traits>
 
 #include "decode_common.cuh"
@@ -22,13 +23,13 @@ constexpr int kMost = CHILL_SELECT_MAX;
 constexpr int kBatch = 4;       // vectors of 16 bytes that a thread has at a time
 constexpr int kMaxParts = 64;   // segments of a row
 constexpr int kRoom = 2304;     // values that wait: those of M threads and more, a whole number for each thread
-constexpr int kQueue = 64;       // vectors of a warp that wait to be looked at, after so many batches that 30 are to be expected
+constexpr int kQueue = 96;       // vectors of a warp that wait to be looked at, after so many batches that 36 are to be expected (M = 64)
 constexpr float kLog2e = 1.4426950408889634f;
 
 struct Sum {
   double sum;
   float top;
-  int unused;
+  int padding;
 };
 
 struct SelectP {
@@ -261,8 +262,9 @@ __device__ __forceinline__ int shrink(Kept& kept, int count, int M, uint64_t& li
 // A thread has vectors of 16 bytes; kShifted, where rows do not begin at multiples of 16 bytes: words of 4 bytes, 256 apart, of which rows that begin in the middle of one
 // put theirs together from two.
 //
-// Warps stream on their own: sums in registers, vectors that reach the limit in a queue of their own, which are looked at value by value
-// after a round of some batches.  32 groups of 8 beams, 128000 tokens, bf16: loads and maxima alone take 14 us of the 19, exponentials 4.
+// Warps stream on their own: sums in registers, vectors that reach the limit in a queue of their own, which are looked at value by value after a round of some batches.  32 groups of
+// 8 beams over 128000 tokens, bf16: a segment's first batch and limit 4 us, the other seven 10 (5.8 TB/s), queue, sorting and sum 4; SMs with four CTAs are done 6 us after those with three.
+// 128 threads a CTA, 8 of them an SM: 33 us instead of 30; half as long segments 31; the next batch's loads ahead of this one's work (3 CTAs an SM) no gain.
 template <class T, bool kShifted>
 __global__ void __launch_bounds__(kThreads, 4) scan_kernel(const __grid_constant__ SelectP p) {
   constexpr int V = 16 / sizeof(T), kWord = 4 / sizeof(T), kStep = kThreads * kBatch;
