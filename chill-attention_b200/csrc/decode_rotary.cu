@@ -2,21 +2,25 @@
 // slots of a paged cache together with v (chill_rotate_append).  include/chill_decode.h has the formula.
 //
 // A copy with little arithmetic: every row is read and written once, so the bound is memory.  A thread owns one vector of pairs of one token and
-// goes over heads with it: the angles, their sines and cosines are the same for all heads and cost it about 40 instructions a pair once.  q and k of (8, 16, 4096, 128) in bf16: 87 us
-// (6.2 TB/s, 0.94 of a copy's rate); (3, 32 and 8, 5003, 128) in fp16, 96 channels turned by three axes: 52 us (0.91); 4,000 tokens of 24 and 8 heads of 128 into pages of 16: 22 us
-// (0.57: two waves of short CTAs).  The next heads' loads ahead of this one's arithmetic, with one loop over the heads of all tensors: 178 us (pointers chosen a head, spills).
+// goes over heads with it.  The sines and cosines are the same for all heads: a block's warps, which have the same vectors of different heads, share them.  q and k of (8, 16, 4096, 128) in bf16:
+// 84 us (6.4 TB/s, 0.97 of a copy's rate; 87 us where every thread works out its own); (3, 32 and 8, 5003, 128) in fp16, 96 channels turned by three axes: 50 us (0.94); 4000 tokens of 24
+// and 8 heads of 128 into pages of 16: 17 us (0.74: two waves of short CTAs).  The next heads' loads ahead of this one's arithmetic, with one loop over the heads of all tensors: 178 us (pointers chosen a head, spills).
 #include "decode_common.cuh"
 
 namespace chill {
 namespace decode {
 
 constexpr int kThreads = 128;
+// Vectors that a block has; its other threads have the same ones of other heads.  Narrow vectors: as many as there are threads, so that a block's accesses lie side by side
+// (102 of 128 channels in halves, fp16, element by element: 31 us, with 32 vectors 50).
+template <class T, int V>
+constexpr int kItems = V * sizeof(T) == 16 ? 32 : kThreads;
 
 struct RotateP {
   int B, L, H, Hkv, pairs, D, n_axes, inverse;
   int per_row;        // threads of a row: vectors of pairs, then vectors of channels that stay
   int turning;        // of these, the ones that turn
-  int heads, slices;  // of q, k (and v); a block goes over heads / slices of them
+  int heads, slices;  // of q, k (and v); a warp goes over heads / slices of them
   unsigned items;     // B * L * per_row
   const float* inv_freq;
   const int *axes, *positions;
@@ -38,7 +42,7 @@ __device__ __forceinline__ float2 turn(int position, float freq) {
   return cs;
 }
 
-// Nobody reads these again here: with plain loads and stores 106 us instead of 87 (q and k of (8, 16, 4096, 128) in bf16).
+// Nobody reads these again here: with plain loads and stores 20 % longer (q and k of (8, 16, 4096, 128) in bf16).
 template <class VecT>
 __device__ __forceinline__ VecT load_once(const char* p) {
   if constexpr (sizeof(VecT) == 16) {
@@ -58,8 +62,8 @@ __device__ __forceinline__ void store_once(char* p, const VecT& v) {
 // vectors.  V > 1 wants channels that lie beside each other.
 template <class T, int V, bool kPaired, bool kAppend>
 __global__ void __launch_bounds__(kThreads, 8) rotate_kernel(const __grid_constant__ RotateP p) {
-  const unsigned at = blockIdx.x * (unsigned)kThreads + threadIdx.x;
-  if (at >= p.items) return;
+  const unsigned at = blockIdx.x * (unsigned)kItems<T, V> + threadIdx.x % kItems<T, V>;
+  const bool inside = at < p.items;
   const unsigned token = at / (unsigned)p.per_row;
   const int part = (int)(at - token * (unsigned)p.per_row);
   const int b = (int)(token / (unsigned)p.L), i = (int)(token - (unsigned)b * (unsigned)p.L);
@@ -70,15 +74,28 @@ __global__ void __launch_bounds__(kThreads, 8) rotate_kernel(const __grid_consta
   const int c0 = turns ? (kPaired ? 2 * first : first) : 2 * p.pairs + (part - p.turning) * V;
   const int apart = kPaired ? 1 : p.pairs;
 
+  // Sines and cosines, by all of the block's threads together
+  constexpr int kFours = (kPairs + 1) / 2;
+  __shared__ float4 both[kFours][kItems<T, V>];
+  for (int i = threadIdx.x; i < kItems<T, V> * kPairs; i += kThreads) {
+    const int item = i % kItems<T, V>, n = i / kItems<T, V>;
+    const unsigned other = blockIdx.x * (unsigned)kItems<T, V> + (unsigned)item, its_token = other / (unsigned)p.per_row;
+    const int its_part = (int)(other - its_token * (unsigned)p.per_row);
+    if (other >= p.items || its_part >= p.turning) continue;
+    const int pair = its_part * kPairs + n, its_b = (int)(its_token / (unsigned)p.L), its_i = (int)(its_token - (unsigned)its_b * (unsigned)p.L);
+    const int axis = p.axes != nullptr ? imin(imax(p.axes[pair], 0), p.n_axes - 1) : 0;
+    float2 x = turn(p.positions[axis * p.pos_axis + its_b * p.pos_batch + its_i * p.pos_token], p.inv_freq[pair]);
+    if (p.inverse) x.y = -x.y;
+    reinterpret_cast<float2*>(&both[n / 2][item])[n & 1] = x;
+  }
+  __syncthreads();
+  if (!inside) return;
   float2 cs[kPairs];
-  if (turns) {
-    const int* at_token = p.positions + b * p.pos_batch + i * p.pos_token;
 #pragma unroll
-    for (int n = 0; n < kPairs; ++n) {
-      const int axis = p.axes != nullptr ? imin(imax(p.axes[first + n], 0), p.n_axes - 1) : 0;
-      cs[n] = turn(at_token[axis * p.pos_axis], p.inv_freq[first + n]);
-      if (p.inverse) cs[n].y = -cs[n].y;
-    }
+  for (int n = 0; n < kPairs; n += 2) {
+    const float4 x = both[n / 2][threadIdx.x % kItems<T, V>];
+    cs[n] = make_float2(x.x, x.y);
+    if (n + 1 < kPairs) cs[n + 1] = make_float2(x.z, x.w);
   }
   int slot = -1, page = 0, row = 0;
   if constexpr (kAppend) {
@@ -88,7 +105,8 @@ __global__ void __launch_bounds__(kThreads, 8) rotate_kernel(const __grid_consta
     row = slot - page * p.page;
   }
 
-  const int h0 = (int)((long long)p.heads * blockIdx.y / p.slices), h1 = (int)((long long)p.heads * (blockIdx.y + 1) / p.slices);
+  const int slice = (int)blockIdx.y * (kThreads / kItems<T, V>) + (int)threadIdx.x / kItems<T, V>;
+  const int h0 = (int)((long long)p.heads * slice / p.slices), h1 = (int)((long long)p.heads * (slice + 1) / p.slices);
   using VecT = Vec<T, V>;
   // Heads [from, to) of one tensor, kBatch at a time: as many loads on their way before the first store.
   auto go = [&](const char* src, long long src_head, char* dst, long long dst_head, long long src_chan, long long dst_chan, int count, bool rotate) {
@@ -152,13 +170,13 @@ static cudaError_t launch_rotate(RotateP& p, int vec, bool paired, cudaStream_t 
   p.per_row = p.turning + (p.D - 2 * p.pairs) / vec;
   const long long items = (long long)p.B * p.L * p.per_row;
   p.items = (unsigned)items;
-  const long long blocks = (items + kThreads - 1) / kThreads;
-  // Heads in as many slices as fill the SMs with 16 blocks each (8: 89 us instead of 87, and 32: 123)
-  const long long want = 16ll * sm_count();
-  p.slices = (int)(blocks >= want ? 1 : (want + blocks - 1) / blocks);
-  p.slices = imax(1, imin(p.slices, p.heads));
-  const dim3 grid((unsigned)blocks, (unsigned)imin(p.slices, 65535));
-  p.slices = (int)grid.y;
+  const int per_block = vec * (int)sizeof(T) == 16 ? 32 : kThreads, shares = kThreads / per_block;  // kItems
+  const long long blocks = (items + per_block - 1) / per_block;
+  // Heads in as many slices as fill the SMs with 8 blocks each (a prompt's 4000 tokens, 24 and 8 heads: 16.9 us, with 16 17.8); a block has `shares` of them
+  const long long want = 8ll * sm_count();
+  const long long more = blocks >= want ? 1 : (want + blocks - 1) / blocks;
+  const dim3 grid((unsigned)blocks, (unsigned)imax(1, imin((int)more, (p.heads + shares - 1) / shares)));
+  p.slices = (int)grid.y * shares;
 #define CHILL_ROTATE(VEC)                                                     \
   case VEC:                                                                   \
     if (paired) rotate_kernel<T, VEC, true, kAppend><<<grid, kThreads, 0, st>>>(p); \
