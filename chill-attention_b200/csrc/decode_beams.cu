@@ -304,9 +304,12 @@ __global__ void __launch_bounds__(kThreads, 4) scan_kernel(const __grid_constant
       uint32_t* words = reinterpret_cast<uint32_t*>(raw);
       const bool odd = reinterpret_cast<uintptr_t>(row) % 4 != 0;
       const uint32_t* at = reinterpret_cast<const uint32_t*>(reinterpret_cast<uintptr_t>(row) / 4 * 4) + n0 * 4 + threadIdx.x;
-      if (whole && n0 > 0 && sizeof(T) == 2 && odd) {
+      if (whole && sizeof(T) == 2 && odd) {
 #pragma unroll
-        for (int i = 0; i < 4 * kBatch; ++i) words[i] = __funnelshift_r(__ldg(at + i * kThreads), __ldg(at + i * kThreads + 1), 16);
+        for (int i = 0; i < 4 * kBatch; ++i) {
+          if (i == 0 && n0 == 0 && threadIdx.x == 0) words[i] = word_of(0);  // half of the first word is another's
+          else words[i] = __funnelshift_r(__ldg(at + i * kThreads), __ldg(at + i * kThreads + 1), 16);
+        }
       } else if (whole && !(sizeof(T) == 2 && odd)) {
 #pragma unroll
         for (int i = 0; i < 4 * kBatch; ++i) words[i] = __ldg(at + i * kThreads);

@@ -66,8 +66,14 @@ __device__ __forceinline__ int block_scan(int v, int& total) {
 //
 // Latency is all there is: one cluster, whose barriers separate the steps, and few trips to memory one after the other.  Every CTA has a share of the rows and keeps them as they
 // were in shared memory, where children in other CTAs find them too (in the workspace where they are too large: kInside false); what goes back is noted there in bits.
-// 4 beams of 700 tokens in pages of 16: 10 us; 16 groups of 16 beams of up to 16384 tokens (256 rows of 1026 blocks): 28 us in a cluster of 16 CTAs (8: 38), of which the rows' way into
+// 4 beams of 700 tokens in pages of 16: 10 us (two of them a launch); 16 groups of 16 beams of up to 16384 tokens (256 rows of 1026 blocks): 28 us in a cluster of 16 CTAs (8: 38), of which the rows' way into
 // shared memory 5, counts 3, claims 6 (scattered reads of shared), new tables 4, barriers 4.  Row by row with an atomic for every entry, and the rows in the workspace: 53 us.
+
+// A cluster's barrier costs one CTA alone 0.5 us more than its own.
+__device__ __forceinline__ void sync_all(const cg::cluster_group& cluster, int ctas) {
+  if (ctas > 1) cluster.sync();
+  else __syncthreads();
+}
 
 // Rows that a warp has at a time, 32 blocks of each: what neighbouring rows share (the beams of a request, nearly everything) is counted in registers before it is
 // counted in memory.
@@ -150,7 +156,7 @@ __global__ void __launch_bounds__(kPageThreads) share_kernel(const __grid_consta
       }
       summary[r] = s;
     }
-    cluster.sync();  // what rows held is written down
+    sync_all(cluster, ctas);  // what rows held is written down
     for (int r = r0 + threadIdx.x; r < r1; r += threads) {
       const int i = r - r0;
       const int2 s = summary[r];
@@ -223,7 +229,7 @@ __global__ void __launch_bounds__(kPageThreads) share_kernel(const __grid_consta
       }
     }
   }
-  cluster.sync();  // the counts are complete
+  sync_all(cluster, ctas);  // the counts are complete
 
   // Claims to the pages that nobody holds.  `back` notes for whose
   auto claim_of = [&](int r, int j) { return (int)(-1 - entries + ((long long)r * p.width + j)); };
@@ -297,7 +303,7 @@ __global__ void __launch_bounds__(kPageThreads) share_kernel(const __grid_consta
       *p.missing = imax(taken - n_free, 0);
     }
   }
-  cluster.sync();  // the lowest claims are there; what was taken from the stack, and other CTAs' rows, have been read
+  sync_all(cluster, ctas);  // the lowest claims are there; what was taken from the stack, and other CTAs' rows, have been read
 
   // How many pages every row puts on the stack: those of which its claim is the lowest
   for (int item = warp; item < (r1 - r0) * words; item += warps) {
@@ -321,7 +327,7 @@ __global__ void __launch_bounds__(kPageThreads) share_kernel(const __grid_consta
     own += total;
   }
   if (threadIdx.x == 0) own_total = own;
-  cluster.sync();
+  sync_all(cluster, ctas);
   int earlier = 0, all = 0;
   for (int c = 0; c < ctas; ++c) {
     const int n = *cluster.map_shared_rank(&own_total, c);
@@ -370,18 +376,18 @@ __global__ void __launch_bounds__(kPageThreads) compact_kernel(const __grid_cons
   int* const moves = totals + kPageCtas;        // [1]
   const int n_free = imin(imax(*p.n_free, 0), p.num_pages);
   for (int q = p0 + threadIdx.x; q < p1; q += kPageThreads) to[q] = q;
-  cluster.sync();
+  sync_all(cluster, ctas);
   for (int i = thread; i < n_free; i += threads) {
     const int q = p.free_pages[i];
     if (q >= 0 && q < p.num_pages) to[q] = -1;
   }
-  cluster.sync();
+  sync_all(cluster, ctas);
   int own = 0;
   for (int q = p0 + threadIdx.x; q < p1; q += kPageThreads) own += __ldcg(&to[q]) < 0 ? 1 : 0;
   int free_here;
   block_scan(own, free_here);
   if (threadIdx.x == 0) totals[cta] = free_here;
-  cluster.sync();
+  sync_all(cluster, ctas);
   int before = 0, all = 0;
   for (int c = 0; c < ctas; ++c) {
     const int n = __ldcg(&totals[c]);
@@ -406,7 +412,7 @@ __global__ void __launch_bounds__(kPageThreads) compact_kernel(const __grid_cons
     if (q == used) *moves = free_before;  // holes
   }
   if (used == p.num_pages && thread == 0) *moves = 0;
-  cluster.sync();
+  sync_all(cluster, ctas);
   const int count = __ldcg(moves);
   for (int i = thread; i < p.orders; i += threads) {
     if (i < count) {
@@ -426,7 +432,7 @@ __global__ void __launch_bounds__(kPageThreads) compact_kernel(const __grid_cons
     *p.count = count;
     *p.n_free = all;
   }
-  cluster.sync();
+  sync_all(cluster, ctas);
   constexpr int kUnroll = 8;
   const int warp = thread >> 5, warps = threads >> 5, lane = threadIdx.x & 31, pieces = (p.width + 32 * kUnroll - 1) / (32 * kUnroll);
   for (long long item = warp; item < (long long)p.B * pieces; item += warps) {
