@@ -33,7 +33,7 @@ def _check_select(logits, scores, count, finished, end_token):
     assert logits.ndim == 2 and logits.numel() > 0 and logits.dtype in cache._DTYPES, "logits must be [groups * beams, vocab], fp16 / bf16 / fp32"
     V = logits.shape[1]
     assert logits.stride(1) == 1 or V == 1, "the elements of a row of logits must lie beside each other"
-    assert V <= 2 ** 30 and logits.shape[0] <= 65535
+    assert V <= 2 ** 26 and logits.shape[0] <= 65535
     assert scores.ndim == 2 and scores.dtype == torch.float32 and scores.is_contiguous() and scores.device == logits.device and \
         scores.numel() == logits.shape[0], "scores must be a contiguous float32 tensor [groups, beams] with a row of logits for each"
     K = scores.shape[1]
@@ -68,7 +68,7 @@ def chill_beam_select(logits: torch.Tensor, scores: torch.Tensor, count: int | N
 
     Candidate (beam, token) of a group has ``scores[group, beam] + log_softmax(logits[row])[token]``, row = group * beams + beam; -inf where the logit or the beam's score
     is -inf (a row of nothing but -inf has no candidates).  They are ranked by that value in 64 bits, and it is rounded to fp32 at the end; of equal ones the lowest
-    beam, then the lowest token comes first.  (Scores beyond 1e13, where 64 bits do not tell the candidates of a beam apart: its largest logits stand for them.)  A NaN or +inf among a row's logits makes its candidates NaN, which rank first: they show.
+    beam, then the largest logit, then the lowest token comes first.  (Logits differ at one value where 64 bits round it, as with scores beyond 1e9.)  A NaN or +inf among a row's logits makes its candidates NaN, which rank first: they show.
 
     Args:
         logits: [groups * beams, vocab], fp16 / bf16 / fp32; rows any stride apart.

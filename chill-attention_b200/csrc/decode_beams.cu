@@ -111,12 +111,18 @@ __device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
   return d;
 }
 
-// A candidate in the order of its 64-bit score, then of its place: beam and token, side by side and inverted (larger is earlier).
+// A candidate in the order of its 64-bit score, then of beam, logit and token, side by side and inverted (larger is earlier).  A row's list is in the order of the logits; 64 bits may
+// round several of them to one score (a beam marked with -1e30), and the logit in the place leaves the list in order, which merging needs.
 struct Candidate {
   uint64_t rank, place;
 };
-constexpr int kTokenBits = 31;
-__device__ __forceinline__ uint64_t place_at(int beam, int token) { return ~((uint64_t)beam << kTokenBits | (uint64_t)token); }
+constexpr int kTokenBits = 26, kBeamBit = kTokenBits + 32;
+static_assert(kMost <= 1 << (64 - kBeamBit), "a beam has too few bits");
+__device__ __forceinline__ uint64_t place_at(int beam, uint32_t order, int token) {
+  return ~((uint64_t)beam << kBeamBit | (uint64_t)~order << kTokenBits | (uint64_t)token);
+}
+__device__ __forceinline__ int beam_at(uint64_t place) { return (int)(~place >> kBeamBit); }
+__device__ __forceinline__ int token_at(uint64_t place) { return (int)(~place & ((1u << kTokenBits) - 1)); }
 __device__ __forceinline__ bool before(const Candidate& a, const Candidate& b) { return a.rank != b.rank ? a.rank > b.rank : a.place > b.place; }
 
 __device__ __forceinline__ bool before(uint64_t a, uint64_t b) { return a > b; }
@@ -549,7 +555,7 @@ __global__ void __launch_bounds__(kMergeWarps * 32) merge_kernel(const __grid_co
   }
   any_flat = __syncthreads_or(any_flat) != 0;
   auto candidate = [&](int k, float x, int v) {
-    return Candidate{rank_of((double)score[k] + ((double)x - lse[k])), place_at(k, v)};
+    return Candidate{rank_of((double)score[k] + ((double)x - lse[k])), place_at(k, flat[k] ? 0 : order_of(x), v)};
   };
   auto usable = [&](int k) { return score[k] != -INFINITY && !over[k] && !flat[k]; };
 
@@ -580,7 +586,7 @@ __global__ void __launch_bounds__(kMergeWarps * 32) merge_kernel(const __grid_co
     const int k = l / p.parts;
     if (usable(k)) return key != 0 ? candidate(k, value_of(key), place_of(key)) : Candidate{0, 0};
     if (over[k] && e == 0 && l == k * p.parts && score[k] != -INFINITY)  // a finished beam: a list of one
-      return Candidate{rank_of((double)score[k]), place_at(k, p.end_token)};
+      return Candidate{rank_of((double)score[k]), place_at(k, 0, p.end_token)};
     return Candidate{0, 0};
   };
   auto merge_all = [&]() {
@@ -697,7 +703,8 @@ __global__ void __launch_bounds__(kMergeWarps * 32) merge_kernel(const __grid_co
       for (int i = 0; i < kEach; ++i) {
         const int l = l0 + i * warps, k = l / p.parts;
         if (l >= lists) break;
-        const float floor = bound == 0 ? -INFINITY : __double2float_rd(least - (double)score[k] + lse[k] - 1e-6);
+        const double s = score[k], error = 1e-15 * (fabs(least) + fabs(s) + fabs(lse[k]));  // of the sum here and of the score's, 2^-53 each
+        const float floor = bound == 0 ? -INFINITY : __double2float_rd(least - s + lse[k] - error);
 #pragma unroll
         for (int r = 0; r < R; ++r) {
           const bool may = over[k] ? l == k * p.parts && lane == 0 && r == 0 : key[i][r] != 0 && !(value_of(key[i][r]) < floor);
@@ -758,7 +765,7 @@ __global__ void __launch_bounds__(kMergeWarps * 32) merge_kernel(const __grid_co
     const int e = lane + 32 * r;
     if (e >= p.M) continue;
     const long long to = (long long)group * p.M + e;
-    int k = (int)(~best.x[r].place >> kTokenBits), v = (int)(~best.x[r].place & ((1u << kTokenBits) - 1));
+    int k = beam_at(best.x[r].place), v = token_at(best.x[r].place);
     double value = -INFINITY;
     if (e < total) {
       value = value_of_rank(best.x[r].rank);
@@ -768,8 +775,8 @@ __global__ void __launch_bounds__(kMergeWarps * 32) merge_kernel(const __grid_co
         so_far = skipped;
         skipped = 0;
         for (int i = 0; i < total; ++i) {
-          const uint64_t place = ~exchange[1][i].place;
-          skipped += (long long)(place >> kTokenBits) * p.V + (long long)(place & ((1u << kTokenBits) - 1)) <= e - total + so_far;
+          const uint64_t place = exchange[1][i].place;
+          skipped += (long long)beam_at(place) * p.V + token_at(place) <= e - total + so_far;
         }
       }
       k = (int)((e - total + skipped) / p.V);
@@ -801,7 +808,7 @@ static size_t workspace_of(const chill_select_args& a) {
 static int check_select(const chill_select_args* a, bool pointers) {
   if (a == nullptr || a->G <= 0 || a->K <= 0 || a->M <= 0 || a->V <= 0) return CHILL_E_INVALID;
   if (!known_dtype(a->dtype)) return CHILL_E_UNSUPPORTED;
-  if (a->K > kMost || a->M > kMost || a->V > (1ll << 30) || (long long)a->G * a->K > kMaxRequests) return CHILL_E_TOO_LARGE;
+  if (a->K > kMost || a->M > kMost || a->V > (1ll << kTokenBits) || (long long)a->G * a->K > kMaxRequests) return CHILL_E_TOO_LARGE;
   if (a->M > a->K * a->V) return CHILL_E_INVALID;
   if (!pointers) return CHILL_OK;
   if (!a->logits || !a->scores || !a->out_scores || !a->out_rows || !a->out_tokens) return CHILL_E_INVALID;

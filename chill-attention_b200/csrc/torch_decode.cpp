@@ -200,7 +200,7 @@ py::object rotate_append(const DecodeLibrary& lib, const Tensor& q, const Tensor
 py::object beam_select(const DecodeLibrary& lib, const Tensor& logits, const Tensor& scores, int64_t count, const std::optional<Tensor>& finished, int64_t end_token) {
   if (watched({&logits, &scores}, finished) || logits.dim() != 2 || logits.numel() == 0 || !fit(logits) || dtype_of(logits) < 0 || !logits.is_cuda()) return py::none();
   const int64_t rows = logits.size(0), V = logits.size(1);
-  if ((logits.stride(1) != 1 && V > 1) || V > (1 << 30)) return py::none();
+  if ((logits.stride(1) != 1 && V > 1) || V > (1 << 26)) return py::none();
   if (scores.dim() != 2 || scores.scalar_type() != at::kFloat || !scores.is_contiguous() || scores.device() != logits.device() || scores.numel() != rows) return py::none();
   const int64_t G = scores.size(0), K = scores.size(1);
   if (K > CHILL_SELECT_MAX || rows > 65535 || count < 1 || count > CHILL_SELECT_MAX || count > K * V) return py::none();

@@ -53,13 +53,13 @@ int chill_rotate_append(const chill_rotate_args* a, void* stream);
 /* ------------------------------------------------------------------------------------------------------------------
  * Selection over beams and vocabulary.  Candidate (k, v) of group g: c = scores[g][k] + x - log sum exp x', x = logits[g * K + k][v], the sum over the
  * row; -inf where the logit or the beam's score is -inf.  A finished beam has one candidate, (k, end_token) with c = scores[g][k], and its
- * logits are not looked at.  The M candidates of the largest c, worked out in 64 bits, in descending order, ties to the lowest k * V + v; NaN counts as
- * largest (a NaN or +inf among a row's logits makes all its candidates NaN, but for those of -inf).  Where 64 bits do not tell the candidates of one beam apart
- * (scores beyond 1e13) those of its M largest logits stand for them. */
+ * logits are not looked at.  The M candidates of the largest c, worked out in 64 bits, in descending order, of equal ones the lowest k, then the largest x (they
+ * differ where 64 bits round c to one number: scores beyond 1e9), then the lowest v; NaN counts as largest (a NaN or +inf among a row's logits makes all its
+ * candidates NaN, but for those of -inf: the lowest v first). */
 #define CHILL_SELECT_MAX 64 /* beams of a group, and candidates that are kept */
 typedef struct chill_select_args {
   int32_t G, K, M, dtype;
-  int64_t V;               /* <= 2^30 */
+  int64_t V;               /* <= 2^26 */
   const void* logits;      /* [G * K][V], rows row_stride elements apart, their elements adjacent */
   int64_t row_stride;
   const float* scores;     /* [G][K], logarithms; -inf: no such beam */
@@ -72,7 +72,7 @@ typedef struct chill_select_args {
   size_t workspace_bytes;
 } chill_select_args;
 /* 1 <= K, M <= CHILL_SELECT_MAX, M <= K * V, G * K <= 65535. */
-size_t chill_select_workspace_bytes(const chill_select_args* a); /* from G, K, M, V and dtype alone */
+size_t chill_select_workspace_bytes(const chill_select_args* a); /* from G, K, M, V, dtype and the current device alone */
 int chill_beam_select(const chill_select_args* a, void* stream);
 
 /* ------------------------------------------------------------------------------------------------------------------

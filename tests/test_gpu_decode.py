@@ -487,6 +487,28 @@ def test_select_with_marks_for_missing_beams(ca, mark):
     assert (out.parents.cpu() == torch.tensor([[0], [4]])).all()
 
 
+@pytest.mark.parametrize("K,M,V", [(4, 64, 500), (4, 64, 20), (3, 17, 30000), (40, 64, 700), (40, 64, 3), (64, 5, 9000)])
+@pytest.mark.parametrize("score", [-2.0 ** 50, -1e30, torch.finfo(torch.float32).min])
+def test_select_where_scores_hide_the_logits(ca, K, M, V, score):
+    """Scores so large that 64 bits round a beam's candidates to few numbers, or to one: the lowest beam, then the largest logit, then the lowest token comes first."""
+    g = torch.Generator().manual_seed(V)
+    row = torch.randint(-12, 12, (V,), generator=g) / 4.0
+    rows = torch.stack([row[torch.randperm(V, generator=g)] for _ in range(K)])  # one row in several orders, for one sum
+    scores = torch.full((1, K), score)
+    scores[0, K // 2] *= 0.5
+    beam, token = torch.arange(K)[:, None].expand(K, V).flatten(), torch.arange(V).repeat(K)
+    value = scores[0].double()[:, None] + (rows.double() - torch.logsumexp(row.double(), 0))
+    order = sorted(range(K * V), key=lambda n: (-value.flatten()[n].item(), beam[n].item(), -rows.flatten()[n].item(), n)) if K * V <= 4000 else None
+    if order is None:  # stable sorts, the last key first
+        order = torch.arange(K * V)
+        for key in (-rows.flatten(), beam, -value.flatten()):
+            order = order[key[order].sort(stable=True).indices]
+    order = torch.as_tensor(order)[:M]
+    out = ca.chill_beam_select(rows.cuda(), scores.cuda(), M)
+    assert out.parents[0].tolist() == beam[order].tolist() and out.tokens[0].tolist() == token[order].tolist()
+    assert torch.equal(out.scores[0].cpu(), value.flatten()[order].float())
+
+
 def test_fork_of_the_largest_batch(ca):
     """8192 requests, every other one twice, in a cluster; shared memory beyond the default limit."""
     B, page = 8192, 4
