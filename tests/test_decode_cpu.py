@@ -106,6 +106,17 @@ def test_selection_refusals(lib):
     assert call(finished=4096, end_token=100) == call(finished=4096, end_token=-1) == -1
 
 
+def test_the_largest_vocabulary(lib):
+    """A token has 26 bits beside its beam and its logit."""
+    from chill_attention import _decode_abi as abi
+
+    def call(V):
+        return lib.chill_beam_select(made(abi.SelectArgs, ("logits", "scores", "out_scores", "out_rows", "out_tokens"), G=1, K=1, M=1, dtype=0, V=V, row_stride=V), None)
+
+    assert call(2 ** 26 + 1) == call(2 ** 31) == -4
+    assert call(2 ** 26) == -1  # what is missing is the workspace
+
+
 def test_page_refusals(lib):
     from chill_attention import _decode_abi as abi
 

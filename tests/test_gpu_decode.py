@@ -509,6 +509,20 @@ def test_select_where_scores_hide_the_logits(ca, K, M, V, score):
     assert torch.equal(out.scores[0].cpu(), value.flatten()[order].float())
 
 
+def test_select_of_the_largest_vocabulary(ca):
+    V = 2 ** 26
+    x = torch.zeros(2, V, dtype=torch.bfloat16, device="cuda")
+    places = [(0, V - 1, 30.0), (1, 0, 29.0), (1, V - 1, 28.0), (0, V // 2, 27.0)]
+    for beam, token, value in places:
+        x[beam, token] = value
+    out = ca.chill_beam_select(x, torch.zeros(1, 2, device="cuda"), 4)
+    lse = [math.log((V - 2) + sum(math.exp(v) for b, _, v in places if b == beam)) for beam in range(2)]
+    want = sorted(((v - lse[b], b, t) for b, t, v in places), reverse=True)
+    assert list(zip(out.parents[0].tolist(), out.tokens[0].tolist())) == [(b, t) for _, b, t in want]
+    # half a step of fp32, of the results; a batch's 32 terms of at most 1 are added up in fp32 (2^-19 of their sum, below 2^-26 of the whole)
+    assert all(abs(got - w[0]) <= 2.0 ** -24 * abs(w[0]) + 2.0 ** -18 for got, w in zip(out.scores[0].tolist(), want))
+
+
 def test_fork_of_the_largest_batch(ca):
     """8192 requests, every other one twice, in a cluster; shared memory beyond the default limit."""
     B, page = 8192, 4
