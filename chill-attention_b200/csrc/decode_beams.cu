@@ -270,7 +270,7 @@ __device__ __forceinline__ int shrink(Kept& kept, int count, int M, uint64_t& li
 //
 // Warps stream on their own: sums in registers, vectors that reach the limit in a queue of their own, which are looked at value by value after a round of some batches.  32 groups of
 // 8 beams over 128000 tokens, bf16: a segment's first batch and limit 4 us, the other seven 10 (5.8 TB/s), queue, sorting and sum 4; SMs with four CTAs are done 6 us after those with three.
-// 128 threads a CTA, 8 of them an SM: 33 us instead of 30; half as long segments 31; the next batch's loads ahead of this one's work (3 CTAs an SM) no gain.
+// 128 threads a CTA, 8 of them an SM: 33 us instead of 30; half as long segments 31; the next batch's loads ahead of this one's work (3 CTAs an SM) no gain; the segment's rest prefetched into L2 31 to 33.
 template <class T, bool kShifted>
 __global__ void __launch_bounds__(kThreads, 4) scan_kernel(const __grid_constant__ SelectP p) {
   constexpr int V = 16 / sizeof(T), kWord = 4 / sizeof(T), kStep = kThreads * kBatch;
