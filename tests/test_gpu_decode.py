@@ -475,6 +475,19 @@ def test_cache_copy_of_one_tensor(ca):
     assert torch.equal(cache, expected)
 
 
+@pytest.mark.parametrize("dtype,V", [(torch.float32, 5000), (torch.bfloat16, 40001)])
+def test_select_of_one_row_for_all_beams(ca, dtype, V):
+    """Rows no elements apart, and rows that overlap: equal beams are ties, the lowest first."""
+    row = torch.randn(V + 40, generator=torch.Generator().manual_seed(V)).to(dtype)
+    for step in (0, 1, 8):
+        rows = row.cuda().as_strided((6, V), (step, 1))
+        scores = torch.tensor([[-1.0, 0.0, 0.0], [0.0, 0.0, -0.5]])
+        out = ca.chill_beam_select(rows, scores.cuda(), 7)
+        want, parents, tokens = orc.select(rows.cpu(), scores, 7)
+        assert torch.equal(out.parents.cpu().long(), parents) and torch.equal(out.tokens.cpu().long(), tokens)
+        check_select(out, rows, scores, 7)
+
+
 @pytest.mark.parametrize("mark", [-1e9, torch.finfo(torch.float32).min])
 def test_select_with_marks_for_missing_beams(ca, mark):
     """The first step with a low score instead of -inf for the beams that are not there yet."""
