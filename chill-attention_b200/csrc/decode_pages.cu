@@ -14,6 +14,7 @@ constexpr int kPageCtas = 8;
 constexpr int kMaxCtas = 16;
 constexpr int kForkRequests = 8192;
 constexpr int kMostShared = 200 * 1024;
+constexpr size_t kUnasked = 40 * 1024;  // dynamic shared memory that every kernel here gets beside its static one
 
 struct ShareP {
   int B, page, num_pages, width;
@@ -483,7 +484,8 @@ template <class F>
 static int launch_cluster(F kernel, const ShareP& p, int ctas, int threads, size_t smem, cudaStream_t st, const char* what) {
   cudaLaunchConfig_t cfg{};
   cudaLaunchAttribute attr[1];
-  if (smem > 48 * 1024) {  // always to the same limit: host threads may be here at once
+  // 48 KB without asking, of which a kernel's static shared memory takes its part.  Always to the same limit: host threads may be here at once
+  if (smem > kUnasked) {
     const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kMostShared);
     if (e != cudaSuccess) return record_cuda_failure(e, what);
   }
