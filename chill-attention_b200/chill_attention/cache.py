@@ -118,6 +118,13 @@ def _check_sizes(**named):
             assert size < 2 ** 31, f"the sizes of {name} must fit 32 bits"
 
 
+def _check_changed(**named):
+    """Tensors that a call changes in place: torch cannot apply a pending sign there for an operator that also returns something."""
+    if not _is_compiling():
+        for name, t in named.items():
+            assert not t.is_neg(), f"{name} is changed in place and has a sign that is still to be applied: resolve_neg() makes a tensor of its own"
+
+
 def _check_table(table):
     _check_sizes(table=table)
     assert table.is_cuda, "the paged cache runs on CUDA tensors only"
@@ -131,6 +138,7 @@ def _check_pages(pages, lens, page_size):
     assert 1 <= page_size < 2 ** 31 and pages.free.ndim == 1 and pages.free.numel() >= 1
     _check_sizes(free=pages.free)
     _check_ints(pages.table, held=(pages.held, (B,)), free=(pages.free, pages.free.shape), n_free=(pages.n_free, (1,)), lens=(lens, (B,)))
+    _check_changed(table=pages.table, held=pages.held, free=pages.free, n_free=pages.n_free)
 
 
 def _check_caches(k_cache, v_cache):
@@ -155,6 +163,7 @@ def _check_rows(k_cache, v_cache, k, v, slots):
     assert k.shape[1] == k_cache.shape[1] and k.shape[3] == k_cache.shape[3], "kv heads and head dim must be those of the caches"
     assert k.dtype == v.dtype == k_cache.dtype and k.device == v.device == k_cache.device
     _check_ints(k_cache, slots=(slots, (k.shape[0], k.shape[2])))
+    _check_changed(k_cache=k_cache, v_cache=v_cache)
     _check_grad(k_cache, v_cache, k, v)
 
 
@@ -166,6 +175,7 @@ def _check_commit(k_cache, v_cache, table, lens, new_lens, path, accepted):
     _check_sizes(path=path)
     assert path.ndim == 2 and path.shape[1] >= 1, "path must be [batch, longest path]"
     _check_ints(k_cache, lens=(lens, (B,)), new_lens=(new_lens, (B,)), path=(path, (B, path.shape[1])), accepted=(accepted, (B,)))
+    _check_changed(k_cache=k_cache, v_cache=v_cache)
     _check_grad(k_cache, v_cache)
 
 
@@ -280,12 +290,14 @@ def _check_fork(pages, shared, lens, parents, page_size):
     B = pages.table.shape[0]
     assert B <= 8192, "a fork takes at most 8192 requests"
     _check_ints(pages.table, missing=(pages.missing, (1,)), shared=(shared, pages.free.shape), parents=(parents, (B,)))
+    _check_changed(missing=pages.missing, shared=shared)
 
 
 def _check_compact(pages, page_size, shared):
     _check_pages(pages, pages.held, page_size)
     if shared is not None:
         _check_ints(pages.table, shared=(shared, pages.free.shape))
+        _check_changed(shared=shared)
 
 
 def _check_copy(k_cache, v_cache, copies):
@@ -298,6 +310,7 @@ def _check_copy(k_cache, v_cache, copies):
     assert isinstance(source, torch.Tensor) and source.ndim == 1 and source.numel() > 0
     _check_sizes(source=source)
     _check_ints(k_cache, source=(source, source.shape), target=(target, source.shape), rows=(rows, source.shape), count=(count, (1,)))
+    _check_changed(k_cache=k_cache, v_cache=v_cache)
     _check_grad(k_cache, v_cache)
 
 
@@ -356,10 +369,12 @@ def _check_reserve(pages, new_lens, max_new, parents, stored):
     B = pages.table.shape[0]
     assert 1 <= max_new < 2 ** 31
     _check_ints(pages.table, missing=(pages.missing, (1,)), new_lens=(new_lens, (B,)))
+    _check_changed(missing=pages.missing)
     if parents is not None:
         _check_ints(pages.table, parents=(parents, (B, max_new)))
     if stored is not None:
         _check_ints(pages.table, stored=(stored, (B,)))
+        _check_changed(stored=stored)
 
 
 def chill_pages_reserve(pages: ChillPages, lens: torch.Tensor, new_lens: torch.Tensor, max_new: int, page_size: int,
@@ -408,6 +423,7 @@ def chill_pages_trim(pages: ChillPages, lens: torch.Tensor, page_size: int, shar
             return
         _check_pages(pages, lens, page_size)
         _check_ints(pages.table, shared=(shared, pages.free.shape))
+        _check_changed(shared=shared)
         _trim_shared_op(*_places(pages), shared, lens, page_size)
         return
     if _direct() and _eager.extension().pages_trim(_NATIVE.get(None) or _native(), pages.table, pages.held, pages.free, pages.n_free, lens, page_size):

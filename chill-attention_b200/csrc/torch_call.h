@@ -18,9 +18,11 @@ using at::Tensor;
 // Without the dispatcher: 0.7 us instead of 1.1, and a call makes up to three.
 inline Tensor empty(at::IntArrayRef sizes, at::ScalarType type, const Tensor& like) { return at::detail::empty_cuda(sizes, type, like.device(), std::nullopt); }
 
-// A tensor that something looks in on (a subclass with its own dispatch, a transform): the dispatcher ops serve it.
+// A tensor that something looks in on (a subclass with its own dispatch, a transform), or of which the memory is not the numbers: a sign still to be applied (z.conj().imag),
+// zeros that were never written.  The dispatcher ops serve it.
 inline bool watched(std::initializer_list<const Tensor*> tensors, const std::optional<Tensor>& one_more = std::nullopt, const std::optional<Tensor>& another = std::nullopt) {
-  auto looked_at = [](const Tensor& t) { return t.unsafeGetTensorImpl()->key_set().has_any(c10::python_ks | c10::functorch_transforms_ks); };
+  constexpr c10::DispatchKeySet kOthers = c10::python_ks | c10::functorch_transforms_ks | c10::DispatchKeySet({c10::DispatchKey::Negative, c10::DispatchKey::ZeroTensor});
+  auto looked_at = [](const Tensor& t) { return t.unsafeGetTensorImpl()->key_set().has_any(kOthers); };
   for (const Tensor* t : tensors)
     if (looked_at(*t)) return true;
   return (one_more.has_value() && looked_at(*one_more)) || (another.has_value() && looked_at(*another));
