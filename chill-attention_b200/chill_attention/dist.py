@@ -226,7 +226,7 @@ class _SequenceShardedAttention(torch.autograd.Function):
         else:
             kbuf, vbuf = halo_buffers
             for buf, t in ((kbuf, k), (vbuf, v)):
-                if buf.local.data_ptr() != t.data_ptr() or buf.local.shape != t.shape or buf.local.stride() != t.stride():
+                if buf.local.data_ptr() != t.data_ptr() or buf.local.shape != t.shape or buf.local.stride() != t.stride() or t.is_neg():
                     raise ValueError("halo_buffers must be the HaloBuffers whose .local views were passed as k and v")
                 if buf.left < cap_l or buf.right < cap_r:
                     raise ValueError(f"HaloBuffer has ({buf.left}, {buf.right}) spare rows, the mask needs ({cap_l}, {cap_r})")
@@ -261,7 +261,7 @@ class _SequenceShardedAttention(torch.autograd.Function):
         Hkv = k.shape[1]
         dev = q.device
         acc_dtype = torch.float64 if k.dtype == torch.float64 else torch.float32
-        do = do.contiguous()
+        do = do.resolve_neg().contiguous()
         # Gradients in the memory order of their tensors (a dense K / V view of a HaloBuffer is position-major):
         # autograd then accumulates them as they are instead of re-laying them out with a strided copy.
         dq, dk, dv = torch.empty_like(q), torch.empty_like(k), torch.empty_like(v)
@@ -355,5 +355,6 @@ def sequence_sharded_attention(q, k, v, mask: ChillMask, seq_len: int, sm_scale=
     copies k and v into them once."""
     if sm_scale is None:
         sm_scale = q.shape[-1] ** -0.5
+    q = q.resolve_neg()  # k and v are copied, or lie in the caller's buffers
     return _SequenceShardedAttention.apply(q, k, v, mask, seq_len, sm_scale, group, local_forward, local_backward,
                                            halo_buffers)

@@ -57,11 +57,11 @@ def attention_fwd_bwd_host(q, k, v, do, mask: ChillMask, sm_scale=None, out=None
     if sm_scale is None:
         sm_scale = D ** -0.5
     lib, functor = _resolve_functor(mask)
-    q, k, v, do = (t if t.is_contiguous() else t.contiguous() for t in (q, k, v, do))
+    q, k, v, do = (t.resolve_neg().contiguous() for t in (q, k, v, do))  # as they are, where memory holds the numbers
     if out is None:
         out = tuple(torch.empty(t.shape, dtype=t.dtype).pin_memory() for t in (q, q, k, v))
     for t, like in zip(out, (q, q, k, v)):
-        assert t.shape == like.shape and t.dtype == like.dtype and t.is_contiguous() and not t.is_cuda
+        assert t.shape == like.shape and t.dtype == like.dtype and t.is_contiguous() and not t.is_cuda and not t.is_neg()
     G = H // Hkv
     if chunk_heads is None:
         per_group = L * D * q.element_size() * (2 * G + 2)

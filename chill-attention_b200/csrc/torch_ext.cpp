@@ -81,6 +81,9 @@ bool tma_compatible(const Tensor& t) {
 // otherwise take the call.
 Tensor packed(const Tensor& t) { return t.scalar_type() == at::kFloat || tma_compatible(t) ? t : t.contiguous(); }
 
+// Memory that holds the numbers themselves: of a tensor with a sign still to be applied (z.conj().imag) a copy.
+Tensor signed_as_stored(const Tensor& t) { return t.is_neg() ? t.resolve_neg() : t; }
+
 void set_strides(int64_t* dst, const Tensor& t) {
   for (int64_t d = 0; d < t.dim(); ++d) dst[d] = t.stride(d);
 }
@@ -136,10 +139,10 @@ struct AttentionFn : torch::autograd::Function<AttentionFn> {
     const auto holder = ctx->saved_data["call"].toCapsule();
     const Call& c = *static_cast<const Call*>(holder.get());
     c10::cuda::CUDAGuard guard(q.device());
-    Tensor d_o = grads[0].defined() ? grads[0] : at::zeros_like(o);
+    Tensor d_o = grads[0].defined() ? signed_as_stored(grads[0]) : at::zeros_like(o);
     // Autograd often hands over an expanded tensor (all strides 0 after o.sum().backward()) or a transposed view
     if (!tma_compatible(d_o)) d_o = d_o.contiguous();
-    Tensor d_lse = grads[1].defined() ? grads[1].to(at::kFloat) : Tensor();  // gradient through a returned LSE
+    Tensor d_lse = grads[1].defined() ? signed_as_stored(grads[1]).to(at::kFloat) : Tensor();  // gradient through a returned LSE
     Tensor dq = at::empty(q.sizes(), q.options()), dk = at::empty(k.sizes(), k.options()), dv = at::empty(v.sizes(), v.options());
     chill_bwd_args a{};
     a.s = make_shape(q, k, lens, c);
@@ -211,9 +214,11 @@ void throw_chill_error(const std::string& message) { throw ChillError(message); 
 namespace {
 
 // O, (O, LSE) when return_lse, or None when the arguments do not pass the checks.
-py::object attention(std::shared_ptr<Library> lib, const Tensor& q, const Tensor& k, const Tensor& v, std::optional<Tensor> lens,
+py::object attention(std::shared_ptr<Library> lib, const Tensor& q_in, const Tensor& k_in, const Tensor& v_in, std::optional<Tensor> lens,
                      const py::tuple& mask_args, double sm_scale, bool return_lse, uint32_t flags) {
-  if (!arguments_ok(q, k, v, lens)) return py::none();
+  if (!arguments_ok(q_in, k_in, v_in, lens)) return py::none();
+  const Tensor q = signed_as_stored(q_in), k = signed_as_stored(k_in), v = signed_as_stored(v_in);
+  if (lens.has_value()) lens = signed_as_stored(*lens);
   auto call = c10::make_intrusive<Call>();
   call->mask = chill_mask_desc{};
   call->mask.id = lib->functor_id;

@@ -127,3 +127,49 @@ def test_what_is_changed_in_place_is_refused(ca, monkeypatch, fast):
             call()
     for t, was in zip((*caches, *pages, shared), before):
         assert torch.equal(t, was)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("which", range(5))
+def test_attention_and_its_gradients(ca, dtype, which):
+    """q, k, v, the gradient of O and that of the LSE."""
+    g = torch.Generator().manual_seed(which)
+    q, k, v, do = (torch.randn(1, h, 70, 64, generator=g).to(dtype).cuda() for h in (4, 2, 2, 4))
+    dlse = torch.randn(1, 4, 70, generator=g).cuda()
+    mask = ca.CausalChillMask()
+
+    def step(q, k, v, do, dlse):
+        leaves = [t.detach().requires_grad_() for t in (q, k, v)]
+        out = ca.chill_attention(*leaves, mask, return_lse=True)
+        return [t.detach() for t in out] + list(torch.autograd.grad(out, leaves, (do, dlse)))
+
+    was = ca.is_deterministic()
+    ca.set_deterministic(True)
+    try:
+        args = [q, k, v, do, dlse]
+        want = step(*args)
+        args[which] = lazy(args[which])
+        for x, y in zip(step(*args), want):
+            assert torch.equal(x, y)
+        with torch.no_grad():
+            assert torch.equal(ca.chill_attention(*args[:3], mask, lens=lazy(ints([33]))), ca.chill_attention(q, k, v, mask, lens=ints([33])))
+    finally:
+        ca.set_deterministic(was)
+
+
+@pytest.mark.parametrize("which", range(4))
+def test_attention_of_host_tensors(ca, which):
+    from chill_attention.host import attention_fwd_bwd_host
+
+    was = ca.is_deterministic()
+    ca.set_deterministic(True)
+    try:
+        args = [torch.randn(1, h, 64, 64).bfloat16() for h in (4, 2, 2, 4)]
+        want = attention_fwd_bwd_host(*args, ca.CausalChillMask())
+        args[which] = lazy(args[which])
+        for x, y in zip(attention_fwd_bwd_host(*args, ca.CausalChillMask()), want):
+            assert torch.equal(x, y)
+        with pytest.raises(AssertionError):
+            attention_fwd_bwd_host(*args, ca.CausalChillMask(), out=tuple(torch._neg_view(x) for x in want))
+    finally:
+        ca.set_deterministic(was)
