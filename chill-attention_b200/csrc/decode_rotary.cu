@@ -202,8 +202,8 @@ static int rotate(const chill_rotate_args* a, bool append, cudaStream_t st) {
   if (!a->inv_freq || !a->positions) return CHILL_E_INVALID;
   if ((a->interleaved | a->inverse) & ~1) return CHILL_E_INVALID;
   if (a->q == nullptr && a->k == nullptr) return CHILL_E_INVALID;
-  if (a->q != nullptr && (a->H <= 0 || a->q_out == nullptr)) return CHILL_E_INVALID;
-  if (a->k != nullptr && (a->H_kv <= 0 || (!append && a->k_out == nullptr))) return CHILL_E_INVALID;
+  if ((a->q == nullptr) != (a->q_out == nullptr) || (!append && (a->k == nullptr) != (a->k_out == nullptr))) return CHILL_E_INVALID;
+  if ((a->q != nullptr && a->H <= 0) || (a->k != nullptr && a->H_kv <= 0)) return CHILL_E_INVALID;
   if (append) {
     if (!a->q || !a->k || !a->v || !a->k_cache || !a->v_cache || !a->slots || a->num_pages <= 0 || a->page_size <= 0 || a->inverse) return CHILL_E_INVALID;
     if ((long long)a->num_pages * a->page_size > 0x7fffffffll) return CHILL_E_TOO_LARGE;

@@ -1,6 +1,7 @@
 // Eager-mode call path of the operators around attention (chill_attention/rotary.py, beams.py, cache.py): argument checks, outputs and
 // workspace from torch's allocator, C-ABI calls of include/chill_decode.h, and the rotation's autograd node.  Part of the native module that torch_ext.cpp
 // defines.  A check that fails returns None; the caller repeats the checks in Python for the message.
+#include <ATen/core/dispatch/Dispatcher.h>
 #include <ATen/ops/empty_like.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <torch/csrc/Exceptions.h>
@@ -97,6 +98,16 @@ std::pair<Tensor, Tensor> launch_rotate(const DecodeLibrary& lib, const Tensor& 
 
 std::pair<Tensor, Tensor> rotate_any(const Tensor& x, const Tensor& y, const Where& w, c10::intrusive_ptr<Turn> turn);
 
+// The dispatcher op (rotary.py), for gradients that are more than their memory: subclasses, several at a time, signs still to be applied.
+std::pair<Tensor, Tensor> rotate_by_dispatcher(const Tensor& x, const Tensor& y, const Where& w, const Turn& turn) {
+  static const auto op = c10::Dispatcher::singleton()
+                             .findSchemaOrThrow("chill_attention::rotate", "")
+                             .typed<std::tuple<Tensor, Tensor>(const Tensor&, const std::optional<Tensor>&, const Tensor&, const Tensor&, const std::optional<Tensor>&, bool, bool)>();
+  auto optional = [](const Tensor& t) { return t.defined() ? std::optional<Tensor>(t) : std::nullopt; };
+  auto [x_out, y_out] = op.call(x, optional(y), w.positions, w.inv_freq, optional(w.axes), turn.interleaved, turn.inverse);
+  return {x_out, y.defined() ? y_out : Tensor()};
+}
+
 // Linear in its input: the gradient is turned by the opposite angle, and nothing but the positions is kept.  The backward is this function again, so it can
 // be differentiated in its turn.
 struct RotateFn : torch::autograd::Function<RotateFn> {
@@ -129,6 +140,7 @@ struct RotateFn : torch::autograd::Function<RotateFn> {
 };
 
 std::pair<Tensor, Tensor> rotate_any(const Tensor& x, const Tensor& y, const Where& w, c10::intrusive_ptr<Turn> turn) {
+  if (watched({&x}, y.defined() ? std::optional<Tensor>(y) : std::nullopt)) return rotate_by_dispatcher(x, y, w, *turn);
   if (at::GradMode::is_enabled() && (x.requires_grad() || (y.defined() && y.requires_grad()))) {
     auto optional = [](const Tensor& t) { return t.defined() ? std::optional<Tensor>(t) : std::nullopt; };
     variable_list out = RotateFn::apply(x, optional(y), w.positions, w.inv_freq, optional(w.axes), std::move(turn));

@@ -33,7 +33,7 @@ typedef struct chill_rotate_args {
   const int32_t* axes;           /* [pairs], row of positions that turns a pair (clamped to [0, n_axes)), or NULL: the first one */
   const int32_t* positions;      /* [axis][batch][token] */
   int64_t position_strides[3];
-  const void *q, *k;             /* [batch][head][token][channel]; q with H heads, k with H_kv; either may be NULL in chill_rotate */
+  const void *q, *k;             /* [batch][head][token][channel]; q with H heads, k with H_kv; either may be NULL in chill_rotate, with its result */
   int64_t q_strides[4], k_strides[4];
   void *q_out, *k_out;           /* results; neither may overlap an input.  chill_rotate_append does not look at k_out */
   int64_t q_out_strides[4], k_out_strides[4];
