@@ -107,8 +107,10 @@ def _(q, k, positions, inv_freq, axes, interleaved, inverse):
 
 
 def _rotate_setup(ctx, inputs, output):
-    _, k, positions, inv_freq, axes, ctx.interleaved, ctx.inverse = inputs
+    q, k, positions, inv_freq, axes, ctx.interleaved, ctx.inverse = inputs
     ctx.has_k = k is not None
+    # a constant turned is a constant: nothing behind it works out a gradient
+    ctx.mark_non_differentiable(*(y for x, y in zip((q, k), output) if x is None or not x.requires_grad))
     ctx.save_for_backward(positions, inv_freq, axes)
     ctx.set_materialize_grads(False)
 

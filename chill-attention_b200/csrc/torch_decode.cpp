@@ -119,6 +119,8 @@ struct RotateFn : torch::autograd::Function<RotateFn> {
     ctx->saved_data["turn"] = c10::IValue::make_capsule(std::move(turn));
     ctx->set_materialize_grads(false);
     if (!y.has_value()) return {x_out};
+    if (!x.requires_grad()) ctx->mark_non_differentiable({x_out});  // a constant turned is a constant
+    if (!y->requires_grad()) ctx->mark_non_differentiable({y_out});
     return {x_out, y_out};
   }
 

@@ -1,4 +1,4 @@
-"""Gradients that reach the rotation's backward in other forms than plain memory."""
+"""Gradients that reach the rotation's backward in other forms than plain memory, and inputs that need none."""
 import pytest
 import torch
 
@@ -115,3 +115,42 @@ def test_saved_tensors_may_be_packed(ca):
     with torch.autograd.graph.save_on_cpu():
         out = ca.chill_rotate(q, k, positions.expand(2, 7), rotary)
     assert all(torch.equal(x, y) for x, y in zip(torch.autograd.grad(out, (q, k), (gq, gk)), want))
+
+
+@pytest.mark.parametrize("fast", [True, False])
+@pytest.mark.parametrize("needs_q", [True, False])
+def test_only_what_needs_a_gradient_gets_one(ca, monkeypatch, needs_q, fast):
+    """The turned form of a constant is a constant: nothing behind it works out a gradient for it, and the backward turns the other one alone."""
+    from chill_attention import _decode_abi, _eager
+
+    monkeypatch.setattr(_eager, "ENABLED", fast)
+    q, k, gq, gk, positions, rotary = problem(ca)
+    (k if needs_q else q).requires_grad_(False)
+    out = ca.chill_rotate(q, k, positions, rotary)
+    assert [x.requires_grad for x in out] == [needs_q, not needs_q]
+    asked = []
+    needed = out[0 if needs_q else 1]
+    needed.register_hook(lambda g: asked.append(g.shape))
+    (out[0].sum() * out[1].sum()).backward()
+    leaf, constant = (q, k) if needs_q else (k, q)
+    assert constant.grad is None and asked == [leaf.shape]
+    (want,) = torch.autograd.grad(ca.chill_rotate(leaf, None, positions, rotary)[0], leaf, torch.ones_like(leaf) * out[1 if needs_q else 0].sum().detach())
+    assert torch.equal(leaf.grad, want)
+    for y in out:  # and once more, both ways of asking
+        if y.requires_grad:
+            (again,) = torch.autograd.grad(ca.chill_rotate(q, k, positions, rotary)[0 if needs_q else 1], leaf, gq if needs_q else gk)
+            with torch.no_grad():
+                assert torch.equal(again, ca.chill_rotate(gq if needs_q else gk, None, positions, rotary._replace(inv_freq=-rotary.inv_freq))[0])
+
+
+@pytest.mark.parametrize("needs_q", [True, False])
+def test_a_compiled_call_with_a_constant(ca, needs_q):
+    torch._dynamo.reset()
+    q, k, gq, gk, positions, rotary = problem(ca)
+    leaf, constant = (q, k) if needs_q else (k, q)
+    constant.requires_grad_(False)
+    loss = lambda q, k: (lambda out: (out[0].sum() * out[1].sum(), out))(ca.chill_rotate(q, k, positions, rotary))  # noqa: E731
+    got, out = torch.compile(loss, fullgraph=True, backend="aot_eager")(q, k)
+    assert [x.requires_grad for x in out] == [needs_q, not needs_q]
+    want, _ = loss(q, k)
+    assert torch.allclose(torch.autograd.grad(got, leaf)[0], torch.autograd.grad(want, leaf)[0], rtol=1e-6, atol=1e-6)
