@@ -71,6 +71,7 @@ def _check_where(x, positions, rotary):
     assert isinstance(positions, torch.Tensor) and positions.dtype == torch.int32 and positions.device == x.device, f"positions must be int32 on {x.device}"
     assert positions.ndim in (2, 3) and tuple(positions.shape[-2:]) == (B, L) and positions.shape[0] >= 1, \
         f"positions must be [{B}, {L}] or [axes, {B}, {L}], not {tuple(positions.shape)}"
+    assert positions.ndim == 2 or positions.shape[0] == 1 or axes is not None, "several rows of positions, and no rotary.axes that says which pair turns by which"
 
 
 def _check_rotate(q, k, positions, rotary):
@@ -149,7 +150,8 @@ def chill_rotate(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tenso
     Args:
         q: [batch, heads, tokens, channels], fp16 / bf16 / fp32, any strides.
         k: the same with kv_heads, or None: q alone is turned.
-        positions: int32 [batch, tokens], or for several axes [axes, batch, tokens]; any strides (``.expand`` for one row of positions).
+        positions: int32 [batch, tokens], or for several axes (``rotary.axes``) [axes, batch, tokens]; any strides (``.expand`` for one row of positions).
+            A pair whose axis is beyond the rows takes the last one: with one row every axis has it.
         rotary: frequencies, axes and pairing.
 
     Returns: (q, k) turned, with the strides of the inputs where these are dense; k is None where it was.
@@ -174,7 +176,8 @@ def chill_rotate_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, k_cac
         q: [batch, heads, max_new, head_dim]; k, v: [batch, kv_heads, max_new, head_dim]; any strides.
         k_cache, v_cache: [num_pages, kv_heads, page_size, head_dim], any strides; the rows of ``step.slots`` are written (-1: none).
         step: of ``chill_pages_reserve``.
-        positions: default ``step.positions``; for several axes int32 [axes, batch, max_new].  With one row of positions every axis has these.
+        positions: default ``step.positions``; for several axes int32 [axes, batch, max_new].  With one row of positions every axis has these
+            (a pair whose axis is beyond the rows takes the last one).
 
     There are no gradients: tensors that require them are refused.
     """

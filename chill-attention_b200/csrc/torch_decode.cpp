@@ -163,6 +163,7 @@ bool where_ok(const Tensor& x, const Tensor& positions, const Tensor& inv_freq, 
   if (axes.has_value() && !ints(*axes, {pairs}, x)) return false;
   if (positions.scalar_type() != at::kInt || positions.device() != x.device()) return false;
   const int64_t d = positions.dim();
+  if (d == 3 && positions.size(0) > 1 && !axes.has_value()) return false;
   return (d == 2 || (d == 3 && positions.size(0) >= 1 && positions.size(0) <= INT32_MAX)) && positions.size(d - 2) == B && positions.size(d - 1) == L;
 }
 

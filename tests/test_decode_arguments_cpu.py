@@ -26,3 +26,14 @@ def test_a_result_without_its_input(lib):
 
     assert call(q=None) == call(k=None) == call(q_out=None) == call(k_out=None) == -1
     assert call(q=None, q_out=None, H_kv=0) == call(k=None, k_out=None, H=0) == -1
+
+
+def test_rows_of_positions_and_axes():
+    from chill_attention import ChillRotary, rotary
+
+    x, at = torch.zeros(2, 4, 3, 16), torch.zeros(3, 2, 3, dtype=torch.int32)
+    plain, three = ChillRotary.of(16, device="cpu"), ChillRotary.of(16, axes=(0, 1, 2, 2, 1, 0, 0, 0), device="cpu")
+    with pytest.raises(AssertionError, match="rotary.axes"):
+        rotary._check_where(x, at, plain)
+    for positions, which in ((at, three), (at[:2], three), (at[:1], three), (at[0], three), (at[:1], plain), (at[0], plain)):
+        rotary._check_where(x, positions, which)
