@@ -65,7 +65,7 @@ def _check_where(x, positions, rotary):
     assert isinstance(inv_freq, torch.Tensor) and inv_freq.dtype == torch.float32 and inv_freq.ndim == 1 and inv_freq.is_contiguous(), \
         "rotary.inv_freq must be a contiguous float32 tensor [pairs]"
     assert inv_freq.device == x.device and 1 <= inv_freq.shape[0] and 2 * inv_freq.shape[0] <= D, "rotary has more channels than a head, or is elsewhere"
-    assert not inv_freq.requires_grad, "there is no gradient for rotary.inv_freq"
+    assert not (torch.is_grad_enabled() and inv_freq.requires_grad), "there is no gradient for rotary.inv_freq"
     if axes is not None:
         cache._check_ints(x, axes=(axes, inv_freq.shape))
     assert isinstance(positions, torch.Tensor) and positions.dtype == torch.int32 and positions.device == x.device, f"positions must be int32 on {x.device}"

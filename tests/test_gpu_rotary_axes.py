@@ -1,4 +1,4 @@
-"""Rows of positions and the axes that name them."""
+"""Rows of positions, the axes that name them, and frequencies."""
 import pytest
 import torch
 
@@ -38,3 +38,20 @@ def test_axes_beyond_the_rows_take_the_last_one(ca, rows):
     check_turned(y, x, orc.rotate(x, positions, rotary.inv_freq, which), 8, False, torch.float32)
     if rows == 1:  # a step's own positions: every axis has these
         assert torch.equal(y, ca.chill_rotate(x, None, positions[0], rotary)[0])
+
+
+def test_frequencies_that_ask_for_gradients(ca):
+    """Refused while gradients are recorded, taken where they are not, whichever way a call goes."""
+    from chill_attention import _eager
+
+    x, at = torch.randn(1, 2, 3, 8, device="cuda"), ints([[4, 5, 6]])
+    rotary = ca.ChillRotary.of(8)
+    held = rotary._replace(inv_freq=rotary.inv_freq.clone().requires_grad_())
+    want = ca.chill_rotate(x, None, at, rotary)[0]
+    for fast in (True, False):
+        with pytest.MonkeyPatch.context() as m:
+            m.setattr(_eager, "ENABLED", fast)
+            with pytest.raises(AssertionError, match="gradient"):
+                ca.chill_rotate(x, None, at, held)
+            with torch.no_grad():
+                assert torch.equal(ca.chill_rotate(x, None, at, held)[0], want)
