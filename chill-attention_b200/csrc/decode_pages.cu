@@ -13,6 +13,7 @@ constexpr int kPageWarps = kPageThreads / 32;
 constexpr int kPageCtas = 8;
 constexpr int kMaxCtas = 16;
 constexpr int kForkRequests = 8192;
+constexpr int kMostPages = 1 << 30;  // the number of a page and what a cluster's CTAs step beyond it fit 32 bits
 constexpr int kMostShared = 200 * 1024;
 constexpr size_t kUnasked = 40 * 1024;  // dynamic shared memory that every kernel here gets beside its static one
 
@@ -458,7 +459,7 @@ static size_t workspace_of(const chill_share_args& a) {
 
 static int check_share(const chill_share_args* a, bool pointers) {
   if (a == nullptr || a->B <= 0 || a->page_size <= 0 || a->num_pages <= 0 || a->table_width <= 0) return CHILL_E_INVALID;
-  if (a->B > kMaxRequests || (long long)a->num_pages * a->page_size > 0x7fffffffll || (long long)a->table_width * a->page_size > kMaxLen ||
+  if (a->B > kMaxRequests || a->num_pages > kMostPages || (long long)a->num_pages * a->page_size > 0x7fffffffll || (long long)a->table_width * a->page_size > kMaxLen ||
       (long long)a->B * a->table_width > 0x7ffffff0ll)  // the number of an entry is a claim, below -1
     return CHILL_E_TOO_LARGE;
   if (!pointers) return CHILL_OK;

@@ -77,7 +77,8 @@ int chill_beam_select(const chill_select_args* a, void* stream);
 
 /* ------------------------------------------------------------------------------------------------------------------
  * Pages that several requests hold.  shared[page] counts the holders beyond one: 0 for a page that one request holds and for a free one, so that
- * chill_pages_reserve hands out pages as ever.  Tables, held, free_pages and n_free are those of chill_pages_args. */
+ * chill_pages_reserve hands out pages as ever.  Tables, held, free_pages and n_free are those of chill_pages_args.  Sizes: num_pages <= 2^30,
+ * num_pages * page_size < 2^31, table_width * page_size <= 2^29, B <= 65535, B * table_width <= 2^31 - 16 (CHILL_E_TOO_LARGE). */
 typedef struct chill_share_args {
   int32_t B, page_size, num_pages, table_width;
   int32_t* table; /* [B][table_width], rows table_stride apart */

@@ -37,3 +37,19 @@ def test_rows_of_positions_and_axes():
         rotary._check_where(x, at, plain)
     for positions, which in ((at, three), (at[:2], three), (at[:1], three), (at[0], three), (at[:1], plain), (at[0], plain)):
         rotary._check_where(x, positions, which)
+
+
+def test_pools_of_so_many_pages_that_their_numbers_leave_32_bits(lib):
+    """A cluster's shares of 2^31 - 1 pages end beyond what an int holds."""
+    from chill_attention import _decode_abi as abi
+
+    every = ("table", "held", "free_pages", "n_free", "shared", "lens", "missing", "parents", "source", "target", "rows", "count", "workspace")
+
+    def args(num_pages, **changes):
+        return made(abi.ShareArgs, every, **{**dict(B=4, page_size=1, num_pages=num_pages, table_width=20, table_stride=20, workspace_bytes=1 << 40, out_lens=8192), **changes})
+
+    for n in (2 ** 31 - 1, 2 ** 31 - 8, 2 ** 30 + 1):
+        assert lib.chill_share_workspace_bytes(args(n)) == 0
+        assert all(call(args(n), None) == -4 for call in (lib.chill_pages_fork, lib.chill_pages_trim_shared, lib.chill_pages_compact))
+    assert lib.chill_share_workspace_bytes(args(2 ** 30)) > 4 * 2 ** 30
+    assert all(call(args(2 ** 30, workspace_bytes=100), None) == -1 for call in (lib.chill_pages_fork, lib.chill_pages_trim_shared, lib.chill_pages_compact))
