@@ -29,7 +29,7 @@ import typing
 import torch
 from torch.autograd import forward_ad
 
-from . import _cabi, _cache_abi, _eager, chill
+from . import _cabi, _cache_abi, _decode_abi, _eager, chill
 from .mask import ChillMask
 
 _HEAD_DIMS = chill._HEAD_DIMS
@@ -288,7 +288,7 @@ def _places(pages):
 def _check_fork(pages, shared, lens, parents, page_size):
     _check_pages(pages, lens, page_size)
     B = pages.table.shape[0]
-    assert B <= 8192, "a fork takes at most 8192 requests"
+    assert B <= _decode_abi.FORK_MAX, f"a fork takes at most {_decode_abi.FORK_MAX} requests"
     _check_ints(pages.table, missing=(pages.missing, (1,)), shared=(shared, pages.free.shape), parents=(parents, (B,)))
     _check_changed(missing=pages.missing, shared=shared)
 
