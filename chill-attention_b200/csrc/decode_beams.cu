@@ -279,8 +279,7 @@ __global__ void __launch_bounds__(kThreads, 4) scan_kernel(const __grid_constant
   asm volatile("griddepcontrol.launch_dependents;");
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int beam = (int)blockIdx.x / p.parts, part = (int)blockIdx.x - beam * p.parts;
-  const int from = (int)((long long)part * p.segment < p.V ? (long long)part * p.segment : p.V);
-  const int to = (int)((long long)from + p.segment < p.V ? from + p.segment : p.V);
+  const int from = part * p.segment, to = imin(from + p.segment, p.V);  // every segment has a value (parts_of)
   const T* row = reinterpret_cast<const T*>(p.logits) + beam * p.row_stride + from;
   const int size = to - from;
   if (p.scores[beam] == -INFINITY || (p.finished != nullptr && p.finished[beam] != 0)) return;  // nothing of it is looked at
@@ -348,7 +347,6 @@ __global__ void __launch_bounds__(kThreads, 4) scan_kernel(const __grid_constant
     for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
     if (lane == 0) of_warps[warp] = {sum, highest, 0};
   };
-  if (size == 0) add_up();
   const int round_step = imin(imax(192 / p.M, 1), 16) * kStep;
   for (int round = 0; round * V < size; round += round_step) {
     int queued = 0;
@@ -732,7 +730,6 @@ __global__ void __launch_bounds__(kMergeWarps * 32) merge_kernel(const __grid_co
     for (int i = threadIdx.x; i < n; i += blockDim.x) {
       const Candidate c = found[i];
       int place = i & 31;
-      if (c.rank == 0) continue;
       for (int run = 0; run < n; run += 32) {
         if (run == (i & ~31) || !before(found[run], c)) continue;
         int larger = 0;
