@@ -68,7 +68,10 @@ def chill_beam_select(logits: torch.Tensor, scores: torch.Tensor, count: int | N
 
     Candidate (beam, token) of a group has ``scores[group, beam] + log_softmax(logits[row])[token]``, row = group * beams + beam; -inf where the logit or the beam's score
     is -inf (a row of nothing but -inf has no candidates).  They are ranked by that value in 64 bits, and it is rounded to fp32 at the end; of equal ones the lowest
-    beam, then the largest logit, then the lowest token comes first.  (Logits differ at one value where 64 bits round it, as with scores beyond 1e9.)  A NaN or +inf among a row's logits makes its candidates NaN, which rank first: they show.
+    beam, then the largest logit, then the lowest token comes first.  The exponentials of the row's sum are fp32, so its logarithm is good to 1e-7 (1e-5 where the
+    maximum rises again and again along the row): a beam's candidates are in the exact order of their logits, those of different beams may change places where they are
+    nearer than that.  Equal rows have equal sums, bit for bit.  A NaN or +inf among a row's logits, or a NaN as score, makes its candidates NaN, which rank first: they
+    show.  They are all alike, and so are those of a score of +inf: the lowest token first.
 
     Args:
         logits: [groups * beams, vocab], fp16 / bf16 / fp32; rows any stride apart.

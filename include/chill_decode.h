@@ -53,9 +53,12 @@ int chill_rotate_append(const chill_rotate_args* a, void* stream);
 /* ------------------------------------------------------------------------------------------------------------------
  * Selection over beams and vocabulary.  Candidate (k, v) of group g: c = scores[g][k] + x - log sum exp x', x = logits[g * K + k][v], the sum over the
  * row; -inf where the logit or the beam's score is -inf.  A finished beam has one candidate, (k, end_token) with c = scores[g][k], and its
- * logits are not looked at.  The M candidates of the largest c, worked out in 64 bits, in descending order, of equal ones the lowest k, then the largest x (they
- * differ where 64 bits round c to one number: scores beyond 1e9), then the lowest v; NaN counts as largest (a NaN or +inf among a row's logits makes all its
- * candidates NaN, but for those of -inf: the lowest v first). */
+ * logits are not looked at.  The M candidates of the largest c in descending order, of equal ones the lowest k, then the largest x (64 bits round c, and neighbouring
+ * logits may share it), then the lowest v.  c is worked out, ranked and kept in 64 bits until it is written, but the terms of its sum are fp32 exponentials, up to 32 of them
+ * a thread added in fp32: the logarithm is good to 1e-7 in ordinary rows, and to 1e-5 where a row's maximum rises again and again along it (measured: 6e-8, 3e-6).  Candidates of one beam are in the exact
+ * order of their logits; those of different beams that are nearer than that may change places.  Equal rows (not permutations of one another) have equal sums, bit
+ * for bit.  NaN counts as largest: a NaN or +inf among a row's logits, or a NaN as score, makes all its candidates NaN, but for those of -inf; these, and those of a beam of score
+ * +inf, are alike, the lowest v first. */
 #define CHILL_SELECT_MAX 64 /* beams of a group, and candidates that are kept */
 typedef struct chill_select_args {
   int32_t G, K, M, dtype;
