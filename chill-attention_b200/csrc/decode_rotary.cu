@@ -3,8 +3,9 @@
 //
 // A copy with little arithmetic: every row is read and written once, so the bound is memory.  A thread owns one vector of pairs of one token and
 // goes over heads with it.  The sines and cosines are the same for all heads: a block's warps, which have the same vectors of different heads, share them.  q and k of (8, 16, 4096, 128) in bf16:
-// 84 us (6.4 TB/s, 0.97 of a copy's rate; 87 us where every thread works out its own); (3, 32 and 8, 5003, 128) in fp16, 96 channels turned by three axes: 50 us (0.94); 4000 tokens of 24
-// and 8 heads of 128 into pages of 16: 17 us (0.74: two waves of short CTAs).  The next heads' loads ahead of this one's arithmetic, with one loop over the heads of all tensors: 178 us (pointers chosen a head, spills).
+// 84 us (6.4 TB/s, 0.97 of a copy's rate; 87 us where every thread works out its own); (3, 32 and 8, 5003, 128) in fp16, 96 channels turned by three axes: 52 us (0.91).  Into pages of 16, 24
+// and 8 heads of 128 in fp16: 3 prompts of 5000 tokens 55 us (0.85), 4 of 1000 18.7 us (0.67; 16.5 where inputs and outputs, 81 MB, stay in L2): two waves of short CTAs, the second
+// not full.  The next heads' loads ahead of this one's arithmetic, with one loop over the heads of all tensors: 178 us (pointers chosen a head, spills).
 #include "decode_common.cuh"
 
 namespace chill {
@@ -172,7 +173,7 @@ static cudaError_t launch_rotate(RotateP& p, int vec, bool paired, cudaStream_t 
   p.items = (unsigned)items;
   const int per_block = vec * (int)sizeof(T) == 16 ? 32 : kThreads, shares = kThreads / per_block;  // kItems
   const long long blocks = (items + per_block - 1) / per_block;
-  // Heads in as many slices as fill the SMs with 8 blocks each (a prompt's 4000 tokens, 24 and 8 heads: 16.9 us, with 16 17.8); a block has `shares` of them
+  // Heads in as many slices as fill the SMs with 8 blocks each (4 prompts of 1000 tokens, 24 and 8 heads of 128: 18.7 us, with 16 19.0); a block has `shares` of them
   const long long want = 8ll * sm_count();
   const long long more = blocks >= want ? 1 : (want + blocks - 1) / blocks;
   const dim3 grid((unsigned)blocks, (unsigned)imax(1, imin((int)more, (p.heads + shares - 1) / shares)));
