@@ -541,17 +541,6 @@ struct CopyP {
   bool both;
 };
 
-template <class V>
-__device__ __forceinline__ V load_once(const char* p) {
-  if constexpr (sizeof(V) == 16) return __ldcs(reinterpret_cast<const V*>(p));
-  else return *reinterpret_cast<const V*>(p);
-}
-template <class V>
-__device__ __forceinline__ void store_once(char* p, const V& v) {
-  if constexpr (sizeof(V) == 16) __stcs(reinterpret_cast<V*>(p), v);
-  else *reinterpret_cast<V*>(p) = v;
-}
-
 constexpr int kCopyThreads = 256, kCopyEach = 4;
 
 template <class V>

@@ -43,22 +43,6 @@ __device__ __forceinline__ float2 turn(int position, float freq) {
   return cs;
 }
 
-// Nobody reads these again here: with plain loads and stores 20 % longer (q and k of (8, 16, 4096, 128) in bf16).
-template <class VecT>
-__device__ __forceinline__ VecT load_once(const char* p) {
-  if constexpr (sizeof(VecT) == 16) {
-    const uint4 raw = __ldcs(reinterpret_cast<const uint4*>(p));
-    return *reinterpret_cast<const VecT*>(&raw);
-  } else {
-    return *reinterpret_cast<const VecT*>(p);
-  }
-}
-template <class VecT>
-__device__ __forceinline__ void store_once(char* p, const VecT& v) {
-  if constexpr (sizeof(VecT) == 16) __stcs(reinterpret_cast<uint4*>(p), *reinterpret_cast<const uint4*>(&v));
-  else *reinterpret_cast<VecT*>(p) = v;
-}
-
 // kPaired: pairs (2 i, 2 i + 1); a vector of V channels is V / 2 pairs (V = 1: a thread moves a pair as two elements).  Otherwise pairs (i, i + pairs): two
 // vectors.  V > 1 wants channels that lie beside each other.
 template <class T, int V, bool kPaired, bool kAppend>
