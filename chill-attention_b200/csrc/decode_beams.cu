@@ -3,7 +3,7 @@
 //
 // The logits are read once, and that is the floor.  Within a row the order is that of x, so a CTA that streams a segment of a row keeps the M largest x beside the
 // maximum and sum of the softmax, without knowing lse yet; a second kernel, a CTA for each group, turns the segments' lists into candidates and merges them.  Replayed from a
-// graph: 32 groups of 8 beams over 128000 tokens in bf16, 16 candidates 30 us (floor 9), 4 groups of 32 beams over 50021 in fp32, 64 candidates 26 us (floor 4), one group of 4 beams
+// graph: 32 groups of 8 beams over 128000 tokens in bf16, 16 candidates 30 us (floor 9), 4 groups of 32 beams over 50021 in fp32, 64 candidates 27 us (floor 4), one group of 4 beams
 // over 32000 in fp32 10 us (floor: two launches).  One kernel with a group in a cluster of 16 CTAs, which exchange sums and lists through distributed shared memory, takes
 // 62, 75 and 14 us: 64 CTAs do not fill the GPU, and lists that are kept sorted while they grow cost more than the logits.
 //

@@ -68,7 +68,7 @@ __device__ __forceinline__ int block_scan(int v, int& total) {
 //
 // Latency is all there is: one cluster, whose barriers separate the steps, and few trips to memory one after the other.  Every CTA has a share of the rows and keeps them as they
 // were in shared memory, where children in other CTAs find them too (in the workspace where they are too large: kInside false); what goes back is noted there in bits.
-// 4 beams of 700 tokens in pages of 16: 10 us (two of them a launch); 16 groups of 16 beams of up to 16384 tokens (256 rows of 1026 blocks): 28 us in a cluster of 16 CTAs (8: 38), of which the rows' way into
+// 4 beams of 700 tokens in pages of 16: 11 us (two of them a launch); 16 groups of 16 beams of up to 16384 tokens (256 rows of 1026 blocks): 29 us in a cluster of 16 CTAs (8: 38), of which the rows' way into
 // shared memory 5, counts 3, claims 6 (scattered reads of shared), new tables 4, barriers 4.  Row by row with an atomic for every entry, and the rows in the workspace: 53 us.
 
 // A cluster's barrier costs one CTA alone 0.5 us more than its own.
